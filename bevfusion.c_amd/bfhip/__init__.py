@@ -11,6 +11,7 @@ is no fallback: if the library is missing, importing an entry point raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import pathlib
 
@@ -188,6 +189,40 @@ SIGNATURES = {
     "bf_cuda_runtime_debug_hashes": (_i, [_vp, C.POINTER(C.c_ulonglong), C.c_char_p, _sz]),
 }
 
+class Rows(C.Structure):
+    """``bfhip_rows`` (include/bfhip_transformer.h)."""
+    _fields_ = [("data", _vp), ("token_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
+class AttentionDesc(C.Structure):
+    """``bfhip_attention_desc`` (include/bfhip_transformer.h)."""
+    _fields_ = [(n, _i) for n in ("type", "sequences", "heads", "kv_heads", "head_dim", "causal",
+                                  "reach")] + \
+               [("scale", C.c_float), ("q_tokens", C.c_longlong), ("k_tokens", C.c_longlong),
+                ("q_starts", _vp), ("k_starts", _vp), ("bias", _vp)]
+
+
+_ll, _rowsp, _attnp = C.c_longlong, C.POINTER(Rows), C.POINTER(AttentionDesc)
+
+# The operators of include/bfhip_transformer.h, which the reference's ABI does not have.
+TRANSFORMER_SIGNATURES = {
+    "bfhip_layer_norm_forward": (_i, [_i, _vp, _ll, _vp, _vp, _vp, _ll, _vp, _vp, _ll, _i,
+                                      C.c_float, _vp, C.c_char_p, _sz]),
+    "bfhip_layer_norm_backward_workspace": (_sz, [_ll, _i]),
+    "bfhip_layer_norm_backward": (_i, [_i, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _vp,
+                                       _ll, _i, _vp, _sz, _vp, C.c_char_p, _sz]),
+    "bfhip_position_bias_forward": (_i, [_vp, _vp, _vp, _i, _i, _ll, _vp, C.c_char_p, _sz]),
+    "bfhip_position_bias_backward_workspace": (_sz, [_i, _i, _ll]),
+    "bfhip_position_bias_backward": (_i, [_vp, _vp, _vp, _i, _i, _ll, _vp, _sz, _vp, C.c_char_p,
+                                          _sz]),
+    "bfhip_attention_forward_workspace": (_sz, [_attnp]),
+    "bfhip_attention_backward_workspace": (_sz, [_attnp]),
+    "bfhip_attention_forward": (_i, [_attnp] + [_rowsp] * 4 + [_vp, _vp, _sz, _vp, C.c_char_p,
+                                                               _sz]),
+    "bfhip_attention_backward": (_i, [_attnp] + [_rowsp] * 4 + [_vp] + [_rowsp] * 4
+                                 + [_vp, _vp, _sz, _vp, C.c_char_p, _sz]),
+}
+
 SWIN_OPS = ("ln1", "qkv", "attention", "proj", "ln2", "fc1", "fc2", "merge", "mlp", "wmsa")
 
 MODEL_SIGNATURES = {
@@ -222,7 +257,7 @@ def _bind(lib, table):
 def missing_symbols():
     """Entry points declared in include/*.h that libbfhip.so does not export."""
     lib = hip_lib()
-    return [n for n in SIGNATURES if not hasattr(lib, n)]
+    return [n for n in (*SIGNATURES, *TRANSFORMER_SIGNATURES) if not hasattr(lib, n)]
 
 
 def model_lib():
@@ -241,7 +276,7 @@ def hip_lib():
         model_lib()
         if not HIP_LIB.exists():
             raise BfHipError(f"{HIP_LIB} is not built (run __graft_entry__.build())")
-        _hip_lib = _bind(C.CDLL(str(HIP_LIB)), SIGNATURES)
+        _hip_lib = _bind(_bind(C.CDLL(str(HIP_LIB)), SIGNATURES), TRANSFORMER_SIGNATURES)
     return _hip_lib
 
 
@@ -373,6 +408,255 @@ def conv2d_raw(desc, x, w, b, out, stream=None):
     err = _err()
     ok = hip_lib().bf_cuda_conv2d_f32(C.byref(desc), x, w, b, out, _stream(stream), err, 512)
     return bool(ok), err.value.decode(errors="replace")
+
+
+# ------------------------------------------------------ transformer operators
+# Layer norm, position bias by buckets and packed attention, each with its
+# backward pass (include/bfhip_transformer.h).  The calls run on the device of
+# their tensors, whichever device is current, on that device's current stream
+# or on `stream`; results and scratch memory are allocated for that stream.
+def _type_code(t):
+    torch = _torch()
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+    if code is None:
+        raise BfHipError(f"expected a float32, float16 or bfloat16 tensor, not {t.dtype}")
+    return code
+
+
+def _expect(what, t, like, shape, dtype):
+    """`t` is a contiguous device tensor of `shape` on the device of `like`."""
+    if (t.device != like.device or not t.is_cuda or t.dtype != dtype or tuple(t.shape) != shape
+            or not t.is_contiguous()):
+        raise BfHipError(f"{what} must be a contiguous {dtype} {list(shape)} tensor on "
+                         f"{like.device}")
+    return _vp(t.data_ptr())
+
+
+_HERE = contextlib.nullcontext()
+
+
+@contextlib.contextmanager
+def _elsewhere(device, stream, tensors):
+    torch = _torch()
+    with torch.cuda.device(device):
+        if stream is None:
+            yield
+            return
+        if stream.device != device:
+            raise BfHipError(f"stream of {stream.device}, tensors on {device}")
+        with torch.cuda.stream(stream):
+            yield
+        for t in tensors:  # keeps their memory until the stream is done with it
+            if t is not None:
+                t.record_stream(stream)
+
+
+def _place(stream, *tensors):
+    """Context in which a call on `tensors` (the first one names the device)
+    allocates and launches."""
+    torch = _torch()
+    device = tensors[0].device
+    if not tensors[0].is_cuda:
+        raise BfHipError("expected a device tensor")
+    if stream is None and device.index == torch.cuda.current_device():
+        return _HERE
+    return _elsewhere(device, stream, tensors)
+
+
+def _scratch(size, device):
+    if not size:
+        return None, None
+    torch = _torch()
+    t = torch.empty(size, dtype=torch.uint8, device=device)
+    return t, _vp(t.data_ptr())
+
+
+def _matrix(what, t, like=None):
+    """[rows, features] with contiguous rows -> (pointer, row stride)."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise BfHipError(f"{what} must be [rows, features] with contiguous rows")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype
+                             or t.device != like.device):
+        raise BfHipError(f"{what} must match {list(like.shape)} {like.dtype} on {like.device}")
+    return _vp(t.data_ptr()), t.stride(0)
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream=None):
+    """Layer norm of the rows of x [rows, features] (bfhip_layer_norm_forward);
+    gamma, beta fp32 [features].  Returns y, or (y, mean, rstd) with `stats`,
+    which layer_norm_backward takes."""
+    torch = _torch()
+    code = _type_code(x)
+    px, sx = _matrix("x", x)
+    rows, n = x.shape
+    pg, pb = (None if t is None else _expect(name, t, x, (n,), torch.float32)
+              for name, t in (("gamma", gamma), ("beta", beta)))
+    with _place(stream, x, gamma, beta, out):
+        y = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else out
+        py, sy = _matrix("out", y, x)
+        pm = pr = None
+        if stats:
+            mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+            pm, pr = _vp(mean.data_ptr()), _vp(rstd.data_ptr())
+        err = _err()
+        _check(hip_lib().bfhip_layer_norm_forward(code, px, sx, pg, pb, py, sy, pm, pr, rows, n,
+                                                  eps, _stream(), err, 512),
+               err, "bfhip_layer_norm_forward")
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_backward(dy, x, mean, rstd, gamma=None, out=None, stream=None):
+    """Gradients of layer_norm (bfhip_layer_norm_backward): (dx, dgamma, dbeta)."""
+    torch = _torch()
+    code = _type_code(x)
+    px, sx = _matrix("x", x)
+    pdy, sdy = _matrix("dy", dy, x)
+    rows, n = x.shape
+    pm, pr = (_expect(name, t, x, (rows,), torch.float32)
+              for name, t in (("mean", mean), ("rstd", rstd)))
+    pg = None if gamma is None else _expect("gamma", gamma, x, (n,), torch.float32)
+    lib = hip_lib()
+    with _place(stream, x, dy, mean, rstd, gamma, out):
+        dx = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else out
+        pdx, sdx = _matrix("out", dx, x)
+        dgamma = torch.empty(n, dtype=torch.float32, device=x.device)
+        dbeta = torch.empty(n, dtype=torch.float32, device=x.device)
+        size = lib.bfhip_layer_norm_backward_workspace(rows, n)
+        work, pw = _scratch(size, x.device)
+        err = _err()
+        _check(lib.bfhip_layer_norm_backward(
+            code, pdy, sdy, px, sx, pg, pm, pr, pdx, sdx, _vp(dgamma.data_ptr()),
+            _vp(dbeta.data_ptr()), rows, n, pw, size, _stream(), err, 512),
+            err, "bfhip_layer_norm_backward")
+    return dx, dgamma, dbeta
+
+
+def position_bias(table, buckets, out=None, stream=None):
+    """A learned table [count, heads] spread over an int32 map of buckets of any
+    shape (bfhip_position_bias_forward): fp32 [heads, *buckets.shape]."""
+    torch = _torch()
+    if table.dim() != 2:
+        raise BfHipError("table must be [buckets, heads]")
+    count, heads = table.shape
+    pt = _expect("table", table, table, (count, heads), torch.float32)
+    pm = _expect("buckets", buckets, table, tuple(buckets.shape), torch.int32)
+    shape = (heads, *buckets.shape)
+    with _place(stream, table, buckets, out):
+        bias = torch.empty(shape, dtype=torch.float32, device=table.device) if out is None else out
+        pb = _expect("out", bias, table, shape, torch.float32)
+        err = _err()
+        _check(hip_lib().bfhip_position_bias_forward(pt, pm, pb, count, heads, buckets.numel(),
+                                                     _stream(), err, 512),
+               err, "bfhip_position_bias_forward")
+    return bias
+
+
+def position_bias_backward(dbias, buckets, count, stream=None):
+    """Gradient of position_bias's table (bfhip_position_bias_backward): fp32
+    [count, heads]."""
+    torch = _torch()
+    heads = dbias.shape[0] if dbias.dim() else 0
+    pd = _expect("dbias", dbias, dbias, (heads, *buckets.shape), torch.float32)
+    pm = _expect("buckets", buckets, dbias, tuple(buckets.shape), torch.int32)
+    lib, n = hip_lib(), buckets.numel()
+    with _place(stream, dbias, buckets):
+        dtable = torch.empty((count, heads), dtype=torch.float32, device=dbias.device)
+        size = lib.bfhip_position_bias_backward_workspace(count, heads, n)
+        work, pw = _scratch(size, dbias.device)
+        err = _err()
+        _check(lib.bfhip_position_bias_backward(pd, pm, _vp(dtable.data_ptr()), count, heads, n,
+                                                pw, size, _stream(), err, 512),
+               err, "bfhip_position_bias_backward")
+    return dtable
+
+
+def _head_rows(what, t, like, heads=None):
+    """[tokens, heads, head_dim] with contiguous heads -> Rows."""
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise BfHipError(f"{what} must be [tokens, heads, head_dim] with contiguous heads")
+    if (t.dtype != like.dtype or t.device != like.device or t.shape[2] != like.shape[2]
+            or (heads is not None and t.shape[1] != heads)):
+        raise BfHipError(f"{what} must match {like.dtype}, head_dim {like.shape[2]} and its "
+                         f"heads on {like.device}")
+    return Rows(t.data_ptr(), t.stride(0), t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias):
+    torch = _torch()
+    code = _type_code(q)
+    rows = [_head_rows("q", q, q), _head_rows("k", k, q), _head_rows("v", v, q)]
+    if v.shape != k.shape:
+        raise BfHipError("k and v must have one shape")
+    n = q_starts.numel() - 1
+    if n < 0:
+        raise BfHipError("starts must hold one entry more than there are sequences")
+    ps = [_expect(name, t, q, (n + 1,), torch.int32)
+          for name, t in (("q_starts", q_starts), ("k_starts", k_starts))]
+    heads, reach, pb = q.shape[1], 0, None
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[1] % 2 == 0:
+            raise BfHipError("bias must be [heads, 2 * reach + 1]")
+        reach = bias.shape[1] // 2
+        pb = _expect("bias", bias, q, (heads, 2 * reach + 1), torch.float32)
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    return AttentionDesc(code, n, heads, k.shape[1], q.shape[2], int(causal), reach, scale,
+                         q.shape[0], k.shape[0], *ps, pb), rows
+
+
+def attention(q, k, v, q_starts, k_starts, causal=False, scale=None, bias=None, out=None,
+              lse=False, stream=None):
+    """Attention over packed sequences (bfhip_attention_forward).  q [tokens,
+    heads, head_dim], k and v [tokens, kv_heads, head_dim], each with contiguous
+    heads (views of a fused projection will do); starts int32 [sequences + 1];
+    bias fp32 [heads, 2 * reach + 1] by signed distance, or None; scale
+    1 / sqrt(head_dim) by default.  Returns out like q, or (out, lse) with
+    `lse`, which attention_backward takes.  Rows that belong to no sequence are
+    not written."""
+    torch = _torch()
+    desc, rows = _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias)
+    lib = hip_lib()
+    with _place(stream, q, k, v, q_starts, k_starts, bias, out):
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        if o.shape[0] != q.shape[0]:
+            raise BfHipError("out must have the shape of q")
+        ro = _head_rows("out", o, q, q.shape[1])
+        stat, ps = None, None
+        if lse:
+            stat = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+            ps = _vp(stat.data_ptr())
+        size = lib.bfhip_attention_forward_workspace(desc)
+        work, pw = _scratch(size, q.device)
+        err = _err()
+        _check(lib.bfhip_attention_forward(desc, *rows, ro, ps, pw, size, _stream(), err, 512),
+               err, "bfhip_attention_forward")
+    return (o, stat) if lse else o
+
+
+def attention_backward(dout, q, k, v, out, lse, q_starts, k_starts, causal=False, scale=None,
+                       bias=None, stream=None):
+    """Gradients of attention (bfhip_attention_backward) from its out and lse:
+    (dq, dk, dv), and dbias after them if there is a bias.  Rows that belong to
+    no sequence are not written."""
+    torch = _torch()
+    desc, rows = _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise BfHipError("out and dout must have the shape of q")
+    ro, rg = _head_rows("out", out, q), _head_rows("dout", dout, q)
+    pl = _expect("lse", lse, q, (q.shape[1], q.shape[0]), torch.float32)
+    lib = hip_lib()
+    with _place(stream, q, k, v, q_starts, k_starts, bias, out, lse, dout):
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+        pb = None
+        if bias is not None:
+            grads.append(torch.empty_like(bias))
+            pb = _vp(grads[3].data_ptr())
+        size = lib.bfhip_attention_backward_workspace(desc)
+        work, pw = _scratch(size, q.device)
+        err = _err()
+        _check(lib.bfhip_attention_backward(
+            desc, *rows, ro, pl, rg, *(_head_rows("gradient", t, q) for t in grads[:3]), pb, pw,
+            size, _stream(), err, 512), err, "bfhip_attention_backward")
+    return tuple(grads)
 
 
 def window_map(batches, height, width, shift, device, stream=None):

@@ -1,0 +1,269 @@
+// Shared parts of the packed-sequence attention kernels: where a workgroup's
+// rows are, operand tiles in LDS, and their matrix-core fragments.
+#pragma once
+
+#include "bfhip_transformer.h"
+#include "element.h"
+#include "gemm_core.h"
+
+namespace bfhip {
+
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// One tensor of the call: bytes between tokens and heads.
+struct AttnRows {
+    char *data;
+    long long token, head;
+    // Address of `head` of `token`.
+    __device__ __forceinline__ char *at(long long t, int h) const { return data + t * token + h * head; }
+};
+
+struct AttnArgs {
+    AttnRows q, k, v, out;
+    const int *q_starts, *k_starts;
+    const float *bias;  // [heads, 2 reach + 1] or null
+    float *lse;         // [heads, q_tokens] or null
+    long long q_tokens, k_tokens;
+    int sequences, heads, kv_heads, dim, causal, reach;
+    float scale, scale2;  // scale2 = scale * log2(e): softmax runs in base 2
+};
+
+// Work on packed sequences is dealt in slots of `rows` rows without knowing the
+// lengths on the host: sequence b owns the slots
+//   floor(start_b / rows) + b  ..  floor(start_{b+1} / rows) + b,
+// which are at least ceil(length / rows) (at most one more), so slot_count()
+// slots always suffice and a slot finds its sequence by searching the starts.
+inline long long slot_count(long long tokens, int sequences, int rows) { return tokens / rows + sequences; }
+
+struct Slot {
+    int sequence;  // -1: none
+    int first;     // row within the sequence
+    int start, length;
+};
+
+__device__ __forceinline__ long long clamp_start(const int *starts, int b, long long tokens) {
+    const long long s = starts[b];
+    return s < 0 ? 0 : s > tokens ? tokens : s;
+}
+
+// The rows of sequence b: ascending starts within the tensor whatever the array holds.
+__device__ __forceinline__ void sequence_rows(const int *starts, int b, long long tokens, int &start, int &length) {
+    const long long s = clamp_start(starts, b, tokens), e = clamp_start(starts, b + 1, tokens);
+    start = __builtin_amdgcn_readfirstlane((int)s);
+    length = __builtin_amdgcn_readfirstlane((int)(e > s ? e - s : 0));
+}
+
+// One wave searches 64 candidates at a time (one load for up to 64 sequences,
+// two for up to 4096).
+template <int ROWS>
+__device__ __forceinline__ Slot find_slot(const int *starts, int sequences, long long tokens, int slot) {
+    const int lane = threadIdx.x % kWave;
+    int lo = 0, span = sequences;
+    while (span > 1) {
+        const int step = (span + kWave - 1) / kWave;
+        const int at = lo + lane * step;
+        const bool below = lane * step < span && clamp_start(starts, at, tokens) / ROWS + at <= slot;
+        const int n = __popcll(__ballot(below));  // a prefix of the lanes
+        const int skip = n > 0 ? (n - 1) * step : 0;
+        lo += skip;
+        span = min(step, span - skip);
+    }
+    Slot s;
+    s.sequence = __builtin_amdgcn_readfirstlane(lo);
+    sequence_rows(starts, s.sequence, tokens, s.start, s.length);
+    s.first = (slot - (s.start / ROWS + s.sequence)) * ROWS;
+    if (s.first < 0 || s.first >= s.length) s.sequence = -1;
+    return s;
+}
+
+// ------------------------------------------------------------- operand tiles
+// A tile of ROWS rows x DIM elements in LDS, in 16-byte chunks: chunk c of row
+// r sits at chunk c ^ swizzle(r) of its row, so that the sixteen rows a
+// fragment reads at the same c spread over all banks.
+template <class E, int DIM>
+struct AttnTile {
+    static constexpr int kRow = DIM * E::kSize;  // bytes
+    static constexpr int kChunks = kRow / 16;
+    __device__ __forceinline__ static int swizzle(int r) {
+        constexpr int per = kRow >= 256 ? 1 : 256 / kRow;  // rows in one pass over the banks
+        return r / per & ((kChunks < 16 ? kChunks : 16) - 1);
+    }
+};
+
+// Copies ROWS rows to LDS with THREADS threads by LDS-DMA.  Rows past `left`
+// and elements past dim read as zero.
+template <class E, int DIM, int ROWS, int THREADS>
+struct AttnTileCopy {
+    using T = AttnTile<E, DIM>;
+    static constexpr int kIssue = ROWS * T::kChunks / THREADS;
+    static_assert(ROWS * T::kChunks % THREADS == 0, "whole chunks per thread");
+    uint32_t off[kIssue];
+    uint32_t stride, row;  // bytes between rows, bytes of a row
+    int wave;
+    __device__ __forceinline__ void init(long long token_bytes, int dim, int thread) {
+        stride = (uint32_t)token_bytes;
+        row = (uint32_t)dim * E::kSize;
+        wave = __builtin_amdgcn_readfirstlane(thread / kWave);
+#pragma unroll
+        for (int j = 0; j < kIssue; ++j) {
+            const int id = j * THREADS + thread, r = id / T::kChunks;
+            const uint32_t c = 16u * ((uint32_t)(id % T::kChunks) ^ (uint32_t)T::swizzle(r));
+            off[j] = c < row ? (uint32_t)r * stride + c : kDmaOutOfRange;
+        }
+    }
+    __device__ __forceinline__ void issue(const char *base, int left, char *lds) const {
+        const int n = left < ROWS ? left : ROWS;
+        const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(base, n > 0 ? (uint32_t)(n - 1) * stride + row : 0u);
+#pragma unroll
+        for (int j = 0; j < kIssue; ++j)
+            dma16(rsrc, reinterpret_cast<bf16 *>(lds + (j * THREADS + wave * kWave) * 16), off[j]);
+    }
+};
+
+// Fragment of 16 rows from `r0` (a multiple of 16), elements 32 kk ..+31 of
+// each: lane l holds row l & 15, elements 8 (l >> 4) ..+7.
+template <class E, int DIM>
+__device__ __forceinline__ typename E::Frag row_frag(const char *lds, int r0, int kk, int lane) {
+    using T = AttnTile<E, DIM>;
+    const int r = lane & 15, g = lane >> 4, f = T::swizzle(r);
+    const char *p = lds + (r0 + r) * T::kRow;
+    if constexpr (E::kSize == 2) {
+        return *reinterpret_cast<const bf16x8 *>(p + 16 * ((4 * kk + g) ^ f));
+    } else {
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(p + 16 * ((8 * kk + 2 * g) ^ f));
+        const f32x4 b = *reinterpret_cast<const f32x4 *>(p + 16 * ((8 * kk + 2 * g + 1) ^ f));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// Fragment of the transposed tile: rows are elements 16 db ..+15, the k axis
+// the 32 tile rows from `r0`.  Lane l holds element 16 db + (l & 15); its slot
+// e (of 8) is tile row r0 + 16 (e >> 2) + 4 (l >> 4) + (e & 3): the order in
+// which two 16-row product blocks leave their rows in a lane's accumulators,
+// so a product can be the other operand without leaving its registers.
+template <class E, int DIM>
+__device__ __forceinline__ typename E::Frag col_frag(const char *lds, int r0, int db, int lane) {
+    using T = AttnTile<E, DIM>;
+    const int c16 = lane & 15, g = lane >> 4;
+    if constexpr (E::kSize == 2) {
+        // ds_read_b64_tr_b16: of 16 lanes, lane i gets column i of the 4 x 16
+        // words whose row e the lanes 4 e .. 4 e + 3 address, 8 bytes each.
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 *Ptr;
+        const int r = 4 * g + (c16 >> 2);
+        const char *p = lds + (r0 + r) * T::kRow + 16 * ((2 * db + ((c16 & 3) >> 1)) ^ T::swizzle(r)) + 8 * (c16 & 1);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(p));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(p + 16 * T::kRow));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        f32x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int r = 4 * g + (e & 3);
+            v[e] = *reinterpret_cast<const float *>(lds + (r0 + 16 * (e >> 2) + r) * T::kRow +
+                                                    16 * ((4 * db + (c16 >> 2)) ^ T::swizzle(r)) + 4 * (c16 & 3));
+        }
+        return v;
+    }
+}
+
+// Fragment of 16 rows in global memory (row 0 at `base`): elements 32 kk ..+31.
+// Rows past `rows` and elements past dim are zero.
+template <class E>
+__device__ __forceinline__ typename E::Frag global_frag(const char *base, long long token_bytes, int rows, int dim,
+                                                        int kk, int lane) {
+    const int r = lane & 15, d = 32 * kk + 8 * (lane >> 4);
+    typename E::Frag f = {};
+    if (r < rows && d < dim)
+        f = *reinterpret_cast<const typename E::Frag *>(base + r * token_bytes + d * E::kSize);
+    return f;
+}
+
+// Eight fp32 values as operand words, rounded to nearest even.
+template <class E>
+__device__ __forceinline__ typename E::Frag to_frag(const f32x4 &a, const f32x4 &b) {
+    const f32x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    if constexpr (E::kSize == 4) {
+        return v;
+    } else {
+        Words<E, 8> w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w.w[e] = (typename E::Word)v[e];
+        return __builtin_bit_cast(bf16x8, w);
+    }
+}
+
+// Stores an accumulated transposed product of DB x 16 elements by 16 rows: lane
+// l holds row l & 15 (at `row`, if `live`), elements 16 db + 4 (l >> 4) ..+3.
+template <class E, int DB>
+__device__ __forceinline__ void store_rows(const f32x4 (&o)[DB], float scale, char *row, bool live, int dim, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+        const int d = 16 * db + 4 * g;
+        if (!live || d >= dim) continue;
+        Words<E, 4> w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.put(e, o[db][e] * scale);
+        __builtin_memcpy(__builtin_assume_aligned(row + d * E::kSize, 4 * E::kSize), &w, sizeof w);
+    }
+}
+
+// 2^v where v may be -inf (0).
+__device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// ------------------------------------------------------------------ the host
+inline bool bad_rows(const bfhip_rows *r, long long tokens, int dim, int size) {
+    if (!r || (!r->data && tokens)) return true;
+    const long long step = 16 / size;
+    return ((uintptr_t)r->data & 15) || r->head_stride % step || r->token_stride % step || r->head_stride < 0 ||
+           (tokens > 1 && (r->token_stride < dim || r->token_stride >= 4 << 20)) || r->token_stride < 0;
+}
+
+inline AttnRows attn_rows(const bfhip_rows *r, long long tokens, int dim, int size) {
+    const long long t = tokens > 1 ? r->token_stride : dim;
+    return AttnRows{(char *)r->data, t * size, r->head_stride * size};
+}
+
+inline bool bad_attention(const bfhip_attention_desc *d) {
+    return !d || d->type < BFHIP_F32 || d->type > BFHIP_BF16 || d->sequences < 0 || d->heads <= 0 || d->kv_heads <= 0 ||
+           d->heads % d->kv_heads || d->head_dim <= 0 || d->head_dim > 128 || d->head_dim % 8 || d->heads > 65535 ||
+           (d->causal != 0 && d->causal != 1) || d->q_tokens < 0 || d->k_tokens < 0 || d->q_tokens > 0x7fffffff ||
+           d->k_tokens > 0x7fffffff || !(d->scale == d->scale) || __builtin_isinf(d->scale) ||
+           (d->sequences && (!d->q_starts || !d->k_starts)) || (d->bias && (d->reach < 0 || d->reach > 2047));
+}
+
+inline AttnArgs attn_args(const bfhip_attention_desc *d, const bfhip_rows *q, const bfhip_rows *k, const bfhip_rows *v,
+                          const bfhip_rows *out, float *lse) {
+    const int size = d->type == BFHIP_F32 ? 4 : 2;
+    AttnArgs a{};
+    a.q = attn_rows(q, d->q_tokens, d->head_dim, size);
+    a.k = attn_rows(k, d->k_tokens, d->head_dim, size);
+    a.v = attn_rows(v, d->k_tokens, d->head_dim, size);
+    a.out = attn_rows(out, d->q_tokens, d->head_dim, size);
+    a.q_starts = d->q_starts;
+    a.k_starts = d->k_starts;
+    a.bias = d->bias;
+    a.lse = lse;
+    a.q_tokens = d->q_tokens;
+    a.k_tokens = d->k_tokens;
+    a.sequences = d->sequences;
+    a.heads = d->heads;
+    a.kv_heads = d->kv_heads;
+    a.dim = d->head_dim;
+    a.causal = d->causal;
+    a.reach = d->bias ? d->reach : 0;
+    a.scale = d->scale;
+    a.scale2 = d->scale * kLog2E;
+    return a;
+}
+
+// Calls f with the padded head size.
+template <class F>
+inline void with_dim(int dim, F f) {
+    if (dim <= 32) f(std::integral_constant<int, 32>{});
+    else if (dim <= 64) f(std::integral_constant<int, 64>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
+}  // namespace bfhip
