@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 import pathlib
 
 PKG = pathlib.Path(__file__).resolve().parent.parent
@@ -415,24 +416,26 @@ def conv2d_raw(desc, x, w, b, out, stream=None):
 # backward pass (include/bfhip_transformer.h).  The calls run on the device of
 # their tensors, whichever device is current, on that device's current stream
 # or on `stream`; results and scratch memory are allocated for that stream.
-def _type_code(t):
+@functools.cache
+def _types():
     torch = _torch()
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _type_code(t):
+    code = _types().get(t.dtype)
     if code is None:
         raise BfHipError(f"expected a float32, float16 or bfloat16 tensor, not {t.dtype}")
     return code
 
 
 def _expect(what, t, like, shape, dtype):
-    """`t` is a contiguous device tensor of `shape` on the device of `like`."""
-    if (t.device != like.device or not t.is_cuda or t.dtype != dtype or tuple(t.shape) != shape
+    """Address of `t`, a contiguous tensor of `shape` on the device of `like`."""
+    if (t.dtype != dtype or t.shape != shape or t.device != like.device
             or not t.is_contiguous()):
         raise BfHipError(f"{what} must be a contiguous {dtype} {list(shape)} tensor on "
                          f"{like.device}")
-    return _vp(t.data_ptr())
-
-
-_HERE = contextlib.nullcontext()
+    return t.data_ptr()
 
 
 @contextlib.contextmanager
@@ -440,45 +443,66 @@ def _elsewhere(device, stream, tensors):
     torch = _torch()
     with torch.cuda.device(device):
         if stream is None:
-            yield
+            yield torch.cuda.current_stream().cuda_stream
             return
         if stream.device != device:
             raise BfHipError(f"stream of {stream.device}, tensors on {device}")
         with torch.cuda.stream(stream):
-            yield
+            yield stream.cuda_stream
         for t in tensors:  # keeps their memory until the stream is done with it
             if t is not None:
                 t.record_stream(stream)
 
 
+class _Here:
+    """Context of a call on the current device and its current stream."""
+
+    def __init__(self, stream):
+        self.stream = stream
+
+    def __enter__(self):
+        return self.stream
+
+    def __exit__(self, *exc):
+        return False
+
+
+@functools.cache
+def _current():
+    """Functions that give the current device's number and, of a device, the
+    current stream's handle (the handle alone: a Stream object costs 2.6 us)."""
+    torch = _torch()
+    return torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+
+
 def _place(stream, *tensors):
     """Context in which a call on `tensors` (the first one names the device)
-    allocates and launches."""
-    torch = _torch()
-    device = tensors[0].device
+    allocates and launches; gives the stream's handle."""
     if not tensors[0].is_cuda:
         raise BfHipError("expected a device tensor")
-    if stream is None and device.index == torch.cuda.current_device():
-        return _HERE
+    device, (current, handle) = tensors[0].device, _current()
+    if stream is None and device.index == current():
+        return _Here(handle(device.index))
     return _elsewhere(device, stream, tensors)
 
 
-def _scratch(size, device):
+def _scratch(size, like):
+    """(tensor that holds the memory, its address)"""
     if not size:
         return None, None
-    torch = _torch()
-    t = torch.empty(size, dtype=torch.uint8, device=device)
-    return t, _vp(t.data_ptr())
+    t = like.new_empty(size, dtype=_torch().uint8)
+    return t, t.data_ptr()
 
 
-def _matrix(what, t, like=None):
+def _matrix(what, t, like):
     """[rows, features] with contiguous rows -> (pointer, row stride)."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    stride = t.stride()
+    if len(stride) != 2 or (stride[1] != 1 and t.shape[1] > 1):
         raise BfHipError(f"{what} must be [rows, features] with contiguous rows")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype
-                             or t.device != like.device):
+    if t is not like and (t.shape != like.shape or t.dtype != like.dtype
+                          or t.device != like.device):
         raise BfHipError(f"{what} must match {list(like.shape)} {like.dtype} on {like.device}")
-    return _vp(t.data_ptr()), t.stride(0)
+    return t.data_ptr(), stride[0]
 
 
 def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream=None):
@@ -487,20 +511,20 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5, out=None, stats=False, stream
     which layer_norm_backward takes."""
     torch = _torch()
     code = _type_code(x)
-    px, sx = _matrix("x", x)
+    px, sx = _matrix("x", x, x)
     rows, n = x.shape
-    pg, pb = (None if t is None else _expect(name, t, x, (n,), torch.float32)
-              for name, t in (("gamma", gamma), ("beta", beta)))
-    with _place(stream, x, gamma, beta, out):
-        y = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else out
+    pg = None if gamma is None else _expect("gamma", gamma, x, (n,), torch.float32)
+    pb = None if beta is None else _expect("beta", beta, x, (n,), torch.float32)
+    with _place(stream, x, gamma, beta, out) as queue:
+        y = x.new_empty((rows, n)) if out is None else out
         py, sy = _matrix("out", y, x)
         pm = pr = None
         if stats:
-            mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-            pm, pr = _vp(mean.data_ptr()), _vp(rstd.data_ptr())
+            mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+            pm, pr = mean.data_ptr(), rstd.data_ptr()
         err = _err()
         _check(hip_lib().bfhip_layer_norm_forward(code, px, sx, pg, pb, py, sy, pm, pr, rows, n,
-                                                  eps, _stream(), err, 512),
+                                                  eps, queue, err, 512),
                err, "bfhip_layer_norm_forward")
     return (y, mean, rstd) if stats else y
 
@@ -509,24 +533,23 @@ def layer_norm_backward(dy, x, mean, rstd, gamma=None, out=None, stream=None):
     """Gradients of layer_norm (bfhip_layer_norm_backward): (dx, dgamma, dbeta)."""
     torch = _torch()
     code = _type_code(x)
-    px, sx = _matrix("x", x)
+    px, sx = _matrix("x", x, x)
     pdy, sdy = _matrix("dy", dy, x)
     rows, n = x.shape
-    pm, pr = (_expect(name, t, x, (rows,), torch.float32)
-              for name, t in (("mean", mean), ("rstd", rstd)))
+    pm = _expect("mean", mean, x, (rows,), torch.float32)
+    pr = _expect("rstd", rstd, x, (rows,), torch.float32)
     pg = None if gamma is None else _expect("gamma", gamma, x, (n,), torch.float32)
     lib = hip_lib()
-    with _place(stream, x, dy, mean, rstd, gamma, out):
-        dx = torch.empty((rows, n), dtype=x.dtype, device=x.device) if out is None else out
+    with _place(stream, x, dy, mean, rstd, gamma, out) as queue:
+        dx = x.new_empty((rows, n)) if out is None else out
         pdx, sdx = _matrix("out", dx, x)
-        dgamma = torch.empty(n, dtype=torch.float32, device=x.device)
-        dbeta = torch.empty(n, dtype=torch.float32, device=x.device)
+        dgamma, dbeta = x.new_empty(n, dtype=torch.float32), x.new_empty(n, dtype=torch.float32)
         size = lib.bfhip_layer_norm_backward_workspace(rows, n)
-        work, pw = _scratch(size, x.device)
+        work, pw = _scratch(size, x)
         err = _err()
         _check(lib.bfhip_layer_norm_backward(
-            code, pdy, sdy, px, sx, pg, pm, pr, pdx, sdx, _vp(dgamma.data_ptr()),
-            _vp(dbeta.data_ptr()), rows, n, pw, size, _stream(), err, 512),
+            code, pdy, sdy, px, sx, pg, pm, pr, pdx, sdx, dgamma.data_ptr(),
+            dbeta.data_ptr(), rows, n, pw, size, queue, err, 512),
             err, "bfhip_layer_norm_backward")
     return dx, dgamma, dbeta
 
@@ -541,12 +564,12 @@ def position_bias(table, buckets, out=None, stream=None):
     pt = _expect("table", table, table, (count, heads), torch.float32)
     pm = _expect("buckets", buckets, table, tuple(buckets.shape), torch.int32)
     shape = (heads, *buckets.shape)
-    with _place(stream, table, buckets, out):
-        bias = torch.empty(shape, dtype=torch.float32, device=table.device) if out is None else out
+    with _place(stream, table, buckets, out) as queue:
+        bias = table.new_empty(shape) if out is None else out
         pb = _expect("out", bias, table, shape, torch.float32)
         err = _err()
         _check(hip_lib().bfhip_position_bias_forward(pt, pm, pb, count, heads, buckets.numel(),
-                                                     _stream(), err, 512),
+                                                     queue, err, 512),
                err, "bfhip_position_bias_forward")
     return bias
 
@@ -559,26 +582,27 @@ def position_bias_backward(dbias, buckets, count, stream=None):
     pd = _expect("dbias", dbias, dbias, (heads, *buckets.shape), torch.float32)
     pm = _expect("buckets", buckets, dbias, tuple(buckets.shape), torch.int32)
     lib, n = hip_lib(), buckets.numel()
-    with _place(stream, dbias, buckets):
-        dtable = torch.empty((count, heads), dtype=torch.float32, device=dbias.device)
+    with _place(stream, dbias, buckets) as queue:
+        dtable = dbias.new_empty((count, heads))
         size = lib.bfhip_position_bias_backward_workspace(count, heads, n)
-        work, pw = _scratch(size, dbias.device)
+        work, pw = _scratch(size, dbias)
         err = _err()
-        _check(lib.bfhip_position_bias_backward(pd, pm, _vp(dtable.data_ptr()), count, heads, n,
-                                                pw, size, _stream(), err, 512),
+        _check(lib.bfhip_position_bias_backward(pd, pm, dtable.data_ptr(), count, heads, n,
+                                                pw, size, queue, err, 512),
                err, "bfhip_position_bias_backward")
     return dtable
 
 
-def _head_rows(what, t, like, heads=None):
+def _head_rows(what, t, like):
     """[tokens, heads, head_dim] with contiguous heads -> Rows."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1):
         raise BfHipError(f"{what} must be [tokens, heads, head_dim] with contiguous heads")
-    if (t.dtype != like.dtype or t.device != like.device or t.shape[2] != like.shape[2]
-            or (heads is not None and t.shape[1] != heads)):
-        raise BfHipError(f"{what} must match {like.dtype}, head_dim {like.shape[2]} and its "
-                         f"heads on {like.device}")
-    return Rows(t.data_ptr(), t.stride(0), t.stride(1) if t.shape[1] > 1 else 0)
+    if t is not like and (t.dtype != like.dtype or t.device != like.device
+                          or shape[2] != like.shape[2]):
+        raise BfHipError(f"{what} must be {like.dtype} of head_dim {like.shape[2]} on "
+                         f"{like.device}")
+    return Rows(t.data_ptr(), stride[0], stride[1] if shape[1] > 1 else 0)
 
 
 def _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias):
@@ -590,8 +614,8 @@ def _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias):
     n = q_starts.numel() - 1
     if n < 0:
         raise BfHipError("starts must hold one entry more than there are sequences")
-    ps = [_expect(name, t, q, (n + 1,), torch.int32)
-          for name, t in (("q_starts", q_starts), ("k_starts", k_starts))]
+    ps = [_expect("q_starts", q_starts, q, (n + 1,), torch.int32),
+          _expect("k_starts", k_starts, q, (n + 1,), torch.int32)]
     heads, reach, pb = q.shape[1], 0, None
     if bias is not None:
         if bias.dim() != 2 or bias.shape[1] % 2 == 0:
@@ -615,19 +639,19 @@ def attention(q, k, v, q_starts, k_starts, causal=False, scale=None, bias=None, 
     torch = _torch()
     desc, rows = _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias)
     lib = hip_lib()
-    with _place(stream, q, k, v, q_starts, k_starts, bias, out):
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        if o.shape[0] != q.shape[0]:
+    with _place(stream, q, k, v, q_starts, k_starts, bias, out) as queue:
+        o = q.new_empty(q.shape) if out is None else out
+        if o.shape != q.shape:
             raise BfHipError("out must have the shape of q")
-        ro = _head_rows("out", o, q, q.shape[1])
+        ro = _head_rows("out", o, q)
         stat, ps = None, None
         if lse:
-            stat = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-            ps = _vp(stat.data_ptr())
+            stat = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+            ps = stat.data_ptr()
         size = lib.bfhip_attention_forward_workspace(desc)
-        work, pw = _scratch(size, q.device)
+        work, pw = _scratch(size, q)
         err = _err()
-        _check(lib.bfhip_attention_forward(desc, *rows, ro, ps, pw, size, _stream(), err, 512),
+        _check(lib.bfhip_attention_forward(desc, *rows, ro, ps, pw, size, queue, err, 512),
                err, "bfhip_attention_forward")
     return (o, stat) if lse else o
 
@@ -644,18 +668,18 @@ def attention_backward(dout, q, k, v, out, lse, q_starts, k_starts, causal=False
     ro, rg = _head_rows("out", out, q), _head_rows("dout", dout, q)
     pl = _expect("lse", lse, q, (q.shape[1], q.shape[0]), torch.float32)
     lib = hip_lib()
-    with _place(stream, q, k, v, q_starts, k_starts, bias, out, lse, dout):
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+    with _place(stream, q, k, v, q_starts, k_starts, bias, out, lse, dout) as queue:
+        grads = [t.new_empty(t.shape) for t in (q, k, v)]
         pb = None
         if bias is not None:
             grads.append(torch.empty_like(bias))
-            pb = _vp(grads[3].data_ptr())
+            pb = grads[3].data_ptr()
         size = lib.bfhip_attention_backward_workspace(desc)
-        work, pw = _scratch(size, q.device)
+        work, pw = _scratch(size, q)
         err = _err()
         _check(lib.bfhip_attention_backward(
             desc, *rows, ro, pl, rg, *(_head_rows("gradient", t, q) for t in grads[:3]), pb, pw,
-            size, _stream(), err, 512), err, "bfhip_attention_backward")
+            size, queue, err, 512), err, "bfhip_attention_backward")
     return tuple(grads)
 
 

@@ -49,13 +49,14 @@ struct ElemBf16 {
 // unaligned vector accesses).
 template <class E, int N>
 struct Words {
-    typename E::Word w[N];
-    __device__ __forceinline__ static Words load(const typename E::Word *p) {
+    using Word = typename E::Word;
+    Word w[N];
+    __device__ __forceinline__ static Words load(const Word *p) {
         Words v;
         __builtin_memcpy(v.w, p, sizeof v.w);
         return v;
     }
-    __device__ __forceinline__ void store(typename E::Word *p) const { __builtin_memcpy(p, w, sizeof w); }
+    __device__ __forceinline__ void store(Word *p) const { __builtin_memcpy(p, w, sizeof w); }
     __device__ __forceinline__ float get(int i) const { return E::get(w[i]); }
     __device__ __forceinline__ void put(int i, float v) { w[i] = E::put(v); }
 };

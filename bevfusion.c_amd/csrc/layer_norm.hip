@@ -3,109 +3,330 @@
 #include "element.h"
 #include "gemm_core.h"
 
+#include <type_traits>
+
 using namespace bfhip;
 
 namespace {
 
-constexpr int kRowWaves = 4;  // rows of a workgroup, one wave each
-
-// One wave per row: the mean, then the centred squares (not E[x^2] - E[x]^2,
-// which loses a spread that is small beside the mean), then the result.
-template <class E>
-__global__ __launch_bounds__(kRowWaves *kWave) void norm_forward_kernel(
-    const typename E::Word *x, long long xs, const float *gamma, const float *beta,
-    typename E::Word *y, long long ys, float *mean, float *rstd, long long rows, int n, float eps) {
-    const int lane = threadIdx.x % kWave;
-    const long long r = (long long)blockIdx.x * kRowWaves + threadIdx.x / kWave;
-    if (r >= rows) return;
-    x += r * xs;
-    y += r * ys;
-    float sum = 0.f, dev = 0.f;
-    for (int c = lane; c < n; c += kWave) sum += E::get(x[c]);
-    const float m = group_sum<kWave>(sum) / (float)n;
-    for (int c = lane; c < n; c += kWave) {
-        const float d = E::get(x[c]) - m;
-        dev = fmaf(d, d, dev);
-    }
-    const float s = 1.f / sqrtf(group_sum<kWave>(dev) / (float)n + eps);
-    for (int c = lane; c < n; c += kWave) {
-        float v = (E::get(x[c]) - m) * s;
-        if (gamma) v *= gamma[c];
-        if (beta) v += beta[c];
-        y[c] = E::put(v);
-    }
-    if (mean && lane == 0) {
-        mean[r] = m;
-        rstd[r] = s;
-    }
-}
-
-template <class E>
-__global__ __launch_bounds__(kRowWaves *kWave) void norm_backward_kernel(
-    const typename E::Word *dy, long long dys, const typename E::Word *x, long long xs,
-    const float *gamma, const float *mean, const float *rstd, typename E::Word *dx, long long dxs,
-    long long rows, int n) {
-    const int lane = threadIdx.x % kWave;
-    const long long r = (long long)blockIdx.x * kRowWaves + threadIdx.x / kWave;
-    if (r >= rows) return;
-    dy += r * dys;
-    x += r * xs;
-    dx += r * dxs;
-    const float m = mean[r], s = rstd[r];
-    float sg = 0.f, sgh = 0.f;
-    for (int c = lane; c < n; c += kWave) {
-        const float g = E::get(dy[c]) * (gamma ? gamma[c] : 1.f);
-        sg += g;
-        sgh = fmaf(g, (E::get(x[c]) - m) * s, sgh);
-    }
-    sg = group_sum<kWave>(sg) / (float)n;
-    sgh = group_sum<kWave>(sgh) / (float)n;
-    for (int c = lane; c < n; c += kWave) {
-        const float g = E::get(dy[c]) * (gamma ? gamma[c] : 1.f), h = (E::get(x[c]) - m) * s;
-        dx[c] = E::put(s * (g - sg - h * sgh));
-    }
-}
-
-// Sums over rows of dy * h and dy: workgroup (column block, part) sums every
-// parts-th group of 4 rows; partial [parts][2][n].
-template <class E>
-__global__ __launch_bounds__(256) void norm_weight_kernel(
-    const typename E::Word *dy, long long dys, const typename E::Word *x, long long xs,
-    const float *mean, const float *rstd, float *partial, long long rows, int n) {
-    __shared__ float sum[2][4][64];
-    const int c = blockIdx.x * 64 + threadIdx.x % 64, w = threadIdx.x / 64;
-    float a = 0.f, b = 0.f;
-    if (c < n)
-        for (long long r = 4ll * blockIdx.y + w; r < rows; r += 4ll * gridDim.y) {
-            const float g = E::get(dy[r * dys + c]);
-            a = fmaf(g, (E::get(x[r * xs + c]) - mean[r]) * rstd[r], a);
-            b += g;
-        }
-    sum[0][w][threadIdx.x % 64] = a;
-    sum[1][w][threadIdx.x % 64] = b;
-    __syncthreads();
-    if (w > 1 || c >= n) return;
-    const float(*q)[64] = sum[w];
-    const int t = threadIdx.x % 64;
-    partial[(size_t)(2 * blockIdx.y + w) * n + c] = (q[0][t] + q[1][t]) + (q[2][t] + q[3][t]);
-}
-
-__global__ __launch_bounds__(256) void norm_weight_sum_kernel(const float *partial, int parts,
-                                                              float *dgamma, float *dbeta, int n) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
-    float a = 0.f, b = 0.f;
-    for (int p = 0; p < parts; ++p) {
-        a += partial[(size_t)(2 * p) * n + c];
-        b += partial[(size_t)(2 * p + 1) * n + c];
-    }
-    dgamma[c] = a;
-    dbeta[c] = b;
-}
-
+constexpr int kThreads = 256;
 constexpr int kMaxFeatures = 65536;
 
-int norm_parts(long long rows) { return (int)(rows <= 0 ? 0 : rows >= 256 ? 64 : (rows + 3) / 4); }
+// What bounds these kernels is memory: a row is read once, held in registers
+// (as words, converted where they are used) by a group of LANES threads, CHUNKS
+// 16-byte chunks each, and written once.  Chunks of a group's lanes are
+// neighbours in memory; a group walks rows with the norm's weights and, in the
+// backward pass, its columns' gradient sums in registers.
+template <class E, int LANES, int CHUNKS>
+struct NormRow {
+    static constexpr int kWords = 16 / E::kSize, kGroups = kThreads / LANES;
+    using Chunk = Words<E, kWords>;
+    using Floats = Words<ElemF32, kWords>;
+    // Threads of one group; LANES > 64: the workgroup's waves together.
+    __device__ static int lane() { return threadIdx.x % LANES; }
+    __device__ static int group() { return threadIdx.x / LANES; }
+    __device__ static int column(int k) { return (k * LANES + lane()) * kWords; }
+
+    // Elements past the row's end read as zero.
+    template <class W>
+    __device__ __forceinline__ static void load(const typename W::Word *row, int n, W (&v)[CHUNKS]) {
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int c = column(k);
+            if (c + kWords <= n) {
+                v[k] = W::load(row + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kWords; ++e) v[k].w[e] = c + e < n ? row[c + e] : (typename W::Word)0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ static void store(typename E::Word *row, int n, const Chunk (&v)[CHUNKS]) {
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int c = column(k);
+            if (c + kWords <= n) {
+                v[k].store(row + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kWords; ++e)
+                    if (c + e < n) row[c + e] = v[k].w[e];
+            }
+        }
+    }
+    // The group's sums of two values, in a fixed order.
+    __device__ __forceinline__ static float2 sum(float a, float b) {
+        constexpr int wave = LANES < kWave ? LANES : kWave;
+        a = group_sum<wave>(a);
+        b = group_sum<wave>(b);
+        if constexpr (LANES > kWave) {
+            __shared__ float2 part[2][LANES / kWave];
+            const int w = threadIdx.x / kWave;
+            __syncthreads();  // the sums before have been read
+            if (threadIdx.x % kWave == 0) part[0][w] = make_float2(a, b);
+            __syncthreads();
+            a = b = 0.f;
+#pragma unroll
+            for (int i = 0; i < LANES / kWave; ++i) {
+                a += part[0][i].x;
+                b += part[0][i].y;
+            }
+        }
+        return make_float2(a, b);
+    }
+};
+
+struct NormArgs {
+    const void *x, *dy;
+    void *y;  // y or dx
+    long long xs, dys, ys, rows;
+    const float *gamma, *beta;
+    float *mean, *rstd;
+    float *partial;  // [workgroups][2][n]
+    int n;
+    float eps;
+};
+
+// The mean, then the centred squares (not E[x^2] - E[x]^2, which loses a
+// spread that is small beside the mean), then the result.
+template <class E, int LANES, int CHUNKS>
+__global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
+    using R = NormRow<E, LANES, CHUNKS>;
+    using W = typename E::Word;
+    typename R::Floats gamma[CHUNKS], beta[CHUNKS];
+    if (a.gamma) R::load(a.gamma, a.n, gamma);
+    if (a.beta) R::load(a.beta, a.n, beta);
+    const float n = (float)a.n;
+    for (long long r = (long long)blockIdx.x * R::kGroups + R::group(); r < a.rows; r += (long long)gridDim.x * R::kGroups) {
+        typename R::Chunk x[CHUNKS];
+        R::load((const W *)a.x + r * a.xs, a.n, x);
+        float s = 0.f, d = 0.f;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int e = 0; e < R::kWords; ++e) s += x[k].get(e);
+        const float m = R::sum(s, 0.f).x / n;  // (a row of equal values has exactly their mean)
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int e = 0; e < R::kWords; ++e) {
+                const float v = R::column(k) + e < a.n ? x[k].get(e) - m : 0.f;
+                d = fmaf(v, v, d);
+            }
+        const float rs = 1.f / sqrtf(R::sum(d, 0.f).x / n + a.eps);
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int e = 0; e < R::kWords; ++e) {
+                float v = (x[k].get(e) - m) * rs;
+                if (a.gamma) v *= gamma[k].w[e];
+                if (a.beta) v += beta[k].w[e];
+                x[k].put(e, v);
+            }
+        R::store((W *)a.y + r * a.ys, a.n, x);
+        if (a.mean && R::lane() == 0) {
+            a.mean[r] = m;
+            a.rstd[r] = rs;
+        }
+    }
+}
+
+// dx row by row, and the workgroup's share of dgamma and dbeta: each thread
+// keeps its columns' sums over its group's rows, then the groups' are added in
+// order through LDS.
+template <class E, int LANES, int CHUNKS>
+__global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
+    using R = NormRow<E, LANES, CHUNKS>;
+    using W = typename E::Word;
+    __shared__ float sums[2][LANES * CHUNKS * R::kWords];
+    typename R::Floats gamma[CHUNKS], dg[CHUNKS], db[CHUNKS];
+    if (a.gamma) R::load(a.gamma, a.n, gamma);
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+        for (int e = 0; e < R::kWords; ++e) {
+            if (!a.gamma) gamma[k].w[e] = 1.f;
+            dg[k].w[e] = db[k].w[e] = 0.f;
+        }
+    const float per = 1.f / (float)a.n;
+    for (long long r = (long long)blockIdx.x * R::kGroups + R::group(); r < a.rows; r += (long long)gridDim.x * R::kGroups) {
+        typename R::Chunk x[CHUNKS], dy[CHUNKS];
+        R::load((const W *)a.x + r * a.xs, a.n, x);
+        R::load((const W *)a.dy + r * a.dys, a.n, dy);
+        const float m = a.mean[r], rs = a.rstd[r];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int e = 0; e < R::kWords; ++e) {
+                // Past the row's end dy is zero, and so is all it is part of.
+                const float d = dy[k].get(e), h = (x[k].get(e) - m) * rs, g = d * gamma[k].w[e];
+                dg[k].w[e] = fmaf(d, h, dg[k].w[e]);
+                db[k].w[e] += d;
+                s1 += g;
+                s2 = fmaf(g, h, s2);
+            }
+        const float2 s = R::sum(s1, s2);
+        s1 = s.x * per;
+        s2 = s.y * per;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+            for (int e = 0; e < R::kWords; ++e)
+                x[k].put(e, rs * (dy[k].get(e) * gamma[k].w[e] - s1 - (x[k].get(e) - m) * rs * s2));
+        R::store((W *)a.y + r * a.ys, a.n, x);
+    }
+    if (!a.partial) return;
+    for (int q = 0; q < R::kGroups; ++q) {
+        if (R::group() == q)
+#pragma unroll
+            for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                for (int e = 0; e < R::kWords; ++e) {
+                    const int c = R::column(k) + e;
+                    sums[0][c] = q ? sums[0][c] + dg[k].w[e] : dg[k].w[e];
+                    sums[1][c] = q ? sums[1][c] + db[k].w[e] : db[k].w[e];
+                }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * a.n; c += kThreads)
+        a.partial[(size_t)blockIdx.x * 2 * a.n + c] = c < a.n ? sums[0][c] : sums[1][c - a.n];
+}
+
+// Rows too long for a workgroup's registers: the row is read again for each
+// step.  dx may overwrite x or dy, so the weights' sums have a kernel of their
+// own, which runs first.
+template <class E>
+__global__ __launch_bounds__(kThreads) void norm_forward_long_kernel(NormArgs a) {
+    using W = typename E::Word;
+    using R = NormRow<E, kThreads, 1>;
+    const long long r = blockIdx.x;
+    const W *x = (const W *)a.x + r * a.xs;
+    W *y = (W *)a.y + r * a.ys;
+    float s = 0.f, d = 0.f;
+    for (int c = threadIdx.x; c < a.n; c += kThreads) s += E::get(x[c]);
+    const float m = R::sum(s, 0.f).x / (float)a.n;
+    for (int c = threadIdx.x; c < a.n; c += kThreads) {
+        const float v = E::get(x[c]) - m;
+        d = fmaf(v, v, d);
+    }
+    const float rs = 1.f / sqrtf(R::sum(d, 0.f).x / (float)a.n + a.eps);
+    for (int c = threadIdx.x; c < a.n; c += kThreads) {
+        float v = (E::get(x[c]) - m) * rs;
+        if (a.gamma) v *= a.gamma[c];
+        if (a.beta) v += a.beta[c];
+        y[c] = E::put(v);
+    }
+    if (a.mean && threadIdx.x == 0) {
+        a.mean[r] = m;
+        a.rstd[r] = rs;
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(kThreads) void norm_backward_long_kernel(NormArgs a) {
+    using W = typename E::Word;
+    using R = NormRow<E, kThreads, 1>;
+    const long long r = blockIdx.x;
+    const W *x = (const W *)a.x + r * a.xs, *dy = (const W *)a.dy + r * a.dys;
+    W *dx = (W *)a.y + r * a.ys;
+    const float m = a.mean[r], rs = a.rstd[r];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < a.n; c += kThreads) {
+        const float g = E::get(dy[c]) * (a.gamma ? a.gamma[c] : 1.f);
+        s1 += g;
+        s2 = fmaf(g, (E::get(x[c]) - m) * rs, s2);
+    }
+    const float2 s = R::sum(s1, s2);
+    s1 = s.x / (float)a.n;
+    s2 = s.y / (float)a.n;
+    for (int c = threadIdx.x; c < a.n; c += kThreads) {
+        const float g = E::get(dy[c]) * (a.gamma ? a.gamma[c] : 1.f), h = (E::get(x[c]) - m) * rs;
+        dx[c] = E::put(rs * (g - s1 - h * s2));
+    }
+}
+
+// Sums over every parts-th group of 4 rows; workgroup (column block, part).
+template <class E>
+__global__ __launch_bounds__(kThreads) void norm_weight_long_kernel(NormArgs a) {
+    using W = typename E::Word;
+    __shared__ float sum[2][4][64];
+    const int t = threadIdx.x % 64, c = blockIdx.x * 64 + t, w = threadIdx.x / 64;
+    float dg = 0.f, db = 0.f;
+    if (c < a.n)
+        for (long long r = 4ll * blockIdx.y + w; r < a.rows; r += 4ll * gridDim.y) {
+            const float g = E::get(((const W *)a.dy)[r * a.dys + c]);
+            dg = fmaf(g, (E::get(((const W *)a.x)[r * a.xs + c]) - a.mean[r]) * a.rstd[r], dg);
+            db += g;
+        }
+    sum[0][w][t] = dg;
+    sum[1][w][t] = db;
+    __syncthreads();
+    if (w > 1 || c >= a.n) return;
+    const float(*q)[64] = sum[w];
+    a.partial[(size_t)(2 * blockIdx.y + w) * a.n + c] = (q[0][t] + q[1][t]) + (q[2][t] + q[3][t]);
+}
+
+// dgamma, dbeta: the partial sums of 16 columns per workgroup, 16 threads each.
+__global__ __launch_bounds__(kThreads) void norm_weight_sum_kernel(const float *partial, int parts, float *dgamma,
+                                                                   float *dbeta, int n) {
+    __shared__ float sum[16][17];
+    const int c = blockIdx.x * 16 + threadIdx.x % 16, w = threadIdx.x / 16;
+    float s = 0.f;
+    if (c < 2 * n)
+        for (int p = w; p < parts; p += 16) s += partial[(size_t)p * 2 * n + c];
+    sum[w][threadIdx.x % 16] = s;
+    __syncthreads();
+    if (w || c >= 2 * n) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sum[i][threadIdx.x];
+    (c < n ? dgamma : dbeta - n)[c] = s;
+}
+
+// Lanes of a row's group: the fewest of 16, 32 and 64 that hold the row in at
+// most 16 elements each, or a workgroup's 256 with up to four chunks (0: none
+// does).  Fewer lanes leave fewer of them without a chunk and need fewer steps
+// to add up; more elements per lane leave too few waves to hide the loads.
+int norm_lanes(int n, int size) {
+    const int words = 16 / size, chunks = (n + words - 1) / words;
+    for (int lanes : {16, 32, 64})
+        if (n <= 16 * lanes) return lanes;
+    return chunks <= 4 * 256 ? 256 : 0;
+}
+
+template <class E, class F>
+void with_row(int n, F f) {
+    const int lanes = norm_lanes(n, E::kSize), words = 16 / E::kSize;
+    const auto with_chunks = [&](auto l) {
+        constexpr int L = decltype(l)::value;
+        const int chunks = (n + L * words - 1) / (L * words);
+        if (chunks <= 1) f(l, std::integral_constant<int, 1>{});
+        else if (chunks == 2) f(l, std::integral_constant<int, 2>{});
+        else if constexpr (L == 256 || E::kSize == 4) {
+            if (chunks == 3) f(l, std::integral_constant<int, 3>{});
+            else f(l, std::integral_constant<int, 4>{});
+        }
+    };
+    if (lanes == 16) with_chunks(std::integral_constant<int, 16>{});
+    else if (lanes == 32) with_chunks(std::integral_constant<int, 32>{});
+    else if (lanes == 64) with_chunks(std::integral_constant<int, 64>{});
+    else with_chunks(std::integral_constant<int, 256>{});
+}
+
+// Workgroups for rows of `groups` groups each: eight per CU, which walk the rest.
+long long norm_grid(long long rows, int groups) {
+    const long long grid = (rows + groups - 1) / groups;
+    return grid < 2048 ? grid : 2048;
+}
+
+// Partial sums of the weights' gradients: one per workgroup of the backward
+// pass, at most two workgroups per CU (more of them wait less for memory, but
+// their sums have to be written and read again).
+long long norm_parts(long long rows, int n, int size) {
+    const int lanes = norm_lanes(n, size);
+    const long long parts = lanes ? (rows + kThreads / lanes - 1) / (kThreads / lanes) : (rows + 3) / 4, most = lanes ? 512 : 64;
+    return parts < most ? parts : most;
+}
 
 bool bad_norm(int type, long long rows, int n) {
     return type < BFHIP_F32 || type > BFHIP_BF16 || rows < 0 || n <= 0 || n > kMaxFeatures;
@@ -113,67 +334,89 @@ bool bad_norm(int type, long long rows, int n) {
 
 }  // namespace
 
-extern "C" int bfhip_layer_norm_forward(int type, const void *x, long long x_stride,
-                                        const float *gamma, const float *beta, void *y,
-                                        long long y_stride, float *mean, float *rstd,
-                                        long long rows, int features, float eps, void *stream,
-                                        char *error, size_t cap) {
+extern "C" int bfhip_layer_norm_forward(int type, const void *x, long long x_stride, const float *gamma, const float *beta,
+                                        void *y, long long y_stride, float *mean, float *rstd, long long rows,
+                                        int features, float eps, void *stream, char *error, size_t cap) {
     if (bad_norm(type, rows, features) || !(eps >= 0.f) || !mean != !rstd)
         return fail(error, cap, "invalid layer norm contract");
     if (rows == 0) return 1;
     if (!x || !y || (rows > 1 && (x_stride < 0 || y_stride < features)))
         return fail(error, cap, "invalid layer norm contract");
-    const long long grid = (rows + kRowWaves - 1) / kRowWaves;
-    if (!launch_fits(grid, kRowWaves * kWave)) return fail(error, cap, "layer norm has too many rows");
+    NormArgs a{};
+    a.x = x; a.xs = x_stride;
+    a.y = y; a.ys = y_stride;
+    a.gamma = gamma; a.beta = beta;
+    a.mean = mean; a.rstd = rstd;
+    a.rows = rows; a.n = features; a.eps = eps;
+    hipStream_t s = (hipStream_t)stream;
+    int ok = 1;
     with_element(type, [&](auto e) {
         using E = decltype(e);
-        using W = typename E::Word;
-        hipLaunchKernelGGL(norm_forward_kernel<E>, dim3((unsigned)grid), dim3(kRowWaves * kWave), 0,
-                           (hipStream_t)stream, (const W *)x, x_stride, gamma, beta, (W *)y,
-                           y_stride, mean, rstd, rows, features, eps);
+        if (!norm_lanes(features, E::kSize)) {
+            ok = launch_fits(rows, kThreads);
+            if (ok) hipLaunchKernelGGL(norm_forward_long_kernel<E>, dim3((unsigned)rows), dim3(kThreads), 0, s, a);
+            return;
+        }
+        with_row<E>(features, [&](auto lanes, auto chunks) {
+            constexpr int L = decltype(lanes)::value, K = decltype(chunks)::value;
+            hipLaunchKernelGGL((norm_forward_kernel<E, L, K>), dim3((unsigned)norm_grid(rows, kThreads / L)), dim3(kThreads),
+                               0, s, a);
+        });
     });
+    if (!ok) return fail(error, cap, "layer norm has too many rows");
     return launch_ok(error, cap, "layer norm launch");
 }
 
 extern "C" size_t bfhip_layer_norm_backward_workspace(long long rows, int features) {
     if (bad_norm(BFHIP_F32, rows, features)) return 0;
-    return (size_t)norm_parts(rows) * 2 * features * sizeof(float);
+    // The type that needs more.
+    const long long a = norm_parts(rows, features, 4), b = norm_parts(rows, features, 2);
+    return (size_t)(a > b ? a : b) * 2 * features * sizeof(float);
 }
 
-extern "C" int bfhip_layer_norm_backward(int type, const void *dy, long long dy_stride,
-                                         const void *x, long long x_stride, const float *gamma,
-                                         const float *mean, const float *rstd, void *dx,
-                                         long long dx_stride, float *dgamma, float *dbeta,
-                                         long long rows, int features, void *workspace,
-                                         size_t workspace_bytes, void *stream, char *error,
-                                         size_t cap) {
+extern "C" int bfhip_layer_norm_backward(int type, const void *dy, long long dy_stride, const void *x, long long x_stride,
+                                         const float *gamma, const float *mean, const float *rstd, void *dx,
+                                         long long dx_stride, float *dgamma, float *dbeta, long long rows, int features,
+                                         void *workspace, size_t workspace_bytes, void *stream, char *error, size_t cap) {
     if (bad_norm(type, rows, features) || !dgamma != !dbeta)
         return fail(error, cap, "invalid layer norm contract");
     if (rows > 0 && (!dy || !x || !mean || !rstd || !dx ||
                      (rows > 1 && (dy_stride < 0 || x_stride < 0 || dx_stride < features))))
         return fail(error, cap, "invalid layer norm contract");
-    const long long grid = (rows + kRowWaves - 1) / kRowWaves;
-    if (!launch_fits(grid, kRowWaves * kWave)) return fail(error, cap, "layer norm has too many rows");
-    const int parts = norm_parts(rows);
-    if (dgamma && parts && (!workspace || ((uintptr_t)workspace & 15) ||
-                            workspace_bytes < bfhip_layer_norm_backward_workspace(rows, features)))
+    if (dgamma && rows && (!workspace || ((uintptr_t)workspace & 15) ||
+                           workspace_bytes < bfhip_layer_norm_backward_workspace(rows, features)))
         return fail(error, cap, "layer norm workspace too small or not 16-byte aligned");
+    NormArgs a{};
+    a.x = x; a.xs = x_stride;
+    a.dy = dy; a.dys = dy_stride;
+    a.y = dx; a.ys = dx_stride;
+    a.gamma = gamma;
+    a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+    a.partial = dgamma ? (float *)workspace : nullptr;
+    a.rows = rows; a.n = features;
     hipStream_t s = (hipStream_t)stream;
-    with_element(type, [&](auto e) {
+    long long parts = 0;
+    int ok = 1;
+    if (rows) with_element(type, [&](auto e) {
         using E = decltype(e);
-        using W = typename E::Word;
-        // The weights' sums first: dx may overwrite dy or x.
-        if (dgamma && parts)
-            hipLaunchKernelGGL(norm_weight_kernel<E>, dim3((features + 63) / 64, parts), dim3(256),
-                               0, s, (const W *)dy, dy_stride, (const W *)x, x_stride, mean, rstd,
-                               (float *)workspace, rows, features);
-        if (grid)
-            hipLaunchKernelGGL(norm_backward_kernel<E>, dim3((unsigned)grid), dim3(kRowWaves * kWave),
-                               0, s, (const W *)dy, dy_stride, (const W *)x, x_stride, gamma, mean,
-                               rstd, (W *)dx, dx_stride, rows, features);
+        parts = norm_parts(rows, features, E::kSize);
+        if (!norm_lanes(features, E::kSize)) {
+            ok = launch_fits(rows, kThreads);
+            if (!ok) return;
+            if (dgamma)
+                hipLaunchKernelGGL(norm_weight_long_kernel<E>, dim3((features + 63) / 64, (unsigned)parts), dim3(kThreads), 0,
+                                   s, a);
+            hipLaunchKernelGGL(norm_backward_long_kernel<E>, dim3((unsigned)rows), dim3(kThreads), 0, s, a);
+            return;
+        }
+        with_row<E>(features, [&](auto lanes, auto chunks) {
+            constexpr int L = decltype(lanes)::value, K = decltype(chunks)::value;
+            hipLaunchKernelGGL((norm_backward_kernel<E, L, K>), dim3((unsigned)parts), dim3(kThreads), 0, s, a);
+        });
     });
+    if (!ok) return fail(error, cap, "layer norm has too many rows");
     if (dgamma)
-        hipLaunchKernelGGL(norm_weight_sum_kernel, dim3((features + 255) / 256), dim3(256), 0, s,
-                           (const float *)workspace, parts, dgamma, dbeta, features);
+        hipLaunchKernelGGL(norm_weight_sum_kernel, dim3((2 * features + 15) / 16), dim3(kThreads), 0, s,
+                           (const float *)workspace, (int)parts, dgamma, dbeta, features);
     return launch_ok(error, cap, "layer norm launch");
 }

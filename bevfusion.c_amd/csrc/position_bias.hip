@@ -7,31 +7,137 @@ using namespace bfhip;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kAhead = 4;  // quads of positions per thread
 
-__global__ __launch_bounds__(kThreads) void bias_forward_kernel(const float *table, const int *map,
-                                                                float *bias, int buckets, int heads,
-                                                                long long n) {
-    const long long p = (long long)blockIdx.x * kThreads + threadIdx.x;
+// Bound by writing heads x positions: a thread writes four neighbouring
+// positions of a head as one float4.  The map is read once; a position's table
+// row is read head by head from the caches (a table row is heads neighbours, so
+// a line serves many heads).
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void bias_forward_kernel(const float *table, const int *map, float *bias,
+                                                                int buckets, int heads, int per, long long n) {
+    constexpr int N = VEC ? 4 : 1;
+    const long long p = ((long long)blockIdx.x * kThreads + threadIdx.x) * N;
     if (p >= n) return;
-    const int b = map[p];
-    for (int h = 0; h < heads; ++h)
-        bias[h * n + p] = (unsigned)b < (unsigned)buckets ? table[(size_t)b * heads + h] : 0.f;
+    const int h0 = blockIdx.y * per, h1 = min(heads, h0 + per);
+    long long row[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int b = map[p + e];
+        row[e] = (unsigned)b < (unsigned)buckets ? (long long)b * heads : -1;
+    }
+#pragma unroll 4
+    for (int h = h0; h < h1; ++h) {
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = row[e] >= 0 ? table[row[e] + h] : 0.f;
+        if constexpr (VEC) *reinterpret_cast<float4 *>(bias + h * n + p) = make_float4(v[0], v[1], v[2], v[3]);
+        else bias[h * n + p] = v[0];
+    }
 }
 
-// One workgroup per (bucket, head): the sum over the map in a fixed order.
-__global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *dbias, const int *map,
-                                                                 float *dtable, int heads,
+// Sums by bucket without atomics between lanes: a wave takes HEADS heads by
+// 64 / HEADS quads of neighbouring positions at a time, and every lane adds
+// into sums of its own (bucket by lane, in LDS), so each address is one lane's
+// and the order of every sum is fixed.  LDS holds `range` buckets per wave; a
+// table with more is walked in ranges, a workgroup each.  The lanes of a head
+// and the waves are added up in order at the end: partial [parts][range x
+// ranges][HEADS x head tiles], or the result where there is one part.
+template <int HEADS>
+__global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *dbias, const int *map, float *out,
+                                                                 int buckets, int heads, int range, int waves, bool vec,
                                                                  long long n) {
-    __shared__ float part[kThreads / kWave];
-    const int b = blockIdx.x / heads, h = blockIdx.x % heads;
-    float sum = 0.f;
-    for (long long p = threadIdx.x; p < n; p += kThreads)
-        if (map[p] == b) sum += dbias[h * n + p];
-    sum = group_sum<kWave>(sum);
-    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = sum;
+    constexpr int QUADS = kWave / HEADS;
+    extern __shared__ float smem[];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int tiles = (heads + HEADS - 1) / HEADS, tile = blockIdx.y % tiles, b0 = blockIdx.y / tiles * range;
+    const int count = min(range, buckets - b0);
+    // Neighbouring lanes take neighbouring quads of one head.
+    const int head = tile * HEADS + lane / QUADS, quad = lane % QUADS;
+    float *const sums = smem + (size_t)wave * range * kWave + lane;
+    for (int b = 0; b < count; ++b) sums[b * kWave] = 0.f;
+    const float *const row = dbias + (size_t)min(head, heads - 1) * n;
+    const bool live = head < heads;
+    const long long step = (long long)gridDim.x * waves * QUADS * 4;
+    for (long long p0 = ((long long)blockIdx.x * waves + wave) * QUADS * 4 + quad * 4; p0 < n; p0 += step * kAhead) {
+        float v[kAhead][4];
+        int at[kAhead][4];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const long long p = p0 + a * step;
+            if (vec && p < n) {
+                const float4 f = *reinterpret_cast<const float4 *>(row + p);
+                const int4 m = *reinterpret_cast<const int4 *>(map + p);
+                v[a][0] = f.x, v[a][1] = f.y, v[a][2] = f.z, v[a][3] = f.w;
+                at[a][0] = m.x, at[a][1] = m.y, at[a][2] = m.z, at[a][3] = m.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[a][e] = p + e < n ? row[p + e] : 0.f;
+                    at[a][e] = p + e < n ? map[p + e] : -1;
+                }
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned b = (unsigned)(at[a][e] - b0);
+                if (live && b < (unsigned)count)
+                    __hip_atomic_fetch_add(sums + b * kWave, v[a][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+    }
     __syncthreads();
-    if (threadIdx.x == 0) dtable[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+    for (int i = threadIdx.x; i < count * HEADS; i += blockDim.x) {
+        const int b = i / HEADS, h = i % HEADS;
+        if (tile * HEADS + h >= heads) continue;
+        float s = 0.f;
+        for (int w = 0; w < waves; ++w)
+#pragma unroll
+            for (int q = 0; q < QUADS; ++q) s += smem[((size_t)w * range + b) * kWave + h * QUADS + q];
+        out[((size_t)blockIdx.x * buckets + b0 + b) * heads + tile * HEADS + h] = s;
+    }
+}
+
+// Sums of the parts, in order: 16 results per workgroup, 16 threads each.
+__global__ __launch_bounds__(kThreads) void bias_sum_kernel(const float *partial, int parts, float *dtable, int n) {
+    __shared__ float sum[16][17];
+    const int c = blockIdx.x * 16 + threadIdx.x % 16, w = threadIdx.x / 16;
+    float s = 0.f;
+    if (c < n)
+        for (int p = w; p < parts; p += 16) s += partial[(size_t)p * n + c];
+    sum[w][threadIdx.x % 16] = s;
+    __syncthreads();
+    if (w || c >= n) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sum[i][threadIdx.x];
+    dtable[c] = s;
+}
+
+// How a gradient is dealt: heads per wave (the fewest of 1, 4 and 16 that hold
+// them, 16 beyond), buckets per range and waves by the LDS they need, and
+// parts so that a thread has at least two rounds of loads.
+struct BiasPlan {
+    int lanes, range, waves, ranges, tiles, parts;
+};
+
+BiasPlan bias_plan(int buckets, int heads, long long positions) {
+    constexpr int kLds = 128 << 10, kRow = kWave * sizeof(float);
+    BiasPlan p{};
+    p.lanes = heads == 1 ? 1 : heads <= 4 ? 4 : 16;
+    p.range = buckets < kLds / kRow ? buckets : kLds / kRow;
+    p.waves = kLds / (p.range * kRow);
+    p.waves = p.waves < kWaves ? p.waves : kWaves;
+    p.ranges = (buckets + p.range - 1) / p.range;
+    p.tiles = (heads + p.lanes - 1) / p.lanes;
+    const long long round = (long long)p.waves * (kWave / p.lanes) * 4 * kAhead;
+    const long long most = (positions + round - 1) / round;
+    // One workgroup per CU or as many as the LDS of two rounds of them holds.
+    long long parts = 512 / ((long long)p.ranges * p.tiles);
+    parts = parts < 1 ? 1 : parts;
+    p.parts = (int)(most < 1 ? 1 : most < parts ? most : parts);
+    return p;
 }
 
 bool bad_bias(int buckets, int heads, long long positions) {
@@ -47,28 +153,55 @@ extern "C" int bfhip_position_bias_forward(const float *table, const int *map, f
     if (bad_bias(buckets, heads, positions) || (positions && (!table || !map || !bias)))
         return fail(error, cap, "invalid position bias contract");
     if (positions == 0) return 1;
-    const long long grid = (positions + kThreads - 1) / kThreads;
+    const bool vec = positions % 4 == 0 && !(((uintptr_t)bias | (uintptr_t)map) & 15);
+    const long long threads = vec ? positions / 4 : positions, grid = (threads + kThreads - 1) / kThreads;
     if (!launch_fits(grid, kThreads)) return fail(error, cap, "position bias has too many positions");
-    hipLaunchKernelGGL(bias_forward_kernel, dim3((unsigned)grid), dim3(kThreads), 0,
-                       (hipStream_t)stream, table, map, bias, buckets, heads, positions);
+    // Heads are split over workgroups while the grid leaves CUs without one.
+    int parts = grid >= 1024 ? 1 : (int)(1024 / grid);
+    parts = parts < heads ? parts : heads;
+    parts = parts < 65535 ? parts : 65535;
+    const int per = (heads + parts - 1) / parts;
+    const dim3 blocks((unsigned)grid, (heads + per - 1) / per);
+    if (vec)
+        hipLaunchKernelGGL(bias_forward_kernel<true>, blocks, dim3(kThreads), 0, (hipStream_t)stream, table, map, bias,
+                           buckets, heads, per, positions);
+    else
+        hipLaunchKernelGGL(bias_forward_kernel<false>, blocks, dim3(kThreads), 0, (hipStream_t)stream, table, map, bias,
+                           buckets, heads, per, positions);
     return launch_ok(error, cap, "position bias launch");
 }
 
 extern "C" size_t bfhip_position_bias_backward_workspace(int buckets, int heads, long long positions) {
-    (void)buckets, (void)heads, (void)positions;
-    return 0;
+    if (bad_bias(buckets, heads, positions)) return 0;
+    const BiasPlan p = bias_plan(buckets, heads, positions);
+    return p.parts > 1 ? (size_t)p.parts * buckets * heads * sizeof(float) : 0;
 }
 
-extern "C" int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtable,
-                                            int buckets, int heads, long long positions,
-                                            void *workspace, size_t workspace_bytes, void *stream,
+extern "C" int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtable, int buckets, int heads,
+                                            long long positions, void *workspace, size_t workspace_bytes, void *stream,
                                             char *error, size_t cap) {
-    (void)workspace, (void)workspace_bytes;
     if (bad_bias(buckets, heads, positions) || !dtable || (positions && (!dbias || !map)))
         return fail(error, cap, "invalid position bias contract");
-    if (!launch_fits((long long)buckets * heads, kThreads))
-        return fail(error, cap, "position bias has too many buckets");
-    hipLaunchKernelGGL(bias_backward_kernel, dim3(buckets * heads), dim3(kThreads), 0,
-                       (hipStream_t)stream, dbias, map, dtable, heads, positions);
+    const BiasPlan p = bias_plan(buckets, heads, positions);
+    const long long blocks = (long long)p.ranges * p.tiles;
+    if (blocks > 65535) return fail(error, cap, "position bias has too many buckets and heads");
+    const size_t need = bfhip_position_bias_backward_workspace(buckets, heads, positions);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
+        return fail(error, cap, "position bias workspace too small or not 16-byte aligned");
+    hipStream_t s = (hipStream_t)stream;
+    const bool vec = positions % 4 == 0 && !(((uintptr_t)dbias | (uintptr_t)map) & 15);
+    float *const out = p.parts > 1 ? (float *)workspace : dtable;
+    const auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(p.parts, (unsigned)blocks), dim3(p.waves * kWave),
+                           (size_t)p.waves * p.range * kWave * sizeof(float), s, dbias, map, out, buckets, heads, p.range,
+                           p.waves, vec, positions);
+    };
+    if (p.lanes == 1) launch(bias_backward_kernel<1>);
+    else if (p.lanes == 4) launch(bias_backward_kernel<4>);
+    else launch(bias_backward_kernel<16>);
+    if (p.parts > 1) {
+        const int n = buckets * heads;
+        hipLaunchKernelGGL(bias_sum_kernel, dim3((n + 15) / 16), dim3(kThreads), 0, s, (const float *)out, p.parts, dtable, n);
+    }
     return launch_ok(error, cap, "position bias launch");
 }
