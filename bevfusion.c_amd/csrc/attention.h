@@ -26,6 +26,12 @@ struct AttnArgs {
     long long q_tokens, k_tokens;
     int sequences, heads, kv_heads, dim, causal, reach;
     float scale, scale2;  // scale2 = scale * log2(e): softmax runs in base 2
+    int slots;            // of the grid
+    int flip;             // the queries' signs change (forward)
+    int parts;            // most parts that a sequence's keys are split into
+    int chunk;            // keys of a part, at least (few queries)
+    float *part_out;      // parts > 1: sums of each part, [parts][q_tokens][heads][padded dim]
+    float2 *part_stat;    // and their (m, l), [parts][q_tokens][heads]
 };
 
 // Work on packed sequences is dealt in slots of `rows` rows without knowing the
@@ -36,9 +42,10 @@ struct AttnArgs {
 inline long long slot_count(long long tokens, int sequences, int rows) { return tokens / rows + sequences; }
 
 struct Slot {
-    int sequence;  // -1: none
-    int first;     // row within the sequence
-    int start, length;
+    int sequence;       // -1: none
+    int index;          // of the sequence's slots
+    int first;          // row within the sequence (find_rows)
+    int start, length;  // the sequence's rows
 };
 
 __device__ __forceinline__ long long clamp_start(const int *starts, int b, long long tokens) {
@@ -55,14 +62,13 @@ __device__ __forceinline__ void sequence_rows(const int *starts, int b, long lon
 
 // One wave searches 64 candidates at a time (one load for up to 64 sequences,
 // two for up to 4096).
-template <int ROWS>
-__device__ __forceinline__ Slot find_slot(const int *starts, int sequences, long long tokens, int slot) {
+__device__ __forceinline__ Slot find_slot(const int *starts, int sequences, long long tokens, int slot, int rows) {
     const int lane = threadIdx.x % kWave;
     int lo = 0, span = sequences;
     while (span > 1) {
         const int step = (span + kWave - 1) / kWave;
         const int at = lo + lane * step;
-        const bool below = lane * step < span && clamp_start(starts, at, tokens) / ROWS + at <= slot;
+        const bool below = lane * step < span && clamp_start(starts, at, tokens) / rows + at <= slot;
         const int n = __popcll(__ballot(below));  // a prefix of the lanes
         const int skip = n > 0 ? (n - 1) * step : 0;
         lo += skip;
@@ -71,9 +77,65 @@ __device__ __forceinline__ Slot find_slot(const int *starts, int sequences, long
     Slot s;
     s.sequence = __builtin_amdgcn_readfirstlane(lo);
     sequence_rows(starts, s.sequence, tokens, s.start, s.length);
-    s.first = (slot - (s.start / ROWS + s.sequence)) * ROWS;
-    if (s.first < 0 || s.first >= s.length) s.sequence = -1;
+    s.index = max(0, slot - (s.start / rows + s.sequence));
     return s;
+}
+
+// The sequence of a row, -1 for rows outside every sequence.
+__device__ __forceinline__ int find_token(const int *starts, int sequences, long long tokens, int token) {
+    const int lane = threadIdx.x % kWave;
+    int lo = 0, span = sequences;
+    while (span > 1) {
+        const int step = (span + kWave - 1) / kWave;
+        const int n = __popcll(__ballot(lane * step < span && clamp_start(starts, lo + lane * step, tokens) <= token));
+        const int skip = n > 0 ? (n - 1) * step : 0;
+        lo += skip;
+        span = min(step, span - skip);
+    }
+    int start, length;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    sequence_rows(starts, lo, tokens, start, length);
+    return token >= start && token - start < length ? lo : -1;
+}
+
+// Slots that have rows of their sequence.
+template <int ROWS>
+__device__ __forceinline__ Slot find_rows(const int *starts, int sequences, long long tokens, int slot) {
+    Slot s = find_slot(starts, sequences, tokens, slot, ROWS);
+    if (s.index * (long long)ROWS >= s.length) s.sequence = -1;
+    s.first = s.index * ROWS;
+    return s;
+}
+
+// Workgroup `id` of slots x heads: its slot and head.  Workgroups are dealt
+// round-robin over the eight XCDs, each with an L2 of its own, so the deal keeps
+// a key head's workgroups on as few XCDs as it can: with kv_heads a multiple or
+// a divisor of eight, id % 8 names the key head (and which share of its work).
+// Slots come from the last one on: in causal sequences the last queries see
+// the most keys, and the longest work should start first.
+struct Deal {
+    int slot, head;
+};
+
+__host__ __device__ __forceinline__ Deal deal(int id, int slots, int heads, int kv_heads) {
+    const int group = heads / kv_heads;
+    int kv = id % kv_heads, rest = id / kv_heads;
+    if (kv_heads % 8 == 0) {
+        const int per = kv_heads / 8, l = id / 8;
+        kv = id % 8 + 8 * (l % per);
+        rest = l / per;
+    }
+    Deal d;
+    d.slot = slots - 1 - rest / group;
+    d.head = kv * group + rest % group;
+    return d;
+}
+
+// Key tiles per part when `tiles` of them are split evenly into parts of about
+// `least` or more, at most `parts` of them.
+__device__ __forceinline__ int part_tiles(int tiles, int parts, int least) {
+    const int n = min(parts, max(1, tiles / least));
+    return max(1, (tiles + n - 1) / n);
 }
 
 // ------------------------------------------------------------- operand tiles
@@ -167,6 +229,35 @@ __device__ __forceinline__ typename E::Frag col_frag(const char *lds, int r0, in
     }
 }
 
+// All fragments of the transposed 32-row tile at `lds`, as col_frag gives them,
+// read and waited for in one piece.  The compiler waits for every LDS-DMA copy
+// in flight before a transposing read of its own; this form leaves them in
+// flight, for loops that keep copies running behind the products.
+template <class E, int DIM>
+__device__ __forceinline__ void col_frags_in_flight(const char *lds, int lane, typename E::Frag (&f)[DIM / 16]) {
+    if constexpr (E::kSize == 4) {
+#pragma unroll
+        for (int db = 0; db < DIM / 16; ++db) f[db] = col_frag<E, DIM>(lds, 0, db, lane);
+    } else {
+        using T = AttnTile<E, DIM>;
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const int c16 = lane & 15, r = 4 * (lane >> 4) + (c16 >> 2);
+        const uint32_t row = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)(lds) + r * T::kRow + 8 * (c16 & 1);
+#pragma unroll
+        for (int db = 0; db < DIM / 16; db += 2) {
+            const uint32_t c = (c16 & 3) >> 1, p = row + 16 * ((2 * db + c) ^ T::swizzle(r)), q = row + 16 * ((2 * db + 2 + c) ^ T::swizzle(r));
+            s16x4 a, b, x, y;
+            asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                         "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(a), "=&v"(b), "=&v"(x), "=&v"(y)
+                         : "v"(p), "v"(q), "n"(16 * T::kRow)
+                         : "memory");
+            f[db] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+            f[db + 1] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+}
+
 // Fragment of 16 rows in global memory (row 0 at `base`): elements 32 kk ..+31.
 // Rows past `rows` and elements past dim are zero.
 template <class E>
@@ -177,6 +268,18 @@ __device__ __forceinline__ typename E::Frag global_frag(const char *base, long l
     if (r < rows && d < dim)
         f = *reinterpret_cast<const typename E::Frag *>(base + r * token_bytes + d * E::kSize);
     return f;
+}
+
+// The fragment, its signs changed if `flip`.
+template <class E>
+__device__ __forceinline__ typename E::Frag signed_frag(typename E::Frag f, int flip) {
+    if (!flip) return f;
+    if constexpr (E::kSize == 4) {
+        return -f;
+    } else {
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(bf16x8, __builtin_bit_cast(s16x8, f) ^ (short)0x8000);
+    }
 }
 
 // Eight fp32 values as operand words, rounded to nearest even.
@@ -253,6 +356,7 @@ inline AttnArgs attn_args(const bfhip_attention_desc *d, const bfhip_rows *q, co
     a.dim = d->head_dim;
     a.causal = d->causal;
     a.reach = d->bias ? d->reach : 0;
+    a.slots = 0;
     a.scale = d->scale;
     a.scale2 = d->scale * kLog2E;
     return a;

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256, 1) void attention_keys_kernel(GradArgs a) {
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4, group = f.heads / f.kv_heads;
     const int kv = blockIdx.x % f.kv_heads, slot_id = blockIdx.x / f.kv_heads;
-    const Slot s = find_slot<kRows>(f.k_starts, f.sequences, f.k_tokens, slot_id);
+    const Slot s = find_rows<kRows>(f.k_starts, f.sequences, f.k_tokens, slot_id);
     if (s.sequence < 0) return;
     int q_start, q_len;
     sequence_rows(f.q_starts, s.sequence, f.q_tokens, q_start, q_len);
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     const int l16 = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % f.heads, slot_id = blockIdx.x / f.heads, kv = head / (f.heads / f.kv_heads);
     const int width = 2 * f.reach + 1;
-    const Slot s = find_slot<kRows>(f.q_starts, f.sequences, f.q_tokens, slot_id);
+    const Slot s = find_rows<kRows>(f.q_starts, f.sequences, f.q_tokens, slot_id);
     float *const part = BIAS && a.part ? a.part + (size_t)blockIdx.x * width : nullptr;
     if (s.sequence < 0) {
         if (part)
