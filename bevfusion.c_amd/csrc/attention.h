@@ -117,7 +117,7 @@ struct Deal {
     int slot, head;
 };
 
-__host__ __device__ __forceinline__ Deal deal(int id, int slots, int heads, int kv_heads) {
+__device__ __forceinline__ Deal deal(int id, int slots, int heads, int kv_heads) {
     const int group = heads / kv_heads;
     int kv = id % kv_heads, rest = id / kv_heads;
     if (kv_heads % 8 == 0) {
@@ -151,6 +151,11 @@ struct AttnTile {
         return r / per & ((kChunks < 16 ? kChunks : 16) - 1);
     }
 };
+
+// One 4-byte LDS-DMA per lane: LDS[lds + 4 * lane] = buffer[voffset].
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rsrc, char *lds, uint32_t voffset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds), 4, voffset, 0, 0, 0);
+}
 
 // Copies ROWS rows to LDS with THREADS threads by LDS-DMA.  Rows past `left`
 // and elements past dim read as zero.

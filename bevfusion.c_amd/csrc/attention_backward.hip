@@ -4,11 +4,16 @@
 //   delta_i = dout_i . out_i,  ds_ij = p_ij (dout_i . v_j - delta_i),
 //   dv_j = sum_i p_ij dout_i,  dk_j = scale sum_i ds_ij q_i,
 //   dq_i = scale sum_j ds_ij k_j,  dbias[e] = sum of ds over pairs at e.
-// Three launches: the row terms (delta and lse); dk and dv, a workgroup per
-// tile of keys and key head that walks the queries of the group's heads; dq
-// and dbias, a workgroup per tile of queries and head that walks the keys.
-// Walking twice costs two products of seven more than adding dq up with
-// atomics would, and gives the same bits every time.
+// Three passes: the row terms (delta and lse); dq and dbias, a workgroup per
+// tile of queries and head that walks the keys; dk and dv, a workgroup per tile
+// of keys and key head that walks the queries of the group's heads.  Walking
+// twice costs two products of seven more than adding dq up with atomics would,
+// and gives the same bits every time.
+//
+// A bias's gradient sums very many ds, whose sum over a row is zero but for
+// delta's error; out's rounding to 16 bits is too large an error there.  With
+// dbias, delta is therefore summed from p and dout . v in fp32, in a walk of its
+// own over the keys, before dq's.
 #include <type_traits>
 
 #include "attention.h"
@@ -17,16 +22,18 @@ using namespace bfhip;
 
 namespace {
 
-constexpr int kTile = 64;  // rows per LDS tile
+constexpr int kTile = 64;       // rows per LDS tile
+constexpr int kPartSteps = 16;  // fewest tiles of queries of a part
 
 struct GradArgs {
     AttnArgs f;
     AttnRows dout, dq, dk, dv;
-    float *lse2, *delta;  // [heads, q_tokens]
-    float *part;          // [query slots, heads, 2 reach + 1] or null
+    float *nlse, *delta;  // [heads, q_tokens]
+    float *part;          // dbias: [query slots, heads, 2 reach + 1] or null
+    float *part_kv;       // f.parts > 1: [parts][k_tokens][kv_heads][dk, dv][padded dim]
 };
 
-// lse in base 2, +inf for a query without keys (every p of it is then 0), and
+// -lse in base 2 (-inf for a query without keys: every p of it is then 0), and
 // delta; 16 lanes per (token, head).
 template <class E>
 __global__ __launch_bounds__(256) void attention_terms_kernel(GradArgs a) {
@@ -35,7 +42,7 @@ __global__ __launch_bounds__(256) void attention_terms_kernel(GradArgs a) {
     const long long t = id / a.f.heads;
     const int h = (int)(id % a.f.heads), d = 8 * (threadIdx.x % 16);
     float sum = 0.f;
-    if (d < a.f.dim) {
+    if (d < a.f.dim && !a.part) {
         using W = Words<E, 8>;
         const W o = *reinterpret_cast<const W *>(__builtin_assume_aligned(a.f.out.at(t, h) + d * E::kSize, 16));
         const W g = *reinterpret_cast<const W *>(__builtin_assume_aligned(a.dout.at(t, h) + d * E::kSize, 16));
@@ -46,32 +53,83 @@ __global__ __launch_bounds__(256) void attention_terms_kernel(GradArgs a) {
     if (threadIdx.x % 16) return;
     const size_t at = (size_t)h * a.f.q_tokens + t;
     const float lse = a.f.lse[at];
-    a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2E;
+    a.nlse[at] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;
     a.delta[at] = sum;
 }
 
-// KB blocks of 16 keys per wave, four waves.  Scores come out with a key per
-// lane, so P and dS are the second operands of dv^T = dout^T P and dk^T = q^T
-// dS without leaving their registers.
-template <class E, int DIM, int KB, bool BIAS>
-__global__ __launch_bounds__(256, 1) void attention_keys_kernel(GradArgs a) {
-    constexpr int kRows = 64 * KB, kKB = DIM / 32, kDB = DIM / 16;
-    using T = AttnTile<E, DIM>;
+// The queries that a tile of keys meets, as steps of 64 queries of one head.
+struct Steps {
+    int begin, tiles;  // first query (a multiple of 64), tiles of each head
+};
+__device__ __forceinline__ Steps query_steps(int causal, int first_key, int offset, int q_len) {
+    Steps s;
+    s.begin = causal ? max(0, first_key - offset) / kTile * kTile : 0;
+    s.tiles = s.begin < q_len ? (q_len - s.begin + kTile - 1) / kTile : 0;
+    return s;
+}
+
+// Bias and scale of one lane's four scores: the biases are looked up where
+// distances within the reach occur, else all have one.
+struct BiasRow {
+    const float *row;  // times log2 e
+    int reach;
+    __device__ __forceinline__ float at(int far) const { return row[min(max(far, -reach), reach) + reach]; }
+    // 1: all distances of low .. high are beyond the reach; `value` is theirs.
+    __device__ __forceinline__ bool one(int low, int high, float &value) const {
+        if (high <= -reach) value = row[0];
+        else if (low >= reach) value = row[2 * reach];
+        else return false;
+        return true;
+    }
+};
+
+template <class E, int DIM, int KB, int WAVES>
+struct KeyTile {
+    static constexpr int kRows = WAVES * 16 * KB, kThreads = WAVES * kWave;
+    static constexpr int kQ = kTile * AttnTile<E, DIM>::kRow;  // bytes of a tile of q or dout
+    static constexpr int kStage = 2 * kQ + 2 * kTile * (int)sizeof(float);
+};
+
+// KB blocks of 16 keys per wave.  Scores come out with a key per lane, so P and
+// dS are the second operands of dv^T = dout^T P and dk^T = q^T dS without
+// leaving their registers.  Bound by the matrix cores and LDS reads: q and dout
+// are read from LDS twice, as rows and transposed, for KB x 16 keys per wave.
+template <class E, int DIM, int KB, int WAVES, bool BIAS>
+__global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArgs a) {
+    using K = KeyTile<E, DIM, KB, WAVES>;
+    constexpr int kRows = K::kRows, kKB = DIM / 32, kDB = DIM / 16, kThreads = K::kThreads;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char *const qt = smem, *const gt = smem + kTile * T::kRow;
-    float *const terms = reinterpret_cast<float *>(gt + kTile * T::kRow);  // lse2 [64], delta [64]
-    float *const bias = terms + 2 * kTile;
     const AttnArgs &f = a.f;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4, group = f.heads / f.kv_heads;
-    const int kv = blockIdx.x % f.kv_heads, slot_id = blockIdx.x / f.kv_heads;
-    const Slot s = find_rows<kRows>(f.k_starts, f.sequences, f.k_tokens, slot_id);
+    const int items = f.slots * f.kv_heads, part = blockIdx.x / items;
+    // In causal sequences the first keys are seen by the most queries.
+    const Deal deal_ = deal(blockIdx.x % items, f.slots, f.kv_heads, f.kv_heads);
+    const int kv = deal_.head;
+    const Slot s = find_rows<kRows>(f.k_starts, f.sequences, f.k_tokens, f.slots - 1 - deal_.slot);
     if (s.sequence < 0) return;
     int q_start, q_len;
     sequence_rows(f.q_starts, s.sequence, f.q_tokens, q_start, q_len);
     const int offset = s.length - q_len;
     const int key0 = s.first + wave * 16 * KB;
+    const Steps steps = query_steps(f.causal, s.first, offset, q_len);
+    const int all = steps.tiles * group, per = part_tiles(all, f.parts, kPartSteps);
+    if (part && part >= (all + per - 1) / per) return;  // (the first part is always there)
+    const int first = part * per, end = min(all, first + per);
 
+    AttnTileCopy<E, DIM, kTile, kThreads> qc, gc;
+    qc.init(f.q.token, f.dim, threadIdx.x);
+    gc.init(a.dout.token, f.dim, threadIdx.x);
+    const auto issue = [&](int step) {
+        const int head = kv * group + step / steps.tiles, i0 = steps.begin + step % steps.tiles * kTile, left = q_len - i0;
+        char *const to = smem + (step & 1) * K::kStage;
+        qc.issue(f.q.at((long long)q_start + i0, head), left, to);
+        gc.issue(a.dout.at((long long)q_start + i0, head), left, to + K::kQ);
+        // Past the last query q, dout and the terms are zero: p is 1, but dout and ds are 0.
+        if (wave < 2)
+            dma4(buffer_rsrc((wave ? a.delta : a.nlse) + (size_t)head * f.q_tokens + q_start + i0, 4u * min(left, kTile)),
+                 to + 2 * K::kQ + wave * kTile * sizeof(float), 4u * lane);
+    };
     typename E::Frag kf[KB][kKB], vf[KB][kKB];
     f32x4 dk[KB][kDB], dv[KB][kDB];
 #pragma unroll
@@ -85,79 +143,88 @@ __global__ __launch_bounds__(256, 1) void attention_keys_kernel(GradArgs a) {
 #pragma unroll
         for (int db = 0; db < kDB; ++db) dk[kb][db] = dv[kb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    AttnTileCopy<E, DIM, kTile, 256> qc, gc;
-    qc.init(f.q.token, f.dim, threadIdx.x);
-    gc.init(a.dout.token, f.dim, threadIdx.x);
-    // The first query that sees the tile's first key.
-    const int begin = f.causal ? max(0, s.first - offset) / kTile * kTile : 0;
-
-    for (int hg = 0; hg < group; ++hg) {
-        const int head = kv * group + hg;
+    BiasRow bias{};
+    int bias_head = -1;
+    if (first < end) issue(first);
+    for (int step = first; step < end; ++step) {
+        wait_vmcnt<0>();
+        lds_barrier();  // this tile is there, and the one before has been read
+        if (step + 1 < end) issue(step + 1);
+        const char *const qt = smem + (step & 1) * K::kStage, *const gt = qt + K::kQ;
+        const float *const terms = reinterpret_cast<const float *>(gt + K::kQ);
+        const int hg = step / steps.tiles, i0 = steps.begin + step % steps.tiles * kTile;
         if constexpr (BIAS) {
-            lds_barrier();
-            const float *b = f.bias + (size_t)head * (2 * f.reach + 1);
-            for (int i = threadIdx.x; i <= 2 * f.reach; i += 256) bias[i] = b[i] * kLog2E;
-        }
-        for (int i0 = begin; i0 < q_len; i0 += kTile) {
-            lds_barrier();  // the tile before has been read
-            qc.issue(f.q.at((long long)q_start + i0, head), q_len - i0, qt);
-            gc.issue(a.dout.at((long long)q_start + i0, head), q_len - i0, gt);
-            if (threadIdx.x < 2 * kTile) {
-                const int i = threadIdx.x % kTile;
-                const bool lse = threadIdx.x < kTile;
-                const size_t at = (size_t)head * f.q_tokens + q_start + i0 + i;
-                terms[threadIdx.x] = i0 + i < q_len ? (lse ? a.lse2 : a.delta)[at] : lse ? INFINITY : 0.f;
+            if (hg != bias_head) {
+                bias_head = hg;
+                float *const row = reinterpret_cast<float *>(smem + 2 * K::kStage);
+                const float *b = f.bias + (size_t)(kv * group + hg) * (2 * f.reach + 1);
+                for (int i = threadIdx.x; i <= 2 * f.reach; i += kThreads) row[i] = b[i] * kLog2E;
+                lds_barrier();
+                bias = BiasRow{row, f.reach};
             }
-            wait_vmcnt<0>();
-            lds_barrier();
-            // A query that does not see every key of the tile.
-            const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
+        }
+        // A query that does not see every key of the wave's.
+        const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                f32x4 p[2][KB], ds[2][KB];
+        for (int c = 0; c < 2; ++c) {
+            f32x4 p[2][KB], ds[2][KB];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int r0 = 32 * c + 16 * b;
+            for (int b = 0; b < 2; ++b) {
+                const int r0 = 32 * c + 16 * b;
 #pragma unroll
-                    for (int kb = 0; kb < KB; ++kb) p[b][kb] = ds[b][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int kb = 0; kb < KB; ++kb) p[b][kb] = ds[b][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int kk = 0; kk < kKB; ++kk) {
-                        const typename E::Frag qf = row_frag<E, DIM>(qt, r0, kk, lane);
+                for (int kk = 0; kk < kKB; ++kk) {
+                    const typename E::Frag qf = row_frag<E, DIM>(qt, r0, kk, lane);
 #pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) p[b][kb] = E::mfma(qf, kf[kb][kk], p[b][kb]);
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < kKB; ++kk) {
-                        const typename E::Frag gf = row_frag<E, DIM>(gt, r0, kk, lane);
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb) ds[b][kb] = E::mfma(gf, vf[kb][kk], ds[b][kb]);
-                    }
-                    const f32x4 lse = *reinterpret_cast<const f32x4 *>(terms + r0 + 4 * g);
-                    const f32x4 delta = *reinterpret_cast<const f32x4 *>(terms + kTile + r0 + 4 * g);
-#pragma unroll
-                    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            // Position of the query before the key.
-                            const int far = key0 + 16 * kb + l16 - (i0 + r0 + 4 * g + e + offset);
-                            float x = p[b][kb][e] * f.scale2;
-                            if constexpr (BIAS) x += bias[min(max(far, -f.reach), f.reach) + f.reach];
-                            x = exp2_raw(x - lse[e]);
-                            float y = x * (ds[b][kb][e] - delta[e]);
-                            if (edge && far > 0) x = y = 0.f;
-                            p[b][kb][e] = x;
-                            ds[b][kb][e] = y;
-                        }
+                    for (int kb = 0; kb < KB; ++kb) p[b][kb] = E::mfma(qf, kf[kb][kk], p[b][kb]);
                 }
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const typename E::Frag pf = to_frag<E>(p[0][kb], p[1][kb]);
-                    const typename E::Frag sf = to_frag<E>(ds[0][kb], ds[1][kb]);
+                for (int kk = 0; kk < kKB; ++kk) {
+                    const typename E::Frag gf = row_frag<E, DIM>(gt, r0, kk, lane);
 #pragma unroll
-                    for (int db = 0; db < kDB; ++db) {
-                        dv[kb][db] = E::mfma(col_frag<E, DIM>(gt, 32 * c, db, lane), pf, dv[kb][db]);
-                        dk[kb][db] = E::mfma(col_frag<E, DIM>(qt, 32 * c, db, lane), sf, dk[kb][db]);
+                    for (int kb = 0; kb < KB; ++kb) ds[b][kb] = E::mfma(gf, vf[kb][kk], ds[b][kb]);
+                }
+                const f32x4 nlse = *reinterpret_cast<const f32x4 *>(terms + r0 + 4 * g);
+                const f32x4 delta = *reinterpret_cast<const f32x4 *>(terms + kTile + r0 + 4 * g);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    // Key minus query of the block's first ones.
+                    const int far0 = key0 + 16 * kb - (i0 + r0 + offset);
+                    f32x4 add = nlse;
+                    if constexpr (BIAS) {
+                        float one;
+                        if (bias.one(far0 - 15, far0 + 15, one)) {
+                            add += one;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) add[e] += bias.at(far0 + l16 - 4 * g - e);
+                        }
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = exp2_raw(fmaf(p[b][kb][e], f.scale2, add[e]));
+                        float y = x * (ds[b][kb][e] - delta[e]);
+                        if (edge && far0 + l16 > 4 * g + e) x = y = 0.f;
+                        p[b][kb][e] = x;
+                        ds[b][kb][e] = y;
+                    }
+                }
+            }
+            typename E::Frag pf[KB], sf[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                pf[kb] = to_frag<E>(p[0][kb], p[1][kb]);
+                sf[kb] = to_frag<E>(ds[0][kb], ds[1][kb]);
+            }
+#pragma unroll
+            for (int db = 0; db < kDB; ++db) {
+                const typename E::Frag gf = col_frag<E, DIM>(gt, 32 * c, db, lane);
+                const typename E::Frag qf = col_frag<E, DIM>(qt, 32 * c, db, lane);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    dv[kb][db] = E::mfma(gf, pf[kb], dv[kb][db]);
+                    dk[kb][db] = E::mfma(qf, sf[kb], dk[kb][db]);
                 }
             }
         }
@@ -166,9 +233,50 @@ __global__ __launch_bounds__(256, 1) void attention_keys_kernel(GradArgs a) {
     for (int kb = 0; kb < KB; ++kb) {
         const int r = key0 + 16 * kb + l16;
         const bool live = r < s.length;
-        store_rows<E, kDB>(dk[kb], f.scale, a.dk.at((long long)s.start + r, kv), live, f.dim, lane);
-        store_rows<E, kDB>(dv[kb], 1.f, a.dv.at((long long)s.start + r, kv), live, f.dim, lane);
+        if (per < all) {
+            if (!live) continue;
+            float *const row = a.part_kv + (((size_t)part * f.k_tokens + s.start + r) * f.kv_heads + kv) * 2 * DIM + 4 * g;
+#pragma unroll
+            for (int db = 0; db < kDB; ++db) {
+                *reinterpret_cast<f32x4 *>(row + 16 * db) = dk[kb][db];
+                *reinterpret_cast<f32x4 *>(row + DIM + 16 * db) = dv[kb][db];
+            }
+        } else {
+            store_rows<E, kDB>(dk[kb], f.scale, a.dk.at((long long)s.start + r, kv), live, f.dim, lane);
+            store_rows<E, kDB>(dv[kb], 1.f, a.dv.at((long long)s.start + r, kv), live, f.dim, lane);
+        }
     }
+}
+
+// dk and dv from the parts' sums, in order: four elements per thread, 2 DIM / 4
+// threads per key and key head.
+template <class E, int DIM, int ROWS>
+__global__ __launch_bounds__(256) void attention_keys_join_kernel(GradArgs a) {
+    constexpr int kPer = 256 * 4 / (2 * DIM);  // key heads of a workgroup, all of one token
+    const AttnArgs &f = a.f;
+    const int per_token = (f.kv_heads + kPer - 1) / kPer, token = blockIdx.x / per_token;
+    const int kv = blockIdx.x % per_token * kPer + threadIdx.x / (DIM / 2), d = threadIdx.x % (DIM / 2) * 4;
+    const int sequence = find_token(f.k_starts, f.sequences, f.k_tokens, token);
+    if (sequence < 0 || kv >= f.kv_heads) return;
+    int q_start, q_len, k_start, k_len;
+    sequence_rows(f.q_starts, sequence, f.q_tokens, q_start, q_len);
+    sequence_rows(f.k_starts, sequence, f.k_tokens, k_start, k_len);
+    const Steps steps = query_steps(f.causal, (token - k_start) / ROWS * ROWS, k_len - q_len, q_len);
+    const int all = steps.tiles * (f.heads / f.kv_heads), per = part_tiles(all, f.parts, kPartSteps);
+    if (per >= all) return;  // written by the kernel before
+    const int used = (all + per - 1) / per;
+    const size_t step = (size_t)f.k_tokens * f.kv_heads * 2 * DIM;
+    const float *const at = a.part_kv + ((size_t)token * f.kv_heads + kv) * 2 * DIM + d;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < used; ++p) v += *reinterpret_cast<const f32x4 *>(at + p * step);
+    const bool is_k = d < DIM;
+    const int e0 = is_k ? d : d - DIM;
+    if (e0 >= f.dim) return;
+    Words<E, 4> w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w.put(e, v[e] * (is_k ? f.scale : 1.f));
+    w.store(reinterpret_cast<typename E::Word *>((is_k ? a.dk : a.dv).at(token, kv)) + e0);
 }
 
 // Sums of a 16 x 16 block of dS^T along its diagonals into `sum` (this wave's
@@ -202,21 +310,27 @@ __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int rea
     }
 }
 
-// IB blocks of 16 queries per wave, four waves.
+// Keys per tile: two tiles of keys and values, and five rows of the longest
+// bias, have to fit the LDS.
+constexpr int tile_keys(int size, int dim) { return size == 4 && dim > 64 ? 32 : 64; }
+
+// IB blocks of 16 queries per wave, four waves.  Scores come out with a query
+// per lane, so dS is the second operand of dq^T = k^T dS^T without leaving its
+// registers.
 template <class E, int DIM, int IB, bool BIAS>
 __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
-    constexpr int kRows = 64 * IB, kKB = DIM / 32, kDB = DIM / 16;
+    constexpr int kRows = 64 * IB, kKB = DIM / 32, kDB = DIM / 16, kKeys = tile_keys(E::kSize, DIM);
     using T = AttnTile<E, DIM>;
+    constexpr int kStage = 2 * kKeys * T::kRow;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char *const kt = smem, *const vt = smem + kTile * T::kRow;
-    float *const bias = reinterpret_cast<float *>(vt + kTile * T::kRow);
+    float *const bias_row = reinterpret_cast<float *>(smem + 2 * kStage);
     const AttnArgs &f = a.f;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4;
-    const int head = blockIdx.x % f.heads, slot_id = blockIdx.x / f.heads, kv = head / (f.heads / f.kv_heads);
-    const int width = 2 * f.reach + 1;
-    const Slot s = find_rows<kRows>(f.q_starts, f.sequences, f.q_tokens, slot_id);
-    float *const part = BIAS && a.part ? a.part + (size_t)blockIdx.x * width : nullptr;
+    const Deal deal_ = deal(blockIdx.x, f.slots, f.heads, f.kv_heads);
+    const int head = deal_.head, kv = head / (f.heads / f.kv_heads), width = 2 * f.reach + 1;
+    const Slot s = find_rows<kRows>(f.q_starts, f.sequences, f.q_tokens, deal_.slot);
+    float *const part = BIAS && a.part ? a.part + ((size_t)deal_.slot * f.heads + head) * width : nullptr;
     if (s.sequence < 0) {
         if (part)
             for (int i = threadIdx.x; i < width; i += 256) part[i] = 0.f;
@@ -225,18 +339,31 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     int k_start, k_len;
     sequence_rows(f.k_starts, s.sequence, f.k_tokens, k_start, k_len);
     const int offset = k_len - s.length, row0 = s.first + wave * 16 * IB;
-    float *const sums = bias + width * (1 + wave);
+    const int last = f.causal ? min(k_len, min(s.first + kRows, s.length) + offset) : k_len;
+    const int full = f.causal ? min(k_len, row0 + offset + 1) : k_len;
+    const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0;
+
+    AttnTileCopy<E, DIM, kKeys, 256> kc, vc;
+    kc.init(f.k.token, f.dim, threadIdx.x);
+    vc.init(f.v.token, f.dim, threadIdx.x);
+    const auto issue = [&](int t, int buffer) {
+        const int j0 = t * kKeys;
+        char *const to = smem + buffer * kStage;
+        kc.issue(f.k.at((long long)k_start + j0, kv), k_len - j0, to);
+        vc.issue(f.v.at((long long)k_start + j0, kv), k_len - j0, to + kKeys * T::kRow);
+    };
+    float *const sums = bias_row + width * (1 + wave);
     if constexpr (BIAS) {
         const float *b = f.bias + (size_t)head * width;
-        for (int i = threadIdx.x; i < width; i += 256) bias[i] = b[i] * kLog2E;
+        for (int i = threadIdx.x; i < width; i += 256) bias_row[i] = b[i] * kLog2E;
         if (part)
             for (int i = lane; i < width; i += kWave) sums[i] = 0.f;
     }
-    float low = 0.f, high = 0.f;
+    const BiasRow bias{bias_row, f.reach};
 
     typename E::Frag qf[IB][kKB], gf[IB][kKB];
     f32x4 dq[IB][kDB];
-    float lse[IB], delta[IB];
+    float nlse[IB], delta[IB];
     int limit[IB];
 #pragma unroll
     for (int ib = 0; ib < IB; ++ib) {
@@ -247,59 +374,100 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             gf[ib][kk] = global_frag<E>(a.dout.at((long long)s.start + r0, head), a.dout.token, s.length - r0, f.dim, kk, lane);
         }
         const size_t at = (size_t)head * f.q_tokens + s.start + r;
-        lse[ib] = r < s.length ? a.lse2[at] : INFINITY;
+        nlse[ib] = r < s.length ? a.nlse[at] : -INFINITY;
         delta[ib] = r < s.length ? a.delta[at] : 0.f;
         limit[ib] = f.causal ? min(k_len, r + offset + 1) : k_len;
 #pragma unroll
         for (int db = 0; db < kDB; ++db) dq[ib][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int last = f.causal ? min(k_len, min(s.first + kRows, s.length) + offset) : k_len;
-    const int full = f.causal ? min(k_len, row0 + offset + 1) : k_len;
-
-    AttnTileCopy<E, DIM, kTile, 256> kc, vc;
-    kc.init(f.k.token, f.dim, threadIdx.x);
-    vc.init(f.v.token, f.dim, threadIdx.x);
-    for (int j0 = 0; j0 < last; j0 += kTile) {
-        lds_barrier();  // the tile before has been read
-        kc.issue(f.k.at((long long)k_start + j0, kv), k_len - j0, kt);
-        vc.issue(f.v.at((long long)k_start + j0, kv), k_len - j0, vt);
-        wait_vmcnt<0>();
-        lds_barrier();
-        const bool edge = j0 + kTile > full;
+    // p and dp = dout . v of 16 keys from tile row r0.
+    const auto products = [&](const char *kt, const char *vt, int j0, int r0, f32x4 (&p)[IB], f32x4 (&dp)[IB]) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            f32x4 p[2][IB], ds[2][IB];
+        for (int ib = 0; ib < IB; ++ib) p[ib] = dp[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < kKB; ++kk) {
+            const typename E::Frag kf = row_frag<E, DIM>(kt, r0, kk, lane);
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) p[ib] = E::mfma(kf, qf[ib][kk], p[ib]);
+        }
+#pragma unroll
+        for (int kk = 0; kk < kKB; ++kk) {
+            const typename E::Frag vf = row_frag<E, DIM>(vt, r0, kk, lane);
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) dp[ib] = E::mfma(vf, gf[ib][kk], dp[ib]);
+        }
+        const bool edge = j0 + kKeys > full;
+#pragma unroll
+        for (int ib = 0; ib < IB; ++ib) {
+            const int far0 = j0 + r0 - (row0 + 16 * ib + offset);
+            f32x4 add = {nlse[ib], nlse[ib], nlse[ib], nlse[ib]};
+            if constexpr (BIAS) {
+                float one;
+                if (bias.one(far0 - 15, far0 + 15, one)) {
+                    add += one;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) add[e] += bias.at(far0 + 4 * g + e - l16);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, add[e]));
+                if (edge && j0 + r0 + 4 * g + e >= limit[ib]) p[ib][e] = dp[ib][e] = 0.f;
+            }
+        }
+    };
+    int buffer = 0;
+    if constexpr (BIAS) {
+        if (part) {
+            // delta in fp32 for the sums of ds.
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) delta[ib] = 0.f;
+            if (tiles > 0) issue(0, buffer);
+            for (int t = 0; t < tiles; ++t, buffer ^= 1) {
+                wait_vmcnt<0>();
+                lds_barrier();
+                issue(t + 1 < tiles ? t + 1 : 0, buffer ^ 1);  // (the first tile again for the walk below)
+                const char *const kt = smem + buffer * kStage, *const vt = kt + kKeys * T::kRow;
+#pragma unroll
+                for (int r0 = 0; r0 < kKeys; r0 += 16) {
+                    f32x4 p[IB], dp[IB];
+                    products(kt, vt, t * kKeys, r0, p, dp);
+#pragma unroll
+                    for (int ib = 0; ib < IB; ++ib)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) delta[ib] = fmaf(p[ib][e], dp[ib][e], delta[ib]);
+                }
+            }
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) {
+                delta[ib] += __shfl_xor(delta[ib], 16);
+                delta[ib] += __shfl_xor(delta[ib], 32);
+                const int r = row0 + 16 * ib + l16;
+                if (g == 0 && r < s.length) a.delta[(size_t)head * f.q_tokens + s.start + r] = delta[ib];
+            }
+        }
+    }
+    if (tiles > 0 && !part) issue(0, buffer);
+    float low = 0.f, high = 0.f;
+    for (int t = 0; t < tiles; ++t, buffer ^= 1) {
+        wait_vmcnt<0>();
+        lds_barrier();  // this tile is there, and the one before has been read
+        if (t + 1 < tiles) issue(t + 1, buffer ^ 1);
+        const char *const kt = smem + buffer * kStage, *const vt = kt + kKeys * T::kRow;
+        const int j0 = t * kKeys;
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+            f32x4 ds[2][IB];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int r0 = 32 * c + 16 * b;
-#pragma unroll
-                for (int ib = 0; ib < IB; ++ib) p[b][ib] = ds[b][ib] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < kKB; ++kk) {
-                    const typename E::Frag kf = row_frag<E, DIM>(kt, r0, kk, lane);
-#pragma unroll
-                    for (int ib = 0; ib < IB; ++ib) p[b][ib] = E::mfma(kf, qf[ib][kk], p[b][ib]);
-                }
-#pragma unroll
-                for (int kk = 0; kk < kKB; ++kk) {
-                    const typename E::Frag vf = row_frag<E, DIM>(vt, r0, kk, lane);
-#pragma unroll
-                    for (int ib = 0; ib < IB; ++ib) ds[b][ib] = E::mfma(vf, gf[ib][kk], ds[b][ib]);
-                }
+                f32x4 p[IB];
+                products(kt, vt, j0, r0, p, ds[b]);
 #pragma unroll
                 for (int ib = 0; ib < IB; ++ib) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = j0 + r0 + 4 * g + e;
-                        float x = p[b][ib][e] * f.scale2;
-                        if constexpr (BIAS) {
-                            const int far = j - (row0 + 16 * ib + l16 + offset);
-                            x += bias[min(max(far, -f.reach), f.reach) + f.reach];
-                        }
-                        float y = exp2_raw(x - lse[ib]) * (ds[b][ib][e] - delta[ib]);
-                        if (edge && j >= limit[ib]) y = 0.f;
-                        ds[b][ib][e] = y;
-                    }
+                    for (int e = 0; e < 4; ++e) ds[b][ib][e] = p[ib][e] * (ds[b][ib][e] - delta[ib]);
                     if constexpr (BIAS)
                         if (part) diagonal_sums(ds[b][ib], j0 + r0 - (row0 + 16 * ib + offset), f.reach, sums, low, high, lane);
                 }
@@ -328,37 +496,64 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         }
         lds_barrier();
         for (int i = threadIdx.x; i < width; i += 256) {
-            const float *q = bias + width + i;
+            const float *q = bias_row + width + i;
             part[i] = (q[0] + q[width]) + (q[2 * width] + q[3 * width]);
         }
     }
 }
 
-// dbias[h, i] = sum over the slots of part[slot, h, i].
+// dbias[i] = sum over the slots of part[slot][i]: 16 results per workgroup, 16
+// threads each.
 __global__ __launch_bounds__(256) void attention_bias_sum_kernel(const float *part, float *dbias, long long n, int slots) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float sum = 0.f;
-    for (int s = 0; s < slots; ++s) sum += part[s * n + i];
-    dbias[i] = sum;
+    __shared__ float sum[16][17];
+    const long long i = (long long)blockIdx.x * 16 + threadIdx.x % 16;
+    const int w = threadIdx.x / 16;
+    float s = 0.f;
+    if (i < n)
+        for (int p = w; p < slots; p += 16) s += part[p * n + i];
+    sum[w][threadIdx.x % 16] = s;
+    __syncthreads();
+    if (w || i >= n) return;
+#pragma unroll
+    for (int q = 1; q < 16; ++q) s += sum[q][threadIdx.x];
+    dbias[i] = s;
 }
 
-template <class E, int DIM>
-constexpr int row_blocks() { return E::kSize == 4 && DIM == 128 ? 1 : 2; }
+constexpr int query_blocks(int size, int dim) { return size == 4 && dim > 64 ? 1 : 2; }
 
-int query_rows(const bfhip_attention_desc *d) { return d->type == BFHIP_F32 && d->head_dim > 64 ? 64 : 128; }
+// How a call is dealt: slots of queries and of keys, and parts of the queries
+// that a tile of keys meets, so that uneven tiles even out over the CUs.
+struct BackwardPlan {
+    int dim, q_rows, k_rows, parts;
+    long long q_slots, k_slots;
+    size_t terms, part, part_kv;  // bytes
+};
 
-size_t terms_bytes(const bfhip_attention_desc *d) {
-    return ((size_t)d->heads * d->q_tokens * 2 * sizeof(float) + 255) / 256 * 256;
+BackwardPlan backward_plan(const bfhip_attention_desc *d) {
+    BackwardPlan p{};
+    const int size = d->type == BFHIP_F32 ? 4 : 2;
+    p.dim = d->head_dim <= 32 ? 32 : d->head_dim <= 64 ? 64 : 128;
+    p.q_rows = p.k_rows = 64 * query_blocks(size, p.dim);
+    p.q_slots = slot_count(d->q_tokens, d->sequences, p.q_rows);
+    p.k_slots = slot_count(d->k_tokens, d->sequences, p.k_rows);
+    const long long units = p.k_slots * d->kv_heads, parts = units ? 2048 / units : 1;
+    p.parts = (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
+    // No tile of keys meets more steps than these.
+    const long long steps = (d->q_tokens + kTile - 1) / kTile * (d->heads / d->kv_heads) / kPartSteps;
+    if (p.parts > steps) p.parts = steps < 1 ? 1 : (int)steps;
+    const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
+    p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float));
+    p.part = d->bias ? round((size_t)p.q_slots * d->heads * (2 * d->reach + 1) * sizeof(float)) : 0;
+    p.part_kv = p.parts > 1 ? (size_t)p.parts * d->k_tokens * d->kv_heads * 2 * p.dim * sizeof(float) : 0;
+    return p;
 }
 
 }  // namespace
 
 extern "C" size_t bfhip_attention_backward_workspace(const bfhip_attention_desc *d) {
     if (bad_attention(d)) return 0;
-    size_t n = terms_bytes(d);
-    if (d->bias) n += (size_t)slot_count(d->q_tokens, d->sequences, query_rows(d)) * d->heads * (2 * d->reach + 1) * sizeof(float);
-    return n;
+    const BackwardPlan p = backward_plan(d);
+    return 2 * p.terms + p.part + p.part_kv;
 }
 
 extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfhip_rows *q, const bfhip_rows *k,
@@ -372,52 +567,62 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         bad_rows(out, d->q_tokens, n, size) || bad_rows(dout, d->q_tokens, n, size) || bad_rows(dq, d->q_tokens, n, size) ||
         bad_rows(dk, d->k_tokens, n, size) || bad_rows(dv, d->k_tokens, n, size))
         return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim");
-    const size_t need = bfhip_attention_backward_workspace(d);
+    const BackwardPlan p = backward_plan(d);
+    const size_t need = 2 * p.terms + p.part + p.part_kv;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
+    const long long terms = (d->q_tokens * d->heads + 15) / 16, q_grid = p.q_slots * d->heads;
+    const long long k_grid = p.k_slots * d->kv_heads * p.parts;
+    const long long joins = p.parts > 1 ? ((long long)d->kv_heads * 2 * p.dim + 1023) / 1024 * d->k_tokens : 0;
+    if (!launch_fits(terms, 256) || !launch_fits(q_grid, 256) || !launch_fits(k_grid, 256) || !launch_fits(joins, 256))
+        return fail(error, cap, "attention has too many rows");
     GradArgs a{};
     a.f = attn_args(d, q, k, v, out, const_cast<float *>(lse));
+    a.f.parts = p.parts;
     a.dout = attn_rows(dout, d->q_tokens, n, size);
     a.dq = attn_rows(dq, d->q_tokens, n, size);
     a.dk = attn_rows(dk, d->k_tokens, n, size);
     a.dv = attn_rows(dv, d->k_tokens, n, size);
-    a.lse2 = (float *)workspace;
-    a.delta = a.lse2 + (size_t)d->heads * d->q_tokens;
-    a.part = dbias ? (float *)((char *)workspace + terms_bytes(d)) : nullptr;
+    char *const work = (char *)workspace;
+    a.nlse = (float *)work;
+    a.delta = (float *)(work + p.terms);
+    a.part = dbias ? (float *)(work + 2 * p.terms) : nullptr;
+    a.part_kv = (float *)(work + 2 * p.terms + p.part);
     hipStream_t s = (hipStream_t)stream;
-    const long long terms = (d->q_tokens * d->heads + 15) / 16, width = 2 * a.f.reach + 1;
-    int ok = launch_fits(terms, 256);
-    long long q_slots = 0;
-    with_element(d->type, [&](auto e) {
-        with_dim(n, [&](auto dim) {
-            using E = decltype(e);
-            constexpr int DIM = decltype(dim)::value, RB = row_blocks<E, DIM>();
-            q_slots = slot_count(d->q_tokens, d->sequences, 64 * RB);
-            const long long q_grid = q_slots * d->heads;
-            const long long k_grid = slot_count(d->k_tokens, d->sequences, 64 * RB) * d->kv_heads;
-            ok = ok && launch_fits(q_grid, 256) && launch_fits(k_grid, 256);
-            if (!ok) return;
-            const size_t tiles = 2 * kTile * AttnTile<E, DIM>::kRow, terms_lds = 2 * kTile * sizeof(float);
-            if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);
-            const auto run = [&](auto with_bias) {
-                constexpr bool B = decltype(with_bias)::value;
-                const size_t row = B ? width * sizeof(float) : 0;
-                if (d->k_tokens && d->sequences)
-                    hipLaunchKernelGGL((attention_keys_kernel<E, DIM, RB, B>), dim3((unsigned)k_grid), dim3(256),
-                                       tiles + terms_lds + row, s, a);
-                if (d->q_tokens && d->sequences)
-                    hipLaunchKernelGGL((attention_queries_kernel<E, DIM, RB, B>), dim3((unsigned)q_grid), dim3(256),
-                                       tiles + (a.part ? 5 : 1) * row, s, a);
-            };
-            if (d->bias) run(std::true_type{});
-            else run(std::false_type{});
+    const long long width = 2 * a.f.reach + 1;
+    if (d->sequences)
+        with_element(d->type, [&](auto e) {
+            with_dim(n, [&](auto dim) {
+                using E = decltype(e);
+                constexpr int DIM = decltype(dim)::value, QB = query_blocks(E::kSize, DIM), KB = QB, WAVES = 4;
+                using K = KeyTile<E, DIM, KB, WAVES>;
+                using T = AttnTile<E, DIM>;
+                if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);
+                const auto run = [&](auto with_bias) {
+                    constexpr bool B = decltype(with_bias)::value;
+                    const size_t row = B ? width * sizeof(float) : 0;
+                    GradArgs b = a;
+                    if (d->q_tokens) {
+                        b.f.slots = (int)p.q_slots;
+                        hipLaunchKernelGGL((attention_queries_kernel<E, DIM, QB, B>), dim3((unsigned)q_grid), dim3(256),
+                                           4 * tile_keys(E::kSize, DIM) * T::kRow + (a.part ? 5 : 1) * row, s, b);
+                    }
+                    if (d->k_tokens) {
+                        b.f.slots = (int)p.k_slots;
+                        hipLaunchKernelGGL((attention_keys_kernel<E, DIM, KB, WAVES, B>), dim3((unsigned)k_grid),
+                                           dim3(K::kThreads), 2 * K::kStage + row, s, b);
+                    }
+                };
+                if (d->bias) run(std::true_type{});
+                else run(std::false_type{});
+                if (joins)
+                    hipLaunchKernelGGL((attention_keys_join_kernel<E, DIM, K::kRows>), dim3((unsigned)joins), dim3(256), 0, s, a);
+            });
         });
-    });
-    if (!ok) return fail(error, cap, "attention has too many rows");
     if (dbias) {
         const long long count = width * d->heads;
-        hipLaunchKernelGGL(attention_bias_sum_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, a.part,
-                           dbias, count, d->q_tokens && d->sequences ? (int)q_slots : 0);
+        hipLaunchKernelGGL(attention_bias_sum_kernel, dim3((unsigned)((count + 15) / 16)), dim3(256), 0, s, a.part, dbias,
+                           count, d->q_tokens && d->sequences ? (int)p.q_slots : 0);
     }
     return launch_ok(error, cap, "attention launch");
 }

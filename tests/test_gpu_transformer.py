@@ -213,6 +213,10 @@ CASES = [
     (BF16, 2, 2, 64, [150], [5000], True, 300),
     (F32, 3, 1, 96, [70, 1], [3000, 40], False, 9),
     (BF16, 32, 4, 80, [1, 1, 2, 0], [0, 1, 6000, 77], True, 5),
+    # The longest bias beside the largest rows; queries of a key tile in parts.
+    (F32, 2, 1, 128, [70, 5], [90, 300], False, 2047),
+    (BF16, 8, 1, 128, [1500, 40], None, True, 2047),
+    (F16, 8, 2, 32, [2100], [700], False, None),
 ]
 
 
