@@ -103,10 +103,9 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4, group = f.heads / f.kv_heads;
     const int items = f.slots * f.kv_heads, part = blockIdx.x / items;
-    // In causal sequences the first keys are seen by the most queries.
-    const Deal deal_ = deal(blockIdx.x % items, f.slots, f.kv_heads, f.kv_heads);
+    const Deal deal_ = deal(blockIdx.x % items, f.kv_heads, f.kv_heads);
     const int kv = deal_.head;
-    const Slot s = find_rows<kRows>(f.k_starts, f.sequences, f.k_tokens, f.slots - 1 - deal_.slot);
+    const Slot s = ranked_rows<kRows, true>(f.k_starts, f.sequences, f.k_tokens, deal_.rank, f.slots, f.causal);
     if (s.sequence < 0) return;
     int q_start, q_len;
     sequence_rows(f.q_starts, s.sequence, f.q_tokens, q_start, q_len);
@@ -165,6 +164,9 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         }
         // A query that does not see every key of the wave's.
         const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
+        // Scores of the whole tile first: the compiler waits for the copies in
+        // flight before the transposed reads, which by then have had the time.
+        typename E::Frag pf[2][KB], sf[2][KB];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             f32x4 p[2][KB], ds[2][KB];
@@ -203,28 +205,37 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float x = exp2_raw(fmaf(p[b][kb][e], f.scale2, add[e]));
-                        float y = x * (ds[b][kb][e] - delta[e]);
-                        if (edge && far0 + l16 > 4 * g + e) x = y = 0.f;
-                        p[b][kb][e] = x;
-                        ds[b][kb][e] = y;
+                        p[b][kb][e] = exp2_raw(fmaf(p[b][kb][e], f.scale2, add[e]));
+                        ds[b][kb][e] = p[b][kb][e] * (ds[b][kb][e] - delta[e]);
                     }
                 }
             }
-            typename E::Frag pf[KB], sf[KB];
+            if (edge) {
+                const int far = key0 + l16 - (i0 + 32 * c + 4 * g + offset);
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (far > 16 * (b - kb) + e) p[b][kb][e] = ds[b][kb][e] = 0.f;
+            }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                pf[kb] = to_frag<E>(p[0][kb], p[1][kb]);
-                sf[kb] = to_frag<E>(ds[0][kb], ds[1][kb]);
+                pf[c][kb] = to_frag<E>(p[0][kb], p[1][kb]);
+                sf[c][kb] = to_frag<E>(ds[0][kb], ds[1][kb]);
             }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int db = 0; db < kDB; ++db) {
                 const typename E::Frag gf = col_frag<E, DIM>(gt, 32 * c, db, lane);
                 const typename E::Frag qf = col_frag<E, DIM>(qt, 32 * c, db, lane);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    dv[kb][db] = E::mfma(gf, pf[kb], dv[kb][db]);
-                    dk[kb][db] = E::mfma(qf, sf[kb], dk[kb][db]);
+                    dv[kb][db] = E::mfma(gf, pf[c][kb], dv[kb][db]);
+                    dk[kb][db] = E::mfma(qf, sf[c][kb], dk[kb][db]);
                 }
             }
         }
@@ -327,10 +338,10 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     const AttnArgs &f = a.f;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4;
-    const Deal deal_ = deal(blockIdx.x, f.slots, f.heads, f.kv_heads);
+    const Deal deal_ = deal(blockIdx.x, f.heads, f.kv_heads);
     const int head = deal_.head, kv = head / (f.heads / f.kv_heads), width = 2 * f.reach + 1;
-    const Slot s = find_rows<kRows>(f.q_starts, f.sequences, f.q_tokens, deal_.slot);
-    float *const part = BIAS && a.part ? a.part + ((size_t)deal_.slot * f.heads + head) * width : nullptr;
+    const Slot s = ranked_rows<kRows, false>(f.q_starts, f.sequences, f.q_tokens, deal_.rank, f.slots, f.causal);
+    float *const part = BIAS && a.part ? a.part + ((size_t)deal_.rank * f.heads + head) * width : nullptr;
     if (s.sequence < 0) {
         if (part)
             for (int i = threadIdx.x; i < width; i += 256) part[i] = 0.f;
@@ -396,7 +407,6 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib) dp[ib] = E::mfma(vf, gf[ib][kk], dp[ib]);
         }
-        const bool edge = j0 + kKeys > full;
 #pragma unroll
         for (int ib = 0; ib < IB; ++ib) {
             const int far0 = j0 + r0 - (row0 + 16 * ib + offset);
@@ -411,10 +421,15 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, add[e]));
-                if (edge && j0 + r0 + 4 * g + e >= limit[ib]) p[ib][e] = dp[ib][e] = 0.f;
-            }
+            for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, add[e]));
+        }
+        if (j0 + r0 + 16 > full) {
+            const int j = j0 + r0 + 4 * g;
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j + e >= limit[ib]) p[ib][e] = dp[ib][e] = 0.f;
         }
     };
     int buffer = 0;
@@ -456,6 +471,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         if (t + 1 < tiles) issue(t + 1, buffer ^ 1);
         const char *const kt = smem + buffer * kStage, *const vt = kt + kKeys * T::kRow;
         const int j0 = t * kKeys;
+        typename E::Frag sf[kKeys / 32][IB];  // (the whole tile first, as above)
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {
             f32x4 ds[2][IB];
@@ -473,11 +489,15 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 }
             }
 #pragma unroll
-            for (int ib = 0; ib < IB; ++ib) {
-                const typename E::Frag sf = to_frag<E>(ds[0][ib], ds[1][ib]);
+            for (int ib = 0; ib < IB; ++ib) sf[c][ib] = to_frag<E>(ds[0][ib], ds[1][ib]);
+        }
 #pragma unroll
-                for (int db = 0; db < kDB; ++db)
-                    dq[ib][db] = E::mfma(col_frag<E, DIM>(kt, 32 * c, db, lane), sf, dq[ib][db]);
+        for (int c = 0; c < kKeys / 32; ++c) {
+#pragma unroll
+            for (int db = 0; db < kDB; ++db) {
+                const typename E::Frag kf = col_frag<E, DIM>(kt, 32 * c, db, lane);
+#pragma unroll
+                for (int ib = 0; ib < IB; ++ib) dq[ib][db] = E::mfma(kf, sf[c][ib], dq[ib][db]);
             }
         }
     }
@@ -538,8 +558,8 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     p.k_slots = slot_count(d->k_tokens, d->sequences, p.k_rows);
     const long long units = p.k_slots * d->kv_heads, parts = units ? 2048 / units : 1;
     p.parts = (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
-    // No tile of keys meets more steps than these.
-    const long long steps = (d->q_tokens + kTile - 1) / kTile * (d->heads / d->kv_heads) / kPartSteps;
+    // As many as the average sequence has queries for.
+    const long long steps = d->sequences ? d->q_tokens / d->sequences / kTile * (d->heads / d->kv_heads) / kPartSteps : 0;
     if (p.parts > steps) p.parts = steps < 1 ? 1 : (int)steps;
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float));
@@ -594,7 +614,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         with_element(d->type, [&](auto e) {
             with_dim(n, [&](auto dim) {
                 using E = decltype(e);
-                constexpr int DIM = decltype(dim)::value, QB = query_blocks(E::kSize, DIM), KB = QB, WAVES = 4;
+                constexpr int DIM = decltype(dim)::value, QB = query_blocks(E::kSize, DIM), WAVES = E::kSize == 2 && DIM == 128 ? 8 : 4, KB = 64 * QB / (16 * WAVES);
                 using K = KeyTile<E, DIM, KB, WAVES>;
                 using T = AttnTile<E, DIM>;
                 if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);

@@ -109,9 +109,9 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4;
     const int items = a.slots * a.heads, part = blockIdx.x / items;
-    const Deal deal_ = deal(blockIdx.x % items, a.slots, a.heads, a.kv_heads);
+    const Deal deal_ = deal(blockIdx.x % items, a.heads, a.kv_heads);
     const int head = deal_.head, kv = head / (a.heads / a.kv_heads);
-    const Slot s = find_rows<kRows>(a.q_starts, a.sequences, a.q_tokens, deal_.slot);
+    const Slot s = ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.causal);
     if (s.sequence < 0) return;
     int k_start, k_len;
     sequence_rows(a.k_starts, s.sequence, a.k_tokens, k_start, k_len);
@@ -194,13 +194,14 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
             }
         }
         if (j0 + kKeys > full) {
+            const int j = j0 + 4 * g;
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib)
 #pragma unroll
                 for (int jb = 0; jb < 4; ++jb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        sc[jb][ib][e] = j0 + 16 * jb + 4 * g + e < limit[ib] ? sc[jb][ib][e] : -INFINITY;
+                        sc[jb][ib][e] = j + 16 * jb + e < limit[ib] ? sc[jb][ib][e] : -INFINITY;
         }
         run.template take<4>(sc, scale, add);
 #pragma unroll
@@ -338,10 +339,11 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
                     }
             }
             if (j0 + kKeyRows > full) {
+                const int j = j0 + 4 * g;
 #pragma unroll
                 for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[jb][0][e] = j0 + 16 * jb + 4 * g + e < limit ? sc[jb][0][e] : -INFINITY;
+                    for (int e = 0; e < 4; ++e) sc[jb][0][e] = j + 16 * jb + e < limit ? sc[jb][0][e] : -INFINITY;
             }
             run.template take<2>(sc, BIAS ? 1.f : a.scale2, {0.f});
             const typename E::Frag pf = to_frag<E>(sc[0][0], sc[1][0]);
