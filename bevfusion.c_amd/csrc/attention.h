@@ -28,6 +28,7 @@ struct AttnArgs {
     float scale, scale2;  // scale2 = scale * log2(e): softmax runs in base 2
     int slots;            // of the grid
     int flip;             // the queries' signs change (forward)
+    int ordered;          // tiles in the order of their work
     int parts;            // most parts that a sequence's keys are split into
     int chunk;            // keys of a part, at least (few queries)
     float *part_out;      // parts > 1: sums of each part, [parts][q_tokens][heads][padded dim]
@@ -112,12 +113,11 @@ __device__ __forceinline__ Slot find_rows(const int *starts, int sequences, long
 // sequences a tile's work grows with its place in its sequence, from the front
 // (queries: the keys before them) or the back (keys: the queries after them):
 // rank 0 is the last (first) tile of the longest sequence, and the tiles of one
-// level come one after the other.  The search has a lane per sequence; with more
-// than 64 of them, or without a mask, tiles come in the rows' own order.
-// (forward, 8192 + 4097 + .. tokens, 32 heads of 128: 737 us in the rows' order.)
+// level come one after the other.  The search has a lane per sequence.
+// Where `ordered` says no (by_work below), tiles come in the rows' own order.
 template <int ROWS, bool FRONT>
-__device__ __forceinline__ Slot ranked_rows(const int *starts, int sequences, long long tokens, int rank, int slots, int causal) {
-    if (!causal || sequences > kWave) return find_rows<ROWS>(starts, sequences, tokens, FRONT ? rank : slots - 1 - rank);
+__device__ __forceinline__ Slot ranked_rows(const int *starts, int sequences, long long tokens, int rank, int slots, int ordered) {
+    if (!ordered) return find_rows<ROWS>(starts, sequences, tokens, FRONT ? rank : slots - 1 - rank);
     const int lane = threadIdx.x % kWave;
     int start = 0, length = 0;
     if (lane < sequences) {
@@ -412,6 +412,15 @@ inline AttnArgs attn_args(const bfhip_attention_desc *d, const bfhip_rows *q, co
     a.scale = d->scale;
     a.scale2 = d->scale * kLog2E;
     return a;
+}
+
+// Whether tiles are dealt in the order of their work: up to four rounds of two
+// workgroups per CU, where the last round's tail counts (forward of 4096 + 2049
+// + .. causal tokens, 16 heads of 128, 1104 workgroups: 124 us, 149 in the rows'
+// order); in more rounds the rows' order reads keys while the XCD's L2 still
+// has them (8192 + 4097 + .. tokens, 32 heads, 4352 workgroups: 761 us, 741).
+inline int by_work(const bfhip_attention_desc *d, long long workgroups) {
+    return d->causal && d->sequences <= kWave && workgroups <= 2048;
 }
 
 // Calls f with the padded head size.

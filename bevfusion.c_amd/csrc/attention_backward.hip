@@ -105,7 +105,7 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
     const int items = f.slots * f.kv_heads, part = blockIdx.x / items;
     const Deal deal_ = deal(blockIdx.x % items, f.kv_heads, f.kv_heads);
     const int kv = deal_.head;
-    const Slot s = ranked_rows<kRows, true>(f.k_starts, f.sequences, f.k_tokens, deal_.rank, f.slots, f.causal);
+    const Slot s = ranked_rows<kRows, true>(f.k_starts, f.sequences, f.k_tokens, deal_.rank, f.slots, f.ordered);
     if (s.sequence < 0) return;
     int q_start, q_len;
     sequence_rows(f.q_starts, s.sequence, f.q_tokens, q_start, q_len);
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     const int l16 = lane & 15, g = lane >> 4;
     const Deal deal_ = deal(blockIdx.x, f.heads, f.kv_heads);
     const int head = deal_.head, kv = head / (f.heads / f.kv_heads), width = 2 * f.reach + 1;
-    const Slot s = ranked_rows<kRows, false>(f.q_starts, f.sequences, f.q_tokens, deal_.rank, f.slots, f.causal);
+    const Slot s = ranked_rows<kRows, false>(f.q_starts, f.sequences, f.q_tokens, deal_.rank, f.slots, f.ordered);
     float *const part = BIAS && a.part ? a.part + ((size_t)deal_.rank * f.heads + head) * width : nullptr;
     if (s.sequence < 0) {
         if (part)
@@ -624,11 +624,13 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                     GradArgs b = a;
                     if (d->q_tokens) {
                         b.f.slots = (int)p.q_slots;
+                        b.f.ordered = by_work(d, q_grid);
                         hipLaunchKernelGGL((attention_queries_kernel<E, DIM, QB, B>), dim3((unsigned)q_grid), dim3(256),
                                            4 * tile_keys(E::kSize, DIM) * T::kRow + (a.part ? 5 : 1) * row, s, b);
                     }
                     if (d->k_tokens) {
                         b.f.slots = (int)p.k_slots;
+                        b.f.ordered = by_work(d, k_grid);
                         hipLaunchKernelGGL((attention_keys_kernel<E, DIM, KB, WAVES, B>), dim3((unsigned)k_grid),
                                            dim3(K::kThreads), 2 * K::kStage + row, s, b);
                     }

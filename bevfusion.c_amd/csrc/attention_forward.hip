@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     const int items = a.slots * a.heads, part = blockIdx.x / items;
     const Deal deal_ = deal(blockIdx.x % items, a.heads, a.kv_heads);
     const int head = deal_.head, kv = head / (a.heads / a.kv_heads);
-    const Slot s = ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.causal);
+    const Slot s = ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.ordered);
     if (s.sequence < 0) return;
     int k_start, k_len;
     sequence_rows(a.k_starts, s.sequence, a.k_tokens, k_start, k_len);
@@ -543,6 +543,7 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
     a.slots = (int)p.slots;
     a.parts = p.parts;
     a.chunk = p.chunk;
+    a.ordered = by_work(d, p.grid);
     // Scores are compared before they are scaled, which takes a positive scale:
     // a negative one flips the queries' signs, and zero becomes one so small
     // that it makes no score differ.
