@@ -189,15 +189,23 @@ __device__ __forceinline__ int part_tiles(int tiles, int parts, int least) {
 
 // ------------------------------------------------------------- operand tiles
 // A tile of ROWS rows x DIM elements in LDS, in 16-byte chunks: chunk c of row
-// r sits at chunk c ^ swizzle(r) of its row, so that the sixteen rows a
-// fragment reads at the same c spread over all banks.
+// r sits at chunk c ^ swizzle(r) of its row.  16-byte reads are served for the
+// rows 0-3 and 12-15 of one lane group together with the rows 4-11 of the next,
+// which reads chunk c ^ 1; a transposing read of 16-bit words takes two
+// neighbouring chunks of eight neighbouring rows.  With x the row's number among
+// those that share their banks, t its highest bit and s the one below, the
+// swizzle (s ^ t, the bits below s, t) puts either set on all banks (x itself
+// and x turned by one bit each leave one of them two-way conflicts).
 template <class E, int DIM>
 struct AttnTile {
     static constexpr int kRow = DIM * E::kSize;  // bytes
     static constexpr int kChunks = kRow / 16;
     __device__ __forceinline__ static int swizzle(int r) {
         constexpr int per = kRow >= 256 ? 1 : 256 / kRow;  // rows in one pass over the banks
-        return r / per & ((kChunks < 16 ? kChunks : 16) - 1);
+        constexpr int n = kChunks < 16 ? kChunks : 16;
+        const int x = r / per & (n - 1);
+        const int t = x / (n / 2);
+        return E::kSize == 2 ? ((x ^ t * (n / 4)) << 1 & (n - 1)) | t : x;
     }
 };
 
