@@ -320,6 +320,34 @@ __device__ __forceinline__ void col_frags_in_flight(const char *lds, int lane, t
     }
 }
 
+// A head's bias row in LDS, times log2 e, with its ends repeated kPad times so
+// that a block of 16 x 16 scores that meets distances within the reach is read
+// without clamping.
+struct BiasRow {
+    static constexpr int kPad = 32;
+    const float *zero;  // the bias of distance 0
+    int reach;
+    __host__ __device__ __forceinline__ static int floats(int reach) { return 2 * (reach + kPad) + 1; }
+    // Copies `bias` [2 reach + 1] to `lds` (the caller waits).
+    __device__ __forceinline__ static BiasRow fill(float *lds, const float *bias, int reach, int thread, int threads) {
+        for (int i = thread; i < floats(reach); i += threads) lds[i] = bias[min(max(i - kPad, 0), 2 * reach)] * kLog2E;
+        return BiasRow{lds + reach + kPad, reach};
+    }
+    // Of the four distances from `far` on; far is at most kPad beyond the reach.
+    __device__ __forceinline__ f32x4 four(int far) const {
+        f32x4 v;
+        __builtin_memcpy(&v, zero + far, sizeof v);
+        return v;
+    }
+    // Whether all distances of low .. high have one bias; `value` is it.
+    __device__ __forceinline__ bool one(int low, int high, float &value) const {
+        if (high <= -reach) value = zero[-reach];
+        else if (low >= reach) value = zero[reach];
+        else return false;
+        return true;
+    }
+};
+
 // Fragment of 16 rows in global memory (row 0 at `base`): elements 32 kk ..+31.
 // Rows past `rows` and elements past dim are zero.
 template <class E>

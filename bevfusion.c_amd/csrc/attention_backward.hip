@@ -68,21 +68,6 @@ __device__ __forceinline__ Steps query_steps(int causal, int first_key, int offs
     return s;
 }
 
-// Bias and scale of one lane's four scores: the biases are looked up where
-// distances within the reach occur, else all have one.
-struct BiasRow {
-    const float *row;  // times log2 e
-    int reach;
-    __device__ __forceinline__ float at(int far) const { return row[min(max(far, -reach), reach) + reach]; }
-    // 1: all distances of low .. high are beyond the reach; `value` is theirs.
-    __device__ __forceinline__ bool one(int low, int high, float &value) const {
-        if (high <= -reach) value = row[0];
-        else if (low >= reach) value = row[2 * reach];
-        else return false;
-        return true;
-    }
-};
-
 template <class E, int DIM, int KB, int WAVES>
 struct KeyTile {
     static constexpr int kRows = WAVES * 16 * KB, kThreads = WAVES * kWave;
@@ -155,11 +140,9 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         if constexpr (BIAS) {
             if (hg != bias_head) {
                 bias_head = hg;
-                float *const row = reinterpret_cast<float *>(smem + 2 * K::kStage);
-                const float *b = f.bias + (size_t)(kv * group + hg) * (2 * f.reach + 1);
-                for (int i = threadIdx.x; i <= 2 * f.reach; i += kThreads) row[i] = b[i] * kLog2E;
+                bias = BiasRow::fill(reinterpret_cast<float *>(smem + 2 * K::kStage),
+                                     f.bias + (size_t)(kv * group + hg) * (2 * f.reach + 1), f.reach, threadIdx.x, kThreads);
                 lds_barrier();
-                bias = BiasRow{row, f.reach};
             }
         }
         // A query that does not see every key of the wave's.
@@ -199,8 +182,8 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                         if (bias.one(far0 - 15, far0 + 15, one)) {
                             add += one;
                         } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) add[e] += bias.at(far0 + l16 - 4 * g - e);
+                            const f32x4 b4 = bias.four(far0 + l16 - 4 * g - 3);
+                            add += __builtin_shufflevector(b4, b4, 3, 2, 1, 0);
                         }
                     }
 #pragma unroll
@@ -290,11 +273,22 @@ __global__ __launch_bounds__(256) void attention_keys_join_kernel(GradArgs a) {
     w.store(reinterpret_cast<typename E::Word *>((is_k ? a.dk : a.dv).at(token, kv)) + e0);
 }
 
+// The value of the lane N places on (SHL) or back (SHR) in the row of 16, 0
+// past its ends.
+template <bool SHL, int N>
+__device__ __forceinline__ float row_shift(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), (SHL ? 0x100 : 0x110) + N, 0xf, 0xf, true));
+}
+
 // Sums of a 16 x 16 block of dS^T along its diagonals into `sum` (this wave's
-// own array): the lane (query i, group g) holds keys 4 g + e, so for one e the
-// lanes (i + 4 n, g + n) lie on one diagonal; two shuffles add them up in the
-// lane that starts the diagonal, and no two such lanes share an address.
-// Distances at or beyond the reach are left to the caller's low and high sums.
+// own array).  Lane (query i, group g) holds the keys 4 g + e, distance far0 +
+// 4 g + e - i.  Within a group, shifts along the row of lanes add the four e up
+// where the diagonal meets e = 0 (`main`) and, for the three diagonals that
+// begin left of it, in the last lanes (`rest`).  The groups' lanes (i + 4 n, g +
+// n) lie on one diagonal: two shuffles add them in the lane that starts it.
+// Either write is then to addresses of one lane each, in the wave's order, so
+// the sums' order is fixed.  Distances at or beyond the reach are left to the
+// caller's low and high sums.
 __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int reach, float *sum, float &low, float &high,
                                               int lane) {
     const int i = lane & 15, g = lane >> 4;
@@ -306,19 +300,19 @@ __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int rea
         high += (ds[0] + ds[1]) + (ds[2] + ds[3]);
         return;
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        float v = ds[e], w = __shfl(v, (lane + 20) & 63);
-        if (g < 3 && i < 12) v += w;
-        w = __shfl(v, (lane + 40) & 63);
-        if (g < 2 && i < 8) v += w;
-        if (g == 0 || i < 4) {
-            const int far = far0 + 4 * g + e - i;
-            if (far <= -reach) low += v;
-            else if (far >= reach) high += v;
-            else __hip_atomic_fetch_add(sum + far + reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-    }
+    float main = (ds[0] + row_shift<true, 1>(ds[1])) + (row_shift<true, 2>(ds[2]) + row_shift<true, 3>(ds[3]));
+    const float rest = row_shift<false, 15>(ds[1]) + row_shift<false, 14>(ds[2]) + row_shift<false, 13>(ds[3]);
+    float next = __shfl(main, (lane + 20) & 63);
+    if (g < 3 && i < 12) main += next;
+    next = __shfl(main, (lane + 40) & 63);
+    if (g < 2 && i < 8) main += next;
+    const auto add = [&](int far, float v) {
+        if (far <= -reach) low += v;
+        else if (far >= reach) high += v;
+        else __hip_atomic_fetch_add(sum + far + reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    if (g == 0 || i < 4) add(far0 + 4 * g - i, main);
+    if (i >= 13) add(far0 + 4 * g + 16 - i, rest);
 }
 
 // Keys per tile: two tiles of keys and values, and five rows of the longest
@@ -363,14 +357,13 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         kc.issue(f.k.at((long long)k_start + j0, kv), k_len - j0, to);
         vc.issue(f.v.at((long long)k_start + j0, kv), k_len - j0, to + kKeys * T::kRow);
     };
-    float *const sums = bias_row + width * (1 + wave);
+    float *const sums = bias_row + BiasRow::floats(f.reach) + width * wave;
+    BiasRow bias{};
     if constexpr (BIAS) {
-        const float *b = f.bias + (size_t)head * width;
-        for (int i = threadIdx.x; i < width; i += 256) bias_row[i] = b[i] * kLog2E;
+        bias = BiasRow::fill(bias_row, f.bias + (size_t)head * width, f.reach, threadIdx.x, 256);
         if (part)
             for (int i = lane; i < width; i += kWave) sums[i] = 0.f;
     }
-    const BiasRow bias{bias_row, f.reach};
 
     typename E::Frag qf[IB][kKB], gf[IB][kKB];
     f32x4 dq[IB][kDB];
@@ -416,8 +409,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 if (bias.one(far0 - 15, far0 + 15, one)) {
                     add += one;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) add[e] += bias.at(far0 + 4 * g + e - l16);
+                    add += bias.four(far0 + 4 * g - l16);
                 }
             }
 #pragma unroll
@@ -484,10 +476,20 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 for (int ib = 0; ib < IB; ++ib) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ds[b][ib][e] = p[ib][e] * (ds[b][ib][e] - delta[ib]);
-                    if constexpr (BIAS)
-                        if (part) diagonal_sums(ds[b][ib], j0 + r0 - (row0 + 16 * ib + offset), f.reach, sums, low, high, lane);
                 }
             }
+            if constexpr (BIAS)
+                if (part) {
+                    // Blocks on one diagonal first.
+                    const int far0 = j0 + 32 * c - (row0 + offset);
+                    if constexpr (IB == 1) {
+                        diagonal_sums(ds[0][0], far0, f.reach, sums, low, high, lane);
+                    } else {
+                        diagonal_sums(ds[0][0] + ds[1][1], far0, f.reach, sums, low, high, lane);
+                        diagonal_sums(ds[0][1], far0 - 16, f.reach, sums, low, high, lane);
+                    }
+                    diagonal_sums(ds[1][0], far0 + 16, f.reach, sums, low, high, lane);
+                }
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib) sf[c][ib] = to_frag<E>(ds[0][ib], ds[1][ib]);
         }
@@ -516,7 +518,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         }
         lds_barrier();
         for (int i = threadIdx.x; i < width; i += 256) {
-            const float *q = bias_row + width + i;
+            const float *q = bias_row + BiasRow::floats(f.reach) + i;
             part[i] = (q[0] + q[width]) + (q[2 * width] + q[3 * width]);
         }
     }
@@ -620,13 +622,13 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                 if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);
                 const auto run = [&](auto with_bias) {
                     constexpr bool B = decltype(with_bias)::value;
-                    const size_t row = B ? width * sizeof(float) : 0;
+                    const size_t row = B ? BiasRow::floats(d->reach) * sizeof(float) : 0;
                     GradArgs b = a;
                     if (d->q_tokens) {
                         b.f.slots = (int)p.q_slots;
                         b.f.ordered = by_work(d, q_grid);
                         hipLaunchKernelGGL((attention_queries_kernel<E, DIM, QB, B>), dim3((unsigned)q_grid), dim3(256),
-                                           4 * tile_keys(E::kSize, DIM) * T::kRow + (a.part ? 5 : 1) * row, s, b);
+                                           4 * tile_keys(E::kSize, DIM) * T::kRow + row + (a.part ? 4 * width * sizeof(float) : 0), s, b);
                     }
                     if (d->k_tokens) {
                         b.f.slots = (int)p.k_slots;

@@ -105,7 +105,6 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     using T = AttnTile<E, DIM>;
     constexpr int kStage = 2 * kKeys * T::kRow;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float *const bias = reinterpret_cast<float *>(smem + 2 * kStage);
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4;
     const int items = a.slots * a.heads, part = blockIdx.x / items;
@@ -133,10 +132,10 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
         kc.issue(a.k.at((long long)k_start + j0, kv), k_len - j0, to);
         vc.issue(a.v.at((long long)k_start + j0, kv), k_len - j0, to + kKeys * T::kRow);
     };
-    if constexpr (BIAS) {
-        const float *b = a.bias + (size_t)head * (2 * a.reach + 1);
-        for (int i = threadIdx.x; i <= 2 * a.reach; i += 256) bias[i] = b[i] * kLog2E;
-    }
+    BiasRow bias{};
+    if constexpr (BIAS)
+        bias = BiasRow::fill(reinterpret_cast<float *>(smem + 2 * kStage), a.bias + (size_t)head * (2 * a.reach + 1),
+                             a.reach, threadIdx.x, 256);
     typename E::Frag qf[IB][kKB];
     int limit[IB];  // keys that the lane's query sees
 #pragma unroll
@@ -174,23 +173,24 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
         for (int ib = 0; ib < IB; ++ib) add[ib] = 0.f;
         if constexpr (BIAS) {
             // Beyond the reach on either side all distances have one bias;
-            // nearer ones are looked up score by score.
+            // nearer ones are looked up.
             const int far0 = j0 - (row0 + offset);  // key 0 of the tile, query 0 of the wave
-            const bool low = far0 + kKeys - 1 <= -a.reach, high = far0 - (16 * IB - 1) >= a.reach;
-            if (low || high) {
+            float one;
+            if (bias.one(far0 - (16 * IB - 1), far0 + kKeys - 1, one)) {
 #pragma unroll
-                for (int ib = 0; ib < IB; ++ib) add[ib] = bias[low ? 0 : 2 * a.reach];
+                for (int ib = 0; ib < IB; ++ib) add[ib] = one;
             } else {
                 scale = 1.f;
 #pragma unroll
                 for (int ib = 0; ib < IB; ++ib)
 #pragma unroll
-                    for (int jb = 0; jb < 4; ++jb)
+                    for (int jb = 0; jb < 4; ++jb) {
+                        const int far = far0 + 16 * (jb - ib);
+                        const f32x4 b = bias.one(far - 15, far + 15, one) ? f32x4{one, one, one, one}
+                                                                          : bias.four(far + 4 * g - l16);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int far = far0 + 16 * (jb - ib) + 4 * g + e - l16;
-                            sc[jb][ib][e] = fmaf(sc[jb][ib][e], a.scale2, bias[min(max(far, -a.reach), a.reach) + a.reach]);
-                        }
+                        for (int e = 0; e < 4; ++e) sc[jb][ib][e] = fmaf(sc[jb][ib][e], a.scale2, b[e]);
+                    }
             }
         }
         if (j0 + kKeys > full) {
@@ -561,7 +561,7 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
             using T = AttnTile<E, DIM>;
             const auto run = [&](auto bias) {
                 constexpr bool B = decltype(bias)::value;
-                const size_t lds = 4 * kKeys * T::kRow + (B ? (2 * d->reach + 1) * sizeof(float) : 0);
+                const size_t lds = 4 * kKeys * T::kRow + (B ? BiasRow::floats(d->reach) * sizeof(float) : 0);
                 if (p.few) hipLaunchKernelGGL((attention_few_kernel<E, DIM, B>), grid, dim3(Few::kThreads), 0, s, a);
                 else hipLaunchKernelGGL((attention_forward_kernel<E, DIM, IB, B>), grid, dim3(256), lds, s, a);
             };
