@@ -30,7 +30,7 @@ struct AttnArgs {
     int flip;             // the queries' signs change (forward)
     int ordered;          // tiles in the order of their work
     int parts;            // most parts that a sequence's keys are split into
-    int chunk;            // keys of a part, at least (few queries)
+    int chunk;            // keys (few queries) or steps (backward) of a part, at least
     float *part_out;      // parts > 1: sums of each part, [parts][q_tokens][heads][padded dim]
     float2 *part_stat;    // and their (m, l), [parts][q_tokens][heads]
 };
@@ -333,18 +333,17 @@ struct BiasRow {
         for (int i = thread; i < floats(reach); i += threads) lds[i] = bias[min(max(i - kPad, 0), 2 * reach)] * kLog2E;
         return BiasRow{lds + reach + kPad, reach};
     }
-    // Of the four distances from `far` on; far is at most kPad beyond the reach.
-    __device__ __forceinline__ f32x4 four(int far) const {
+    // Of the four distances from `at` on, in a block of 16 x 16 scores with the
+    // distances far0 - 15 .. far0 + 15.  Beyond the reach all have one bias.
+    __device__ __forceinline__ f32x4 block(int far0, int at) const {
         f32x4 v;
-        __builtin_memcpy(&v, zero + far, sizeof v);
+        if (far0 + 15 <= -reach || far0 - 15 >= reach) {
+            const float one = zero[far0 < 0 ? -reach : reach];
+            v = f32x4{one, one, one, one};
+        } else {
+            __builtin_memcpy(&v, zero + at, sizeof v);
+        }
         return v;
-    }
-    // Whether all distances of low .. high have one bias; `value` is it.
-    __device__ __forceinline__ bool one(int low, int high, float &value) const {
-        if (high <= -reach) value = zero[-reach];
-        else if (low >= reach) value = zero[reach];
-        else return false;
-        return true;
     }
 };
 

@@ -14,6 +14,7 @@
 // delta's error; out's rounding to 16 bits is too large an error there.  With
 // dbias, delta is therefore summed from p and dout . v in fp32, in a walk of its
 // own over the keys, before dq's.
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.h"
@@ -22,8 +23,7 @@ using namespace bfhip;
 
 namespace {
 
-constexpr int kTile = 64;       // rows per LDS tile
-constexpr int kPartSteps = 16;  // fewest tiles of queries of a part
+constexpr int kTile = 64;  // rows per LDS tile
 
 struct GradArgs {
     AttnArgs f;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
     const int offset = s.length - q_len;
     const int key0 = s.first + wave * 16 * KB;
     const Steps steps = query_steps(f.causal, s.first, offset, q_len);
-    const int all = steps.tiles * group, per = part_tiles(all, f.parts, kPartSteps);
+    const int all = steps.tiles * group, per = part_tiles(all, f.parts, f.chunk);
     if (part && part >= (all + per - 1) / per) return;  // (the first part is always there)
     const int first = part * per, end = min(all, first + per);
 
@@ -176,19 +176,18 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                 for (int kb = 0; kb < KB; ++kb) {
                     // Key minus query of the block's first ones.
                     const int far0 = key0 + 16 * kb - (i0 + r0 + offset);
-                    f32x4 add = nlse;
-                    if constexpr (BIAS) {
-                        float one;
-                        if (bias.one(far0 - 15, far0 + 15, one)) {
-                            add += one;
-                        } else {
-                            const f32x4 b4 = bias.four(far0 + l16 - 4 * g - 3);
-                            add += __builtin_shufflevector(b4, b4, 3, 2, 1, 0);
-                        }
+                    f32x4 x;
+                    if constexpr (BIAS) {  // (rounded as the forward's scores are)
+                        const f32x4 b4 = bias.block(far0, far0 + l16 - 4 * g - 3);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = fmaf(p[b][kb][e], f.scale2, b4[3 - e]) + nlse[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = fmaf(p[b][kb][e], f.scale2, nlse[e]);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[b][kb][e] = exp2_raw(fmaf(p[b][kb][e], f.scale2, add[e]));
+                        p[b][kb][e] = exp2_raw(x[e]);
                         ds[b][kb][e] = p[b][kb][e] * (ds[b][kb][e] - delta[e]);
                     }
                 }
@@ -256,7 +255,7 @@ __global__ __launch_bounds__(256) void attention_keys_join_kernel(GradArgs a) {
     sequence_rows(f.q_starts, sequence, f.q_tokens, q_start, q_len);
     sequence_rows(f.k_starts, sequence, f.k_tokens, k_start, k_len);
     const Steps steps = query_steps(f.causal, (token - k_start) / ROWS * ROWS, k_len - q_len, q_len);
-    const int all = steps.tiles * (f.heads / f.kv_heads), per = part_tiles(all, f.parts, kPartSteps);
+    const int all = steps.tiles * (f.heads / f.kv_heads), per = part_tiles(all, f.parts, f.chunk);
     if (per >= all) return;  // written by the kernel before
     const int used = (all + per - 1) / per;
     const size_t step = (size_t)f.k_tokens * f.kv_heads * 2 * DIM;
@@ -403,17 +402,14 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
 #pragma unroll
         for (int ib = 0; ib < IB; ++ib) {
             const int far0 = j0 + r0 - (row0 + 16 * ib + offset);
-            f32x4 add = {nlse[ib], nlse[ib], nlse[ib], nlse[ib]};
-            if constexpr (BIAS) {
-                float one;
-                if (bias.one(far0 - 15, far0 + 15, one)) {
-                    add += one;
-                } else {
-                    add += bias.four(far0 + 4 * g - l16);
-                }
-            }
+            if constexpr (BIAS) {  // (rounded as the forward's scores are)
+                const f32x4 b4 = bias.block(far0, far0 + 4 * g - l16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, add[e]));
+                for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, b4[e]) + nlse[ib]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, nlse[ib]));
+            }
         }
         if (j0 + r0 + 16 > full) {
             const int j = j0 + r0 + 4 * g;
@@ -541,12 +537,14 @@ __global__ __launch_bounds__(256) void attention_bias_sum_kernel(const float *pa
     dbias[i] = s;
 }
 
-constexpr int query_blocks(int size, int dim) { return size == 4 && dim > 64 ? 1 : 2; }
+// Blocks of 16 rows per wave: two, so that a fragment read from LDS serves two
+// products; one for fp32, whose products take eight times as long as the reads.
+constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
 
 // How a call is dealt: slots of queries and of keys, and parts of the queries
 // that a tile of keys meets, so that uneven tiles even out over the CUs.
 struct BackwardPlan {
-    int dim, q_rows, k_rows, parts;
+    int dim, q_rows, k_rows, parts, chunk;
     long long q_slots, k_slots;
     size_t terms, part, part_kv;  // bytes
 };
@@ -555,14 +553,16 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     BackwardPlan p{};
     const int size = d->type == BFHIP_F32 ? 4 : 2;
     p.dim = d->head_dim <= 32 ? 32 : d->head_dim <= 64 ? 64 : 128;
-    p.q_rows = p.k_rows = 64 * query_blocks(size, p.dim);
+    p.q_rows = p.k_rows = 64 * row_blocks(size);
     p.q_slots = slot_count(d->q_tokens, d->sequences, p.q_rows);
     p.k_slots = slot_count(d->k_tokens, d->sequences, p.k_rows);
-    const long long units = p.k_slots * d->kv_heads, parts = units ? 2048 / units : 1;
-    p.parts = (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
-    // As many as the average sequence has queries for.
-    const long long steps = d->sequences ? d->q_tokens / d->sequences / kTile * (d->heads / d->kv_heads) / kPartSteps : 0;
-    if (p.parts > steps) p.parts = steps < 1 ? 1 : (int)steps;
+    // Parts of 16 tiles of queries or more, as many as the average sequence has;
+    // of 4 or more where there is less than a workgroup per CU.
+    const long long units = p.k_slots * d->kv_heads, group = d->heads / d->kv_heads;
+    p.chunk = units < 256 ? 4 : 16;
+    const long long rows = units < 256 ? d->q_tokens : d->sequences ? d->q_tokens / d->sequences : 0;
+    const long long parts = units ? 2048 / units : 1, steps = rows * group / (kTile * p.chunk);
+    p.parts = (int)std::max(1ll, std::min({32ll, parts, steps}));
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float));
     p.part = d->bias ? round((size_t)p.q_slots * d->heads * (2 * d->reach + 1) * sizeof(float)) : 0;
@@ -601,6 +601,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     GradArgs a{};
     a.f = attn_args(d, q, k, v, out, const_cast<float *>(lse));
     a.f.parts = p.parts;
+    a.f.chunk = p.chunk;
     a.dout = attn_rows(dout, d->q_tokens, n, size);
     a.dq = attn_rows(dq, d->q_tokens, n, size);
     a.dk = attn_rows(dk, d->k_tokens, n, size);
@@ -616,7 +617,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         with_element(d->type, [&](auto e) {
             with_dim(n, [&](auto dim) {
                 using E = decltype(e);
-                constexpr int DIM = decltype(dim)::value, QB = query_blocks(E::kSize, DIM), WAVES = E::kSize == 2 && DIM == 128 ? 8 : 4, KB = 64 * QB / (16 * WAVES);
+                constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), WAVES = E::kSize == 2 && DIM == 128 ? 8 : 4, KB = 64 * QB / (16 * WAVES);
                 using K = KeyTile<E, DIM, KB, WAVES>;
                 using T = AttnTile<E, DIM>;
                 if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);

@@ -32,13 +32,13 @@ struct Running {
             for (int db = 0; db < DB; ++db) o[ib][db] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
     }
-    // Takes the scores of JB blocks of 16 keys (base 2: score = raw * scale + add,
-    // scale > 0) and leaves 2^(score - m) in their place.  m only has to be near
+    // Takes the scores of JB blocks of 16 keys (base 2: score = raw * scale, scale >
+    // 0) and leaves 2^(score - m) in their place.  m only has to be near
     // the maximum: it moves, and what has been summed is scaled, when a score
     // passes it by more than 8 (probabilities then stay below 2^8, which fp16
     // holds and fp32 sums); most tiles need no scaling.
     template <int JB>
-    __device__ __forceinline__ void take(f32x4 (&sc)[JB][IB], float scale, const float (&add)[IB]) {
+    __device__ __forceinline__ void take(f32x4 (&sc)[JB][IB], float scale) {
         float top[IB];
         bool moves = false;
 #pragma unroll
@@ -51,7 +51,7 @@ struct Running {
             }
             t = fmaxf(t, __shfl_xor(t, 16));
             t = fmaxf(t, __shfl_xor(t, 32));
-            top[ib] = fmaf(t, scale, add[ib]);
+            top[ib] = t * scale;
             moves |= top[ib] > m[ib] + 8.f;
         }
         if (__any(moves)) {
@@ -69,7 +69,7 @@ struct Running {
 #pragma unroll
         for (int ib = 0; ib < IB; ++ib) {
             // No key seen yet: any finite value keeps 2^(-inf - it) at 0.
-            const float at = add[ib] - (m[ib] == -INFINITY ? 0.f : m[ib]);
+            const float at = m[ib] == -INFINITY ? 0.f : -m[ib];
 #pragma unroll
             for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
@@ -168,30 +168,18 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
                 for (int ib = 0; ib < IB; ++ib) sc[jb][ib] = E::mfma(kf, qf[ib][kk], sc[jb][ib]);
             }
         }
-        float scale = a.scale2, add[IB];
-#pragma unroll
-        for (int ib = 0; ib < IB; ++ib) add[ib] = 0.f;
         if constexpr (BIAS) {
             // Beyond the reach on either side all distances have one bias;
             // nearer ones are looked up.
-            const int far0 = j0 - (row0 + offset);  // key 0 of the tile, query 0 of the wave
-            float one;
-            if (bias.one(far0 - (16 * IB - 1), far0 + kKeys - 1, one)) {
 #pragma unroll
-                for (int ib = 0; ib < IB; ++ib) add[ib] = one;
-            } else {
-                scale = 1.f;
+            for (int ib = 0; ib < IB; ++ib)
 #pragma unroll
-                for (int ib = 0; ib < IB; ++ib)
+                for (int jb = 0; jb < 4; ++jb) {
+                    const int far = j0 + 16 * jb - (row0 + 16 * ib + offset);  // of the block's first key and query
+                    const f32x4 b = bias.block(far, far + 4 * g - l16);
 #pragma unroll
-                    for (int jb = 0; jb < 4; ++jb) {
-                        const int far = far0 + 16 * (jb - ib);
-                        const f32x4 b = bias.one(far - 15, far + 15, one) ? f32x4{one, one, one, one}
-                                                                          : bias.four(far + 4 * g - l16);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[jb][ib][e] = fmaf(sc[jb][ib][e], a.scale2, b[e]);
-                    }
-            }
+                    for (int e = 0; e < 4; ++e) sc[jb][ib][e] = fmaf(sc[jb][ib][e], a.scale2, b[e]);
+                }
         }
         if (j0 + kKeys > full) {
             const int j = j0 + 4 * g;
@@ -203,7 +191,7 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
                     for (int e = 0; e < 4; ++e)
                         sc[jb][ib][e] = j + 16 * jb + e < limit[ib] ? sc[jb][ib][e] : -INFINITY;
         }
-        run.template take<4>(sc, scale, add);
+        run.template take<4>(sc, BIAS ? 1.f : a.scale2);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             typename E::Frag pf[IB];
@@ -345,7 +333,7 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sc[jb][0][e] = j + 16 * jb + e < limit ? sc[jb][0][e] : -INFINITY;
             }
-            run.template take<2>(sc, BIAS ? 1.f : a.scale2, {0.f});
+            run.template take<2>(sc, BIAS ? 1.f : a.scale2);
             const typename E::Frag pf = to_frag<E>(sc[0][0], sc[1][0]);
             typename E::Frag vf[kDB];
             col_frags_in_flight<E, DIM>(vt, lane, vf);
@@ -468,7 +456,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
     if (a.lse && d == 0) a.lse[(size_t)head * a.q_tokens + token] = natural_lse(top, total);
 }
 
-constexpr int query_rows(int size, int dim) { return size == 4 && dim > 64 ? 64 : 128; }
+// Queries of a workgroup: two blocks of 16 per wave, so that a fragment read from
+// LDS serves two products; one for fp32, whose products take eight times as long
+// as the reads.
+constexpr int query_rows(int size) { return size == 4 ? 64 : 128; }
 
 // How a call is dealt.  `few`: so few queries per sequence that a key head's
 // group of them fills at most two tiles of 16 rows on average.  The keys are
@@ -491,7 +482,7 @@ ForwardPlan forward_plan(const bfhip_attention_desc *d) {
     p.parts = 1;
     if (!d->sequences || !d->q_tokens) return p;
     p.few = d->q_tokens * group <= 32ll * d->sequences && d->q_tokens * group < 1 << 30;
-    p.rows = query_rows(size, p.dim);
+    p.rows = query_rows(size);
     if (p.few) {
         const long long units = (long long)d->sequences * d->kv_heads, least = size * p.dim <= 128 ? 128 : 64;
         const long long chunk = (d->k_tokens * d->kv_heads / 1536 + least - 1) / least * least;
@@ -556,7 +547,7 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
     with_element(d->type, [&](auto e) {
         with_dim(d->head_dim, [&](auto n) {
             using E = decltype(e);
-            constexpr int DIM = decltype(n)::value, ROWS = query_rows(E::kSize, DIM), IB = ROWS / 64;
+            constexpr int DIM = decltype(n)::value, ROWS = query_rows(E::kSize), IB = ROWS / 64;
             using Few = FewQueries<E, DIM>;
             using T = AttnTile<E, DIM>;
             const auto run = [&](auto bias) {
