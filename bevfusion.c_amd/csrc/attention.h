@@ -383,6 +383,15 @@ __device__ __forceinline__ typename E::Frag to_frag(const f32x4 &a, const f32x4 
     }
 }
 
+// What the rounding of to_frag left, as operand words.
+template <class E>
+__device__ __forceinline__ typename E::Frag rest_frag(const f32x4 &a, const f32x4 &b) {
+    typedef typename E::Word Words4 __attribute__((ext_vector_type(4)));
+    const f32x4 x = a - __builtin_convertvector(__builtin_convertvector(a, Words4), f32x4);
+    const f32x4 y = b - __builtin_convertvector(__builtin_convertvector(b, Words4), f32x4);
+    return to_frag<E>(x, y);
+}
+
 // Stores an accumulated transposed product of DB x 16 elements by 16 rows: lane
 // l holds row l & 15 (at `row`, if `live`), elements 16 db + 4 (l >> 4) ..+3.
 template <class E, int DB>

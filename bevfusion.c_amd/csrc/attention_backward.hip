@@ -10,10 +10,15 @@
 // twice costs two products of seven more than adding dq up with atomics would,
 // and gives the same bits every time.
 //
-// A bias's gradient sums very many ds, whose sum over a row is zero but for
-// delta's error; out's rounding to 16 bits is too large an error there.  With
-// dbias, delta is therefore summed from p and dout . v in fp32, in a walk of its
-// own over the keys, before dq's.
+// Precision of the 16-bit types.  p and ds are rounded to the type for the matrix
+// cores, and delta is computed from the forward's rounded out.  Over many keys
+// these errors average out; a query that sees few keys has large p and a large
+// out, and there they show (64 causal tokens: dq and dk off by 1.7 times what
+// their own rounding is).  So where no query of a tile sees more than kFineKeys
+// keys, the rounding's rest is multiplied too, and delta is summed from p and
+// dout . v in fp32, in a walk of its own over the keys.  A bias's gradient sums
+// very many ds, whose sum over a row is zero but for delta's error: with dbias,
+// delta is always summed so.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,7 +28,8 @@ using namespace bfhip;
 
 namespace {
 
-constexpr int kTile = 64;  // rows per LDS tile
+constexpr int kTile = 64;       // rows per LDS tile
+constexpr int kFineKeys = 256;  // see above
 
 struct GradArgs {
     AttnArgs f;
@@ -147,6 +153,7 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         }
         // A query that does not see every key of the wave's.
         const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
+        const bool fine = E::kSize == 2 && (f.causal ? min(s.length, i0 + kTile + offset) : s.length) <= kFineKeys;
         // Scores of the whole tile first: the compiler waits for the copies in
         // flight before the transposed reads, which by then have had the time.
         typename E::Frag pf[2][KB], sf[2][KB];
@@ -206,6 +213,20 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
             for (int kb = 0; kb < KB; ++kb) {
                 pf[c][kb] = to_frag<E>(p[0][kb], p[1][kb]);
                 sf[c][kb] = to_frag<E>(ds[0][kb], ds[1][kb]);
+            }
+            if constexpr (E::kSize == 2) {
+                if (fine) {
+#pragma unroll
+                    for (int db = 0; db < kDB; ++db) {
+                        const typename E::Frag gf = col_frag<E, DIM>(gt, 32 * c, db, lane);
+                        const typename E::Frag qf = col_frag<E, DIM>(qt, 32 * c, db, lane);
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb) {
+                            dv[kb][db] = E::mfma(gf, rest_frag<E>(p[0][kb], p[1][kb]), dv[kb][db]);
+                            dk[kb][db] = E::mfma(qf, rest_frag<E>(ds[0][kb], ds[1][kb]), dk[kb][db]);
+                        }
+                    }
+                }
             }
         }
 #pragma unroll
@@ -421,9 +442,9 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         }
     };
     int buffer = 0;
-    if constexpr (BIAS) {
-        if (part) {
-            // delta in fp32 for the sums of ds.
+    const bool fine = E::kSize == 2 && last <= kFineKeys, sum_delta = fine || part;
+    if constexpr (BIAS || E::kSize == 2) {
+        if (sum_delta) {
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib) delta[ib] = 0.f;
             if (tiles > 0) issue(0, buffer);
@@ -451,7 +472,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             }
         }
     }
-    if (tiles > 0 && !part) issue(0, buffer);
+    if (tiles > 0 && !sum_delta) issue(0, buffer);
     float low = 0.f, high = 0.f;
     for (int t = 0; t < tiles; ++t, buffer ^= 1) {
         wait_vmcnt<0>();
@@ -488,6 +509,16 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 }
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib) sf[c][ib] = to_frag<E>(ds[0][ib], ds[1][ib]);
+            if constexpr (E::kSize == 2) {
+                if (fine) {
+#pragma unroll
+                    for (int db = 0; db < kDB; ++db) {
+                        const typename E::Frag kf = col_frag<E, DIM>(kt, 32 * c, db, lane);
+#pragma unroll
+                        for (int ib = 0; ib < IB; ++ib) dq[ib][db] = E::mfma(kf, rest_frag<E>(ds[0][ib], ds[1][ib]), dq[ib][db]);
+                    }
+                }
+            }
         }
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {
