@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "column_sum.h"
 
 using namespace bfhip;
 
@@ -551,23 +552,6 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     }
 }
 
-// dbias[i] = sum over the slots of part[slot][i]: 16 results per workgroup, 16
-// threads each.
-__global__ __launch_bounds__(256) void attention_bias_sum_kernel(const float *part, float *dbias, long long n, int slots) {
-    __shared__ float sum[16][17];
-    const long long i = (long long)blockIdx.x * 16 + threadIdx.x % 16;
-    const int w = threadIdx.x / 16;
-    float s = 0.f;
-    if (i < n)
-        for (int p = w; p < slots; p += 16) s += part[p * n + i];
-    sum[w][threadIdx.x % 16] = s;
-    __syncthreads();
-    if (w || i >= n) return;
-#pragma unroll
-    for (int q = 1; q < 16; ++q) s += sum[q][threadIdx.x];
-    dbias[i] = s;
-}
-
 // Blocks of 16 rows per wave: two, so that a fragment read from LDS serves two
 // products; one for fp32, whose products take eight times as long as the reads.
 constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
@@ -675,10 +659,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                     hipLaunchKernelGGL((attention_keys_join_kernel<E, DIM, K::kRows>), dim3((unsigned)joins), dim3(256), 0, s, a);
             });
         });
-    if (dbias) {
-        const long long count = width * d->heads;
-        hipLaunchKernelGGL(attention_bias_sum_kernel, dim3((unsigned)((count + 15) / 16)), dim3(256), 0, s, a.part, dbias,
-                           count, d->q_tokens && d->sequences ? (int)p.q_slots : 0);
-    }
+    const long long count = width * d->heads;
+    if (dbias) column_sum(a.part, d->q_tokens && d->sequences ? p.q_slots : 0, dbias, dbias, count, count, s);
     return launch_ok(error, cap, "attention launch");
 }

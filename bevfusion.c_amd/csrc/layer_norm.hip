@@ -1,5 +1,6 @@
 // Stateless layer norm, forward and backward (include/bfhip_transformer.h).
 #include "bfhip_transformer.h"
+#include "column_sum.h"
 #include "element.h"
 #include "gemm_core.h"
 
@@ -16,7 +17,8 @@ constexpr int kMaxFeatures = 65536;
 // (as words, converted where they are used) by a group of LANES threads, CHUNKS
 // 16-byte chunks each, and written once.  Chunks of a group's lanes are
 // neighbours in memory; a group walks rows with the norm's weights and, in the
-// backward pass, its columns' gradient sums in registers.
+// backward pass, its columns' gradient sums in registers, and loads the next row
+// before it works on one.
 template <class E, int LANES, int CHUNKS>
 struct NormRow {
     static constexpr int kWords = 16 / E::kSize, kGroups = kThreads / LANES;
@@ -97,9 +99,15 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
     if (a.gamma) R::load(a.gamma, a.n, gamma);
     if (a.beta) R::load(a.beta, a.n, beta);
     const float n = (float)a.n;
-    for (long long r = (long long)blockIdx.x * R::kGroups + R::group(); r < a.rows; r += (long long)gridDim.x * R::kGroups) {
+    const long long step = (long long)gridDim.x * R::kGroups;
+    long long r = (long long)blockIdx.x * R::kGroups + R::group();
+    typename R::Chunk next[CHUNKS];
+    if (r < a.rows) R::load((const W *)a.x + r * a.xs, a.n, next);
+    for (; r < a.rows; r += step) {
         typename R::Chunk x[CHUNKS];
-        R::load((const W *)a.x + r * a.xs, a.n, x);
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) x[k] = next[k];
+        if (r + step < a.rows) R::load((const W *)a.x + (r + step) * a.xs, a.n, next);
         float s = 0.f, d = 0.f;
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k)
@@ -149,11 +157,26 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
             dg[k].w[e] = db[k].w[e] = 0.f;
         }
     const float per = 1.f / (float)a.n;
-    for (long long r = (long long)blockIdx.x * R::kGroups + R::group(); r < a.rows; r += (long long)gridDim.x * R::kGroups) {
+    const long long step = (long long)gridDim.x * R::kGroups;
+    long long r = (long long)blockIdx.x * R::kGroups + R::group();
+    typename R::Chunk next_x[CHUNKS], next_dy[CHUNKS];
+    float next_m = 0.f, next_rs = 0.f;
+    const auto fetch = [&](long long row) {
+        R::load((const W *)a.x + row * a.xs, a.n, next_x);
+        R::load((const W *)a.dy + row * a.dys, a.n, next_dy);
+        next_m = a.mean[row];
+        next_rs = a.rstd[row];
+    };
+    if (r < a.rows) fetch(r);
+    for (; r < a.rows; r += step) {
         typename R::Chunk x[CHUNKS], dy[CHUNKS];
-        R::load((const W *)a.x + r * a.xs, a.n, x);
-        R::load((const W *)a.dy + r * a.dys, a.n, dy);
-        const float m = a.mean[r], rs = a.rstd[r];
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            x[k] = next_x[k];
+            dy[k] = next_dy[k];
+        }
+        const float m = next_m, rs = next_rs;
+        if (r + step < a.rows) fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k)
@@ -267,31 +290,15 @@ __global__ __launch_bounds__(kThreads) void norm_weight_long_kernel(NormArgs a) 
     a.partial[(size_t)(2 * blockIdx.y + w) * a.n + c] = (q[0][t] + q[1][t]) + (q[2][t] + q[3][t]);
 }
 
-// dgamma, dbeta: the partial sums of 16 columns per workgroup, 16 threads each.
-__global__ __launch_bounds__(kThreads) void norm_weight_sum_kernel(const float *partial, int parts, float *dgamma,
-                                                                   float *dbeta, int n) {
-    __shared__ float sum[16][17];
-    const int c = blockIdx.x * 16 + threadIdx.x % 16, w = threadIdx.x / 16;
-    float s = 0.f;
-    if (c < 2 * n)
-        for (int p = w; p < parts; p += 16) s += partial[(size_t)p * 2 * n + c];
-    sum[w][threadIdx.x % 16] = s;
-    __syncthreads();
-    if (w || c >= 2 * n) return;
-#pragma unroll
-    for (int i = 1; i < 16; ++i) s += sum[i][threadIdx.x];
-    (c < n ? dgamma : dbeta - n)[c] = s;
-}
-
-// Lanes of a row's group: the fewest of 16, 32 and 64 that hold the row in at
-// most 16 elements each, or a workgroup's 256 with up to four chunks (0: none
-// does).  Fewer lanes leave fewer of them without a chunk and need fewer steps
-// to add up; more elements per lane leave too few waves to hide the loads.
+// Lanes of a row's group: the fewest of 16, 32, 64 and 256 that hold the row in
+// at most four chunks each (0: none does).  Fewer lanes leave fewer of them
+// without a chunk, need fewer steps to add up, and keep more of a row in flight
+// per wave.
 int norm_lanes(int n, int size) {
     const int words = 16 / size, chunks = (n + words - 1) / words;
-    for (int lanes : {16, 32, 64})
-        if (n <= 16 * lanes) return lanes;
-    return chunks <= 4 * 256 ? 256 : 0;
+    for (int lanes : {16, 32, 64, 256})
+        if (chunks <= 4 * lanes) return lanes;
+    return 0;
 }
 
 template <class E, class F>
@@ -302,10 +309,8 @@ void with_row(int n, F f) {
         const int chunks = (n + L * words - 1) / (L * words);
         if (chunks <= 1) f(l, std::integral_constant<int, 1>{});
         else if (chunks == 2) f(l, std::integral_constant<int, 2>{});
-        else if constexpr (L == 256 || E::kSize == 4) {
-            if (chunks == 3) f(l, std::integral_constant<int, 3>{});
-            else f(l, std::integral_constant<int, 4>{});
-        }
+        else if (chunks == 3) f(l, std::integral_constant<int, 3>{});
+        else f(l, std::integral_constant<int, 4>{});
     };
     if (lanes == 16) with_chunks(std::integral_constant<int, 16>{});
     else if (lanes == 32) with_chunks(std::integral_constant<int, 32>{});
@@ -415,8 +420,6 @@ extern "C" int bfhip_layer_norm_backward(int type, const void *dy, long long dy_
         });
     });
     if (!ok) return fail(error, cap, "layer norm has too many rows");
-    if (dgamma)
-        hipLaunchKernelGGL(norm_weight_sum_kernel, dim3((2 * features + 15) / 16), dim3(kThreads), 0, s,
-                           (const float *)workspace, (int)parts, dgamma, dbeta, features);
+    if (dgamma) column_sum((const float *)workspace, parts, dgamma, dbeta, features, 2ll * features, s);
     return launch_ok(error, cap, "layer norm launch");
 }

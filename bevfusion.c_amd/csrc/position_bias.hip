@@ -1,6 +1,7 @@
 // Learned position bias by buckets: a table spread over a map, and the table's
 // gradient (include/bfhip_transformer.h).
 #include "bfhip_transformer.h"
+#include "column_sum.h"
 #include "gemm_core.h"
 
 using namespace bfhip;
@@ -44,9 +45,9 @@ __global__ __launch_bounds__(kThreads) void bias_forward_kernel(const float *tab
 // table with more is walked in ranges, a workgroup each.  The lanes of a head
 // and the waves are added up in order at the end: partial [parts][range x
 // ranges][HEADS x head tiles], or the result where there is one part.
-template <int HEADS>
+template <int HEADS, bool VEC>
 __global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *dbias, const int *map, float *out,
-                                                                 int buckets, int heads, int range, int waves, bool vec,
+                                                                 int buckets, int heads, int range, int waves,
                                                                  long long n) {
     constexpr int QUADS = kWave / HEADS;
     extern __shared__ float smem[];
@@ -58,24 +59,26 @@ __global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *db
     float *const sums = smem + (size_t)wave * range * kWave + lane;
     for (int b = 0; b < count; ++b) sums[b * kWave] = 0.f;
     const float *const row = dbias + (size_t)min(head, heads - 1) * n;
-    const bool live = head < heads;
     const long long step = (long long)gridDim.x * waves * QUADS * 4;
     for (long long p0 = ((long long)blockIdx.x * waves + wave) * QUADS * 4 + quad * 4; p0 < n; p0 += step * kAhead) {
+        // Positions past the end are loaded from within it and add 0 to the
+        // first bucket, as do those of other buckets: no lane branches.
         float v[kAhead][4];
         int at[kAhead][4];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
             const long long p = p0 + a * step;
-            if (vec && p < n) {
-                const float4 f = *reinterpret_cast<const float4 *>(row + p);
-                const int4 m = *reinterpret_cast<const int4 *>(map + p);
+            if constexpr (VEC) {
+                const long long q = min(p, n - 4);
+                const float4 f = *reinterpret_cast<const float4 *>(row + q);
+                const int4 m = *reinterpret_cast<const int4 *>(map + q);
                 v[a][0] = f.x, v[a][1] = f.y, v[a][2] = f.z, v[a][3] = f.w;
                 at[a][0] = m.x, at[a][1] = m.y, at[a][2] = m.z, at[a][3] = m.w;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    v[a][e] = p + e < n ? row[p + e] : 0.f;
-                    at[a][e] = p + e < n ? map[p + e] : -1;
+                    v[a][e] = row[min(p + e, n - 1)];
+                    at[a][e] = map[min(p + e, n - 1)];
                 }
             }
         }
@@ -84,8 +87,9 @@ __global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *db
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const unsigned b = (unsigned)(at[a][e] - b0);
-                if (live && b < (unsigned)count)
-                    __hip_atomic_fetch_add(sums + b * kWave, v[a][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                const bool in = b < (unsigned)count && p0 + a * step + e < n;
+                __hip_atomic_fetch_add(sums + (in ? b : 0) * kWave, in ? v[a][e] : 0.f, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_WORKGROUP);
             }
     }
     __syncthreads();
@@ -98,21 +102,6 @@ __global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *db
             for (int q = 0; q < QUADS; ++q) s += smem[((size_t)w * range + b) * kWave + h * QUADS + q];
         out[((size_t)blockIdx.x * buckets + b0 + b) * heads + tile * HEADS + h] = s;
     }
-}
-
-// Sums of the parts, in order: 16 results per workgroup, 16 threads each.
-__global__ __launch_bounds__(kThreads) void bias_sum_kernel(const float *partial, int parts, float *dtable, int n) {
-    __shared__ float sum[16][17];
-    const int c = blockIdx.x * 16 + threadIdx.x % 16, w = threadIdx.x / 16;
-    float s = 0.f;
-    if (c < n)
-        for (int p = w; p < parts; p += 16) s += partial[(size_t)p * n + c];
-    sum[w][threadIdx.x % 16] = s;
-    __syncthreads();
-    if (w || c >= n) return;
-#pragma unroll
-    for (int i = 1; i < 16; ++i) s += sum[i][threadIdx.x];
-    dtable[c] = s;
 }
 
 // How a gradient is dealt: heads per wave (the fewest of 1, 4 and 16 that hold
@@ -133,8 +122,8 @@ BiasPlan bias_plan(int buckets, int heads, long long positions) {
     p.tiles = (heads + p.lanes - 1) / p.lanes;
     const long long round = (long long)p.waves * (kWave / p.lanes) * 4 * kAhead;
     const long long most = (positions + round - 1) / round;
-    // One workgroup per CU or as many as the LDS of two rounds of them holds.
-    long long parts = 512 / ((long long)p.ranges * p.tiles);
+    // Four workgroups per CU.
+    long long parts = 1024 / ((long long)p.ranges * p.tiles);
     parts = parts < 1 ? 1 : parts;
     p.parts = (int)(most < 1 ? 1 : most < parts ? most : parts);
     return p;
@@ -194,14 +183,12 @@ extern "C" int bfhip_position_bias_backward(const float *dbias, const int *map, 
     const auto launch = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(p.parts, (unsigned)blocks), dim3(p.waves * kWave),
                            (size_t)p.waves * p.range * kWave * sizeof(float), s, dbias, map, out, buckets, heads, p.range,
-                           p.waves, vec, positions);
+                           p.waves, positions);
     };
-    if (p.lanes == 1) launch(bias_backward_kernel<1>);
-    else if (p.lanes == 4) launch(bias_backward_kernel<4>);
-    else launch(bias_backward_kernel<16>);
-    if (p.parts > 1) {
-        const int n = buckets * heads;
-        hipLaunchKernelGGL(bias_sum_kernel, dim3((n + 15) / 16), dim3(kThreads), 0, s, (const float *)out, p.parts, dtable, n);
-    }
+    if (p.lanes == 1) launch(vec ? bias_backward_kernel<1, true> : bias_backward_kernel<1, false>);
+    else if (p.lanes == 4) launch(vec ? bias_backward_kernel<4, true> : bias_backward_kernel<4, false>);
+    else launch(vec ? bias_backward_kernel<16, true> : bias_backward_kernel<16, false>);
+    const long long n = (long long)buckets * heads;
+    if (p.parts > 1) column_sum(out, p.parts, dtable, dtable, n, n, s);
     return launch_ok(error, cap, "position bias launch");
 }
