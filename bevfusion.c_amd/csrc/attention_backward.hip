@@ -330,7 +330,7 @@ __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int rea
     const auto add = [&](int far, float v) {
         if (far <= -reach) low += v;
         else if (far >= reach) high += v;
-        else __hip_atomic_fetch_add(sum + far + reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        else sum[far + reach] += v;
     };
     if (g == 0 || i < 4) add(far0 + 4 * g - i, main);
     if (i >= 13) add(far0 + 4 * g + 16 - i, rest);
