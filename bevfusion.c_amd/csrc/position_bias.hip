@@ -99,14 +99,17 @@ __global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *db
         float s = 0.f;
         for (int w = 0; w < waves; ++w)
 #pragma unroll
-            for (int q = 0; q < QUADS; ++q) s += smem[((size_t)w * range + b) * kWave + h * QUADS + q];
+            for (int q = 0; q < QUADS; ++q)  // (from a place that differs by bucket: by bank)
+                s += smem[((size_t)w * range + b) * kWave + h * QUADS + (q + b) % QUADS];
         out[((size_t)blockIdx.x * buckets + b0 + b) * heads + tile * HEADS + h] = s;
     }
 }
 
-// How a gradient is dealt: heads per wave (the fewest of 1, 4 and 16 that hold
-// them, 16 beyond), buckets per range and waves by the LDS they need, and
-// parts so that a thread has at least two rounds of loads.
+// How a gradient is dealt: buckets per range and waves by the LDS they need;
+// heads per wave, 16 or the fewest of 1 and 4 that hold them, so that the map is
+// read once for them; and parts of a round of loads or more.  Where a workgroup
+// per head gets through all positions in four rounds, one launch is all: heads
+// one by one, and no parts.
 struct BiasPlan {
     int lanes, range, waves, ranges, tiles, parts;
 };
@@ -119,13 +122,15 @@ BiasPlan bias_plan(int buckets, int heads, long long positions) {
     p.waves = kLds / (p.range * kRow);
     p.waves = p.waves < kWaves ? p.waves : kWaves;
     p.ranges = (buckets + p.range - 1) / p.range;
+    const bool small = positions <= 4ll * p.waves * kWave * 4 * kAhead;
+    if (small) p.lanes = 1;
     p.tiles = (heads + p.lanes - 1) / p.lanes;
     const long long round = (long long)p.waves * (kWave / p.lanes) * 4 * kAhead;
     const long long most = (positions + round - 1) / round;
     // Four workgroups per CU.
     long long parts = 1024 / ((long long)p.ranges * p.tiles);
     parts = parts < 1 ? 1 : parts;
-    p.parts = (int)(most < 1 ? 1 : most < parts ? most : parts);
+    p.parts = (int)(small || most < 1 ? 1 : most < parts ? most : parts);
     return p;
 }
 
