@@ -46,17 +46,19 @@ struct ElemBf16 {
 
 // N words at p as floats and back, in one access where N words are a power of
 // two of bytes; p needs no alignment beyond the word's (gfx950 serves
-// unaligned vector accesses).
+// unaligned vector accesses).  A vector, so that 16-bit words stay packed in
+// registers.
 template <class E, int N>
 struct Words {
     using Word = typename E::Word;
-    Word w[N];
+    typedef Word Vec __attribute__((ext_vector_type(N)));
+    Vec w;
     __device__ __forceinline__ static Words load(const Word *p) {
         Words v;
-        __builtin_memcpy(v.w, p, sizeof v.w);
+        __builtin_memcpy(&v.w, p, sizeof v.w);
         return v;
     }
-    __device__ __forceinline__ void store(Word *p) const { __builtin_memcpy(p, w, sizeof w); }
+    __device__ __forceinline__ void store(Word *p) const { __builtin_memcpy(p, &w, sizeof w); }
     __device__ __forceinline__ float get(int i) const { return E::get(w[i]); }
     __device__ __forceinline__ void put(int i, float v) { w[i] = E::put(v); }
 };
