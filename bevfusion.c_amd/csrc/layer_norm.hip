@@ -298,8 +298,8 @@ __global__ __launch_bounds__(kThreads) void norm_weight_long_kernel(NormArgs a) 
 // at most four chunks each (0: none does).  Fewer lanes leave fewer of them
 // without a chunk, need fewer steps to add up, and keep more of a row in flight
 // per wave.  The backward pass of 16-bit types takes at most two chunks where
-// four would leave less than four waves per SIMD: 9999 x 257 fp16 12.4 us with
-// two, 15.4 with three; 65536 x 768 bf16 125 us with two, 93 with three.
+// four would leave less than four waves per SIMD: 9999 x 257 fp16 12.3 us with
+// two, 14.9 with three; 65536 x 768 bf16 94 us with two, 58 with three.
 int norm_lanes(long long rows, int n, int size, bool backward) {
     const int words = 16 / size, chunks = (n + words - 1) / words;
     for (int lanes : {16, 32, 64})
