@@ -556,6 +556,8 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
 // products; one for fp32, whose products take eight times as long as the reads.
 constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
 
+constexpr int key_blocks(int size, int dim) { return size == 4 || dim > 64 ? 1 : 2; }
+
 // How a call is dealt: slots of queries and of keys, and parts of the queries
 // that a tile of keys meets, so that uneven tiles even out over the CUs.
 struct BackwardPlan {
@@ -568,7 +570,8 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     BackwardPlan p{};
     const int size = d->type == BFHIP_F32 ? 4 : 2;
     p.dim = d->head_dim <= 32 ? 32 : d->head_dim <= 64 ? 64 : 128;
-    p.q_rows = p.k_rows = 64 * row_blocks(size);
+    p.q_rows = 64 * row_blocks(size);
+    p.k_rows = 64 * key_blocks(size, p.dim);
     p.q_slots = slot_count(d->q_tokens, d->sequences, p.q_rows);
     p.k_slots = slot_count(d->k_tokens, d->sequences, p.k_rows);
     // Parts of 16 tiles of queries or more, as many as the average sequence has;
@@ -632,7 +635,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         with_element(d->type, [&](auto e) {
             with_dim(n, [&](auto dim) {
                 using E = decltype(e);
-                constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), WAVES = E::kSize == 2 && DIM == 128 ? 8 : 4, KB = 64 * QB / (16 * WAVES);
+                constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), WAVES = 4, KB = key_blocks(E::kSize, DIM);
                 using K = KeyTile<E, DIM, KB, WAVES>;
                 using T = AttnTile<E, DIM>;
                 if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);
