@@ -62,16 +62,16 @@ struct NormRow {
         a = group_sum<wave>(a);
         b = group_sum<wave>(b);
         if constexpr (LANES > kWave) {
-            __shared__ float2 part[2][LANES / kWave];
+            __shared__ float2 part[LANES / kWave];
             const int w = threadIdx.x / kWave;
             __syncthreads();  // the sums before have been read
-            if (threadIdx.x % kWave == 0) part[0][w] = make_float2(a, b);
+            if (threadIdx.x % kWave == 0) part[w] = make_float2(a, b);
             __syncthreads();
             a = b = 0.f;
 #pragma unroll
             for (int i = 0; i < LANES / kWave; ++i) {
-                a += part[0][i].x;
-                b += part[0][i].y;
+                a += part[i].x;
+                b += part[i].y;
             }
         }
         return make_float2(a, b);

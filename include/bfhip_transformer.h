@@ -44,12 +44,13 @@ enum { BFHIP_F32 = 0, BFHIP_F16 = 1, BFHIP_BF16 = 2 };
  *
  *   y = (x - mean) * rstd * gamma + beta,  rstd = 1 / sqrt(var + eps), var the
  *   mean squared deviation.  gamma, beta: [features] or NULL (1 and 0).  mean,
- *   rstd: [rows], both or neither NULL.  y may be x (in place).
+ *   rstd: [rows], both or neither NULL.  y may be x (in place, one stride).
  *
  * Backward, with g = dy * gamma and h = (x - mean) * rstd:
  *   dx     = rstd * (g - mean_c(g) - h * mean_c(g * h))
  *   dgamma = sum over rows of dy * h,   dbeta = sum over rows of dy
- *   dgamma, dbeta: [features], both or neither NULL.  dx may be dy or x.
+ *   dgamma, dbeta: [features], both or neither NULL.  dx may be dy or x (one
+ *   stride).
  *   rows == 0 writes zeros to dgamma and dbeta. */
 int bfhip_layer_norm_forward(int type, const void *x, long long x_stride, const float *gamma,
                              const float *beta, void *y, long long y_stride, float *mean,
@@ -107,14 +108,21 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  *
  * Scores and the softmax are fp32; for 16-bit types the probabilities, and in
  * the backward pass the gradients of the scores, are rounded to the type where
- * they enter the matrix cores.  fp32 is multiplied in fp32.
+ * they enter the matrix cores (where a query sees few keys, their rounding's rest
+ * enters too).  fp32 is multiplied in fp32.  A score and its bias are added in
+ * fp32: a bias near the lowest fp32 value swallows the score.
+ *
+ * Workspaces: the forward's holds the sums of keys that are split (few queries
+ * on many keys, at most some 300 MB; mostly none), the backward's two fp32 per
+ * query and head, sums of queries that are split (at most some 150 MB), and with
+ * a bias 2 * reach + 1 fp32 per head and 64 or 128 queries.
  *
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
  * stride in elements; the elements of one head are contiguous, pointers and
  * strides are multiples of 16 bytes, token strides at least head_dim (unless
  * there is one token) and below 4 Mi elements.
  * bias: [heads, 2 * reach + 1] or NULL (reach is then ignored); reach in
- * [0, 2047].  lse and the gradients below: see each function. */
+ * [0, 2047].  out must not overlap the other tensors. */
 typedef struct {
     void *data;
     long long token_stride;

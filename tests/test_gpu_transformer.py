@@ -268,6 +268,52 @@ def test_attention(device, case, layout):
     assert all(torch.equal(a, b) for a, b in zip(back, grads(call, dout, out, lse)))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
+@pytest.mark.parametrize("case", [(F32, 2, 1, 32, [70, 3], [90, 3], True, 4), (BF16, 4, 2, 64, [1, 2], [700, 3], True, None),
+                                  (F16, 2, 2, 16, [130], [260], False, None)], ids=str)
+def test_attention_scales(device, case, scale):
+    """No scale, a negative one and a large one."""
+    call, dout = inputs(device, case)
+    call["scale"] = scale
+    want = ref.attention(**call, dout=dout)
+    out, lse = bfhip.attention(**call, lse=True)
+    ref.check("out", out, *want["out"])
+    for name, t in zip(("dq", "dk", "dv", "dbias"), grads(call, dout, out, lse)):
+        ref.check(name, t, *want[name])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [65, 300, 4100])
+def test_attention_of_very_many_sequences(device, n, causal):
+    """More sequences than a search step has lanes, most of them a few tokens
+    long, some empty, and a long one among single tokens."""
+    ql = [(i * 7) % 4 for i in range(n)]
+    kl = [(i * 5) % 7 for i in range(n)]
+    ql[n // 2], kl[n // 2] = 150, 170
+    case = (BF16, 2, 1, 32, ql, kl, causal, None)
+    call, dout = inputs(device, case)
+    out, lse = bfhip.attention(**call, lse=True)
+    back = grads(call, dout, out, lse)
+    # The reference goes sequence by sequence: every 9th, and the long one.
+    qs, ks = call["q_starts"].tolist(), call["k_starts"].tolist()
+    some = [i for i in range(n) if i % max(1, n // 40) == 0 or i == n // 2]
+    rows = torch.cat([torch.arange(qs[i], qs[i + 1], device=device) for i in some])
+    keys = torch.cat([torch.arange(ks[i], ks[i + 1], device=device) for i in some])
+    part = dict(call, q=call["q"][rows], k=call["k"][keys], v=call["v"][keys],
+                q_starts=starts([ql[i] for i in some], device), k_starts=starts([kl[i] for i in some], device))
+    want = ref.attention(**part, dout=dout[rows])
+    for name, t, at in (("out", out, rows), ("dq", back[0], rows), ("dk", back[1], keys), ("dv", back[2], keys)):
+        ref.check(name, t[at], *want[name])
+
+
+def test_attention_of_a_prompt_among_single_tokens(device):
+    """A batch that is dealt for single tokens and one that is dealt for
+    prompts, the same sequences in both."""
+    ql, kl = [1] * 60 + [90], [400] * 60 + [500]
+    call, _ = inputs(device, (F16, 4, 2, 64, ql, kl, True, 20))
+    ref.check("out", bfhip.attention(**call), *ref.attention(**call)["out"])
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("reach", [None, 5])
 def test_attention_leaves_rows_outside_sequences(device, dtype, reach):
@@ -466,6 +512,30 @@ def test_captured_and_replayed(device):
             assert all(torch.equal(a, b) for a, b in zip(out, w)), rep
             bfhip.attention(**small)
             torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("case", [CASES[4], CASES[10], CASES[17], (BF16, 8, 2, 128, [2500], None, True, 60)], ids=str)
+def test_split_work_captured_and_replayed(device, case):
+    """Keys and queries in parts: a workspace between the launches of a graph."""
+    call, dout = inputs(device, case)
+
+    def run():
+        out, lse = bfhip.attention(**call, lse=True)
+        return out, lse, *grads(call, dout, out, lse)
+
+    want = run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for rep in range(3):
+        for t in got:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
+        run()
+        torch.cuda.synchronize()
 
 
 def test_on_a_stream_of_its_own(device):
