@@ -152,6 +152,8 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                 lds_barrier();
             }
         }
+        // No key of the wave's is there, or is seen.
+        if (key0 >= s.length || (f.causal && i0 + kTile - 1 + offset < key0)) continue;
         // A query that does not see every key of the wave's.
         const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
         const bool fine = E::kSize == 2 && (f.causal ? min(s.length, i0 + kTile + offset) : s.length) <= kFineKeys;
@@ -367,6 +369,8 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     const int offset = k_len - s.length, row0 = s.first + wave * 16 * IB;
     const int last = f.causal ? min(k_len, min(s.first + kRows, s.length) + offset) : k_len;
     const int full = f.causal ? min(k_len, row0 + offset + 1) : k_len;
+    // Keys that the wave has work on.
+    const int own = row0 >= s.length ? 0 : f.causal ? min(k_len, min(row0 + 16 * IB, s.length) + offset) : k_len;
     const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0;
 
     AttnTileCopy<E, DIM, kKeys, 256> kc, vc;
@@ -454,6 +458,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 lds_barrier();
                 issue(t + 1 < tiles ? t + 1 : 0, buffer ^ 1);  // (the first tile again for the walk below)
                 const char *const kt = smem + buffer * kStage, *const vt = kt + kKeys * T::kRow;
+                if (t * kKeys >= own) continue;
 #pragma unroll
                 for (int r0 = 0; r0 < kKeys; r0 += 16) {
                     f32x4 p[IB], dp[IB];
@@ -481,6 +486,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         if (t + 1 < tiles) issue(t + 1, buffer ^ 1);
         const char *const kt = smem + buffer * kStage, *const vt = kt + kKeys * T::kRow;
         const int j0 = t * kKeys;
+        if (j0 >= own) continue;
         typename E::Frag sf[kKeys / 32][IB];  // (the whole tile first, as above)
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c) {

@@ -119,6 +119,8 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     // Keys seen by the workgroup's last query, and by the wave's first.
     const int last = a.causal ? min(k_len, min(s.first + kRows, s.length) + offset) : k_len;
     const int full = a.causal ? min(k_len, row0 + offset + 1) : k_len;
+    // Keys that the wave has work on.
+    const int own = row0 >= s.length ? 0 : a.causal ? min(k_len, min(row0 + 16 * IB, s.length) + offset) : k_len;
     const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0;
     const int per = part_tiles(tiles, a.parts, kPartTiles), begin = part * per, end = min(tiles, begin + per);
     if (part && begin >= tiles) return;
@@ -156,6 +158,7 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
         if (t + 1 < end) issue(t + 1);
         const char *const kt = smem + (t & 1) * kStage, *const vt = kt + kKeys * T::kRow;
         const int j0 = t * kKeys;
+        if (j0 >= own) continue;
         f32x4 sc[4][IB];
 #pragma unroll
         for (int jb = 0; jb < 4; ++jb) {
