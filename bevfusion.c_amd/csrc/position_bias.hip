@@ -93,15 +93,18 @@ __global__ __launch_bounds__(kThreads) void bias_backward_kernel(const float *db
             }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < count * HEADS; i += blockDim.x) {
-        const int b = i / HEADS, h = i % HEADS;
-        if (tile * HEADS + h >= heads) continue;
+    // Four threads per result, a quarter of its lanes each (from a place that
+    // differs by bucket, so that a wave's reads lie on different banks).
+    for (int i = threadIdx.x / 4; i < count * HEADS; i += blockDim.x / 4) {
+        const int b = i / HEADS, h = i % HEADS, quarter = threadIdx.x % 4;
         float s = 0.f;
         for (int w = 0; w < waves; ++w)
 #pragma unroll
-            for (int q = 0; q < QUADS; ++q)  // (from a place that differs by bucket: by bank)
-                s += smem[((size_t)w * range + b) * kWave + h * QUADS + (q + b) % QUADS];
-        out[((size_t)blockIdx.x * buckets + b0 + b) * heads + tile * HEADS + h] = s;
+            for (int q = 0; q < QUADS / 4; ++q)
+                s += smem[((size_t)w * range + b) * kWave + h * QUADS + (4 * q + quarter + b) % QUADS];
+        s = group_sum<4>(s);
+        if (quarter == 0 && tile * HEADS + h < heads)
+            out[((size_t)blockIdx.x * buckets + b0 + b) * heads + tile * HEADS + h] = s;
     }
 }
 
