@@ -4,7 +4,9 @@ Thin ctypes mirror of the C ABI in ``include/bf_cuda_ops.h``,
 ``include/bf_cuda_swin.h``, ``include/bf_cuda_camera.h``, ``include/bf_cuda.h``,
 ``include/bf_cuda_bev.h`` and ``include/bf_cuda_transfusion.h`` (the
 reference's operator/plugin interface for this path, the lift-splat pooling
-that consumes it, the BEV stage after it and the TransFusion decoder).  PyTorch supplies device memory and
+that consumes it, the BEV stage after it and the TransFusion decoder), and of the
+stateless transformer operators in ``include/bfhip_transformer.h`` (layer norm,
+position bias, packed attention, forward and backward).  PyTorch supplies device memory and
 the current HIP stream; every computation runs in ``lib/libbfhip.so``.  There
 is no fallback: if the library is missing, importing an entry point raises.
 """
