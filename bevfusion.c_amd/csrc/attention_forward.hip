@@ -111,11 +111,10 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4;
-    // A tile's parts one after the other: the longest work is then dealt first.
-    const int group = a.heads / a.kv_heads;
-    const Deal deal_ = deal(blockIdx.x, a.heads * a.parts, a.kv_heads);
-    const int kv = deal_.head / (group * a.parts), of_kv = deal_.head % (group * a.parts);
-    const int head = kv * group + of_kv % group, part = of_kv / group;
+    // Part after part: workgroups that run together then read the same keys.
+    const int items = a.slots * a.heads, part = blockIdx.x / items;
+    const Deal deal_ = deal(blockIdx.x % items, a.heads, a.kv_heads);
+    const int head = deal_.head, kv = head / (a.heads / a.kv_heads);
     const Slot s = ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.ordered);
     if (s.sequence < 0) return;
     int k_start, k_len;
