@@ -120,7 +120,8 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         char *const to = smem + (step & 1) * K::kStage;
         qc.issue(f.q.at((long long)q_start + i0, head), left, to);
         gc.issue(a.dout.at((long long)q_start + i0, head), left, to + K::kQ);
-        // Past the last query q, dout and the terms are zero: p is 1, but dout and ds are 0.
+        // Past the last query q, dout and the terms are zero: ds is 0, and p is 1
+        // (or what a bias makes it, which may be infinite: masked below).
         if (wave < 2)
             dma4(buffer_rsrc((wave ? a.delta : a.nlse) + (size_t)head * f.q_tokens + q_start + i0, 4u * min(left, kTile)),
                  to + 2 * K::kQ + wave * kTile * sizeof(float), 4u * lane);
@@ -215,6 +216,16 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (far > 16 * (b - kb) + e) p[b][kb][e] = ds[b][kb][e] = 0.f;
+            }
+            if (BIAS && i0 + kTile > q_len) {
+                const int left = q_len - (i0 + 32 * c + 4 * g);
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (16 * b + e >= left) p[b][kb][e] = ds[b][kb][e] = 0.f;
             }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {

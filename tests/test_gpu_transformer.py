@@ -356,6 +356,20 @@ def test_attention_masked_keys_hold_anything(device, dtype):
         assert torch.equal(got[:71], want[:71]), value
 
 
+@pytest.mark.parametrize("dtype,size", [(F16, 20.0), (BF16, 100.0), (F32, 100.0)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_of_large_biases(device, dtype, size, causal):
+    """A bias whose own exponential the type does not hold, on tiles that are
+    not full: it cancels in the softmax and reaches no gradient by itself."""
+    call, dout = inputs(device, (dtype, 4, 2, 32, [70, 3, 130], [70, 90, 131], causal, 6))
+    call["bias"][:, :7] += size
+    want = ref.attention(**call, dout=dout)
+    out, lse = bfhip.attention(**call, lse=True)
+    ref.check("out", out, *want["out"])
+    for name, t in zip(("dq", "dk", "dv", "dbias"), grads(call, dout, out, lse)):
+        ref.check(name, t, *want[name])
+
+
 def test_attention_bias_can_mask(device):
     """Scores of -inf: by distance, and for whole rows; the lowest finite value
     masks too, but leaves a softmax where every key has it."""
