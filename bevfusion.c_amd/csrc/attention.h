@@ -78,7 +78,8 @@ __device__ __forceinline__ Slot find_slot(const int *starts, int sequences, long
     Slot s;
     s.sequence = __builtin_amdgcn_readfirstlane(lo);
     sequence_rows(starts, s.sequence, tokens, s.start, s.length);
-    s.index = max(0, slot - (s.start / rows + s.sequence));
+    s.index = slot - (s.start / rows + s.sequence);
+    if (s.index < 0) s.sequence = -1;  // before the first sequence
     return s;
 }
 

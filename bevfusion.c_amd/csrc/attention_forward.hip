@@ -266,6 +266,7 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
     const int l16 = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads;
     const int kv = blockIdx.x % a.kv_heads;
     const Slot s = find_slot(a.k_starts, a.sequences, a.k_tokens, blockIdx.x / a.kv_heads, a.chunk);
+    if (s.sequence < 0) return;
     const int k_start = s.start, k_len = s.length, all = (k_len + kKeyRows - 1) / kKeyRows;
     const int part = s.index, per = part_tiles(all, a.parts, a.chunk / kKeyRows);
     if (part && part >= (all + per - 1) / per) return;  // (the first part is always there)

@@ -370,6 +370,23 @@ def test_attention_of_large_biases(device, dtype, size, causal):
         ref.check(name, t, *want[name])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("ql", [[33, 200], [1, 2]])
+def test_attention_behind_many_other_rows(device, dtype, causal, ql):
+    """A first sequence that begins tiles away from the tensor's first row."""
+    call, dout = inputs(device, (dtype, 4, 2, 64, [700] + ql, [900, 300, 650], causal, 5))
+    for name in ("q_starts", "k_starts"):
+        call[name] = call[name][1:].contiguous()
+    want = ref.attention(**call, dout=dout)
+    out, lse = bfhip.attention(**call, lse=True)
+    rows, keys = slice(700, None), slice(900, None)
+    ref.check("out", out[rows], want["out"][0][rows], want["out"][1][rows])
+    back = grads(call, dout, out, lse)
+    for name, t, at in zip(("dq", "dk", "dv", "dbias"), back, (rows, keys, keys, slice(None))):
+        ref.check(name, t[at], want[name][0][at], want[name][1][at])
+
+
 def test_attention_bias_can_mask(device):
     """Scores of -inf: by distance, and for whole rows; the lowest finite value
     masks too, but leaves a softmax where every key has it."""
