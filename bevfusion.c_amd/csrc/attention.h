@@ -420,16 +420,26 @@ inline bool bad_rows(const bfhip_rows *r, long long tokens, int dim, int size) {
            (tokens > 1 && (r->token_stride < dim || r->token_stride >= 4 << 20)) || r->token_stride < 0;
 }
 
+// Rows that a call writes: also no row on another, whichever of tokens and
+// heads is the outer one.
+inline bool bad_result(const bfhip_rows *r, long long tokens, int heads, int dim, int size) {
+    if (bad_rows(r, tokens, dim, size)) return true;
+    const long long t = tokens > 1 ? r->token_stride : 0, h = heads > 1 ? r->head_stride : 0;
+    return tokens && ((heads > 1 && h < dim) || (tokens > 1 && heads > 1 && t < (heads - 1) * h + dim && h < (tokens - 1) * t + dim));
+}
+
 inline AttnRows attn_rows(const bfhip_rows *r, long long tokens, int dim, int size) {
     const long long t = tokens > 1 ? r->token_stride : dim;
     return AttnRows{(char *)r->data, t * size, r->head_stride * size};
 }
 
+constexpr long long kMostTokens = 0x7ffff000;  // a tile past the last row is still an int
+
 inline bool bad_attention(const bfhip_attention_desc *d) {
     return !d || d->type < BFHIP_F32 || d->type > BFHIP_BF16 || d->sequences < 0 || d->heads <= 0 || d->kv_heads <= 0 ||
            d->heads % d->kv_heads || d->head_dim <= 0 || d->head_dim > 128 || d->head_dim % 8 || d->heads > 65535 ||
-           (d->causal != 0 && d->causal != 1) || d->q_tokens < 0 || d->k_tokens < 0 || d->q_tokens > 0x7fffffff ||
-           d->k_tokens > 0x7fffffff || !(d->scale == d->scale) || __builtin_isinf(d->scale) ||
+           (d->causal != 0 && d->causal != 1) || d->q_tokens < 0 || d->k_tokens < 0 || d->q_tokens > kMostTokens ||
+           d->k_tokens > kMostTokens || !(d->scale == d->scale) || __builtin_isinf(d->scale) ||
            (d->sequences && (!d->q_starts || !d->k_starts)) || (d->bias && (d->reach < 0 || d->reach > 2047));
 }
 

@@ -626,9 +626,9 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     if (bad_attention(d) || (dbias && !d->bias) || (!lse && d->q_tokens)) return fail(error, cap, "invalid attention contract");
     const int size = d->type == BFHIP_F32 ? 4 : 2, n = d->head_dim;
     if (bad_rows(q, d->q_tokens, n, size) || bad_rows(k, d->k_tokens, n, size) || bad_rows(v, d->k_tokens, n, size) ||
-        bad_rows(out, d->q_tokens, n, size) || bad_rows(dout, d->q_tokens, n, size) || bad_rows(dq, d->q_tokens, n, size) ||
-        bad_rows(dk, d->k_tokens, n, size) || bad_rows(dv, d->k_tokens, n, size))
-        return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim");
+        bad_rows(out, d->q_tokens, n, size) || bad_rows(dout, d->q_tokens, n, size) || bad_result(dq, d->q_tokens, d->heads, n, size) ||
+        bad_result(dk, d->k_tokens, d->kv_heads, n, size) || bad_result(dv, d->k_tokens, d->kv_heads, n, size))
+        return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
     const BackwardPlan p = backward_plan(d);
     const size_t need = 2 * p.terms + p.part + p.part_kv;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))

@@ -530,8 +530,9 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
     if (bad_attention(d)) return fail(error, cap, "invalid attention contract");
     const int size = d->type == BFHIP_F32 ? 4 : 2;
     if (bad_rows(q, d->q_tokens, d->head_dim, size) || bad_rows(k, d->k_tokens, d->head_dim, size) ||
-        bad_rows(v, d->k_tokens, d->head_dim, size) || bad_rows(out, d->q_tokens, d->head_dim, size))
-        return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim");
+        bad_rows(v, d->k_tokens, d->head_dim, size) ||
+        bad_result(out, d->q_tokens, d->heads, d->head_dim, size))
+        return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
     const ForwardPlan p = forward_plan(d);
     const size_t rows = part_rows(d, p), need = rows * (p.dim * sizeof(float) + sizeof(float2));
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))

@@ -104,12 +104,15 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * lse = -inf and no gradient.  Keys that a query does not see do not reach its
  * scores, whatever they hold; a value row reaches every query of its
  * sequence whose tile of the product it shares, so a NaN or infinity in a
- * value can also reach queries of its sequence that do not see it (0 * NaN).
+ * value can also reach queries of its sequence that do not see it (0 * NaN).  In
+ * the backward pass that holds for the keys (dq) and for q and dout (dk, dv)
+ * too.
  *
  * Scores and the softmax are fp32; for 16-bit types the probabilities, and in
  * the backward pass the gradients of the scores, are rounded to the type where
  * they enter the matrix cores (where a query sees few keys, their rounding's rest
- * enters too).  fp32 is multiplied in fp32.  A score and its bias are added in
+ * enters too).  A score's gradient beyond the type's range (fp16:
+ * 65504) becomes infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
  * fp32: a bias near the lowest fp32 value swallows the score.
  *
  * Workspaces: the forward's holds the sums of keys that are split (few queries
@@ -120,7 +123,8 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
  * stride in elements; the elements of one head are contiguous, pointers and
  * strides are multiples of 16 bytes, token strides at least head_dim (unless
- * there is one token) and below 4 Mi elements.
+ * there is one token) and below 4 Mi elements; no row of a result on another.  At
+ * most 0x7ffff000 query and key rows.
  * bias: [heads, 2 * reach + 1] or NULL (reach is then ignored); reach in
  * [0, 2047].  out must not overlap the other tensors. */
 typedef struct {

@@ -145,6 +145,27 @@ def test_attention_refuses_rows(bad):
         assert not ok and b"attention rows" in message, name
 
 
+@pytest.mark.parametrize("bad", [rows(head=0), rows(head=16), rows(token=64), rows(token=36, head=36)])
+def test_attention_refuses_results_on_one_another(bad):
+    """Rows that overlap are read (broadcast keys), but not written."""
+    ok, message = forward(desc(), out=bad)
+    assert not ok and b"results on one another" in message
+    for name in ("dq", "dk", "dv"):
+        ok, message = backward(desc(kv_heads=4), **{name: bad})
+        assert not ok and b"results on one another" in message, name
+    # Read rows pass that check: the workspace is what is missing here.
+    shared = rows(head=0)
+    ok, message = backward(desc(), work=None, q=shared, k=shared, v=shared, out=shared, dout=shared)
+    assert not ok and b"workspace" in message
+
+
+def test_attention_refuses_too_many_rows():
+    for bad in (dict(q_tokens=0x7fffffff), dict(k_tokens=0x7fffffff)):
+        for f in (forward, backward):
+            ok, message = f(desc(**bad))
+            assert not ok and b"invalid attention" in message
+
+
 def test_attention_backward_refuses():
     assert b"invalid" in backward(desc(), lse=None)[1]
     assert b"invalid" in backward(desc(bias=None))[1]  # a bias's gradient without one
