@@ -84,12 +84,13 @@ struct KeyTile {
 
 // KB blocks of 16 keys per wave.  Scores come out with a key per lane, so P and
 // dS are the second operands of dv^T = dout^T P and dk^T = q^T dS without
-// leaving their registers.  8192 causal tokens, 16 heads of 128 on 4, bf16: 305
-// us, 0.61 PFLOP/s: q and dout are read from LDS twice, as rows and transposed,
+// leaving their registers.  8192 causal tokens, 16 heads of 128 on 4, bf16: 267
+// us, 0.70 PFLOP/s: q and dout are read from LDS twice, as rows and transposed,
 // for KB x 16 keys, and with the registers for two waves per SIMD the reads'
-// latency shows (matrix cores 34 % busy, LDS 41 %; two blocks of keys halve the
-// reads but leave one wave per SIMD: 380 us; three waves on tiles of 32 queries
-// 324).
+// latency shows (matrix cores 32 % busy, LDS 36 %).  Measured when this one took
+// 300 us: two blocks of keys, which halve the reads but leave one wave per SIMD,
+// 380; three waves on tiles of 32 queries 324; parts that are dealt last
+// instead of one after the other 300 (the longest work then ends the grid).
 template <class E, int DIM, int KB, int WAVES, bool BIAS>
 __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArgs a) {
     using K = KeyTile<E, DIM, KB, WAVES>;
@@ -360,7 +361,7 @@ constexpr int tile_keys(int size, int dim) { return size == 4 && dim > 64 ? 32 :
 // IB blocks of 16 queries per wave, four waves.  Scores come out with a query
 // per lane, so dS is the second operand of dq^T = k^T dS^T without leaving its
 // registers.  Bound by the matrix cores and the exponentials: the same tokens
-// 147 us, 0.95 PFLOP/s.
+// 149 us, 0.93 PFLOP/s.
 template <class E, int DIM, int IB, bool BIAS>
 __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     constexpr int kRows = 64 * IB, kKB = DIM / 32, kDB = DIM / 16, kKeys = tile_keys(E::kSize, DIM);

@@ -8,7 +8,7 @@ namespace bfhip {
 // out[i] = sum over p of partial[p][i], i < n; from `split` on the results go to
 // out2[i - split].  A workgroup has 16 neighbouring columns and 32 shares of the
 // parts, eight loads in flight each, added up in order at the end.  Bound by the
-// latency of its loads (512 parts of 1536 columns: 5 us, 11 with 16 shares and
+// latency of its loads (512 parts of 1536 columns: 4 us, 11 with 16 shares and
 // one load in flight).
 constexpr int kSumThreads = 512;
 
