@@ -393,6 +393,18 @@ __device__ __forceinline__ typename E::Frag rest_frag(const f32x4 &a, const f32x
     return to_frag<E>(x, y);
 }
 
+// Sum of the products of two fragments' eight values.
+template <class E>
+__device__ __forceinline__ float frag_dot(const typename E::Frag &a, const typename E::Frag &b) {
+    typedef typename E::Word Words8 __attribute__((ext_vector_type(8)));
+    const f32x8 x = __builtin_convertvector(__builtin_bit_cast(Words8, a), f32x8);
+    const f32x8 y = __builtin_convertvector(__builtin_bit_cast(Words8, b), f32x8);
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+    return s;
+}
+
 // Stores an accumulated transposed product of DB x 16 elements by 16 rows: lane
 // l holds row l & 15 (at `row`, if `live`), elements 16 db + 4 (l >> 4) ..+3.
 template <class E, int DB>

@@ -4,10 +4,10 @@
 //   delta_i = dout_i . out_i,  ds_ij = p_ij (dout_i . v_j - delta_i),
 //   dv_j = sum_i p_ij dout_i,  dk_j = scale sum_i ds_ij q_i,
 //   dq_i = scale sum_j ds_ij k_j,  dbias[e] = sum of ds over pairs at e.
-// Three passes: the row terms (delta and lse); dq and dbias, a workgroup per
-// tile of queries and head that walks the keys; dk and dv, a workgroup per tile
-// of keys and key head that walks the queries of the group's heads.  Walking
-// twice costs two products of seven more than adding dq up with atomics would,
+// Two passes: dq and dbias, a workgroup per tile of queries and head that walks
+// the keys, and writes the rows' delta and lse for the second; dk and dv, a
+// workgroup per tile of keys and key head that walks the queries of the group's
+// heads.  Walking twice costs two products of seven more than adding dq up with atomics would,
 // and gives the same bits every time.
 //
 // Precision of the 16-bit types.  p and ds are rounded to the type for the matrix
@@ -35,34 +35,10 @@ constexpr int kFineKeys = 256;  // see above
 struct GradArgs {
     AttnArgs f;
     AttnRows dout, dq, dk, dv;
-    float *nlse, *delta;  // [heads, q_tokens]
+    float *nlse, *delta;  // [heads, q_tokens]; nlse: -lse in base 2, -inf for a query without keys (every p is then 0)
     float *part;          // dbias: [query slots, heads, 2 reach + 1] or null
     float *part_kv;       // f.parts > 1: [parts][k_tokens][kv_heads][dk, dv][padded dim]
 };
-
-// -lse in base 2 (-inf for a query without keys: every p of it is then 0), and
-// delta; 16 lanes per (token, head).
-template <class E>
-__global__ __launch_bounds__(256) void attention_terms_kernel(GradArgs a) {
-    const long long id = (long long)blockIdx.x * 16 + threadIdx.x / 16;
-    if (id >= a.f.q_tokens * a.f.heads) return;
-    const long long t = id / a.f.heads;
-    const int h = (int)(id % a.f.heads), d = 8 * (threadIdx.x % 16);
-    float sum = 0.f;
-    if (d < a.f.dim && !a.part) {
-        using W = Words<E, 8>;
-        const W o = *reinterpret_cast<const W *>(__builtin_assume_aligned(a.f.out.at(t, h) + d * E::kSize, 16));
-        const W g = *reinterpret_cast<const W *>(__builtin_assume_aligned(a.dout.at(t, h) + d * E::kSize, 16));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(o.get(e), g.get(e), sum);
-    }
-    sum = group_sum<16>(sum);
-    if (threadIdx.x % 16) return;
-    const size_t at = (size_t)h * a.f.q_tokens + t;
-    const float lse = a.f.lse[at];
-    a.nlse[at] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;
-    a.delta[at] = sum;
-}
 
 // The queries that a tile of keys meets, as steps of 64 queries of one head.
 struct Steps {
@@ -407,6 +383,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             for (int i = lane; i < width; i += kWave) sums[i] = 0.f;
     }
 
+    const bool fine = E::kSize == 2 && last <= kFineKeys, sum_delta = fine || part;
     typename E::Frag qf[IB][kKB], gf[IB][kKB];
     f32x4 dq[IB][kDB];
     float nlse[IB], delta[IB];
@@ -419,9 +396,21 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             qf[ib][kk] = global_frag<E>(f.q.at((long long)s.start + r0, head), f.q.token, s.length - r0, f.dim, kk, lane);
             gf[ib][kk] = global_frag<E>(a.dout.at((long long)s.start + r0, head), a.dout.token, s.length - r0, f.dim, kk, lane);
         }
+        delta[ib] = 0.f;
+        if (!sum_delta) {
+#pragma unroll
+            for (int kk = 0; kk < kKB; ++kk)
+                delta[ib] += frag_dot<E>(gf[ib][kk], global_frag<E>(f.out.at((long long)s.start + r0, head), f.out.token, s.length - r0, f.dim, kk, lane));
+            delta[ib] += __shfl_xor(delta[ib], 16);
+            delta[ib] += __shfl_xor(delta[ib], 32);
+        }
         const size_t at = (size_t)head * f.q_tokens + s.start + r;
-        nlse[ib] = r < s.length ? a.nlse[at] : -INFINITY;
-        delta[ib] = r < s.length ? a.delta[at] : 0.f;
+        const float lse = r < s.length ? f.lse[at] : -INFINITY;
+        nlse[ib] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;
+        if (g == 0 && r < s.length) {
+            a.nlse[at] = nlse[ib];
+            if (!sum_delta) a.delta[at] = delta[ib];
+        }
         limit[ib] = f.causal ? min(k_len, r + offset + 1) : k_len;
 #pragma unroll
         for (int db = 0; db < kDB; ++db) dq[ib][db] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -464,11 +453,8 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         }
     };
     int buffer = 0;
-    const bool fine = E::kSize == 2 && last <= kFineKeys, sum_delta = fine || part;
     if constexpr (BIAS || E::kSize == 2) {
         if (sum_delta) {
-#pragma unroll
-            for (int ib = 0; ib < IB; ++ib) delta[ib] = 0.f;
             if (tiles > 0) issue(0, buffer);
             for (int t = 0; t < tiles; ++t, buffer ^= 1) {
                 wait_vmcnt<0>();
@@ -634,10 +620,10 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     const size_t need = 2 * p.terms + p.part + p.part_kv;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
-    const long long terms = (d->q_tokens * d->heads + 15) / 16, q_grid = p.q_slots * d->heads;
+    const long long q_grid = p.q_slots * d->heads;
     const long long k_grid = p.k_slots * d->kv_heads * p.parts;
     const long long joins = p.parts > 1 ? ((long long)d->kv_heads * 2 * p.dim + 1023) / 1024 * d->k_tokens : 0;
-    if (!launch_fits(terms, 256) || !launch_fits(q_grid, 256) || !launch_fits(k_grid, 256) || !launch_fits(joins, 256))
+    if (!launch_fits(q_grid, 256) || !launch_fits(k_grid, 256) || !launch_fits(joins, 256))
         return fail(error, cap, "attention has too many rows");
     GradArgs a{};
     a.f = attn_args(d, q, k, v, out, const_cast<float *>(lse));
@@ -661,7 +647,6 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                 constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), WAVES = 4, KB = key_blocks(E::kSize, DIM);
                 using K = KeyTile<E, DIM, KB, WAVES>;
                 using T = AttnTile<E, DIM>;
-                if (terms) hipLaunchKernelGGL(attention_terms_kernel<E>, dim3((unsigned)terms), dim3(256), 0, s, a);
                 const auto run = [&](auto with_bias) {
                     constexpr bool B = decltype(with_bias)::value;
                     const size_t row = B ? BiasRow::floats(d->reach) * sizeof(float) : 0;
