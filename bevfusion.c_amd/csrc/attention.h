@@ -30,7 +30,7 @@ struct AttnArgs {
     int flip;             // the queries' signs change (forward)
     int ordered;          // tiles in the order of their work
     int parts;            // most parts that a sequence's keys are split into
-    int chunk;            // keys (few queries) or steps (backward) of a part, at least
+    int chunk;            // keys (few queries), tiles (forward) or steps (backward) of a part, at least
     float *part_out;      // parts > 1: sums of each part, [parts][q_tokens][heads][padded dim]
     float2 *part_stat;    // and their (m, l), [parts][q_tokens][heads]
 };

@@ -584,9 +584,10 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     p.q_slots = slot_count(d->q_tokens, d->sequences, p.q_rows);
     p.k_slots = slot_count(d->k_tokens, d->sequences, p.k_rows);
     // Parts of 16 tiles of queries or more, as many as the average sequence has;
-    // of 4 or more where there is less than a workgroup per CU.
+    // of 4 or more where there is less than a workgroup per CU, 2 in fp32, whose
+    // products take longer.
     const long long units = p.k_slots * d->kv_heads, group = d->heads / d->kv_heads;
-    p.chunk = units < 256 ? 4 : 16;
+    p.chunk = units >= 256 ? 16 : size == 4 ? 2 : 4;
     const long long rows = units < 256 ? d->q_tokens : d->sequences ? d->q_tokens / d->sequences : 0;
     const long long parts = units ? 2048 / units : 1, steps = rows * group / (kTile * p.chunk);
     p.parts = (int)std::max(1ll, std::min({32ll, parts, steps}));

@@ -16,7 +16,6 @@ using namespace bfhip;
 namespace {
 
 constexpr int kKeys = 64;      // keys per tile
-constexpr int kPartTiles = 4;  // fewest tiles of a part
 
 // Running maximum, sum and result of IB blocks of 16 queries, one wave's.
 template <int IB, int DB>
@@ -128,7 +127,7 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     // Keys that the wave has work on.
     const int own = row0 >= s.length ? 0 : a.causal ? min(k_len, min(row0 + 16 * IB, s.length) + offset) : k_len;
     const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0;
-    const int per = part_tiles(tiles, a.parts, kPartTiles), begin = part * per, end = min(tiles, begin + per);
+    const int per = part_tiles(tiles, a.parts, a.chunk), begin = part * per, end = min(tiles, begin + per);
     if (part && begin >= tiles) return;
 
     AttnTileCopy<E, DIM, kKeys, 256> kc, vc;
@@ -415,14 +414,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
     int q_start, q_len, k_start, k_len;
     sequence_rows(a.q_starts, sequence, a.q_tokens, q_start, q_len);
     sequence_rows(a.k_starts, sequence, a.k_tokens, k_start, k_len);
-    int keys = k_len, least = a.chunk, size = 32;
+    int keys = k_len, size = 32, least = a.chunk / size;
     if constexpr (ROWS > 0) {
         const int tile = (token - q_start) / ROWS * ROWS;
         if (a.causal) keys = min(k_len, min(tile + ROWS, q_len) + k_len - q_len);
         size = kKeys;
-        least = kPartTiles * kKeys;
+        least = a.chunk;
     }
-    const int tiles = keys > 0 ? (keys + size - 1) / size : 0, per = part_tiles(tiles, a.parts, least / size);
+    const int tiles = keys > 0 ? (keys + size - 1) / size : 0, per = part_tiles(tiles, a.parts, least);
     const int used = max(1, (tiles + per - 1) / per);
     if (ROWS == 0 && used == 1) return;  // written by the kernel before
     const size_t step = (size_t)a.q_tokens * a.heads, row = (size_t)token * a.heads + min(head, a.heads - 1);
@@ -478,7 +477,9 @@ constexpr int query_rows(int size) { return size == 4 ? 64 : 128; }
 // workgroups read keys whatever the lengths are, and a sequence has at most
 // `parts` of them; otherwise a tile's keys are split into as many parts as
 // bring about four workgroups per CU, but no more than the average sequence has
-// keys for.
+// keys for, four tiles or more in each.  fp32's products take eight times as long
+// as other types', so that a walk costs more than a join where CUs are idle: parts
+// of two tiles, as many as the longest sequence may have.
 struct ForwardPlan {
     bool few;
     int rows, parts, chunk, dim;
@@ -507,7 +508,9 @@ ForwardPlan forward_plan(const bfhip_attention_desc *d) {
     // Slots are at most one per sequence more than there is work for.
     const long long tiles = (d->q_tokens + p.rows - 1) / p.rows;
     const long long units = (tiles > d->sequences ? tiles : d->sequences) * d->heads;
-    const long long keys = d->k_tokens / d->sequences / (kPartTiles * kKeys), parts = 1024 / units;
+    const bool longest = size == 4 && units < 256;
+    p.chunk = longest ? 2 : 4;
+    const long long keys = (longest ? d->k_tokens : d->k_tokens / d->sequences) / (p.chunk * kKeys), parts = 1024 / units;
     p.parts = (int)(parts < 1 || keys < 1 ? 1 : parts < keys ? parts : keys);
     p.grid = p.slots * d->heads * p.parts;
     return p;
