@@ -38,6 +38,9 @@ struct GradArgs {
     float *nlse, *delta;  // [heads, q_tokens]; nlse: -lse in base 2, -inf for a query without keys (every p is then 0)
     float *part;          // dbias: [query slots, heads, 2 reach + 1] or null
     float *part_kv;       // f.parts > 1: [parts][k_tokens][kv_heads][dk, dv][padded dim]
+    float *part_q;        // q_parts > 1: dq, [parts][q_tokens][heads][padded dim]
+    int q_parts, q_chunk; // most parts that a sequence's keys are split into, and their tiles, at least
+    int joins;            // workgroups that join dk and dv, before those of dq
 };
 
 // The queries that a tile of keys meets, as steps of 64 queries of one head.
@@ -257,12 +260,50 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
     }
 }
 
+// Keys per tile: two tiles of keys and values, and five rows of the longest
+// bias, have to fit the LDS.
+constexpr int tile_keys(int size, int dim) { return size == 4 && dim > 64 ? 32 : 64; }
+
+// Blocks of 16 rows per wave: two, so that a fragment read from LDS serves two
+// products; one for fp32, whose products take eight times as long as the reads.
+constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
+
+// dq of one token from the parts' sums, in order: four elements per thread.
+template <class E, int DIM>
+__device__ __forceinline__ void join_queries(const GradArgs &a, int block) {
+    constexpr int kPer = 256 * 4 / DIM, kRows = 64 * row_blocks(E::kSize), kKeys = tile_keys(E::kSize, DIM);
+    const AttnArgs &f = a.f;
+    const int per_token = (f.heads + kPer - 1) / kPer, token = block / per_token;
+    const int head = block % per_token * kPer + threadIdx.x / (DIM / 4), d = threadIdx.x % (DIM / 4) * 4;
+    const int sequence = find_token(f.q_starts, f.sequences, f.q_tokens, token);
+    if (sequence < 0 || head >= f.heads) return;
+    int q_start, q_len, k_start, k_len;
+    sequence_rows(f.q_starts, sequence, f.q_tokens, q_start, q_len);
+    sequence_rows(f.k_starts, sequence, f.k_tokens, k_start, k_len);
+    const int tile = (token - q_start) / kRows * kRows;
+    const int last = f.causal ? min(k_len, min(tile + kRows, q_len) + k_len - q_len) : k_len;
+    const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0, per = part_tiles(tiles, a.q_parts, a.q_chunk);
+    if (per >= tiles) return;  // written by the queries' walk
+    const int used = (tiles + per - 1) / per;
+    const size_t step = (size_t)f.q_tokens * f.heads * DIM;
+    const float *const at = a.part_q + ((size_t)token * f.heads + head) * DIM + d;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < used; ++p) v += *reinterpret_cast<const f32x4 *>(at + p * step);
+    if (d >= f.dim) return;
+    Words<E, 4> w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w.put(e, v[e] * f.scale);
+    w.store(reinterpret_cast<typename E::Word *>(a.dq.at(token, head)) + d);
+}
+
 // dk and dv from the parts' sums, in order: four elements per thread, 2 DIM / 4
-// threads per key and key head.
+// threads per key and key head; and, by the workgroups behind, dq.
 template <class E, int DIM, int ROWS>
-__global__ __launch_bounds__(256) void attention_keys_join_kernel(GradArgs a) {
+__global__ __launch_bounds__(256) void attention_gradient_join_kernel(GradArgs a) {
     constexpr int kPer = 256 * 4 / (2 * DIM);  // key heads of a workgroup, all of one token
     const AttnArgs &f = a.f;
+    if ((int)blockIdx.x >= a.joins) return join_queries<E, DIM>(a, blockIdx.x - a.joins);
     const int per_token = (f.kv_heads + kPer - 1) / kPer, token = blockIdx.x / per_token;
     const int kv = blockIdx.x % per_token * kPer + threadIdx.x / (DIM / 2), d = threadIdx.x % (DIM / 2) * 4;
     const int sequence = find_token(f.k_starts, f.sequences, f.k_tokens, token);
@@ -330,10 +371,6 @@ __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int rea
     if (i >= 13) add(far0 + 4 * g + 16 - i, rest);
 }
 
-// Keys per tile: two tiles of keys and values, and five rows of the longest
-// bias, have to fit the LDS.
-constexpr int tile_keys(int size, int dim) { return size == 4 && dim > 64 ? 32 : 64; }
-
 // IB blocks of 16 queries per wave, four waves.  Scores come out with a query
 // per lane, so dS is the second operand of dq^T = k^T dS^T without leaving its
 // registers.  Bound by the matrix cores and the exponentials: the same tokens
@@ -348,7 +385,9 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     const AttnArgs &f = a.f;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int l16 = lane & 15, g = lane >> 4;
-    const Deal deal_ = deal(blockIdx.x, f.heads, f.kv_heads);
+    constexpr bool kParts = E::kSize == 4 && !BIAS;  // (backward_plan)
+    const int items = f.slots * f.heads, nth = kParts ? blockIdx.x / items : 0;  // part of the keys
+    const Deal deal_ = deal(kParts ? blockIdx.x % items : blockIdx.x, f.heads, f.kv_heads);
     const int head = deal_.head, kv = head / (f.heads / f.kv_heads), width = 2 * f.reach + 1;
     const Slot s = ranked_rows<kRows, false>(f.q_starts, f.sequences, f.q_tokens, deal_.rank, f.slots, f.ordered);
     float *const part = BIAS && a.part ? a.part + ((size_t)deal_.rank * f.heads + head) * width : nullptr;
@@ -365,6 +404,9 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     // Keys that the wave has work on.
     const int own = row0 >= s.length ? 0 : f.causal ? min(k_len, min(row0 + 16 * IB, s.length) + offset) : k_len;
     const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0;
+    const int per = kParts ? part_tiles(tiles, a.q_parts, a.q_chunk) : tiles;
+    const int begin = nth * per, end = min(tiles, begin + per);
+    if (kParts && nth && begin >= tiles) return;
 
     AttnTileCopy<E, DIM, kKeys, 256> kc, vc;
     kc.init(f.k.token, f.dim, threadIdx.x);
@@ -407,7 +449,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         const size_t at = (size_t)head * f.q_tokens + s.start + r;
         const float lse = r < s.length ? f.lse[at] : -INFINITY;
         nlse[ib] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;
-        if (g == 0 && r < s.length) {
+        if (nth == 0 && g == 0 && r < s.length) {
             a.nlse[at] = nlse[ib];
             if (!sum_delta) a.delta[at] = delta[ib];
         }
@@ -454,7 +496,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     };
     int buffer = 0;
     if constexpr (BIAS || E::kSize == 2) {
-        if (sum_delta) {
+        if (sum_delta) {  // (there is one part then)
             if (tiles > 0) issue(0, buffer);
             for (int t = 0; t < tiles; ++t, buffer ^= 1) {
                 wait_vmcnt<0>();
@@ -481,12 +523,12 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             }
         }
     }
-    if (tiles > 0 && !sum_delta) issue(0, buffer);
+    if (begin < end && !sum_delta) issue(begin, buffer);
     float low = 0.f, high = 0.f;
-    for (int t = 0; t < tiles; ++t, buffer ^= 1) {
+    for (int t = begin; t < end; ++t, buffer ^= 1) {
         wait_vmcnt<0>();
         lds_barrier();  // this tile is there, and the one before has been read
-        if (t + 1 < tiles) issue(t + 1, buffer ^ 1);
+        if (t + 1 < end) issue(t + 1, buffer ^ 1);
         const char *const kt = smem + buffer * kStage, *const vt = kt + kKeys * T::kRow;
         const int j0 = t * kKeys;
         if (j0 >= own) continue;
@@ -543,6 +585,13 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
 #pragma unroll
     for (int ib = 0; ib < IB; ++ib) {
         const int r = row0 + 16 * ib + l16;
+        if (kParts && per < tiles) {
+            if (r >= s.length) continue;
+            float *const row = a.part_q + (((size_t)nth * f.q_tokens + s.start + r) * f.heads + head) * DIM + 4 * g;
+#pragma unroll
+            for (int db = 0; db < kDB; ++db) *reinterpret_cast<f32x4 *>(row + 16 * db) = dq[ib][db];
+            continue;
+        }
         store_rows<E, kDB>(dq[ib], f.scale, a.dq.at((long long)s.start + r, head), r < s.length, f.dim, lane);
     }
     if constexpr (BIAS) {
@@ -561,18 +610,17 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     }
 }
 
-// Blocks of 16 rows per wave: two, so that a fragment read from LDS serves two
-// products; one for fp32, whose products take eight times as long as the reads.
-constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
-
 constexpr int key_blocks(int size, int dim) { return size == 4 || dim > 64 ? 1 : 2; }
 
 // How a call is dealt: slots of queries and of keys, and parts of the queries
-// that a tile of keys meets, so that uneven tiles even out over the CUs.
+// that a tile of keys meets, so that uneven tiles even out over the CUs.  Parts
+// of the keys that a tile of queries meets only in fp32, whose products take eight
+// times as long, and where there is less than a workgroup per CU (not with a
+// bias, whose gradient takes a walk over all keys first).
 struct BackwardPlan {
-    int dim, q_rows, k_rows, parts, chunk;
+    int dim, q_rows, k_rows, parts, chunk, q_parts, q_chunk;
     long long q_slots, k_slots;
-    size_t terms, part, part_kv;  // bytes
+    size_t terms, part, part_kv, part_q;  // bytes
 };
 
 BackwardPlan backward_plan(const bfhip_attention_desc *d) {
@@ -591,10 +639,15 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     const long long rows = units < 256 ? d->q_tokens : d->sequences ? d->q_tokens / d->sequences : 0;
     const long long parts = units ? 2048 / units : 1, steps = rows * group / (kTile * p.chunk);
     p.parts = (int)std::max(1ll, std::min({32ll, parts, steps}));
+    const long long q_units = std::max(1ll, d->q_tokens / p.q_rows) * d->heads;
+    p.q_chunk = 2 * 64 / tile_keys(size, p.dim);
+    p.q_parts = size == 4 && !d->bias && q_units < 256
+                    ? (int)std::max(1ll, std::min({32ll, 1024 / q_units, d->k_tokens / 128})) : 1;
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float));
     p.part = d->bias ? round((size_t)p.q_slots * d->heads * (2 * d->reach + 1) * sizeof(float)) : 0;
     p.part_kv = p.parts > 1 ? (size_t)p.parts * d->k_tokens * d->kv_heads * 2 * p.dim * sizeof(float) : 0;
+    p.part_q = p.q_parts > 1 ? (size_t)p.q_parts * d->q_tokens * d->heads * p.dim * sizeof(float) : 0;
     return p;
 }
 
@@ -603,7 +656,7 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
 extern "C" size_t bfhip_attention_backward_workspace(const bfhip_attention_desc *d) {
     if (bad_attention(d)) return 0;
     const BackwardPlan p = backward_plan(d);
-    return 2 * p.terms + p.part + p.part_kv;
+    return 2 * p.terms + p.part + p.part_kv + p.part_q;
 }
 
 extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfhip_rows *q, const bfhip_rows *k,
@@ -618,12 +671,13 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         bad_result(dk, d->k_tokens, d->kv_heads, n, size) || bad_result(dv, d->k_tokens, d->kv_heads, n, size))
         return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
     const BackwardPlan p = backward_plan(d);
-    const size_t need = 2 * p.terms + p.part + p.part_kv;
+    const size_t need = 2 * p.terms + p.part + p.part_kv + p.part_q;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
-    const long long q_grid = p.q_slots * d->heads;
+    const long long q_grid = p.q_slots * d->heads * p.q_parts;
     const long long k_grid = p.k_slots * d->kv_heads * p.parts;
-    const long long joins = p.parts > 1 ? ((long long)d->kv_heads * 2 * p.dim + 1023) / 1024 * d->k_tokens : 0;
+    const long long k_joins = p.parts > 1 ? ((long long)d->kv_heads * 2 * p.dim + 1023) / 1024 * d->k_tokens : 0;
+    const long long joins = k_joins + (p.q_parts > 1 ? ((long long)d->heads * p.dim + 1023) / 1024 * d->q_tokens : 0);
     if (!launch_fits(q_grid, 256) || !launch_fits(k_grid, 256) || !launch_fits(joins, 256))
         return fail(error, cap, "attention has too many rows");
     GradArgs a{};
@@ -639,6 +693,10 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     a.delta = (float *)(work + p.terms);
     a.part = dbias ? (float *)(work + 2 * p.terms) : nullptr;
     a.part_kv = (float *)(work + 2 * p.terms + p.part);
+    a.part_q = (float *)(work + 2 * p.terms + p.part + p.part_kv);
+    a.q_parts = p.q_parts;
+    a.q_chunk = p.q_chunk;
+    a.joins = (int)k_joins;
     hipStream_t s = (hipStream_t)stream;
     const long long width = 2 * a.f.reach + 1;
     if (d->sequences)
@@ -668,7 +726,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                 if (d->bias) run(std::true_type{});
                 else run(std::false_type{});
                 if (joins)
-                    hipLaunchKernelGGL((attention_keys_join_kernel<E, DIM, K::kRows>), dim3((unsigned)joins), dim3(256), 0, s, a);
+                    hipLaunchKernelGGL((attention_gradient_join_kernel<E, DIM, K::kRows>), dim3((unsigned)joins), dim3(256), 0, s, a);
             });
         });
     const long long count = width * d->heads;

@@ -117,8 +117,8 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  *
  * Workspaces: the forward's holds the sums of keys that are split (few queries
  * on many keys, at most some 300 MB; mostly none), the backward's two fp32 per
- * query and head, sums of queries that are split (at most some 150 MB), and with
- * a bias 2 * reach + 1 fp32 per head and 64 or 128 queries.
+ * query and head, sums of queries that are split (at most some 150 MB; of keys
+ * in fp32, some 35 MB), and with a bias 2 * reach + 1 fp32 per head and 64 or 128 queries.
  *
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
  * stride in elements; the elements of one head are contiguous, pointers and

@@ -569,6 +569,16 @@ def test_split_work_captured_and_replayed(device, case):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("case", [(F32, 6, 3, 32, [65, 1, 200, 0, 333, 9], [60, 130, 200, 17, 500, 9], True, None),
+                                  (F32, 2, 1, 128, [70, 3], [1000, 260], False, None),
+                                  (F32, 5, 5, 40, [129, 64], [33, 700], True, None),
+                                  (F32, 1, 1, 72, [300], [129], False, None)], ids=str)
+def test_queries_on_split_keys(device, case):
+    """fp32 gradients whose walks are split where CUs are idle."""
+    test_attention(device, case, "fused")
+    test_split_work_captured_and_replayed(device, case)
+
+
 def test_on_a_stream_of_its_own(device):
     s = block_inputs(device, 3)
     want = block(*s)
