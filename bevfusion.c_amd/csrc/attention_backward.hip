@@ -374,7 +374,8 @@ __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int rea
 // IB blocks of 16 queries per wave, four waves.  Scores come out with a query
 // per lane, so dS is the second operand of dq^T = k^T dS^T without leaving its
 // registers.  Bound by the matrix cores and the exponentials: the same tokens
-// 149 us, 0.93 PFLOP/s.
+// 156 us, 0.89 PFLOP/s, the rows' delta included (a launch of its own for it took
+// 17 us more).
 template <class E, int DIM, int IB, bool BIAS>
 __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     constexpr int kRows = 64 * IB, kKB = DIM / 32, kDB = DIM / 16, kKeys = tile_keys(E::kSize, DIM);
