@@ -31,6 +31,7 @@ struct AttnArgs {
     int ordered;          // tiles in the order of their work
     int parts;            // most parts that a sequence's keys are split into
     int chunk;            // keys (few queries), tiles (forward) or steps (backward) of a part, at least
+    int few_rows;         // > 0: sequences of no more queries x group are attention_few_kernel's
     float *part_out;      // parts > 1: sums of each part, [parts][q_tokens][heads][padded dim]
     float2 *part_stat;    // and their (m, l), [parts][q_tokens][heads]
 };

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     const Deal deal_ = deal(blockIdx.x % items, a.heads, a.kv_heads);
     const int head = deal_.head, kv = head / (a.heads / a.kv_heads);
     const Slot s = ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.ordered);
-    if (s.sequence < 0) return;
+    if (s.sequence < 0 || s.length <= a.few_rows / (a.heads / a.kv_heads)) return;
     int k_start, k_len;
     sequence_rows(a.k_starts, s.sequence, a.k_tokens, k_start, k_len);
     const int offset = k_len - s.length;  // query i stands at position i + offset
@@ -275,6 +275,7 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
     int q_start, q_len;
     sequence_rows(a.q_starts, s.sequence, a.q_tokens, q_start, q_len);
     const int offset = k_len - q_len, rows = q_len * group;
+    if (a.few_rows && rows > a.few_rows) return;
 
     AttnTileCopy<E, DIM, kKeyRows, kWave> kc, vc;
     kc.init(a.k.token, a.dim, lane);
@@ -414,6 +415,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
     int q_start, q_len, k_start, k_len;
     sequence_rows(a.q_starts, sequence, a.q_tokens, q_start, q_len);
     sequence_rows(a.k_starts, sequence, a.k_tokens, k_start, k_len);
+    if (ROWS == 0 && a.few_rows && q_len * (a.heads / a.kv_heads) > a.few_rows) return;
     int keys = k_len, size = 32, least = a.chunk / size;
     if constexpr (ROWS > 0) {
         const int tile = (token - q_start) / ROWS * ROWS;
@@ -471,7 +473,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
 constexpr int query_rows(int size) { return size == 4 ? 64 : 128; }
 
 // How a call is dealt.  `few`: so few queries per sequence that a key head's
-// group of them fills at most two tiles of 16 rows on average.  The keys are
+// group of them fills at most a tile of 16 rows on average, or one query each; where there are more
+// queries than sequences (`mixed`), only the sequences that do are dealt so, and the
+// others, prompts among single tokens, by a second launch.  On 2000 keys a
+// sequence, 32 heads of 128 on 8, bf16: 48 x 4 queries 110 us, 177 by the
+// launch for prompts alone; 63 single tokens and a prompt of 400 267 us, 1497 if all were
+// dealt as few.
+// The keys are
 // split into parts where the work would leave CUs idle: `few` takes parts of
 // `chunk` keys, a 1536th of all that is read (a tile or more), so that about 1536
 // workgroups read keys whatever the lengths are, and a sequence has at most
@@ -481,8 +489,8 @@ constexpr int query_rows(int size) { return size == 4 ? 64 : 128; }
 // as other types', so that a walk costs more than a join where CUs are idle: parts
 // of two tiles, as many as the longest sequence may have.
 struct ForwardPlan {
-    bool few;
-    int rows, parts, chunk, dim;
+    bool few, mixed;
+    int rows, parts, chunk, dim, few_rows;
     long long slots, grid;
 };
 
@@ -492,7 +500,9 @@ ForwardPlan forward_plan(const bfhip_attention_desc *d) {
     p.dim = d->head_dim <= 32 ? 32 : d->head_dim <= 64 ? 64 : 128;
     p.parts = 1;
     if (!d->sequences || !d->q_tokens) return p;
-    p.few = d->q_tokens * group <= 32ll * d->sequences && d->q_tokens * group < 1 << 30;
+    p.few_rows = group > 16 ? group : 16;
+    p.few = d->q_tokens * group <= (long long)p.few_rows * d->sequences && d->q_tokens * group < 1 << 30;
+    p.mixed = p.few && d->q_tokens > d->sequences;
     p.rows = query_rows(size);
     if (p.few) {
         const long long units = (long long)d->sequences * d->kv_heads, least = size * p.dim <= 128 ? 128 : 64;
@@ -543,12 +553,14 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
     if (!d->sequences || !d->q_tokens) return 1;
     const long long joins = p.parts > 1 ? ((long long)d->heads * p.dim + 255) / 256 * d->q_tokens : 0;
-    if (!launch_fits(p.grid, 256) || !launch_fits(joins, 256)) return fail(error, cap, "attention has too many rows");
+    const long long rest_slots = p.mixed ? slot_count(d->q_tokens, d->sequences, p.rows) : 0, rest = rest_slots * d->heads;
+    if (!launch_fits(p.grid, 256) || !launch_fits(rest, 256) || !launch_fits(joins, 256)) return fail(error, cap, "attention has too many rows");
     AttnArgs a = attn_args(d, q, k, v, out, lse);
     a.slots = (int)p.slots;
     a.parts = p.parts;
     a.chunk = p.chunk;
     a.ordered = by_work(d, p.grid);
+    a.few_rows = p.mixed ? p.few_rows : 0;
     // Scores are compared before they are scaled, which takes a positive scale:
     // a negative one flips the queries' signs, and zero becomes one so small
     // that it makes no score differ.
@@ -569,6 +581,13 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
                 const size_t lds = 4 * kKeys * T::kRow + (B ? BiasRow::floats(d->reach) * sizeof(float) : 0);
                 if (p.few) hipLaunchKernelGGL((attention_few_kernel<E, DIM, B>), grid, dim3(Few::kThreads), 0, s, a);
                 else hipLaunchKernelGGL((attention_forward_kernel<E, DIM, IB, B>), grid, dim3(256), lds, s, a);
+                if (p.mixed) {
+                    AttnArgs b = a;
+                    b.slots = (int)rest_slots;
+                    b.parts = 1;
+                    b.ordered = by_work(d, rest);
+                    hipLaunchKernelGGL((attention_forward_kernel<E, DIM, IB, B>), dim3((unsigned)rest), dim3(256), lds, s, b);
+                }
             };
             if (d->bias) run(std::true_type{});
             else run(std::false_type{});

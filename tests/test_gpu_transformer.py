@@ -579,6 +579,19 @@ def test_queries_on_split_keys(device, case):
     test_split_work_captured_and_replayed(device, case)
 
 
+@pytest.mark.parametrize("case", [(BF16, 8, 2, 128, [1] * 40 + [100, 0, 5, 4], [700] * 43 + [0], True, 30),
+                                  (F32, 4, 1, 40, [2, 0, 1, 0, 0, 0, 17, 0, 0], [3000, 5, 2000, 0, 7, 8, 900, 1, 0], True, None),
+                                  (F16, 3, 3, 64, [1, 16, 17, 3, 0, 0, 1], [90, 4000, 300, 1, 5, 0, 20], False, 4),
+                                  (F16, 20, 1, 32, [1, 2, 0, 0, 0, 0, 0, 0, 9], [900] * 9, True, None),
+                                  (F16, 20, 1, 32, [3, 0, 1, 0, 1, 0, 0, 2, 0, 0], [900] * 10, True, None),
+                                  (BF16, 6, 2, 32, [1] * 70 + [5, 6] + [0] * 8, [64] * 80, False, None)], ids=str)
+def test_prompts_among_single_tokens(device, case):
+    """Batches whose sequences are dealt in two ways, on either side of the
+    border between them."""
+    test_attention(device, case, "heads")
+    test_split_work_captured_and_replayed(device, case)
+
+
 def test_on_a_stream_of_its_own(device):
     s = block_inputs(device, 3)
     want = block(*s)
