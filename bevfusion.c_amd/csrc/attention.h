@@ -2,6 +2,8 @@
 // rows are, operand tiles in LDS, and their matrix-core fragments.
 #pragma once
 
+#include <cfloat>
+
 #include "bfhip_transformer.h"
 #include "element.h"
 #include "gemm_core.h"
@@ -322,7 +324,14 @@ __device__ __forceinline__ void col_frags_in_flight(const char *lds, int lane, t
     }
 }
 
-// A head's bias row in LDS, times log2 e, with its ends repeated kPad times so
+// A bias in base 2.  A finite one stays finite: the lowest fp32 value masks a key
+// beside others, but leaves a softmax where every key has it.
+__device__ __forceinline__ float base2_bias(float bias) {
+    const float b = bias * kLog2E;
+    return __builtin_isinf(b) && !__builtin_isinf(bias) ? __builtin_copysignf(FLT_MAX, bias) : b;
+}
+
+// A head's bias row in LDS, in base 2, with its ends repeated kPad times so
 // that a block of 16 x 16 scores that meets distances within the reach is read
 // without clamping.
 struct BiasRow {
@@ -332,7 +341,7 @@ struct BiasRow {
     __host__ __device__ __forceinline__ static int floats(int reach) { return 2 * (reach + kPad) + 1; }
     // Copies `bias` [2 reach + 1] to `lds` (the caller waits).
     __device__ __forceinline__ static BiasRow fill(float *lds, const float *bias, int reach, int thread, int threads) {
-        for (int i = thread; i < floats(reach); i += threads) lds[i] = bias[min(max(i - kPad, 0), 2 * reach)] * kLog2E;
+        for (int i = thread; i < floats(reach); i += threads) lds[i] = base2_bias(bias[min(max(i - kPad, 0), 2 * reach)]);
         return BiasRow{lds + reach + kPad, reach};
     }
     // Of the four distances from `at` on, in a block of 16 x 16 scores with the

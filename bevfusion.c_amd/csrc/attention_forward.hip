@@ -332,8 +332,8 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int far = min(max(j0 + 16 * jb + 4 * g + e - (token + offset), -a.reach), a.reach) + a.reach;
-                        const float b = live ? a.bias[(size_t)head * (2 * a.reach + 1) + far] : 0.f;
-                        sc[jb][0][e] = fmaf(b, kLog2E, sc[jb][0][e] * a.scale2);
+                        const float b = live ? base2_bias(a.bias[(size_t)head * (2 * a.reach + 1) + far]) : 0.f;
+                        sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, b);  // (rounded as in the other kernels)
                     }
             }
             if (j0 + kKeyRows > full) {

@@ -113,7 +113,9 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * they enter the matrix cores (where a query sees few keys, their rounding's rest
  * enters too).  A score's gradient beyond the type's range (fp16:
  * 65504) becomes infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
- * fp32: a bias near the lowest fp32 value swallows the score.
+ * fp32: a large bias (1e9, the lowest fp32 value) swallows the score, so that a
+ * query all of whose keys have it takes their mean.  Finite biases beyond 2.3e38
+ * of either sign count as that.
  *
  * Workspaces: the forward's holds the sums of keys that are split (few queries
  * on many keys, at most some 300 MB; mostly none), the backward's two fp32 per
