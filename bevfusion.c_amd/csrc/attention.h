@@ -325,7 +325,9 @@ __device__ __forceinline__ void col_frags_in_flight(const char *lds, int lane, t
 }
 
 // A bias in base 2.  A finite one stays finite: the lowest fp32 value masks a key
-// beside others, but leaves a softmax where every key has it.
+// beside others, but leaves a softmax where every key has it.  Up to kLargeBias
+// that takes nothing but the product.
+constexpr float kLargeBias = 2e38f;
 __device__ __forceinline__ float base2_bias(float bias) {
     const float b = bias * kLog2E;
     return __builtin_isinf(b) && !__builtin_isinf(bias) ? __builtin_copysignf(FLT_MAX, bias) : b;

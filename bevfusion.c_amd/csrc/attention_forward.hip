@@ -327,14 +327,21 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
                 for (int kk = 0; kk < kKB; ++kk) sc[jb][0] = E::mfma(row_frag<E, DIM>(kt, 16 * jb, kk, lane), qf[kk], sc[jb][0]);
             }
             if constexpr (BIAS) {
+                float b[2][4], most = 0.f;
 #pragma unroll
                 for (int jb = 0; jb < 2; ++jb)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int far = min(max(j0 + 16 * jb + 4 * g + e - (token + offset), -a.reach), a.reach) + a.reach;
-                        const float b = live ? base2_bias(a.bias[(size_t)head * (2 * a.reach + 1) + far]) : 0.f;
-                        sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, b);  // (rounded as in the other kernels)
+                        b[jb][e] = live ? a.bias[(size_t)head * (2 * a.reach + 1) + far] : 0.f;
+                        most = fmaxf(most, fabsf(b[jb][e]));
                     }
+                const bool large = __any(most > kLargeBias);
+#pragma unroll
+                for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)  // (rounded as in the other kernels)
+                        sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, large ? base2_bias(b[jb][e]) : b[jb][e] * kLog2E);
             }
             if (j0 + kKeyRows > full) {
                 const int j = j0 + 4 * g;
