@@ -19,6 +19,11 @@
 // dout . v in fp32, in a walk of its own over the keys.  A bias's gradient sums
 // very many ds, whose sum over a row is zero but for delta's error: with dbias,
 // delta is always summed so.
+//
+// lse is one fp32, so p is off by a factor of about 1 +- |lse| 2^-22: beside a
+// large bias log l is lost in it, and with it the sum of the row's p.  Where a
+// bias takes |lse| past far_lse, the queries' walk finds the row's maximum m and
+// sum l again, in a walk over the keys of its own, and p = 2^((s - m) - log2 l).
 #include <algorithm>
 #include <type_traits>
 
@@ -32,10 +37,14 @@ namespace {
 constexpr int kTile = 64;       // rows per LDS tile
 constexpr int kFineKeys = 256;  // see above
 
+// 1024 takes p off by less than the 16-bit types' rounding does.
+constexpr float far_lse(int size) { return size == 4 ? 64.f : 1024.f; }
+
 struct GradArgs {
     AttnArgs f;
     AttnRows dout, dq, dk, dv;
     float *nlse, *delta;  // [heads, q_tokens]; nlse: -lse in base 2, -inf for a query without keys (every p is then 0)
+    float *rest;          // with a bias: -log2 l where nlse is -m (see above), 0 elsewhere
     float *part;          // dbias: [query slots, heads, 2 reach + 1] or null
     float *part_kv;       // f.parts > 1: [parts][k_tokens][kv_heads][dk, dv][padded dim]
     float *part_q;        // q_parts > 1: dq, [parts][q_tokens][heads][padded dim]
@@ -54,11 +63,12 @@ __device__ __forceinline__ Steps query_steps(int causal, int first_key, int offs
     return s;
 }
 
-template <class E, int DIM, int KB, int WAVES>
+template <class E, int DIM, int KB, int WAVES, bool BIAS>
 struct KeyTile {
     static constexpr int kRows = WAVES * 16 * KB, kThreads = WAVES * kWave;
+    static constexpr int kTerms = BIAS ? 3 : 2;                // nlse, delta and rest of a query
     static constexpr int kQ = kTile * AttnTile<E, DIM>::kRow;  // bytes of a tile of q or dout
-    static constexpr int kStage = 2 * kQ + 2 * kTile * (int)sizeof(float);
+    static constexpr int kStage = 2 * kQ + kTerms * kTile * (int)sizeof(float);
 };
 
 // KB blocks of 16 keys per wave.  Scores come out with a key per lane, so P and
@@ -72,7 +82,7 @@ struct KeyTile {
 // instead of one after the other 300 (the longest work then ends the grid).
 template <class E, int DIM, int KB, int WAVES, bool BIAS>
 __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArgs a) {
-    using K = KeyTile<E, DIM, KB, WAVES>;
+    using K = KeyTile<E, DIM, KB, WAVES, BIAS>;
     constexpr int kRows = K::kRows, kKB = DIM / 32, kDB = DIM / 16, kThreads = K::kThreads;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const AttnArgs &f = a.f;
@@ -102,8 +112,8 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         gc.issue(a.dout.at((long long)q_start + i0, head), left, to + K::kQ);
         // Past the last query q, dout and the terms are zero: ds is 0, and p is 1
         // (or what a bias makes it, which may be infinite: masked below).
-        if (wave < 2)
-            dma4(buffer_rsrc((wave ? a.delta : a.nlse) + (size_t)head * f.q_tokens + q_start + i0, 4u * min(left, kTile)),
+        if (wave < K::kTerms)
+            dma4(buffer_rsrc((wave == 0 ? a.nlse : wave == 1 ? a.delta : a.rest) + (size_t)head * f.q_tokens + q_start + i0, 4u * min(left, kTile)),
                  to + 2 * K::kQ + wave * kTile * sizeof(float), 4u * lane);
     };
     typename E::Frag kf[KB][kKB], vf[KB][kKB];
@@ -142,6 +152,8 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         // A query that does not see every key of the wave's.
         const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
         const bool fine = E::kSize == 2 && (f.causal ? min(s.length, i0 + kTile + offset) : s.length) <= kFineKeys;
+        // Whether a query of the tile's has a rest.
+        const bool far = BIAS && __any(terms[2 * kTile + lane] != 0.f);
         // Scores of the whole tile first: the compiler waits for the copies in
         // flight before the transposed reads, which by then have had the time.
         typename E::Frag pf[2][KB], sf[2][KB];
@@ -176,6 +188,7 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                         const f32x4 b4 = bias.block(far0, far0 + l16 - 4 * g - 3);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = fmaf(p[b][kb][e], f.scale2, b4[3 - e]) + nlse[e];
+                        if (far) x += *reinterpret_cast<const f32x4 *>(terms + 2 * kTile + r0 + 4 * g);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = fmaf(p[b][kb][e], f.scale2, nlse[e]);
@@ -426,10 +439,22 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             for (int i = lane; i < width; i += kWave) sums[i] = 0.f;
     }
 
+    // Whether a row of the workgroup's is far; every wave looks at all rows.
+    bool far_tile = false;
+    if constexpr (BIAS) {
+        for (int r = s.first + lane; r < min(s.first + kRows, s.length); r += kWave) {
+            const float lse = f.lse[(size_t)head * f.q_tokens + s.start + r];
+            far_tile |= __builtin_isfinite(lse) && fabsf(lse) > far_lse(E::kSize);
+        }
+        far_tile = __any(far_tile);
+    }
+    // This wave's rows' rest, where one is far.
+    float *const rests = bias_row + BiasRow::floats(f.reach) + (part ? 4 * width : 0) + 16 * IB * wave;
     const bool fine = E::kSize == 2 && last <= kFineKeys, sum_delta = fine || part;
     typename E::Frag qf[IB][kKB], gf[IB][kKB];
     f32x4 dq[IB][kDB];
     float nlse[IB], delta[IB];
+    bool far_row[IB];
     int limit[IB];
 #pragma unroll
     for (int ib = 0; ib < IB; ++ib) {
@@ -450,24 +475,32 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         const size_t at = (size_t)head * f.q_tokens + s.start + r;
         const float lse = r < s.length ? f.lse[at] : -INFINITY;
         nlse[ib] = lse == -INFINITY ? -INFINITY : -lse * kLog2E;
+        far_row[ib] = BIAS && __builtin_isfinite(lse) && fabsf(lse) > far_lse(E::kSize);
         if (nth == 0 && g == 0 && r < s.length) {
             a.nlse[at] = nlse[ib];
+            if constexpr (BIAS) a.rest[at] = 0.f;
             if (!sum_delta) a.delta[at] = delta[ib];
         }
         limit[ib] = f.causal ? min(k_len, r + offset + 1) : k_len;
 #pragma unroll
         for (int db = 0; db < kDB; ++db) dq[ib][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // p and dp = dout . v of 16 keys from tile row r0.
-    const auto products = [&](const char *kt, const char *vt, int j0, int r0, f32x4 (&p)[IB], f32x4 (&dp)[IB]) {
+    // q . k of 16 keys from tile row r0.
+    const auto scores = [&](const char *kt, int r0, f32x4 (&p)[IB]) {
 #pragma unroll
-        for (int ib = 0; ib < IB; ++ib) p[ib] = dp[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int ib = 0; ib < IB; ++ib) p[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < kKB; ++kk) {
             const typename E::Frag kf = row_frag<E, DIM>(kt, r0, kk, lane);
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib) p[ib] = E::mfma(kf, qf[ib][kk], p[ib]);
         }
+    };
+    // p and dp = dout . v of 16 keys from tile row r0.
+    const auto products = [&](const char *kt, const char *vt, int j0, int r0, f32x4 (&p)[IB], f32x4 (&dp)[IB]) {
+        scores(kt, r0, p);
+#pragma unroll
+        for (int ib = 0; ib < IB; ++ib) dp[ib] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < kKB; ++kk) {
             const typename E::Frag vf = row_frag<E, DIM>(vt, r0, kk, lane);
@@ -480,7 +513,10 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             if constexpr (BIAS) {  // (rounded as the forward's scores are)
                 const f32x4 b4 = bias.block(far0, far0 + 4 * g - l16);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, b4[e]) + nlse[ib]);
+                for (int e = 0; e < 4; ++e) p[ib][e] = fmaf(p[ib][e], f.scale2, b4[e]) + nlse[ib];
+                if (far_tile) p[ib] += rests[16 * ib + l16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(p[ib][e]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) p[ib][e] = exp2_raw(fmaf(p[ib][e], f.scale2, nlse[ib]));
@@ -496,6 +532,61 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         }
     };
     int buffer = 0;
+    if constexpr (BIAS) {
+        if (far_tile) {
+            float m[IB], l[IB];  // of the keys that the lane meets
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) m[ib] = -INFINITY, l[ib] = 0.f;
+            if (tiles > 0) issue(0, buffer);
+            for (int t = 0; t < tiles; ++t, buffer ^= 1) {
+                wait_vmcnt<0>();
+                lds_barrier();  // this tile is there, and the one before has been read
+                if (t + 1 < tiles) issue(t + 1, buffer ^ 1);
+                const int j0 = t * kKeys;
+                if (j0 >= own) continue;
+#pragma unroll 1
+                for (int r0 = 0; r0 < kKeys; r0 += 16) {
+                    f32x4 x[IB];
+                    scores(smem + buffer * kStage, r0, x);
+#pragma unroll
+                    for (int ib = 0; ib < IB; ++ib) {
+                        const int far0 = j0 + r0 - (row0 + 16 * ib + offset), j = j0 + r0 + 4 * g;
+                        const f32x4 b4 = bias.block(far0, far0 + 4 * g - l16);
+                        float top = m[ib];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[ib][e] = j + e < limit[ib] ? fmaf(x[ib][e], f.scale2, b4[e]) : -INFINITY;
+                            top = fmaxf(top, x[ib][e]);
+                        }
+                        const float at = top == -INFINITY ? 0.f : top;
+                        l[ib] *= exp2_raw(m[ib] - at);
+                        m[ib] = top;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) l[ib] += exp2_raw(x[ib][e] - at);
+                    }
+                }
+            }
+            lds_barrier();  // the last tile has been read
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) {
+                rests[16 * ib + l16] = 0.f;
+                if (!far_row[ib]) continue;  // (a row's four lanes say the same)
+                float top = fmaxf(m[ib], __shfl_xor(m[ib], 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                l[ib] *= exp2_raw(m[ib] - top);
+                l[ib] += __shfl_xor(l[ib], 16);
+                l[ib] += __shfl_xor(l[ib], 32);
+                nlse[ib] = -top;
+                const float rest = -__builtin_amdgcn_logf(l[ib]);
+                rests[16 * ib + l16] = rest;
+                if (g == 0) {
+                    const size_t at = (size_t)head * f.q_tokens + s.start + row0 + 16 * ib + l16;
+                    a.nlse[at] = nlse[ib];
+                    a.rest[at] = rest;
+                }
+            }
+        }
+    }
     if constexpr (BIAS || E::kSize == 2) {
         if (sum_delta) {  // (there is one part then)
             if (tiles > 0) issue(0, buffer);
@@ -645,7 +736,7 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     p.q_parts = size == 4 && !d->bias && q_units < 256
                     ? (int)std::max(1ll, std::min({32ll, 1024 / q_units, d->k_tokens / 128})) : 1;
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
-    p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float));
+    p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float)) * (d->bias ? 3 : 2);
     p.part = d->bias ? round((size_t)p.q_slots * d->heads * (2 * d->reach + 1) * sizeof(float)) : 0;
     p.part_kv = p.parts > 1 ? (size_t)p.parts * d->k_tokens * d->kv_heads * 2 * p.dim * sizeof(float) : 0;
     p.part_q = p.q_parts > 1 ? (size_t)p.q_parts * d->q_tokens * d->heads * p.dim * sizeof(float) : 0;
@@ -657,7 +748,7 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
 extern "C" size_t bfhip_attention_backward_workspace(const bfhip_attention_desc *d) {
     if (bad_attention(d)) return 0;
     const BackwardPlan p = backward_plan(d);
-    return 2 * p.terms + p.part + p.part_kv + p.part_q;
+    return p.terms + p.part + p.part_kv + p.part_q;
 }
 
 extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfhip_rows *q, const bfhip_rows *k,
@@ -672,7 +763,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         bad_result(dk, d->k_tokens, d->kv_heads, n, size) || bad_result(dv, d->k_tokens, d->kv_heads, n, size))
         return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
     const BackwardPlan p = backward_plan(d);
-    const size_t need = 2 * p.terms + p.part + p.part_kv + p.part_q;
+    const size_t need = p.terms + p.part + p.part_kv + p.part_q;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
     const long long q_grid = p.q_slots * d->heads * p.q_parts;
@@ -691,10 +782,12 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     a.dv = attn_rows(dv, d->k_tokens, n, size);
     char *const work = (char *)workspace;
     a.nlse = (float *)work;
-    a.delta = (float *)(work + p.terms);
-    a.part = dbias ? (float *)(work + 2 * p.terms) : nullptr;
-    a.part_kv = (float *)(work + 2 * p.terms + p.part);
-    a.part_q = (float *)(work + 2 * p.terms + p.part + p.part_kv);
+    const size_t term = p.terms / (d->bias ? 3 : 2);
+    a.delta = (float *)(work + term);
+    a.rest = d->bias ? (float *)(work + 2 * term) : nullptr;
+    a.part = dbias ? (float *)(work + p.terms) : nullptr;
+    a.part_kv = (float *)(work + p.terms + p.part);
+    a.part_q = (float *)(work + p.terms + p.part + p.part_kv);
     a.q_parts = p.q_parts;
     a.q_chunk = p.q_chunk;
     a.joins = (int)k_joins;
@@ -705,17 +798,18 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
             with_dim(n, [&](auto dim) {
                 using E = decltype(e);
                 constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), WAVES = 4, KB = key_blocks(E::kSize, DIM);
-                using K = KeyTile<E, DIM, KB, WAVES>;
                 using T = AttnTile<E, DIM>;
                 const auto run = [&](auto with_bias) {
                     constexpr bool B = decltype(with_bias)::value;
+                    using K = KeyTile<E, DIM, KB, WAVES, B>;
                     const size_t row = B ? BiasRow::floats(d->reach) * sizeof(float) : 0;
                     GradArgs b = a;
                     if (d->q_tokens) {
                         b.f.slots = (int)p.q_slots;
                         b.f.ordered = by_work(d, q_grid);
                         hipLaunchKernelGGL((attention_queries_kernel<E, DIM, QB, B>), dim3((unsigned)q_grid), dim3(256),
-                                           4 * tile_keys(E::kSize, DIM) * T::kRow + row + (a.part ? 4 * width * sizeof(float) : 0), s, b);
+                                           4 * tile_keys(E::kSize, DIM) * T::kRow + row + (a.part ? 4 * width * sizeof(float) : 0) +
+                                               (B ? p.q_rows * sizeof(float) : 0), s, b);
                     }
                     if (d->k_tokens) {
                         b.f.slots = (int)p.k_slots;
@@ -727,7 +821,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                 if (d->bias) run(std::true_type{});
                 else run(std::false_type{});
                 if (joins)
-                    hipLaunchKernelGGL((attention_gradient_join_kernel<E, DIM, K::kRows>), dim3((unsigned)joins), dim3(256), 0, s, a);
+                    hipLaunchKernelGGL((attention_gradient_join_kernel<E, DIM, WAVES * 16 * KB>), dim3((unsigned)joins), dim3(256), 0, s, a);
             });
         });
     const long long count = width * d->heads;

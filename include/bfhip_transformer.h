@@ -115,11 +115,13 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * 65504) becomes infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
  * fp32: a large bias (1e9, the lowest fp32 value) swallows the score, so that a
  * query all of whose keys have it takes their mean.  Finite biases beyond 2.3e38
- * of either sign count as that.
+ * of either sign count as that.  The backward pass finds the sum of a query's
+ * probabilities again where a bias has taken its lse far from zero; without a
+ * bias it takes them from lse alone, off by a factor of about 1 +- |lse| 2^-22.
  *
  * Workspaces: the forward's holds the sums of keys that are split (few queries
  * on many keys, at most some 300 MB; mostly none), the backward's two fp32 per
- * query and head, sums of queries that are split (at most some 150 MB; of keys
+ * query and head (three with a bias), sums of queries that are split (at most some 150 MB; of keys
  * in fp32, some 35 MB), and with a bias 2 * reach + 1 fp32 per head and 64 or 128 queries.
  *
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
