@@ -731,7 +731,7 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
     const long long rows = units < 256 ? d->q_tokens : d->sequences ? d->q_tokens / d->sequences : 0;
     const long long parts = units ? 2048 / units : 1, steps = rows * group / (kTile * p.chunk);
     p.parts = (int)std::max(1ll, std::min({32ll, parts, steps}));
-    const long long q_units = std::max(1ll, d->q_tokens / p.q_rows) * d->heads;
+    const long long q_units = std::max(1ll, (d->q_tokens + p.q_rows - 1) / p.q_rows) * d->heads;
     p.q_chunk = 2 * 64 / tile_keys(size, p.dim);
     p.q_parts = size == 4 && !d->bias && q_units < 256
                     ? (int)std::max(1ll, std::min({32ll, 1024 / q_units, d->k_tokens / 128})) : 1;

@@ -7,6 +7,7 @@
 // then O / l and lse = (m + log2 l) ln 2.  Scores come out transposed, so a
 // lane holds scores of one query only: the row statistics are one value per
 // lane, and P is the second product's operand without leaving its registers.
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.h"
@@ -490,11 +491,14 @@ constexpr int query_rows(int size) { return size == 4 ? 64 : 128; }
 // split into parts where the work would leave CUs idle: `few` takes parts of
 // `chunk` keys, a 1536th of all that is read (a tile or more), so that about 1536
 // workgroups read keys whatever the lengths are, and a sequence has at most
-// `parts` of them; otherwise a tile's keys are split into as many parts as
+// `parts` of them, whose sums take kPartBytes at most, which wide groups reach (512 single
+// tokens, 128 heads on one); otherwise a tile's keys are split into as many parts as
 // bring about four workgroups per CU, but no more than the average sequence has
 // keys for, four tiles or more in each.  fp32's products take eight times as long
 // as other types', so that a walk costs more than a join where CUs are idle: parts
 // of two tiles, as many as the longest sequence may have.
+constexpr long long kPartBytes = 1ll << 30;
+
 struct ForwardPlan {
     bool few, mixed;
     int rows, parts, chunk, dim, few_rows;
@@ -515,8 +519,8 @@ ForwardPlan forward_plan(const bfhip_attention_desc *d) {
         const long long units = (long long)d->sequences * d->kv_heads, least = size * p.dim <= 128 ? 128 : 64;
         const long long chunk = (d->k_tokens * d->kv_heads / 1536 + least - 1) / least * least;
         p.chunk = (int)(chunk < least ? least : chunk > 1 << 20 ? 1 << 20 : chunk);
-        const long long most = d->k_tokens / p.chunk < 32 ? d->k_tokens / p.chunk : 32, parts = 16384 / units;
-        p.parts = (int)(parts < 1 || most < 1 ? 1 : parts < most ? parts : most);
+        const long long fit = kPartBytes / (d->q_tokens * d->heads * (long long)(p.dim * sizeof(float) + sizeof(float2)));
+        p.parts = (int)std::max(1ll, std::min({32ll, d->k_tokens / p.chunk, 16384 / units, fit}));
         p.slots = slot_count(d->k_tokens, d->sequences, p.chunk);
         p.grid = p.slots * d->kv_heads;
         return p;

@@ -120,9 +120,10 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * bias it takes them from lse alone, off by a factor of about 1 +- |lse| 2^-22.
  *
  * Workspaces: the forward's holds the sums of keys that are split (few queries
- * on many keys, at most some 300 MB; mostly none), the backward's two fp32 per
- * query and head (three with a bias), sums of queries that are split (at most some 150 MB; of keys
- * in fp32, some 35 MB), and with a bias 2 * reach + 1 fp32 per head and 64 or 128 queries.
+ * on many keys, at most 1 GiB; mostly none), the backward's two fp32 per query
+ * and head (three with a bias), sums of queries that are split (at most 128 MiB;
+ * of keys in fp32, 32 MiB), and with a bias 2 * reach + 1 fp32 per head for
+ * every 64 (fp32) or 128 queries and every sequence.
  *
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
  * stride in elements; the elements of one head are contiguous, pointers and
