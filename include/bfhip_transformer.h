@@ -93,7 +93,9 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * and the key rows k_starts[b] .. k_starts[b+1] (device arrays of sequences + 1
  * ascending int32; lengths may be zero and may differ between queries and
  * keys).  Starts are clamped to [0, tokens]; rows outside every sequence are
- * not written, and what they hold is ignored.  Query head h reads key head h / (heads / kv_heads).
+ * not written, and what they hold is ignored.  (Where starts descend all the
+ * same, what the rows get is open, but nothing outside the rows is touched.)
+ * Query head h reads key head h / (heads / kv_heads).
  *
  * With Lq queries and Lk keys, query i stands at position i + Lk - Lq, so the
  * last query stands at the last key.  Key j is seen if not causal, or if

@@ -11,7 +11,7 @@ import torch
 
 import bfhip
 import transformer_ref as ref
-from test_gpu_transformer import BF16, F16, F32, grads, inputs
+from test_gpu_transformer import BF16, F16, F32, grads, inputs, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,93 @@ def test_attention_gradients_of_some_rows_far_from_zero(device, case):
     ref.check("out", out, *want["out"])
     for name, t in zip(("dq", "dk", "dv", "dbias"), grads(call, dout, out, lse)):
         ref.check(name, t, *want[name])
+
+# (rows of the tensors, starts): a query's and a key's alike.
+STARTS = [[-7, 50, 80, 10 ** 9], [-2 ** 31, -5, 30, 20, 80, 2 ** 31 - 1], [80, 0, 80], [0, 50, 30, 80, 79, 80],
+          [300, -1, 40, 40, 80, -3]]
+
+
+@pytest.mark.parametrize("at", STARTS, ids=str)
+@pytest.mark.parametrize("case", [(BF16, 4, 2, 64, None), (F32, 2, 1, 128, None), (F16, 4, 4, 32, 7), (F32, 3, 1, 40, 3)], ids=str)
+@pytest.mark.parametrize("few", [False, True])
+def test_attention_reads_and_writes_its_rows_only(device, case, at, few):
+    """Starts past the rows, before them and descending are clamped: nothing
+    outside the rows is read into a result or written, in either direction.
+    Where the clamped starts ascend, every sequence comes out right."""
+    dtype, heads, kv_heads, dim, reach = case
+    tq, guard = 80, 70
+    scale_k = 40 if few else 1  # keys per query, so that keys are split
+    call, dout = inputs(device, (dtype, heads, kv_heads, dim, [tq], [tq * scale_k], True, reach), layout="plain")
+    q_at = torch.tensor(at, dtype=torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
+    k_at = (q_at * scale_k).clamp(-2 ** 31, 2 ** 31 - 1)
+    pad = 40 if few else 0  # empty sequences: so few queries per sequence that they are dealt as few
+    q_at, k_at = (torch.cat([t, t[-1:].expand(pad)]).int().to(device) for t in (q_at, k_at))
+
+    def inside(t, fill):
+        wide = torch.full((t.shape[0] + 2 * guard, *t.shape[1:]), fill, dtype=t.dtype, device=device)
+        wide[guard:guard + t.shape[0]] = t
+        return wide, wide[guard:guard + t.shape[0]]
+
+    (_, q), (_, k), (_, v), (_, g) = (inside(t, math.nan) for t in (call["q"], call["k"], call["v"], dout))
+    wide = {}
+    for name, like in (("out", q), ("dq", q), ("dk", k), ("dv", v)):
+        wide[name] = inside(torch.zeros_like(like), 7.0)
+    there = dict(call, q=q, k=k, v=v, q_starts=q_at, k_starts=k_at)
+    out = wide["out"][1]
+    _, lse = bfhip.attention(**there, out=out, lse=True)
+    clamped = [t.clamp(0, n).tolist() for t, n in ((q_at.cpu(), tq), (k_at.cpu(), tq * scale_k))]
+    owned = torch.zeros(tq)
+    for a, b in zip(clamped[0], clamped[0][1:]):
+        owned[a:max(a, b)] += 1
+    lse = torch.where((owned > 0).to(device), lse, 0.0)  # (rows of no sequence have none)
+    dbias = None if reach is None else torch.empty_like(call["bias"])
+    backward_into(there, g, out, lse, wide["dq"][1], wide["dk"][1], wide["dv"][1], dbias)
+    for name, (buffer, _) in wide.items():
+        assert (buffer[:guard] == 7).all() and (buffer[-guard:] == 7).all(), name
+    for a, b, c, d in zip(clamped[0], clamped[0][1:], clamped[1], clamped[1][1:]):
+        if a == b or clamped[0] != sorted(clamped[0]):
+            continue
+        alone = dict(call, q=q[a:b], k=k[c:d], v=v[c:d], q_starts=starts([b - a], device), k_starts=starts([d - c], device))
+        want = ref.attention(**alone, dout=g[a:b])
+        for name, rows in (("out", slice(a, b)), ("dq", slice(a, b)), ("dk", slice(c, d)), ("dv", slice(c, d))):
+            ref.check(name, wide[name][1][rows], *want[name])
+
+
+@pytest.mark.parametrize("ql,kl,skip_q", [([5, 70], [200, 300], 140000), ([1, 1], [700, 900], 0)], ids=str)
+def test_attention_of_rows_past_four_gib(device, ql, kl, skip_q):
+    """A long cache: rows whose offsets no 32-bit number of bytes holds."""
+    call, dout = inputs(device, (BF16, 4, 2, 64, ql, kl, True, None), layout="plain")
+    stride, skip = 16384, 140000  # 32 KiB a token: 4.6 GB before the first row
+    room = torch.zeros(((skip + sum(kl)) * stride,), dtype=BF16, device=device)
+
+    def far(t, at, skip):
+        h = t.shape[1] * t.shape[2]
+        view = room.view(-1, stride)[:, at:at + h].unflatten(1, t.shape[1:])
+        view[skip:skip + t.shape[0]] = t
+        return view[:skip + t.shape[0]]
+
+    there = dict(call, q=far(call["q"], 0, skip_q), k=far(call["k"], 1024, skip), v=far(call["v"], 2048, skip),
+                 q_starts=call["q_starts"] + skip_q, k_starts=call["k_starts"] + skip)
+    out = far(torch.zeros_like(call["q"]), 4096, skip_q)
+    _, lse = bfhip.attention(**there, out=out, lse=True)
+    want = ref.attention(**call, dout=dout)
+    ref.check("out", out[skip_q:], *want["out"])
+    skips = dict(q=skip_q, k=skip, v=skip)
+    back = backward_into(there, far(dout, 5120, skip_q), out, lse, *(far(torch.zeros_like(call[n]), 6144 + 1024 * i, skips[n])
+                                                                     for i, n in enumerate("qkv")))
+    for n, t in zip("qkv", back):
+        ref.check("d" + n, t[skips[n]:], *want["d" + n])
+
+
+@pytest.mark.parametrize("case", [(F16, 4, 2, 64, [1] * 60 + [90], [400] * 60 + [500], True, 20),
+                                  (BF16, 8, 2, 128, [1] * 30 + [40], [700] * 30 + [60], False, None)], ids=str)
+def test_attention_of_the_same_sequences_in_both_deals(device, case):
+    """Single tokens and a prompt as a batch of few queries, and with rows of
+    no sequence behind them as a batch of prompts."""
+    call, dout = inputs(device, case)
+    want = ref.attention(**call)["out"]
+    n = call["q"].shape[0]
+    for extra in (0, 20 * n):
+        q = torch.zeros((n + extra, *call["q"].shape[1:]), dtype=call["q"].dtype, device=device)
+        q[:n] = call["q"]
+        ref.check(f"out, {extra} rows behind", bfhip.attention(**dict(call, q=q))[:n], *want)
