@@ -33,7 +33,7 @@ struct AttnArgs {
     int ordered;          // tiles in the order of their work
     int parts;            // most parts that a sequence's keys are split into
     int chunk;            // keys (few queries), tiles (forward) or steps (backward) of a part, at least
-    int few_rows;         // > 0: sequences of no more queries x group are attention_few_kernel's
+    int few_rows;         // > 0: sequences of no more queries x group are attention_few_kernel's, the others attention_forward_kernel's
     float *part_out;      // parts > 1: sums of each part, [parts][q_tokens][heads][padded dim]
     float2 *part_stat;    // and their (m, l), [parts][q_tokens][heads]
 };
@@ -109,6 +109,22 @@ __device__ __forceinline__ Slot find_rows(const int *starts, int sequences, long
     Slot s = find_slot(starts, sequences, tokens, slot, ROWS);
     if (s.index * (long long)ROWS >= s.length) s.sequence = -1;
     s.first = s.index * ROWS;
+    return s;
+}
+
+// Slots of the sequences of `least` rows or more alone (least <= ROWS), where
+// most have fewer: one for every row whose number is a multiple of `least`.  Such
+// a sequence has at least one of them and as many as it has tiles; rows are few
+// where places of a batch are empty, so that these cost no workgroups.
+template <int ROWS>
+__device__ __forceinline__ Slot long_rows(const int *starts, int sequences, long long tokens, int slot, int least) {
+    Slot s{-1, 0, 0, 0, 0};
+    const int b = find_token(starts, sequences, tokens, slot * least);
+    if (b < 0) return s;
+    sequence_rows(starts, b, tokens, s.start, s.length);
+    s.index = slot - (s.start + least - 1) / least;
+    s.first = s.index * ROWS;
+    if (s.length >= least && s.index * (long long)ROWS < s.length) s.sequence = b;
     return s;
 }
 

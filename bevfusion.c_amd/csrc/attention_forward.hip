@@ -116,8 +116,10 @@ __global__ __launch_bounds__(256, 1) void attention_forward_kernel(AttnArgs a) {
     const int items = a.slots * a.heads, part = blockIdx.x / items;
     const Deal deal_ = deal(blockIdx.x % items, a.heads, a.kv_heads);
     const int head = deal_.head, kv = head / (a.heads / a.kv_heads);
-    const Slot s = ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.ordered);
-    if (s.sequence < 0 || s.length <= a.few_rows / (a.heads / a.kv_heads)) return;
+    const Slot s = a.few_rows
+                       ? long_rows<kRows>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.few_rows / (a.heads / a.kv_heads) + 1)
+                       : ranked_rows<kRows, false>(a.q_starts, a.sequences, a.q_tokens, deal_.rank, a.slots, a.ordered);
+    if (s.sequence < 0) return;
     int k_start, k_len;
     sequence_rows(a.k_starts, s.sequence, a.k_tokens, k_start, k_len);
     const int offset = k_len - s.length;  // query i stands at position i + offset
@@ -481,22 +483,27 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
 constexpr int query_rows(int size) { return size == 4 ? 64 : 128; }
 
 // How a call is dealt.  `few`: so few queries per sequence that a key head's
-// group of them fills at most a tile of 16 rows on average, or one query each; where there are more
-// queries than sequences (`mixed`), only the sequences that do are dealt so, and the
-// others, prompts among single tokens, by a second launch.  On 2000 keys a
-// sequence, 32 heads of 128 on 8, bf16: 48 x 4 queries 110 us, 177 by the
-// launch for prompts alone; 63 single tokens and a prompt of 400 267 us, 1497 if all were
-// dealt as few.
-// The keys are
-// split into parts where the work would leave CUs idle: `few` takes parts of
-// `chunk` keys, a 1536th of all that is read (a tile or more), so that about 1536
-// workgroups read keys whatever the lengths are, and a sequence has at most
-// `parts` of them, whose sums take kPartBytes at most, which wide groups reach (512 single
-// tokens, 128 heads on one); otherwise a tile's keys are split into as many parts as
-// bring about four workgroups per CU, but no more than the average sequence has
-// keys for, four tiles or more in each.  fp32's products take eight times as long
-// as other types', so that a walk costs more than a join where CUs are idle: parts
-// of two tiles, as many as the longest sequence may have.
+// group of them fills at most a tile of 16 rows on average, or one query each.
+// Unless there are as many queries as sequences, the average says little of the
+// longest (places of a batch may be empty): then (`mixed`) only the sequences of
+// no more than few_rows rows are dealt so, and the others, prompts among single
+// tokens, by a second launch.
+// Heads of 128, bf16, 2000 keys per sequence, by this deal and by the prompts'
+// launch alone: 32 heads on 8: 48 x 4 queries 98 and 178 us, 63 single tokens and
+// a prompt of 100 164 and 229, 256 places with 25 single tokens and a prompt of
+// 200 93 and 122, without the prompt 47 and 119; 32 heads on 32, where no head
+// shares its keys, 63 and 100 423 and 363, but with 16000 keys in one sequence and
+// 500 in the others 165 and 471.  Lengths are not known here, so the deal
+// that bears uneven ones is taken.
+// The keys are split into parts where the work would leave CUs idle: `few` takes
+// parts of `chunk` keys, a 1536th of all that is read (a tile or more), so that
+// about 1536 workgroups read keys whatever the lengths are, and a sequence has at
+// most `parts` of them, whose sums take kPartBytes at most (which wide groups
+// reach: 512 single tokens, 128 heads on one); otherwise a tile's keys are split
+// into as many parts as bring about four workgroups per CU, but no more than the
+// average sequence has keys for, four tiles or more in each.  fp32's products take
+// eight times as long as other types', so that a walk costs more than a join
+// where CUs are idle: parts of two tiles, as many as the longest sequence may have.
 constexpr long long kPartBytes = 1ll << 30;
 
 struct ForwardPlan {
@@ -513,7 +520,7 @@ ForwardPlan forward_plan(const bfhip_attention_desc *d) {
     if (!d->sequences || !d->q_tokens) return p;
     p.few_rows = group > 16 ? group : 16;
     p.few = d->q_tokens * group <= (long long)p.few_rows * d->sequences && d->q_tokens * group < 1 << 30;
-    p.mixed = p.few && d->q_tokens > d->sequences;
+    p.mixed = p.few && d->q_tokens != d->sequences;
     p.rows = query_rows(size);
     if (p.few) {
         const long long units = (long long)d->sequences * d->kv_heads, least = size * p.dim <= 128 ? 128 : 64;
@@ -564,7 +571,8 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
     if (!d->sequences || !d->q_tokens) return 1;
     const long long joins = p.parts > 1 ? ((long long)d->heads * p.dim + 255) / 256 * d->q_tokens : 0;
-    const long long rest_slots = p.mixed ? slot_count(d->q_tokens, d->sequences, p.rows) : 0, rest = rest_slots * d->heads;
+    const int least = p.few_rows / (d->heads / d->kv_heads) + 1;  // queries of a prompt
+    const long long rest_slots = p.mixed ? (d->q_tokens + least - 1) / least : 0, rest = rest_slots * d->heads;
     if (!launch_fits(p.grid, 256) || !launch_fits(rest, 256) || !launch_fits(joins, 256)) return fail(error, cap, "attention has too many rows");
     AttnArgs a = attn_args(d, q, k, v, out, lse);
     a.slots = (int)p.slots;
@@ -596,7 +604,6 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
                     AttnArgs b = a;
                     b.slots = (int)rest_slots;
                     b.parts = 1;
-                    b.ordered = by_work(d, rest);
                     hipLaunchKernelGGL((attention_forward_kernel<E, DIM, IB, B>), dim3((unsigned)rest), dim3(256), lds, s, b);
                 }
             };

@@ -200,3 +200,23 @@ def test_attention_of_the_same_sequences_in_both_deals(device, case):
         q = torch.zeros((n + extra, *call["q"].shape[1:]), dtype=call["q"].dtype, device=device)
         q[:n] = call["q"]
         ref.check(f"out, {extra} rows behind", bfhip.attention(**dict(call, q=q))[:n], *want)
+
+
+@pytest.mark.parametrize("case", [(BF16, 8, 2, 64, 150, 200, 256), (F32, 4, 1, 32, 100, 300, 130)], ids=str)
+def test_prompt_in_a_batch_with_empty_places(device, case):
+    """A batch of a fixed number of places, most of them empty: its prompt
+    takes the prompts' launch, whose bits are those of a batch of prompts."""
+    dtype, heads, kv_heads, dim, prompt, keys, places = case
+    ql, kl = [1] * 25 + [prompt], [300] * 25 + [keys]
+    many, _ = inputs(device, (dtype, heads, kv_heads, dim, [prompt] * 80, [keys] * 80, True, None), layout="plain")
+    call, dout = inputs(device, (dtype, heads, kv_heads, dim, ql + [0] * (places - 26), kl + [0] * (places - 26), True, None),
+                        layout="plain")
+    assert call["q"].shape[0] < places
+    for name, n in (("q", prompt), ("k", keys), ("v", keys)):
+        call[name][-n:] = many[name][:n]
+    out, lse = bfhip.attention(**call, lse=True)
+    want = ref.attention(**call, dout=dout)
+    ref.check("out", out, *want["out"])
+    for name, t in zip(("dq", "dk", "dv"), grads(call, dout, out, lse)):
+        ref.check(name, t, *want[name])
+    assert torch.equal(out[-prompt:], bfhip.attention(**many)[:prompt])
