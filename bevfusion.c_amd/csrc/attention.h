@@ -376,6 +376,14 @@ struct BiasRow {
     }
 };
 
+// Eight elements at p, which is on 16 bytes (fp32's are two loads).
+template <class E>
+__device__ __forceinline__ typename E::Frag load_frag(const char *p) {
+    typename E::Frag f;
+    __builtin_memcpy(&f, __builtin_assume_aligned(p, 16), sizeof f);
+    return f;
+}
+
 // Fragment of 16 rows in global memory (row 0 at `base`): elements 32 kk ..+31.
 // Rows past `rows` and elements past dim are zero.
 template <class E>
@@ -383,8 +391,7 @@ __device__ __forceinline__ typename E::Frag global_frag(const char *base, long l
                                                         int kk, int lane) {
     const int r = lane & 15, d = 32 * kk + 8 * (lane >> 4);
     typename E::Frag f = {};
-    if (r < rows && d < dim)
-        f = *reinterpret_cast<const typename E::Frag *>(base + r * token_bytes + d * E::kSize);
+    if (r < rows && d < dim) f = load_frag<E>(base + r * token_bytes + d * E::kSize);
     return f;
 }
 

@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256, 1) void attention_few_kernel(AttnArgs a) {
             for (int kk = 0; kk < kKB; ++kk) {
                 const int d = 32 * kk + 8 * g;
                 qf[kk] = typename E::Frag{};
-                if (live && d < a.dim) qf[kk] = signed_frag<E>(*reinterpret_cast<const typename E::Frag *>(q + d * E::kSize), a.flip);
+                if (live && d < a.dim) qf[kk] = signed_frag<E>(load_frag<E>(q + d * E::kSize), a.flip);
             }
         }
         const int limit = a.causal ? min(k_len, token + offset + 1) : k_len;

@@ -220,3 +220,29 @@ def test_prompt_in_a_batch_with_empty_places(device, case):
     for name, t in zip(("dq", "dk", "dv"), grads(call, dout, out, lse)):
         ref.check(name, t, *want[name])
     assert torch.equal(out[-prompt:], bfhip.attention(**many)[:prompt])
+
+
+@pytest.mark.parametrize("case", [(F32, 2, 1, 40, [70, 3], [90, 30], True, 4), (F32, 4, 2, 12 * 8, [1, 1], [900, 65], True, None),
+                                  (F32, 3, 3, 8, [130], [200], False, None)], ids=str)
+def test_attention_of_rows_on_16_bytes(device, case):
+    """fp32 rows that begin at odd multiples of 16 bytes."""
+    call, dout = inputs(device, case, layout="plain")
+
+    def odd(t):
+        heads, dim = t.shape[1:]
+        wide = torch.full((t.shape[0] * (heads * (dim + 4) + 4 * (heads % 2 == 0)) + 4,), 3.0, device=device)
+        assert (wide.data_ptr() + 16) % 32 == 16
+        view = wide[4:].view(t.shape[0], -1)[:, :heads * (dim + 4)].unflatten(1, (heads, dim + 4))[:, :, :dim]
+        assert view.stride(0) % 8 == 4 and view.stride(1) % 8 == 4
+        view.copy_(t)
+        return view
+
+    call.update({n: odd(call[n]) for n in "qkv"})
+    dout = odd(dout)
+    want = ref.attention(**call, dout=dout)
+    out = odd(torch.zeros_like(dout))
+    _, lse = bfhip.attention(**call, out=out, lse=True)
+    ref.check("out", out, *want["out"])
+    dbias = None if call["bias"] is None else torch.empty_like(call["bias"])
+    for name, t in zip(("dq", "dk", "dv"), backward_into(call, dout, out, lse, *(odd(torch.zeros_like(call[n])) for n in "qkv"), dbias)):
+        ref.check(name, t, *want[name])

@@ -1,7 +1,9 @@
-"""What the transformer operators' header says of sizes
+"""What the transformer operators' header says of sizes and alignment
 (include/bfhip_transformer.h), asked on the CPU."""
 
+import pathlib
 import random
+import re
 
 import bfhip
 
@@ -47,3 +49,12 @@ def test_attention_backward_workspace_of_a_tile_and_a_half():
     size = bfhip.hip_lib().bfhip_attention_backward_workspace
     d = bfhip.AttentionDesc(0, 1, 32, 32, 128, 0, 0, 0.1, 127, 4096, 4096, 4096, None)
     assert 0 < size(d) - 2 * 4 * 32 * 127 <= 32 << 20
+
+
+def test_no_load_of_rows_through_a_fragment_type():
+    """Rows begin on 16 bytes.  A load through a type of a larger alignment would
+    be undefined for them, whatever it does on a machine that serves it."""
+    csrc = pathlib.Path(__file__).resolve().parent.parent / "bevfusion.c_amd" / "csrc"
+    for name in ("attention.h", "attention_forward.hip", "attention_backward.hip"):
+        text = re.sub(r"//[^\n]*", "", (csrc / name).read_text())
+        assert not re.search(r"_cast<\s*(const\s+)?(typename\s+E::Frag|f32x8)\s*\*", text), name
