@@ -419,13 +419,19 @@ __device__ __forceinline__ typename E::Frag to_frag(const f32x4 &a, const f32x4 
     }
 }
 
-// What the rounding of to_frag left, as operand words.
+// What the rounding of to_frag left, as operand words; nothing of a value that the
+// type holds as an infinity.
 template <class E>
 __device__ __forceinline__ typename E::Frag rest_frag(const f32x4 &a, const f32x4 &b) {
     typedef typename E::Word Words4 __attribute__((ext_vector_type(4)));
-    const f32x4 x = a - __builtin_convertvector(__builtin_convertvector(a, Words4), f32x4);
-    const f32x4 y = b - __builtin_convertvector(__builtin_convertvector(b, Words4), f32x4);
-    return to_frag<E>(x, y);
+    const auto rest = [](const f32x4 &v) {
+        const f32x4 w = __builtin_convertvector(__builtin_convertvector(v, Words4), f32x4);
+        f32x4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = __builtin_isinf(w[e]) ? 0.f : v[e] - w[e];
+        return r;
+    };
+    return to_frag<E>(rest(a), rest(b));
 }
 
 // Sum of the products of two fragments' eight values.

@@ -246,3 +246,23 @@ def test_attention_of_rows_on_16_bytes(device, case):
     dbias = None if call["bias"] is None else torch.empty_like(call["bias"])
     for name, t in zip(("dq", "dk", "dv"), backward_into(call, dout, out, lse, *(odd(torch.zeros_like(call[n])) for n in "qkv"), dbias)):
         ref.check(name, t, *want[name])
+
+
+@pytest.mark.parametrize("keys", [2, 300])
+def test_attention_gradients_beyond_the_type(device, keys):
+    """fp16 gradients that the type does not hold are infinite, not NaN."""
+    q = torch.zeros((1, 1, 8), dtype=F16, device=device)
+    k = torch.zeros((keys, 1, 8), dtype=F16, device=device)
+    v = torch.zeros_like(k)
+    k[0, 0, 0], k[1, 0, 0] = 4.0, -4.0
+    q[0, 0, 1] = 6.0
+    k[0, 0, 1] = k[1, 0, 1] = 6.0  # (the others have almost no weight)
+    v[0, 0], v[1, 0] = 300.0, -300.0
+    dout = torch.full_like(q, 300.0)
+    at = starts([1], device), starts([keys], device)
+    out, lse = bfhip.attention(q, k, v, *at, scale=1.0, lse=True)
+    dq, dk, dv = bfhip.attention_backward(dout, q, k, v, out, lse, *at, scale=1.0)
+    # ds = +-1/2 * 8 * 300 * 300 = +-360000 for the first two keys.
+    assert dq[0, 0, 0] == math.inf
+    assert dk[0, 0, 1] == math.inf and dk[1, 0, 1] == -math.inf
+    assert torch.isfinite(dv).all()
