@@ -185,8 +185,9 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
         for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
             for (int e = 0; e < R::kWords; ++e) {
-                // Past the row's end dy is zero, and so is all it is part of.
-                const float d = dy[k].get(e), h = (x[k].get(e) - m) * rs, g = d * gamma[k].w[e];
+                // Past the row's end dy is zero; h could be infinite there.
+                const float d = dy[k].get(e), g = d * gamma[k].w[e];
+                const float h = R::column(k) + e < a.n ? (x[k].get(e) - m) * rs : 0.f;
                 dg[k].w[e] = fmaf(d, h, dg[k].w[e]);
                 db[k].w[e] += d;
                 s1 += g;

@@ -11,7 +11,7 @@ import torch
 
 import bfhip
 import transformer_ref as ref
-from test_gpu_transformer import BF16, F16, F32, grads, inputs, starts
+from test_gpu_transformer import BF16, F16, F32, gen, grads, inputs, randn, starts
 
 pytestmark = pytest.mark.gpu
 
@@ -266,3 +266,20 @@ def test_attention_gradients_beyond_the_type(device, keys):
     assert dq[0, 0, 0] == math.inf
     assert dk[0, 0, 1] == math.inf and dk[1, 0, 1] == -math.inf
     assert torch.isfinite(dv).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [1, 5, 100, 257])
+def test_layer_norm_gradients_of_large_equal_rows(device, dtype, n):
+    """Rows without spread, far from zero: what lies past their end reaches
+    nothing."""
+    x = torch.full((3, n), 2.0 ** 112, dtype=dtype, device=device)
+    x[1] = -1.0
+    g = gen(device, n)
+    gamma, dy = 1 + randn(g, n, scale=0.2), randn(g, 3, n, dtype=dtype)
+    y, mean, rstd = bfhip.layer_norm(x, gamma, eps=1e-10, stats=True)
+    dx, dgamma, dbeta = bfhip.layer_norm_backward(dy, x, mean, rstd, gamma)
+    assert torch.equal(mean, x[:, 0].float()) and not y.any()
+    want = ref.layer_norm(torch.zeros_like(x), gamma, None, 1e-10, dy)  # (the same centred values)
+    for name, got in dict(dx=dx, dgamma=dgamma, dbeta=dbeta).items():
+        ref.check(name, got, *want[name])
