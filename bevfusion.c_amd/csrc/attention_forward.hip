@@ -581,10 +581,10 @@ extern "C" int bfhip_attention_forward(const bfhip_attention_desc *d, const bfhi
     a.ordered = by_work(d, p.grid);
     a.few_rows = p.mixed ? p.few_rows : 0;
     // Scores are compared before they are scaled, which takes a positive scale:
-    // a negative one flips the queries' signs, and zero becomes one so small
-    // that it makes no score differ.
+    // a negative one flips the queries' signs, and zero becomes the smallest
+    // number there is, with which no product that fp32 holds makes scores differ.
     a.flip = d->scale < 0.f;
-    a.scale2 = d->scale == 0.f ? 1e-30f : __builtin_fabsf(a.scale2);
+    a.scale2 = d->scale == 0.f ? __FLT_DENORM_MIN__ : __builtin_fabsf(a.scale2);
     a.part_out = (float *)workspace;
     a.part_stat = (float2 *)(a.part_out + rows * p.dim);
     hipStream_t s = (hipStream_t)stream;

@@ -283,3 +283,14 @@ def test_layer_norm_gradients_of_large_equal_rows(device, dtype, n):
     want = ref.layer_norm(torch.zeros_like(x), gamma, None, 1e-10, dy)  # (the same centred values)
     for name, got in dict(dx=dx, dgamma=dgamma, dbeta=dbeta).items():
         ref.check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("case", [(F32, 2, 1, 32, [70], [90], True, None), (BF16, 4, 2, 64, [1, 2], [700, 3], True, 3)], ids=str)
+def test_attention_without_scale_takes_no_scores(device, case):
+    """Scale 0, and products of queries and keys near 2^120."""
+    call, _ = inputs(device, case)
+    call["scale"] = 0.0
+    want = ref.attention(**dict(call, q=torch.zeros_like(call["q"])))
+    for name in "qk":
+        call[name].mul_(2.0 ** 58)
+    ref.check("out", bfhip.attention(**call), *want["out"])
