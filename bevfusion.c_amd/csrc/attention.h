@@ -469,8 +469,8 @@ __device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp
 inline bool bad_rows(const bfhip_rows *r, long long tokens, int dim, int size) {
     if (!r || (!r->data && tokens)) return true;
     const long long step = 16 / size;
-    return ((uintptr_t)r->data & 15) || r->head_stride % step || r->token_stride % step || r->head_stride < 0 ||
-           (tokens > 1 && (r->token_stride < dim || r->token_stride >= 4 << 20)) || r->token_stride < 0;
+    return ((uintptr_t)r->data & 15) || r->head_stride % step || r->head_stride < 0 ||
+           (tokens > 1 && (r->token_stride % step || r->token_stride < dim || r->token_stride >= 4 << 20));
 }
 
 // Rows that a call writes: also no row on another, whichever of tokens and

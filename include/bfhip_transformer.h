@@ -129,9 +129,9 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  *
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
  * stride in elements; the elements of one head are contiguous, pointers and
- * strides are multiples of 16 bytes, token strides at least head_dim (unless
- * there is one token) and below 4 Mi elements; no row of a result on another.  At
- * most 0x7ffff000 query and key rows.
+ * strides are multiples of 16 bytes, token strides at least head_dim and below
+ * 4 Mi elements (of no account where there is at most one token); no row of a
+ * result on another.  At most 0x7ffff000 query and key rows.
  * bias: [heads, 2 * reach + 1] or NULL (reach is then ignored); reach in
  * [0, 2047].  out must not overlap the other tensors. */
 typedef struct {

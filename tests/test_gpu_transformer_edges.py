@@ -294,3 +294,16 @@ def test_attention_without_scale_takes_no_scores(device, case):
     for name in "qk":
         call[name].mul_(2.0 ** 58)
     ref.check("out", bfhip.attention(**call), *want["out"])
+
+
+def test_attention_of_one_token_of_any_stride(device):
+    """The stride between tokens means nothing where there is one."""
+    call, dout = inputs(device, (F32, 4, 2, 32, [1], [1], True, None), layout="plain")
+    want = bfhip.attention(**call)
+    for stride in (1, 7, 16):
+        odd = {n: call[n].as_strided(call[n].shape, (stride, 32, 1)) for n in "qkv"}
+        out = torch.empty_like(want).as_strided(want.shape, (stride, 32, 1))
+        got, lse = bfhip.attention(**dict(call, **odd), out=out, lse=True)
+        assert torch.equal(got, want)
+        back = grads(dict(call, **odd), dout, got, lse)
+        assert all(torch.isfinite(t).all() for t in back)
