@@ -772,6 +772,8 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     const long long joins = k_joins + (p.q_parts > 1 ? ((long long)d->heads * p.dim + 1023) / 1024 * d->q_tokens : 0);
     if (!launch_fits(q_grid, 256) || !launch_fits(k_grid, 256) || !launch_fits(joins, 256))
         return fail(error, cap, "attention has too many rows");
+    const long long width = 2 * (d->bias ? d->reach : 0) + 1, count = width * d->heads;
+    if (dbias && !column_sum_fits(count)) return fail(error, cap, "attention has too many biases");
     GradArgs a{};
     a.f = attn_args(d, q, k, v, out, const_cast<float *>(lse));
     a.f.parts = p.parts;
@@ -792,7 +794,6 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     a.q_chunk = p.q_chunk;
     a.joins = (int)k_joins;
     hipStream_t s = (hipStream_t)stream;
-    const long long width = 2 * a.f.reach + 1;
     if (d->sequences)
         with_element(d->type, [&](auto e) {
             with_dim(n, [&](auto dim) {
@@ -824,7 +825,6 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                     hipLaunchKernelGGL((attention_gradient_join_kernel<E, DIM, WAVES * 16 * KB>), dim3((unsigned)joins), dim3(256), 0, s, a);
             });
         });
-    const long long count = width * d->heads;
     if (dbias) column_sum(a.part, d->q_tokens && d->sequences ? p.q_slots : 0, dbias, dbias, count, count, s);
     return launch_ok(error, cap, "attention launch");
 }

@@ -1,7 +1,7 @@
 // Sums of partial results over their parts, in a fixed order.
 #pragma once
 
-#include "hip_common.h"
+#include "gemm_core.h"
 
 namespace bfhip {
 
@@ -31,6 +31,9 @@ static __global__ __launch_bounds__(kSumThreads) void column_sum_kernel(const fl
     if (c < split) out[c] = s;
     else out2[c - split] = s;
 }
+
+// Whether a launch holds n columns' workgroups.
+inline bool column_sum_fits(long long n) { return launch_fits((n + 15) / 16, kSumThreads); }
 
 inline void column_sum(const float *partial, long long parts, float *out, float *out2, long long split, long long n, hipStream_t s) {
     hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((n + 15) / 16)), dim3(kSumThreads), 0, s, partial, parts, out, out2,

@@ -1,6 +1,7 @@
 """What the transformer operators' header says of sizes and alignment
 (include/bfhip_transformer.h), asked on the CPU."""
 
+import ctypes as C
 import pathlib
 import random
 import re
@@ -58,3 +59,18 @@ def test_no_load_of_rows_through_a_fragment_type():
     for name in ("attention.h", "attention_forward.hip", "attention_backward.hip"):
         text = re.sub(r"//[^\n]*", "", (csrc / name).read_text())
         assert not re.search(r"_cast<\s*(const\s+)?(typename\s+E::Frag|f32x8)\s*\*", text), name
+
+
+def test_attention_backward_refuses_what_no_launch_holds():
+    """A gradient of more biases than a launch's threads can add up is refused
+    before anything is launched."""
+    lib = bfhip.hip_lib()
+
+    def call(heads, reach):
+        d = bfhip.AttentionDesc(0, 1, heads, heads, 8, 0, reach, 0.1, 1, 1, 4096, 4096, 4096)
+        row, error = bfhip.Rows(4096, 8 * heads, 8), C.create_string_buffer(256)
+        assert not lib.bfhip_attention_backward(d, row, row, row, row, 4096, row, row, row, row, 4096, 4096, 1 << 50, None,
+                                                error, 256)
+        return error.value
+
+    assert b"too many" in call(65535, 2047) and b"too many" in call(33000, 2047)
