@@ -355,8 +355,10 @@ __device__ __forceinline__ float row_shift(float v) {
 // where the diagonal meets e = 0 (`main`) and, for the three diagonals that
 // begin left of it, in the last lanes (`rest`).  The groups' lanes (i + 4 n, g +
 // n) lie on one diagonal: two shuffles add them in the lane that starts it.
-// Either write is then to addresses of one lane each, in the wave's order, so
-// the sums' order is fixed.  Distances at or beyond the reach are left to the
+// Either write is then to addresses of one lane each.  A sum's next addition may
+// be another lane's, which the compiler, who sees one lane's addresses differ,
+// must not move before this one: LDS serves a wave in its order, so that keeping
+// the instructions' order fixes the sums'.  Distances at or beyond the reach are left to the
 // caller's low and high sums.
 __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int reach, float *sum, float &low, float &high,
                                               int lane) {
@@ -376,12 +378,14 @@ __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int rea
     next = __shfl(main, (lane + 40) & 63);
     if (g < 2 && i < 8) main += next;
     const auto add = [&](int far, float v) {
+        asm volatile("" ::: "memory");
         if (far <= -reach) low += v;
         else if (far >= reach) high += v;
         else sum[far + reach] += v;
     };
     if (g == 0 || i < 4) add(far0 + 4 * g - i, main);
     if (i >= 13) add(far0 + 4 * g + 16 - i, rest);
+    asm volatile("" ::: "memory");
 }
 
 // IB blocks of 16 queries per wave, four waves.  Scores come out with a query
