@@ -40,10 +40,83 @@ constexpr int kFineKeys = 256;  // see above
 // 1024 takes p off by less than the 16-bit types' rounding does.
 constexpr float far_lse(int size) { return size == 4 ? 64.f : 1024.f; }
 
+// fp16 holds 2^-24 to 65504; p of many keys and score gradients lie outside.  p is
+// at most 1 and enters the matrix cores times kSpread.  ds enters times a power of
+// two, the growth, one for the 16 to 32 rows of a wave.  In the queries' walk it
+// takes the largest |dout . v| to 2^13 or more (kGrowth at most) where delta is
+// summed: |ds| is at most twice that.  Elsewhere the largest ds is watched, and
+// what has been summed shrinks when one passes kMost.  The keys' walk gets a bound
+// of ds from the queries' (`most`).  So what a wave's rows lose lies 2^-36 below
+// the largest |dout . v|.  Powers of two change no other bits.
+constexpr float kSpread = 0x1p12f, kLogSpread = 12.f, kGrowth = 0x1p40f, kMost = 0x1p15f;
+
+template <class E>
+constexpr bool kScaled = std::is_same_v<E, ElemF16>;
+
+// The wave's largest of each lane's rows' (infinite rows stay so, whatever they
+// grow by).
+template <int B>
+__device__ __forceinline__ float wave_most(const float (&rows)[B]) {
+    float most = 0.f;
+#pragma unroll
+    for (int r = 0; r < B; ++r) most = fmaxf(most, rows[r] < INFINITY ? rows[r] : 0.f);
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, most)));
+}
+
+// The power of two that takes `most` to 2^13 .. 2^14.
+__device__ __forceinline__ float growth_of(float most) {
+    return most > 0.f ? fminf(ldexpf(1.f, 14 - __builtin_amdgcn_frexp_expf(most)), kGrowth) : kGrowth;
+}
+
+// What everything shrinks by where one of ds, grown, passes kMost; 1 otherwise.
+template <int B>
+__device__ __forceinline__ float shrink(const f32x4 (&ds)[2][B]) {
+    float rows[B];
+    bool over = false;
+#pragma unroll
+    for (int r = 0; r < B; ++r) {
+        rows[r] = 0.f;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rows[r] = fmaxf(rows[r], fabsf(ds[b][r][e]));
+        over |= rows[r] > kMost;
+    }
+    if (!__any(over)) return 1.f;
+    const float most = wave_most(rows);
+    return most > kMost ? growth_of(most) : 1.f;
+}
+
+template <int B>
+__device__ __forceinline__ void scale_rows(f32x4 (&ds)[2][B], float by) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < B; ++r) ds[b][r] *= by;
+}
+
+__device__ __forceinline__ bf16x8 scaled_frag(const bf16x8 &f, float by) {
+    typedef _Float16 Words8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(bf16x8, __builtin_bit_cast(Words8, f) * (_Float16)by);
+}
+
+// Keys per tile: two tiles of keys and values, and five rows of the longest
+// bias, have to fit the LDS.
+constexpr int tile_keys(int size, int dim) { return size == 4 && dim > 64 ? 32 : 64; }
+
+// Blocks of 16 rows per wave: two, so that a fragment read from LDS serves two
+// products; one for fp32, whose products take eight times as long as the reads.
+constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
+
 struct GradArgs {
     AttnArgs f;
     AttnRows dout, dq, dk, dv;
     float *nlse, *delta;  // [heads, q_tokens]; nlse: -lse in base 2, -inf for a query without keys (every p is then 0)
+    int sum_delta;        // delta is summed over the keys everywhere: with dbias, and in fp16 with a bias
+    float *most;          // fp16: of ds in each query slot's four waves, [heads][slots][4]
+    int q_slots;
     float *rest;          // with a bias: -log2 l where nlse is -m (see above), 0 elsewhere
     float *part;          // dbias: [query slots, heads, 2 reach + 1] or null
     float *part_kv;       // f.parts > 1: [parts][k_tokens][kv_heads][dk, dv][padded dim]
@@ -129,6 +202,17 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
 #pragma unroll
         for (int db = 0; db < kDB; ++db) dk[kb][db] = dv[kb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    float growth = 1.f;  // of ds
+    if constexpr (kScaled<E>) {
+        constexpr int kQueries = 64 * row_blocks(E::kSize);  // of a slot
+        const int slot = q_start / kQueries + s.sequence, from = 4 * (slot + steps.begin / kQueries);
+        const int to = 4 * (slot + (q_len + kQueries - 1) / kQueries);
+        float most[1] = {0.f};
+        for (int hg = first < end ? first / steps.tiles : group; hg < group && hg * steps.tiles < end; ++hg)
+            for (int i = from + lane; i < to; i += kWave)
+                most[0] = fmaxf(most[0], a.most[(size_t)(kv * group + hg) * a.q_slots * 4 + i]);
+        growth = growth_of(wave_most(most)) / kSpread;  // (ds has p's)
+    }
     BiasRow bias{};
     int bias_head = -1;
     if (first < end) issue(first);
@@ -152,8 +236,8 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         // A query that does not see every key of the wave's.
         const bool edge = f.causal && i0 + offset < key0 + 16 * KB - 1;
         const bool fine = E::kSize == 2 && (f.causal ? min(s.length, i0 + kTile + offset) : s.length) <= kFineKeys;
-        // Whether a query of the tile's has a rest.
-        const bool far = BIAS && __any(terms[2 * kTile + lane] != 0.f);
+        // Whether a query of the tile's may have a rest.
+        const bool far = BIAS && __any(fabsf(terms[lane]) > far_lse(E::kSize) / 2.f && __builtin_isfinite(terms[lane]));
         // Scores of the whole tile first: the compiler waits for the copies in
         // flight before the transposed reads, which by then have had the time.
         typename E::Frag pf[2][KB], sf[2][KB];
@@ -177,7 +261,9 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
 #pragma unroll
                     for (int kb = 0; kb < KB; ++kb) ds[b][kb] = E::mfma(gf, vf[kb][kk], ds[b][kb]);
                 }
-                const f32x4 nlse = *reinterpret_cast<const f32x4 *>(terms + r0 + 4 * g);
+                f32x4 nlse = *reinterpret_cast<const f32x4 *>(terms + r0 + 4 * g);
+                if constexpr (kScaled<E>)  // (part of the exponent; its rounding is nlse's own)
+                    if (!far) nlse += kLogSpread;
                 const f32x4 delta = *reinterpret_cast<const f32x4 *>(terms + kTile + r0 + 4 * g);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
@@ -188,7 +274,7 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                         const f32x4 b4 = bias.block(far0, far0 + l16 - 4 * g - 3);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = fmaf(p[b][kb][e], f.scale2, b4[3 - e]) + nlse[e];
-                        if (far) x += *reinterpret_cast<const f32x4 *>(terms + 2 * kTile + r0 + 4 * g);
+                        if (far) x += *reinterpret_cast<const f32x4 *>(terms + 2 * kTile + r0 + 4 * g) + (kScaled<E> ? kLogSpread : 0.f);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = fmaf(p[b][kb][e], f.scale2, nlse[e]);
@@ -219,6 +305,9 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (16 * b + e >= left) p[b][kb][e] = ds[b][kb][e] = 0.f;
+            }
+            if constexpr (kScaled<E>) {
+                scale_rows(ds, growth);
             }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -258,28 +347,21 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
     for (int kb = 0; kb < KB; ++kb) {
         const int r = key0 + 16 * kb + l16;
         const bool live = r < s.length;
+        const float dk_by = kScaled<E> ? 1.f / (kSpread * growth) : 1.f, dv_by = kScaled<E> ? 1.f / kSpread : 1.f;
         if (per < all) {
             if (!live) continue;
             float *const row = a.part_kv + (((size_t)part * f.k_tokens + s.start + r) * f.kv_heads + kv) * 2 * DIM + 4 * g;
 #pragma unroll
             for (int db = 0; db < kDB; ++db) {
-                *reinterpret_cast<f32x4 *>(row + 16 * db) = dk[kb][db];
-                *reinterpret_cast<f32x4 *>(row + DIM + 16 * db) = dv[kb][db];
+                *reinterpret_cast<f32x4 *>(row + 16 * db) = dk[kb][db] * dk_by;
+                *reinterpret_cast<f32x4 *>(row + DIM + 16 * db) = dv[kb][db] * dv_by;
             }
         } else {
-            store_rows<E, kDB>(dk[kb], f.scale, a.dk.at((long long)s.start + r, kv), live, f.dim, lane);
-            store_rows<E, kDB>(dv[kb], 1.f, a.dv.at((long long)s.start + r, kv), live, f.dim, lane);
+            store_rows<E, kDB>(dk[kb], f.scale * dk_by, a.dk.at((long long)s.start + r, kv), live, f.dim, lane);
+            store_rows<E, kDB>(dv[kb], dv_by, a.dv.at((long long)s.start + r, kv), live, f.dim, lane);
         }
     }
 }
-
-// Keys per tile: two tiles of keys and values, and five rows of the longest
-// bias, have to fit the LDS.
-constexpr int tile_keys(int size, int dim) { return size == 4 && dim > 64 ? 32 : 64; }
-
-// Blocks of 16 rows per wave: two, so that a fragment read from LDS serves two
-// products; one for fp32, whose products take eight times as long as the reads.
-constexpr int row_blocks(int size) { return size == 4 ? 1 : 2; }
 
 // dq of one token from the parts' sums, in order: four elements per thread.
 template <class E, int DIM>
@@ -454,7 +536,7 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
     }
     // This wave's rows' rest, where one is far.
     float *const rests = bias_row + BiasRow::floats(f.reach) + (part ? 4 * width : 0) + 16 * IB * wave;
-    const bool fine = E::kSize == 2 && last <= kFineKeys, sum_delta = fine || part;
+    const bool fine = E::kSize == 2 && last <= kFineKeys, sum_delta = fine || a.sum_delta;
     typename E::Frag qf[IB][kKB], gf[IB][kKB];
     f32x4 dq[IB][kDB];
     float nlse[IB], delta[IB];
@@ -591,8 +673,12 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             }
         }
     }
+    float growth = kGrowth;  // of ds
     if constexpr (BIAS || E::kSize == 2) {
         if (sum_delta) {  // (there is one part then)
+            float most[IB];  // of |dout . v|
+#pragma unroll
+            for (int ib = 0; ib < IB; ++ib) most[ib] = 0.f;
             if (tiles > 0) issue(0, buffer);
             for (int t = 0; t < tiles; ++t, buffer ^= 1) {
                 wait_vmcnt<0>();
@@ -607,7 +693,10 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
 #pragma unroll
                     for (int ib = 0; ib < IB; ++ib)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) delta[ib] = fmaf(p[ib][e], dp[ib][e], delta[ib]);
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (kScaled<E>) most[ib] = fmaxf(most[ib], fabsf(dp[ib][e]));
+                            delta[ib] = fmaf(p[ib][e], dp[ib][e], delta[ib]);
+                        }
                 }
             }
 #pragma unroll
@@ -617,9 +706,19 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                 const int r = row0 + 16 * ib + l16;
                 if (g == 0 && r < s.length) a.delta[(size_t)head * f.q_tokens + s.start + r] = delta[ib];
             }
+            if constexpr (kScaled<E>) growth = growth_of(wave_most(most));
         }
     }
     if (begin < end && !sum_delta) issue(begin, buffer);
+    if constexpr (kScaled<E>) {
+        // From here on p, ds and the sums of ds carry the growth, which is part of
+        // the exponent (its rounding is nlse's own).
+        const float by = __builtin_amdgcn_logf(growth);
+#pragma unroll
+        for (int ib = 0; ib < IB; ++ib)
+            if (far_tile) rests[16 * ib + l16] += by;
+            else nlse[ib] += by;
+    }
     float low = 0.f, high = 0.f;
     for (int t = begin; t < end; ++t, buffer ^= 1) {
         wait_vmcnt<0>();
@@ -655,6 +754,23 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
                     }
                     diagonal_sums(ds[1][0], far0 + 16, f.reach, sums, low, high, lane);
                 }
+            if constexpr (kScaled<E>) {
+                if constexpr (!BIAS)
+                    if (!sum_delta) {
+                        const float by = shrink(ds);
+                        if (by != 1.f) {
+                            growth *= by;
+                            scale_rows(ds, by);
+#pragma unroll
+                            for (int ib = 0; ib < IB; ++ib) {
+                                nlse[ib] += __builtin_amdgcn_logf(by);
+                                if (c) sf[0][ib] = scaled_frag(sf[0][ib], by);
+#pragma unroll
+                                for (int db = 0; db < kDB; ++db) dq[ib][db] *= by;
+                            }
+                        }
+                    }
+            }
 #pragma unroll
             for (int ib = 0; ib < IB; ++ib) sf[c][ib] = to_frag<E>(ds[0][ib], ds[1][ib]);
             if constexpr (E::kSize == 2) {
@@ -688,8 +804,10 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
             for (int db = 0; db < kDB; ++db) *reinterpret_cast<f32x4 *>(row + 16 * db) = dq[ib][db];
             continue;
         }
-        store_rows<E, kDB>(dq[ib], f.scale, a.dq.at((long long)s.start + r, head), r < s.length, f.dim, lane);
+        store_rows<E, kDB>(dq[ib], kScaled<E> ? f.scale / growth : f.scale, a.dq.at((long long)s.start + r, head), r < s.length, f.dim, lane);
     }
+    if constexpr (kScaled<E>)  // ds of this wave's is below 2^15 / growth
+        if (lane == 0) a.most[((size_t)head * a.q_slots + s.start / kRows + s.sequence + s.index) * 4 + wave] = kMost / growth;
     if constexpr (BIAS) {
         if (!part) return;
         low = group_sum<kWave>(low);
@@ -697,6 +815,10 @@ __global__ __launch_bounds__(256, 1) void attention_queries_kernel(GradArgs a) {
         if (lane == 0) {
             sums[0] += low;
             sums[2 * f.reach] += high;
+        }
+        if constexpr (kScaled<E>) {
+            asm volatile("" ::: "memory");  // (other lanes' additions)
+            for (int i = lane; i < width; i += kWave) sums[i] *= 1.f / growth;
         }
         lds_barrier();
         for (int i = threadIdx.x; i < width; i += 256) {
@@ -716,7 +838,7 @@ constexpr int key_blocks(int size, int dim) { return size == 4 || dim > 64 ? 1 :
 struct BackwardPlan {
     int dim, q_rows, k_rows, parts, chunk, q_parts, q_chunk;
     long long q_slots, k_slots;
-    size_t terms, part, part_kv, part_q;  // bytes
+    size_t terms, most, part, part_kv, part_q;  // bytes
 };
 
 BackwardPlan backward_plan(const bfhip_attention_desc *d) {
@@ -741,6 +863,7 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
                     ? (int)std::max(1ll, std::min({32ll, 1024 / q_units, d->k_tokens / 128})) : 1;
     const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
     p.terms = round((size_t)d->heads * d->q_tokens * sizeof(float)) * (d->bias ? 3 : 2);
+    p.most = d->type == BFHIP_F16 ? round((size_t)d->heads * p.q_slots * 4 * sizeof(float)) : 0;
     p.part = d->bias ? round((size_t)p.q_slots * d->heads * (2 * d->reach + 1) * sizeof(float)) : 0;
     p.part_kv = p.parts > 1 ? (size_t)p.parts * d->k_tokens * d->kv_heads * 2 * p.dim * sizeof(float) : 0;
     p.part_q = p.q_parts > 1 ? (size_t)p.q_parts * d->q_tokens * d->heads * p.dim * sizeof(float) : 0;
@@ -752,7 +875,7 @@ BackwardPlan backward_plan(const bfhip_attention_desc *d) {
 extern "C" size_t bfhip_attention_backward_workspace(const bfhip_attention_desc *d) {
     if (bad_attention(d)) return 0;
     const BackwardPlan p = backward_plan(d);
-    return p.terms + p.part + p.part_kv + p.part_q;
+    return p.terms + p.most + p.part + p.part_kv + p.part_q;
 }
 
 extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfhip_rows *q, const bfhip_rows *k,
@@ -767,7 +890,7 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         bad_result(dk, d->k_tokens, d->kv_heads, n, size) || bad_result(dv, d->k_tokens, d->kv_heads, n, size))
         return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
     const BackwardPlan p = backward_plan(d);
-    const size_t need = p.terms + p.part + p.part_kv + p.part_q;
+    const size_t need = p.terms + p.most + p.part + p.part_kv + p.part_q;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "attention workspace too small or not 16-byte aligned");
     const long long q_grid = p.q_slots * d->heads * p.q_parts;
@@ -791,9 +914,12 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
     const size_t term = p.terms / (d->bias ? 3 : 2);
     a.delta = (float *)(work + term);
     a.rest = d->bias ? (float *)(work + 2 * term) : nullptr;
-    a.part = dbias ? (float *)(work + p.terms) : nullptr;
-    a.part_kv = (float *)(work + p.terms + p.part);
-    a.part_q = (float *)(work + p.terms + p.part + p.part_kv);
+    a.most = (float *)(work + p.terms);
+    a.q_slots = (int)p.q_slots;
+    a.sum_delta = dbias || (d->bias && d->type == BFHIP_F16);
+    a.part = dbias ? (float *)(work + p.terms + p.most) : nullptr;
+    a.part_kv = (float *)(work + p.terms + p.most + p.part);
+    a.part_q = (float *)(work + p.terms + p.most + p.part + p.part_kv);
     a.q_parts = p.q_parts;
     a.q_chunk = p.q_chunk;
     a.joins = (int)k_joins;

@@ -113,8 +113,11 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * Scores and the softmax are fp32; for 16-bit types the probabilities, and in
  * the backward pass the gradients of the scores, are rounded to the type where
  * they enter the matrix cores (where a query sees few keys, their rounding's rest
- * enters too).  A score's gradient beyond the type's range (fp16:
- * 65504) becomes infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
+ * enters too).  fp16: the forward pass loses probabilities 2^-25 below a row's
+ * largest; the backward pass multiplies by powers of two on the way, so that
+ * gradients of scores may be of any size: it loses what lies 2^-36 below the
+ * largest |dout . v| of some 32 rows.  Results beyond the type's range become
+ * infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
  * fp32: a large bias (1e9, the lowest fp32 value) swallows the score, so that a
  * query all of whose keys have it takes their mean.  Finite biases beyond 2.3e38
  * of either sign count as that.  The backward pass finds the sum of a query's
@@ -124,8 +127,8 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * Workspaces: the forward's holds the sums of keys that are split (few queries
  * on many keys, at most 1 GiB; mostly none), the backward's two fp32 per query
  * and head (three with a bias), sums of queries that are split (at most 128 MiB;
- * of keys in fp32, 32 MiB), and with a bias 2 * reach + 1 fp32 per head for
- * every 64 (fp32) or 128 queries and every sequence.
+ * of keys in fp32, 32 MiB), and for every head, every 64 (fp32) or 128 queries
+ * and every sequence 2 * reach + 1 fp32 with a bias and four in fp16.
  *
  * head_dim: a multiple of 8, at most 128.  Rows: pointer, token and head
  * stride in elements; the elements of one head are contiguous, pointers and

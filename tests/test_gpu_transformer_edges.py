@@ -268,6 +268,59 @@ def test_attention_gradients_beyond_the_type(device, keys):
     assert torch.isfinite(dv).all()
 
 
+@pytest.fixture
+def whole_range(monkeypatch):
+    """Bounds without what fp16's smallest numbers would cost inside: only
+    results are rounded to them."""
+    small = ref.tiny
+    monkeypatch.setattr(ref, "tiny", lambda dtype: 0.0)
+    return small
+
+
+@pytest.mark.parametrize("case", [(F16, 2, 1, 64, [40, 3], [300, 60], False, 5), (F16, 2, 2, 32, [200], [600], False, 9),
+                                  (F16, 4, 1, 128, [129], None, True, None), (F16, 1, 1, 16, [3], [5000], False, None)], ids=str)
+def test_attention_of_small_gradients(device, case, whole_range):
+    """fp16: probabilities and score gradients far below the type's smallest
+    normal number reach the gradients."""
+    call, dout = inputs(device, case)
+    if call["bias"] is not None:  # most keys' weights near 2^-24
+        call["bias"][:, :3] -= 17.0
+    else:
+        call["q"].mul_(0.05)
+        call["k"].mul_(16.0)
+    heads, kv_heads, t = dout.shape[1], call["k"].shape[1], whole_range(F16)
+    group = heads // kv_heads
+    for size in (1.0, 2.0 ** -17):
+        g = (dout * size).contiguous()
+        want = ref.attention(**call, dout=g)
+        # p enters times 2^12, ds times a power of two that takes the largest
+        # |dout . v| to 2^13 or more, in the keys' walk 4 times it: each loses
+        # 2^-25 there.
+        most = max((g[:, h].double() @ call["v"][:, h // group].double().T).abs().max() for h in range(heads))
+        lost = most * 2.0 ** -38 * abs(call["scale"])
+        total = lambda x: x.abs().double().sum(0)
+        shared = lambda x: total(x).unflatten(0, (kv_heads, group)).sum(1)
+        floor = dict(dq=lost * total(call["k"]).repeat_interleave(group, 0) + t, dk=4 * lost * shared(call["q"]) + t,
+                     dv=2.0 ** -37 * shared(g) + t, dbias=0.0)
+        out, lse = bfhip.attention(**call, lse=True)
+        for name, got in zip(("dq", "dk", "dv", "dbias"), grads(call, g, out, lse)):
+            value, bound = want[name]
+            ref.check(f"{name} x {size}", got, value, bound + floor[name])
+
+
+def test_attention_gradients_of_uneven_rows(device):
+    """fp16: rows and keys whose gradients differ by many powers of two, the
+    small ones first and last."""
+    call, dout = inputs(device, (F16, 4, 2, 64, [300, 90], [300, 500], True, None))
+    size = 2.0 ** torch.randint(-14, 7, (390, 1, 1), generator=gen(device, 5), device=device)
+    size[:64], size[-64:] = 2.0 ** -14, 2.0 ** -14
+    dout = (dout * size).half()
+    want = ref.attention(**call, dout=dout)
+    out, lse = bfhip.attention(**call, lse=True)
+    for name, t in zip(("dq", "dk", "dv"), grads(call, dout, out, lse)):
+        ref.check(name, t, *want[name])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n", [1, 5, 100, 257])
 def test_layer_norm_gradients_of_large_equal_rows(device, dtype, n):

@@ -41,7 +41,8 @@ def test_attention_backward_workspace_is_bounded():
         rows, up = (64 if d.type == 0 else 128), lambda n: (n + 255) // 256 * 256
         terms = (3 if d.bias else 2) * up(4 * d.heads * d.q_tokens)
         part = up(4 * d.heads * (2 * d.reach + 1) * (d.q_tokens // rows + d.sequences)) if d.bias else 0
-        rest = size(d) - terms - part
+        most = up(16 * d.heads * (d.q_tokens // rows + d.sequences)) if d.type == 1 else 0
+        rest = size(d) - terms - part - most
         assert 0 <= rest <= (128 << 20) + ((32 << 20) if d.type == 0 and not d.bias else 0)
 
 
