@@ -42,12 +42,13 @@ constexpr float far_lse(int size) { return size == 4 ? 64.f : 1024.f; }
 
 // fp16 holds 2^-24 to 65504; p of many keys and score gradients lie outside.  p is
 // at most 1 and enters the matrix cores times kSpread.  ds enters times a power of
-// two, the growth, one for the 16 to 32 rows of a wave.  In the queries' walk it
-// takes the largest |dout . v| to 2^13 or more (kGrowth at most) where delta is
+// two, the growth, one per wave.  In the queries' walk it takes the largest
+// |dout . v| of the wave's 32 rows to 2^13 or more (kGrowth at most) where delta is
 // summed: |ds| is at most twice that.  Elsewhere the largest ds is watched, and
 // what has been summed shrinks when one passes kMost.  The keys' walk gets a bound
-// of ds from the queries' (`most`).  So what a wave's rows lose lies 2^-36 below
-// the largest |dout . v|.  Powers of two change no other bits.
+// of ds, over all queries that it meets, from the queries' (`most`).  So what is
+// lost lies 2^-36 below the largest |dout . v|; powers of two change no other
+// bits.
 constexpr float kSpread = 0x1p12f, kLogSpread = 12.f, kGrowth = 0x1p40f, kMost = 0x1p15f;
 
 template <class E>
@@ -136,26 +137,26 @@ __device__ __forceinline__ Steps query_steps(int causal, int first_key, int offs
     return s;
 }
 
-template <class E, int DIM, int KB, int WAVES, bool BIAS>
+template <class E, int DIM, int KB, bool BIAS>
 struct KeyTile {
-    static constexpr int kRows = WAVES * 16 * KB, kThreads = WAVES * kWave;
+    static constexpr int kRows = 64 * KB, kThreads = 4 * kWave;
     static constexpr int kTerms = BIAS ? 3 : 2;                // nlse, delta and rest of a query
     static constexpr int kQ = kTile * AttnTile<E, DIM>::kRow;  // bytes of a tile of q or dout
     static constexpr int kStage = 2 * kQ + kTerms * kTile * (int)sizeof(float);
 };
 
-// KB blocks of 16 keys per wave.  Scores come out with a key per lane, so P and
-// dS are the second operands of dv^T = dout^T P and dk^T = q^T dS without
-// leaving their registers.  8192 causal tokens, 16 heads of 128 on 4, bf16: 267
+// KB blocks of 16 keys per wave, four waves.  Scores come out with a key per
+// lane, so P and dS are the second operands of dv^T = dout^T P and dk^T = q^T dS
+// without leaving their registers.  8192 causal tokens, 16 heads of 128 on 4, bf16: 267
 // us, 0.70 PFLOP/s: q and dout are read from LDS twice, as rows and transposed,
 // for KB x 16 keys, and with the registers for two waves per SIMD the reads'
 // latency shows (matrix cores 32 % busy, LDS 36 %).  Measured when this one took
 // 300 us: two blocks of keys, which halve the reads but leave one wave per SIMD,
 // 380; three waves on tiles of 32 queries 324; parts that are dealt last
 // instead of one after the other 300 (the longest work then ends the grid).
-template <class E, int DIM, int KB, int WAVES, bool BIAS>
-__global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArgs a) {
-    using K = KeyTile<E, DIM, KB, WAVES, BIAS>;
+template <class E, int DIM, int KB, bool BIAS>
+__global__ __launch_bounds__(256, 1) void attention_keys_kernel(GradArgs a) {
+    using K = KeyTile<E, DIM, KB, BIAS>;
     constexpr int kRows = K::kRows, kKB = DIM / 32, kDB = DIM / 16, kThreads = K::kThreads;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const AttnArgs &f = a.f;
@@ -185,9 +186,10 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
         gc.issue(a.dout.at((long long)q_start + i0, head), left, to + K::kQ);
         // Past the last query q, dout and the terms are zero: ds is 0, and p is 1
         // (or what a bias makes it, which may be infinite: masked below).
-        if (wave < K::kTerms)
-            dma4(buffer_rsrc((wave == 0 ? a.nlse : wave == 1 ? a.delta : a.rest) + (size_t)head * f.q_tokens + q_start + i0, 4u * min(left, kTile)),
-                 to + 2 * K::kQ + wave * kTile * sizeof(float), 4u * lane);
+        if (wave < K::kTerms) {
+            const float *const term = (wave == 0 ? a.nlse : wave == 1 ? a.delta : a.rest) + (size_t)head * f.q_tokens + q_start + i0;
+            dma4(buffer_rsrc(term, 4u * min(left, kTile)), to + 2 * K::kQ + wave * kTile * sizeof(float), 4u * lane);
+        }
     };
     typename E::Frag kf[KB][kKB], vf[KB][kKB];
     f32x4 dk[KB][kDB], dv[KB][kDB];
@@ -306,9 +308,7 @@ __global__ __launch_bounds__(WAVES *kWave, 1) void attention_keys_kernel(GradArg
                         for (int e = 0; e < 4; ++e)
                             if (16 * b + e >= left) p[b][kb][e] = ds[b][kb][e] = 0.f;
             }
-            if constexpr (kScaled<E>) {
-                scale_rows(ds, growth);
-            }
+            if constexpr (kScaled<E>) scale_rows(ds, growth);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 pf[c][kb] = to_frag<E>(p[0][kb], p[1][kb]);
@@ -440,8 +440,8 @@ __device__ __forceinline__ float row_shift(float v) {
 // Either write is then to addresses of one lane each.  A sum's next addition may
 // be another lane's, which the compiler, who sees one lane's addresses differ,
 // must not move before this one: LDS serves a wave in its order, so that keeping
-// the instructions' order fixes the sums'.  Distances at or beyond the reach are left to the
-// caller's low and high sums.
+// the instructions' order fixes the sums'.  Distances at or beyond the reach are
+// left to the caller's low and high sums.
 __device__ __forceinline__ void diagonal_sums(const f32x4 &ds, int far0, int reach, float *sum, float &low, float &high,
                                               int lane) {
     const int i = lane & 15, g = lane >> 4;
@@ -928,11 +928,11 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
         with_element(d->type, [&](auto e) {
             with_dim(n, [&](auto dim) {
                 using E = decltype(e);
-                constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), WAVES = 4, KB = key_blocks(E::kSize, DIM);
+                constexpr int DIM = decltype(dim)::value, QB = row_blocks(E::kSize), KB = key_blocks(E::kSize, DIM);
                 using T = AttnTile<E, DIM>;
                 const auto run = [&](auto with_bias) {
                     constexpr bool B = decltype(with_bias)::value;
-                    using K = KeyTile<E, DIM, KB, WAVES, B>;
+                    using K = KeyTile<E, DIM, KB, B>;
                     const size_t row = B ? BiasRow::floats(d->reach) * sizeof(float) : 0;
                     GradArgs b = a;
                     if (d->q_tokens) {
@@ -945,14 +945,14 @@ extern "C" int bfhip_attention_backward(const bfhip_attention_desc *d, const bfh
                     if (d->k_tokens) {
                         b.f.slots = (int)p.k_slots;
                         b.f.ordered = by_work(d, k_grid);
-                        hipLaunchKernelGGL((attention_keys_kernel<E, DIM, KB, WAVES, B>), dim3((unsigned)k_grid),
+                        hipLaunchKernelGGL((attention_keys_kernel<E, DIM, KB, B>), dim3((unsigned)k_grid),
                                            dim3(K::kThreads), 2 * K::kStage + row, s, b);
                     }
                 };
                 if (d->bias) run(std::true_type{});
                 else run(std::false_type{});
                 if (joins)
-                    hipLaunchKernelGGL((attention_gradient_join_kernel<E, DIM, WAVES * 16 * KB>), dim3((unsigned)joins), dim3(256), 0, s, a);
+                    hipLaunchKernelGGL((attention_gradient_join_kernel<E, DIM, 64 * KB>), dim3((unsigned)joins), dim3(256), 0, s, a);
             });
         });
     if (dbias) column_sum(a.part, d->q_tokens && d->sequences ? p.q_slots : 0, dbias, dbias, count, count, s);

@@ -116,8 +116,8 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * enters too).  fp16: the forward pass loses probabilities 2^-25 below a row's
  * largest; the backward pass multiplies by powers of two on the way, so that
  * gradients of scores may be of any size: it loses what lies 2^-36 below the
- * largest |dout . v| of some 32 rows.  Results beyond the type's range become
- * infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
+ * largest |dout . v| of 32 neighbouring queries (dq) or of all queries that meet a
+ * key (dk).  Results beyond the type's range become infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
  * fp32: a large bias (1e9, the lowest fp32 value) swallows the score, so that a
  * query all of whose keys have it takes their mean.  Finite biases beyond 2.3e38
  * of either sign count as that.  The backward pass finds the sum of a query's
