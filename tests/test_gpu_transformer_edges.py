@@ -360,3 +360,81 @@ def test_attention_of_one_token_of_any_stride(device):
         assert torch.equal(got, want)
         back = grads(dict(call, **odd), dout, got, lse)
         assert all(torch.isfinite(t).all() for t in back)
+
+
+@pytest.mark.parametrize("case", [(BF16, 8, 2, 64, [1] * 12, 4000, True), (F16, 4, 1, 128, [1, 3, 1, 2], 900, True),
+                                  (F32, 2, 2, 32, [70, 1, 30], 300, False)], ids=str)
+def test_attention_of_caches_with_room(device, case):
+    """Keys kept in places of a fixed size: what a place has left over is a
+    sequence without queries, whatever lies there."""
+    dtype, heads, kv_heads, dim, ql, room, causal = case
+    g = gen(device, 7)
+    kl = torch.randint(max(ql), room, (len(ql),), generator=g, device=device).tolist()
+    call, dout = inputs(device, (dtype, heads, kv_heads, dim, ql, kl, causal, None), layout="plain")
+    want = ref.attention(**call, dout=dout)
+    wide = {n: torch.full((room * len(ql), kv_heads, dim), math.nan, dtype=dtype, device=device) for n in "kv"}
+    rows = torch.cat([torch.arange(room * i, room * i + n, device=device) for i, n in enumerate(kl)])
+    for n in "kv":
+        wide[n][rows] = call[n]
+    q_at, k_at = [0], [0]
+    for i, (n, m) in enumerate(zip(ql, kl)):
+        q_at += [q_at[-1] + n] * 2
+        k_at += [room * i + m, room * (i + 1)]
+    there = dict(call, **wide, q_starts=torch.tensor(q_at, device=device).int(), k_starts=torch.tensor(k_at, device=device).int())
+    out, lse = bfhip.attention(**there, lse=True)
+    ref.check("out", out, *want["out"])
+    dq, dk, dv = grads(there, dout, out, lse)
+    for name, t in (("dq", dq), ("dk", dk[rows]), ("dv", dv[rows])):
+        ref.check(name, t, *want[name])
+    left = torch.ones(dk.shape[0], dtype=torch.bool, device=device)
+    left[rows] = False
+    assert not dk[left].any() and not dv[left].any()
+
+
+@pytest.mark.parametrize("case", [(BF16, 4, 2, 64, None), (F16, 4, 1, 32, 6), (F32, 2, 1, 128, None)], ids=str)
+def test_attention_replayed_with_other_starts(device, case):
+    """A captured call reads its starts when it runs."""
+    dtype, heads, kv_heads, dim, reach = case
+    lens = [([70, 1, 9], [300, 400, 20]), ([1, 78, 1], [20, 100, 600]), ([0, 80, 0], [360, 355, 5])]
+    call, dout = inputs(device, (dtype, heads, kv_heads, dim, *lens[0], True, reach))
+
+    def run(c):
+        out, lse = bfhip.attention(**c, lse=True)
+        return out, lse, *grads(c, dout, out, lse)
+
+    run(call)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(call)
+    for ql, kl in lens[1:] + lens[:1]:
+        for name, n in (("q_starts", ql), ("k_starts", kl)):
+            call[name].copy_(starts(n, device))
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, run(call)))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("case", [(2, 1, 64, [100, 3], [100, 9], True, None), (2, 2, 32, [70, 30], [500, 30], False, 4),
+                                  (1, 1, 16, [40, 3], [3000, 60], False, None)], ids=str)
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_attention_gradients_that_are_not_finite_show(device, dtype, case, value):
+    """An infinite dout: its query's gradient is not finite, nor are those of the
+    keys that it sees; other queries' and other sequences' are what they were."""
+    call, dout = inputs(device, (dtype, *case))
+    want = ref.attention(**call, dout=dout)
+    out, lse = bfhip.attention(**call, lse=True)
+    dout[17, 0] = value
+    dq, dk, dv, *_ = grads(call, dout, out, lse)
+    assert not torch.isfinite(dq[17, 0]).any()
+    assert not torch.isfinite(dk[:17, 0]).any() and not torch.isfinite(dv[:17, 0]).any()
+    others = torch.ones(dq.shape[:2], dtype=torch.bool, device=device)
+    others[17, 0] = False
+    ref.check("dq", dq[others], want["dq"][0][others], want["dq"][1][others])
+    n = call["k_starts"][1]
+    for name, t in (("dk", dk), ("dv", dv)):
+        ref.check(name, t[n:], want[name][0][n:], want[name][1][n:])
