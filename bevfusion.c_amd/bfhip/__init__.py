@@ -613,6 +613,8 @@ def _attention_desc(q, k, v, q_starts, k_starts, causal, scale, bias):
     rows = [_head_rows("q", q, q), _head_rows("k", k, q), _head_rows("v", v, q)]
     if v.shape != k.shape:
         raise BfHipError("k and v must have one shape")
+    if not q.shape[2]:
+        raise BfHipError("heads must have elements")
     n = q_starts.numel() - 1
     if n < 0:
         raise BfHipError("starts must hold one entry more than there are sequences")

@@ -6,6 +6,9 @@ import pathlib
 import random
 import re
 
+import pytest
+import torch
+
 import bfhip
 
 
@@ -75,3 +78,9 @@ def test_attention_backward_refuses_what_no_launch_holds():
         return error.value
 
     assert b"too many" in call(65535, 2047) and b"too many" in call(33000, 2047)
+
+
+def test_python_refuses_heads_of_no_elements():
+    empty, at = torch.zeros((4, 2, 0)), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(bfhip.BfHipError):
+        bfhip.attention(empty, empty, empty, at, at)
