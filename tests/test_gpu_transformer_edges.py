@@ -438,3 +438,28 @@ def test_attention_gradients_that_are_not_finite_show(device, dtype, case, value
     n = call["k_starts"][1]
     for name, t in (("dk", dk), ("dv", dv)):
         ref.check(name, t[n:], want[name][0][n:], want[name][1][n:])
+
+
+def test_calls_on_two_streams_at_once(device):
+    """Split work, gradients and norms in flight on two streams, each call's
+    workspace its own."""
+    sets = [inputs(device, case) for case in ((BF16, 8, 2, 128, [1500, 40], None, True, 60),
+                                              (F16, 8, 8, 16, [200], [4000], False, None))]
+    g = gen(device, 9)
+    x, gamma = randn(g, 5000, 257, dtype=F16), randn(g, 257)
+
+    def run(call, dout, stream=None):
+        out, lse = bfhip.attention(**call, lse=True, stream=stream)
+        c = dict(call)
+        back = bfhip.attention_backward(dout, c.pop("q"), c.pop("k"), c.pop("v"), out, lse, **c, stream=stream)
+        y, mean, rstd = bfhip.layer_norm(x, gamma, stats=True, stream=stream)
+        return out, lse, *back, y, *bfhip.layer_norm_backward(x, x, mean, rstd, gamma, stream=stream)
+
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = [[run(*s, stream=stream) for _ in range(3)] for s, stream in zip(sets, streams)]
+        torch.cuda.synchronize()
+        for rows, expected in zip(got, want):
+            assert all(torch.equal(a, b) for row in rows for a, b in zip(row, expected))
