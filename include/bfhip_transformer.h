@@ -117,12 +117,15 @@ int bfhip_position_bias_backward(const float *dbias, const int *map, float *dtab
  * largest; the backward pass multiplies by powers of two on the way, so that
  * gradients of scores may be of any size: it loses what lies 2^-36 below the
  * largest |dout . v| of 32 neighbouring queries (dq) or of all queries that meet a
- * key (dk).  Results beyond the type's range become infinite.  fp32 is multiplied in fp32.  A score and its bias are added in
- * fp32: a large bias (1e9, the lowest fp32 value) swallows the score, so that a
- * query all of whose keys have it takes their mean.  Finite biases beyond 2.3e38
- * of either sign count as that.  The backward pass finds the sum of a query's
- * probabilities again where a bias has taken its lse far from zero; without a
- * bias it takes them from lse alone, off by a factor of about 1 +- |lse| 2^-22.
+ * key (dk).  Results beyond the type's range become infinite.  fp32 is multiplied
+ * in fp32.
+ *
+ * A score and its bias are added in fp32: a large bias (1e9, the lowest fp32
+ * value) swallows the score, so that a query all of whose keys have it takes
+ * their mean.  Finite biases beyond 2.3e38 of either sign count as that.  The
+ * backward pass finds the sum of a query's probabilities again where a bias has
+ * taken its lse far from zero; without a bias it takes them from lse alone, off
+ * by a factor of about 1 +- |lse| 2^-22.
  *
  * Workspaces: the forward's holds the sums of keys that are split (few queries
  * on many keys, at most 1 GiB; mostly none), the backward's two fp32 per query
