@@ -205,7 +205,31 @@ class AttentionDesc(C.Structure):
                 ("q_starts", _vp), ("k_starts", _vp), ("bias", _vp)]
 
 
+class RotaryDesc(C.Structure):
+    """``bfhip_rotary_desc`` (include/bfhip_transformer.h)."""
+    _fields_ = [(n, _i) for n in ("type", "head_dim", "part", "interleaved", "inverse", "heads",
+                                  "heads2")] + \
+               [("amplitude", C.c_float), ("tokens", C.c_longlong), ("positions", _vp),
+                ("frequencies", _vp)]
+
+
+class Pages(C.Structure):
+    """``bfhip_pages`` (include/bfhip_transformer.h)."""
+    _fields_ = [("data", _vp), ("page_stride", C.c_longlong), ("token_stride", C.c_longlong),
+                ("head_stride", C.c_longlong)]
+
+
+class PagedDesc(C.Structure):
+    """``bfhip_paged_desc`` (include/bfhip_transformer.h)."""
+    _fields_ = [(n, _i) for n in ("type", "sequences", "heads", "kv_heads", "head_dim", "page_size",
+                                  "table_pages", "reach")] + \
+               [("scale", C.c_float), ("tokens", C.c_longlong), ("pages", C.c_longlong),
+                ("table_stride", C.c_longlong), ("starts", _vp), ("lengths", _vp), ("table", _vp),
+                ("bias", _vp)]
+
+
 _ll, _rowsp, _attnp = C.c_longlong, C.POINTER(Rows), C.POINTER(AttentionDesc)
+_rotaryp, _pagesp, _pagedp = C.POINTER(RotaryDesc), C.POINTER(Pages), C.POINTER(PagedDesc)
 
 # The operators of include/bfhip_transformer.h, which the reference's ABI does not have.
 TRANSFORMER_SIGNATURES = {
@@ -224,6 +248,12 @@ TRANSFORMER_SIGNATURES = {
                                                                _sz]),
     "bfhip_attention_backward": (_i, [_attnp] + [_rowsp] * 4 + [_vp] + [_rowsp] * 4
                                  + [_vp, _vp, _sz, _vp, C.c_char_p, _sz]),
+    "bfhip_rotary": (_i, [_rotaryp] + [_rowsp] * 4 + [_vp, C.c_char_p, _sz]),
+    "bfhip_rotary_frequencies": (_i, [_i] + [C.c_double] * 5 + [_vp, C.c_char_p, _sz]),
+    "bfhip_cache_append": (_i, [_pagedp, _rowsp, _rowsp, _pagesp, _pagesp, _vp, C.c_char_p, _sz]),
+    "bfhip_paged_attention_workspace": (_sz, [_pagedp]),
+    "bfhip_paged_attention": (_i, [_pagedp, _rowsp, _pagesp, _pagesp, _rowsp, _vp, _vp, _sz, _vp,
+                                   C.c_char_p, _sz]),
 }
 
 SWIN_OPS = ("ln1", "qkv", "attention", "proj", "ln2", "fc1", "fc2", "merge", "mlp", "wmsa")
@@ -685,6 +715,151 @@ def attention_backward(dout, q, k, v, out, lse, q_starts, k_starts, causal=False
             desc, *rows, ro, pl, rg, *(_head_rows("gradient", t, q) for t in grads[:3]), pb, pw,
             size, queue, err, 512), err, "bfhip_attention_backward")
     return tuple(grads)
+
+
+def rotary_frequencies(part, base=10000.0, factor=1.0, length=0, low=1.0, high=4.0, device="cuda"):
+    """Radians per position of rotary's part / 2 pairs (bfhip_rotary_frequencies):
+    fp64 on `device`.  Contexts `factor` times as long as the trained ones divide
+    them by factor, all of them, or by parts if the trained `length` is given."""
+    torch, err = _torch(), _err()
+    out = torch.empty(max(part, 0) // 2, dtype=torch.float64)
+    _check(hip_lib().bfhip_rotary_frequencies(part, base, factor, length, low, high,
+                                              out.data_ptr(), err, 512),
+           err, "bfhip_rotary_frequencies")
+    return out.to(device)
+
+
+def rotary(q, k, positions, frequencies, interleaved=False, amplitude=1.0, out=None, stream=None):
+    """Queries and keys turned by their positions (bfhip_rotary).  q [tokens,
+    heads, head_dim] and k [tokens, kv_heads, head_dim] with contiguous heads
+    (views of a fused projection will do), k may be None; positions int32
+    [tokens]; frequencies fp64 [part / 2] of the elements that turn.  `out`: a
+    tensor for each (q and k themselves: in place).  Returns (q, k) turned, or q
+    alone without k."""
+    return _rotary(q, k, positions, frequencies, interleaved, amplitude, out, stream, 0)
+
+
+def rotary_backward(dq, dk, positions, frequencies, interleaved=False, amplitude=1.0, out=None,
+                    stream=None):
+    """Gradients of rotary's q and k from those of its results (bfhip_rotary)."""
+    return _rotary(dq, dk, positions, frequencies, interleaved, amplitude, out, stream, 1)
+
+
+def _rotary(q, k, positions, frequencies, interleaved, amplitude, out, stream, inverse):
+    torch = _torch()
+    code, given = _type_code(q), [q] if k is None else [q, k]
+    rows = [_head_rows(n, t, q) for n, t in zip("qk", given)]
+    tokens, heads, dim = q.shape
+    if any(t.shape[0] != tokens for t in given):
+        raise BfHipError("q and k must have the same tokens")
+    pp = _expect("positions", positions, q, (tokens,), torch.int32)
+    pf = _expect("frequencies", frequencies, q, (frequencies.numel(),), torch.float64)
+    wanted = [None] * len(given) if out is None else [out] if torch.is_tensor(out) else list(out)
+    if len(wanted) != len(given):
+        raise BfHipError("out must hold a tensor for each of q and k")
+    desc = RotaryDesc(code, dim, 2 * frequencies.numel(), int(interleaved), inverse, heads,
+                      0 if k is None else k.shape[1], amplitude, tokens, pp, pf)
+    with _place(stream, *given, positions, frequencies, *wanted) as queue:
+        results = [t.new_empty(t.shape) if o is None else o for t, o in zip(given, wanted)]
+        if any(o.shape != t.shape for o, t in zip(results, given)):
+            raise BfHipError("out must have the shapes of q and k")
+        to = [_head_rows("out", o, q) for o in results]
+        if k is None:
+            rows.append(None)
+            to.append(None)
+        err = _err()
+        _check(hip_lib().bfhip_rotary(desc, rows[0], to[0], rows[1], to[1], queue, err, 512),
+               err, "bfhip_rotary")
+    return results[0] if k is None else tuple(results)
+
+
+def _page_pool(what, t, like):
+    """[pages, page_size, kv_heads, head_dim] with contiguous heads -> Pages."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 4 or (stride[3] != 1 and shape[3] > 1):
+        raise BfHipError(f"{what} must be [pages, page_size, kv_heads, head_dim] with contiguous "
+                         "heads")
+    if t.dtype != like.dtype or t.device != like.device or shape[3] != like.shape[-1]:
+        raise BfHipError(f"{what} must be {like.dtype} of head_dim {like.shape[-1]} on "
+                         f"{like.device}")
+    return Pages(t.data_ptr(), *stride[:3])
+
+
+def _paged_desc(like, heads, k_pages, v_pages, page_table, starts, lengths, scale, bias):
+    torch = _torch()
+    code = _type_code(like)
+    pools = [_page_pool("k_pages", k_pages, like), _page_pool("v_pages", v_pages, like)]
+    if k_pages.shape != v_pages.shape:
+        raise BfHipError("k_pages and v_pages must have one shape")
+    pages, size, kv_heads, dim = k_pages.shape
+    n = starts.numel() - 1
+    if n < 0:
+        raise BfHipError("starts must hold one entry more than there are sequences")
+    if (page_table.dim() != 2 or page_table.shape[0] != n or page_table.dtype != torch.int32
+            or page_table.device != like.device
+            or (page_table.stride(1) != 1 and page_table.shape[1] > 1)):
+        raise BfHipError(f"page_table must be an int32 [{n}, pages of a sequence] tensor with "
+                         f"contiguous rows on {like.device}")
+    ps = _expect("starts", starts, like, (n + 1,), torch.int32)
+    pl = _expect("lengths", lengths, like, (n,), torch.int32)
+    reach, pb = 0, None
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[1] % 2 == 0:
+            raise BfHipError("bias must be [heads, 2 * reach + 1]")
+        reach = bias.shape[1] // 2
+        pb = _expect("bias", bias, like, (heads, 2 * reach + 1), torch.float32)
+    return PagedDesc(code, n, heads, kv_heads, dim, size, page_table.shape[1], reach, scale,
+                     like.shape[0], pages, page_table.stride(0), ps, pl, page_table.data_ptr(),
+                     pb), pools
+
+
+def cache_append(k, v, k_pages, v_pages, page_table, starts, lengths, stream=None):
+    """Copies new tokens' keys and values [tokens, kv_heads, head_dim] into their
+    pages (bfhip_cache_append).  k_pages and v_pages [pages, page_size, kv_heads,
+    head_dim]; page_table int32 [sequences, pages of a sequence]; starts int32
+    [sequences + 1], the sequences' new tokens; lengths int32 [sequences], their
+    keys with the new tokens, which stand at the end."""
+    rows = [_head_rows("k", k, k), _head_rows("v", v, k)]
+    if k.shape != v.shape or k.shape[1] != k_pages.shape[2]:
+        raise BfHipError("k and v must have one shape, with the pages' heads")
+    desc, pools = _paged_desc(k, k.shape[1], k_pages, v_pages, page_table, starts, lengths, 1.0,
+                              None)
+    with _place(stream, k, v, k_pages, v_pages, page_table, starts, lengths) as queue:
+        err = _err()
+        _check(hip_lib().bfhip_cache_append(desc, *rows, *pools, queue, err, 512), err,
+               "bfhip_cache_append")
+
+
+def paged_attention(q, k_pages, v_pages, page_table, starts, lengths, scale=None, bias=None,
+                    out=None, lse=False, stream=None):
+    """Causal attention of new tokens q [tokens, heads, head_dim] over a paged
+    cache that holds their own keys and values already (bfhip_paged_attention;
+    the cache as in cache_append, scale and bias as in attention).  Returns out
+    like q, or (out, lse) with `lse`.  Rows that belong to no sequence are not
+    written."""
+    torch = _torch()
+    rq = _head_rows("q", q, q)
+    if not q.shape[2]:
+        raise BfHipError("heads must have elements")
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    desc, pools = _paged_desc(q, q.shape[1], k_pages, v_pages, page_table, starts, lengths, scale,
+                              bias)
+    lib = hip_lib()
+    with _place(stream, q, k_pages, v_pages, page_table, starts, lengths, bias, out) as queue:
+        o = q.new_empty(q.shape) if out is None else out
+        if o.shape != q.shape:
+            raise BfHipError("out must have the shape of q")
+        ro = _head_rows("out", o, q)
+        stat, pl = None, None
+        if lse:
+            stat = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+            pl = stat.data_ptr()
+        size = lib.bfhip_paged_attention_workspace(desc)
+        work, pw = _scratch(size, q)
+        err = _err()
+        _check(lib.bfhip_paged_attention(desc, rq, *pools, ro, pl, pw, size, queue, err, 512),
+               err, "bfhip_paged_attention")
+    return (o, stat) if lse else o
 
 
 def window_map(batches, height, width, shift, device, stream=None):

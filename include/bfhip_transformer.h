@@ -1,7 +1,8 @@
 /*
  * Stateless transformer operators on AMD gfx950, served by libbfhip.so: layer
- * norm, learned position bias by buckets, and attention over packed sequences,
- * each with its backward pass.  They stand beside the stateless linear and
+ * norm, learned position bias by buckets, rotary positions and attention over
+ * packed sequences, each with its backward pass; and for serving a paged cache
+ * of keys and values with the attention of new tokens over it.  They stand beside the stateless linear and
  * convolution of bf_cuda_ops.h and have no counterpart in the reference, whose
  * transformer blocks exist inside its fixed contexts only.
  *
@@ -181,6 +182,119 @@ int bfhip_attention_backward(const bfhip_attention_desc *desc, const bfhip_rows 
                              const bfhip_rows *dk, const bfhip_rows *dv, float *dbias,
                              void *workspace, size_t workspace_bytes,
                              void *stream, char *error, size_t error_cap);
+
+/* ---------------------------------------------------------- rotary positions
+ * Pairs of a head's elements turned by angles that grow with the token's
+ * position, t_i = position * frequencies[i], i < part / 2, part <= head_dim even:
+ *   (a, b) -> amplitude * (a cos t - b sin t, a sin t + b cos t)
+ * Pair i is the elements (i, i + part / 2), or (2 i, 2 i + 1) if interleaved;
+ * elements from part on are copied.  The gradient is the transposed map: with
+ * `inverse` the angles change their sign (and the amplitude stays).
+ *
+ * x and y: rows of `heads` heads of head_dim elements, strides in elements, of
+ * any alignment; the elements of one head are contiguous, and no head of y lies
+ * on another.  y may be x (in place, the same strides), else they do not
+ * overlap.  A second pair of rows (x2, y2, heads2; heads2 == 0: none) of the same
+ * tokens, type and head_dim shares the angles: queries and keys take one call.
+ * positions: int32 [tokens], of either sign.  frequencies: fp64 [part / 2], in
+ * radians per position.  Angles are reduced in 64 bits, off by at most 2^-51 of
+ * the angle; cosine, sine and products are fp32, results are rounded once.
+ * tokens at most 0x7ffff000, heads and heads2 at most 65535, head_dim at most
+ * 4096. */
+typedef struct {
+    int type;
+    int head_dim;
+    int part;
+    int interleaved;
+    int inverse;
+    int heads;
+    int heads2;
+    float amplitude;
+    long long tokens;
+    const int *positions;
+    const double *frequencies;
+} bfhip_rotary_desc;
+
+int bfhip_rotary(const bfhip_rotary_desc *desc, const bfhip_rows *x, const bfhip_rows *y,
+                 const bfhip_rows *x2, const bfhip_rows *y2,
+                 void *stream, char *error, size_t error_cap);
+
+/* frequencies[i] = base^(-2 i / part) on the host, scaled for contexts `factor`
+ * times as long as the trained one.  length == 0: all of them divided by factor
+ * (positions are interpolated).  Otherwise by parts: a pair that turns r =
+ * length * frequency / 2 pi times over the trained length is kept where
+ * r >= high, divided by factor where r <= low, and mixed linearly in between.
+ * base > 0, factor > 0, length >= 0, low < high. */
+int bfhip_rotary_frequencies(int part, double base, double factor, double length, double low,
+                             double high, double *frequencies, char *error, size_t error_cap);
+
+/* --------------------------------------------------------------- paged cache
+ * Keys and values of many sequences in pages of page_size tokens.  Position j
+ * of sequence b is row j % page_size of page table[b * table_stride +
+ * j / page_size]; a table has table_pages entries per sequence.  Pages may
+ * stand in any order and be shared by sequences.  lengths[b] counts the keys of
+ * sequence b with its new tokens among them: its new tokens, the rows
+ * starts[b] .. starts[b + 1] of q, k and v (starts as in
+ * bfhip_attention_forward; there may be none), stand at its last positions.
+ * Lengths are clamped to [0, table_pages * page_size], which is below 2^31.
+ * starts, lengths and table are int32 on the device.  A table entry outside
+ * [0, pages) is never followed: its positions are written nowhere and seen by no
+ * query.  Entries past a sequence's length are not read.
+ *
+ * Pages: [pages, page_size, kv_heads, head_dim] by strides in elements, of any
+ * size; the elements of one head are contiguous, pointers and strides multiples
+ * of 16 bytes and not negative.  head_dim: a multiple of 8, at most 128. */
+typedef struct {
+    void *data;
+    long long page_stride;
+    long long token_stride;
+    long long head_stride;
+} bfhip_pages;
+
+typedef struct {
+    int type;
+    int sequences;
+    int heads;    /* of the queries; of no account to bfhip_cache_append */
+    int kv_heads;
+    int head_dim;
+    int page_size;
+    int table_pages;
+    int reach;    /* as in bfhip_attention_desc */
+    float scale;
+    long long tokens; /* rows of q, k, v and out */
+    long long pages;
+    long long table_stride;
+    const int *starts;
+    const int *lengths;
+    const int *table;
+    const float *bias;
+} bfhip_paged_desc;
+
+/* Copies the new tokens' keys and values (rows of any alignment) into their
+ * pages.  A token that stands before position 0 (more new tokens than
+ * lengths[b]) or outside every sequence is written nowhere.  Two tokens of one
+ * call must not have the same place. */
+int bfhip_cache_append(const bfhip_paged_desc *desc, const bfhip_rows *k, const bfhip_rows *v,
+                       const bfhip_pages *k_pages, const bfhip_pages *v_pages,
+                       void *stream, char *error, size_t error_cap);
+
+/* Attention of the new tokens over the cache, causal: token i of n stands at
+ * position lengths[b] - n + i and sees the keys up to its own.  Scores, bias,
+ * softmax, roundings, out and lse ([heads, tokens] or NULL) are those of
+ * bfhip_attention_forward, and so is what is said there of rows without keys and
+ * of rows outside every sequence.  Made for few tokens per sequence: a key head's
+ * keys are read once for each 16 rows (token, head of its group); the work is
+ * split over the keys as the lengths on the device say.  Keys past a query's
+ * position and what pages hold past a length reach no result, but a NaN or
+ * infinity in the value of a token reaches the queries of the same sequence in
+ * the same call that stand before it.
+ * The workspace holds the sums of split keys (at most 1 GiB). */
+size_t bfhip_paged_attention_workspace(const bfhip_paged_desc *desc);
+
+int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
+                          const bfhip_pages *k_pages, const bfhip_pages *v_pages,
+                          const bfhip_rows *out, float *lse, void *workspace,
+                          size_t workspace_bytes, void *stream, char *error, size_t error_cap);
 
 #ifdef __cplusplus
 }
