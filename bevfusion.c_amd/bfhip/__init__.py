@@ -228,8 +228,20 @@ class PagedDesc(C.Structure):
                 ("bias", _vp)]
 
 
+class Matrix(C.Structure):
+    """``bfhip_matrix`` (include/bfhip_transformer.h)."""
+    _fields_ = [("data", _vp), ("stride", C.c_longlong)]
+
+
+class GatedDesc(C.Structure):
+    """``bfhip_gated_desc`` (include/bfhip_transformer.h)."""
+    _fields_ = [("type", _i), ("activation", _i), ("rows", C.c_longlong),
+                ("features", C.c_longlong), ("hidden", C.c_longlong)]
+
+
 _ll, _rowsp, _attnp = C.c_longlong, C.POINTER(Rows), C.POINTER(AttentionDesc)
 _rotaryp, _pagesp, _pagedp = C.POINTER(RotaryDesc), C.POINTER(Pages), C.POINTER(PagedDesc)
+_gatedp, _matrixp = C.POINTER(GatedDesc), C.POINTER(Matrix)
 
 # The operators of include/bfhip_transformer.h, which the reference's ABI does not have.
 TRANSFORMER_SIGNATURES = {
@@ -254,7 +266,14 @@ TRANSFORMER_SIGNATURES = {
     "bfhip_paged_attention_workspace": (_sz, [_pagedp]),
     "bfhip_paged_attention": (_i, [_pagedp, _rowsp, _pagesp, _pagesp, _rowsp, _vp, _vp, _sz, _vp,
                                    C.c_char_p, _sz]),
+    "bfhip_gated_linear_workspace": (_sz, [_gatedp]),
+    "bfhip_gated_linear_backward_workspace": (_sz, [_gatedp]),
+    "bfhip_gated_linear": (_i, [_gatedp] + [_matrixp] * 6 + [_vp, _sz, _vp, C.c_char_p, _sz]),
+    "bfhip_gated_linear_backward": (_i, [_gatedp] + [_matrixp] * 9 + [_vp, _sz, _vp, C.c_char_p,
+                                                                       _sz]),
 }
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 
 SWIN_OPS = ("ln1", "qkv", "attention", "proj", "ln2", "fc1", "fc2", "merge", "mlp", "wmsa")
 
@@ -860,6 +879,65 @@ def paged_attention(q, k_pages, v_pages, page_table, starts, lengths, scale=None
         _check(lib.bfhip_paged_attention(desc, rq, *pools, ro, pl, pw, size, queue, err, 512),
                err, "bfhip_paged_attention")
     return (o, stat) if lse else o
+
+
+def _gated_matrix(what, t, shape, like):
+    stride = t.stride()
+    if t.shape != shape or t.dtype != like.dtype or t.device != like.device \
+            or (stride[1] != 1 and shape[1] > 1):
+        raise BfHipError(f"{what} must be a {like.dtype} {list(shape)} tensor with contiguous rows "
+                         f"on {like.device}")
+    return Matrix(t.data_ptr(), stride[0])
+
+
+def _gated_desc(x, w_gate, w_up, activation):
+    code = _type_code(x)
+    if x.dim() != 2 or w_gate.dim() != 2:
+        raise BfHipError("x must be [rows, features], the weights [hidden, features]")
+    if activation not in ACTIVATIONS:
+        raise BfHipError(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    (rows, features), hidden = x.shape, w_gate.shape[0]
+    return GatedDesc(code, ACTIVATIONS[activation], rows, features, hidden), \
+        [_gated_matrix("x", x, (rows, features), x),
+         _gated_matrix("w_gate", w_gate, (hidden, features), x),
+         _gated_matrix("w_up", w_up, (hidden, features), x)]
+
+
+def gated_linear(x, w_gate, w_up, activation="silu", out=None, save=False, stream=None):
+    """act(x @ w_gate^T) * (x @ w_up^T) (bfhip_gated_linear): x [rows, features],
+    the weights [hidden, features] of one stride (views of one tensor will do),
+    all with contiguous rows; activation silu, gelu or relu.  Returns h [rows,
+    hidden], or (h, gate, up) with `save`, which gated_linear_backward takes."""
+    desc, given = _gated_desc(x, w_gate, w_up, activation)
+    shape, lib = (x.shape[0], w_gate.shape[0]), hip_lib()
+    with _place(stream, x, w_gate, w_up, out) as queue:
+        h = x.new_empty(shape) if out is None else out
+        kept = [x.new_empty(shape) for _ in range(2)] if save else [None, None]
+        size = lib.bfhip_gated_linear_workspace(desc)
+        work, pw = _scratch(size, x)
+        err = _err()
+        _check(lib.bfhip_gated_linear(
+            desc, *given, _gated_matrix("out", h, shape, x),
+            *(t if t is None else Matrix(t.data_ptr(), shape[1]) for t in kept), pw, size, queue,
+            err, 512), err, "bfhip_gated_linear")
+    return (h, *kept) if save else h
+
+
+def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation="silu", stream=None):
+    """Gradients of gated_linear (bfhip_gated_linear_backward) from that of h:
+    (dx, dw_gate, dw_up)."""
+    desc, given = _gated_desc(x, w_gate, w_up, activation)
+    shape, lib = (x.shape[0], w_gate.shape[0]), hip_lib()
+    more = [_gated_matrix(n, t, shape, x) for n, t in (("dh", dh), ("gate", gate), ("up", up))]
+    with _place(stream, x, dh, w_gate, w_up, gate, up) as queue:
+        grads = [t.new_empty(t.shape) for t in (x, w_gate, w_up)]
+        size = lib.bfhip_gated_linear_backward_workspace(desc)
+        work, pw = _scratch(size, x)
+        err = _err()
+        _check(lib.bfhip_gated_linear_backward(
+            desc, more[0], *given, *more[1:], *(Matrix(t.data_ptr(), t.shape[1]) for t in grads),
+            pw, size, queue, err, 512), err, "bfhip_gated_linear_backward")
+    return tuple(grads)
 
 
 def window_map(batches, height, width, shift, device, stream=None):

@@ -1,8 +1,9 @@
 /*
  * Stateless transformer operators on AMD gfx950, served by libbfhip.so: layer
- * norm, learned position bias by buckets, rotary positions and attention over
- * packed sequences, each with its backward pass; and for serving a paged cache
- * of keys and values with the attention of new tokens over it.  They stand beside the stateless linear and
+ * norm, learned position bias by buckets, rotary positions, attention over
+ * packed sequences and the gated linear of a feed-forward block, each with its
+ * backward pass; and for serving a paged cache of keys and values with the
+ * attention of new tokens over it.  They stand beside the stateless linear and
  * convolution of bf_cuda_ops.h and have no counterpart in the reference, whose
  * transformer blocks exist inside its fixed contexts only.
  *
@@ -295,6 +296,60 @@ int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
                           const bfhip_pages *k_pages, const bfhip_pages *v_pages,
                           const bfhip_rows *out, float *lse, void *workspace,
                           size_t workspace_bytes, void *stream, char *error, size_t error_cap);
+
+/* -------------------------------------------------------------- gated linear
+ * h = act(x Wg^T) * (x Wu^T), both products, the activation and their product
+ * in one kernel: x [rows, features], Wg and Wu [hidden, features], h [rows,
+ * hidden].  act: silu, v / (1 + e^-v); gelu, v (1 + erf(v / sqrt 2)) / 2; relu,
+ * max(v, 0).  gate and up (both or neither NULL): the two products, rounded to
+ * the type, which the backward pass takes.
+ *
+ * Backward, with g = gate, u = up and dh the gradient of h:
+ *   dg = dh * u * act'(g),  du = dh * act(g)
+ *   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+ * dx, or dWg and dWu together, may be NULL where they are not wanted.  dg and du
+ * are rounded to the type where they enter the matrix cores; fp16's are
+ * multiplied by a power of two on the way (their largest comes near 2^14), so that
+ * they may be of any size.  A result beyond the type's range is infinite.
+ * relu'(0) = 0.
+ *
+ * Matrices: row r at element r * <name>.stride (at least the row's length, of no
+ * account where there is at most one row), the elements of a row contiguous.
+ * Any alignment will do; pointers and strides on 16 bytes, and rows of whole 16
+ * bytes, are faster.  Wg and Wu have one stride.  Results overlap nothing.  Sizes 0 .. 2^31 - 1 each, features and hidden at least 1, no
+ * matrix of more than 2^40 elements.  The workspace holds dg and du and, where
+ * results are few beside the sums' lengths, parts of sums (at most 256 MiB). */
+enum { BFHIP_SILU = 0, BFHIP_GELU = 1, BFHIP_RELU = 2 };
+
+typedef struct {
+    void *data;
+    long long stride;
+} bfhip_matrix;
+
+typedef struct {
+    int type;
+    int activation;
+    long long rows;
+    long long features;
+    long long hidden;
+} bfhip_gated_desc;
+
+size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *desc);
+size_t bfhip_gated_linear_backward_workspace(const bfhip_gated_desc *desc);
+
+int bfhip_gated_linear(const bfhip_gated_desc *desc, const bfhip_matrix *x,
+                       const bfhip_matrix *w_gate, const bfhip_matrix *w_up,
+                       const bfhip_matrix *h, const bfhip_matrix *gate, const bfhip_matrix *up,
+                       void *workspace, size_t workspace_bytes,
+                       void *stream, char *error, size_t error_cap);
+
+int bfhip_gated_linear_backward(const bfhip_gated_desc *desc, const bfhip_matrix *dh,
+                                const bfhip_matrix *x, const bfhip_matrix *w_gate,
+                                const bfhip_matrix *w_up, const bfhip_matrix *gate,
+                                const bfhip_matrix *up, const bfhip_matrix *dx,
+                                const bfhip_matrix *dw_gate, const bfhip_matrix *dw_up,
+                                void *workspace, size_t workspace_bytes,
+                                void *stream, char *error, size_t error_cap);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,117 @@
+"""The gated linear's boundary without a GPU: refusals, which come before any
+launch, and what its workspaces may take."""
+
+import ctypes as C
+import random
+
+import pytest
+import torch
+
+import bfhip
+
+P = C.c_void_p(4096)
+
+
+def mat(data=4096, stride=512):
+    return bfhip.Matrix(data, stride)
+
+
+def desc(**change):
+    d = dict(type=2, activation=0, rows=10, features=256, hidden=512)
+    d.update(change)
+    return bfhip.GatedDesc(*d.values())
+
+
+def call(name, *args):
+    e = C.create_string_buffer(256)
+    f = getattr(bfhip.hip_lib(), name)
+    ok = f(*args, None, e, 256)
+    assert f(*args, None, None, 0) == ok
+    return ok, e.value
+
+
+def forward(d, x=mat(), w_gate=mat(), w_up=mat(), h=mat(), gate=mat(), up=mat(), work=P, size=1 << 40):
+    return call("bfhip_gated_linear", d, x, w_gate, w_up, h, gate, up, work, size)
+
+
+def backward(d, dh=mat(), x=mat(), w_gate=mat(), w_up=mat(), gate=mat(), up=mat(), dx=mat(), dw_gate=mat(), dw_up=mat(), work=P,
+             size=1 << 50):
+    return call("bfhip_gated_linear_backward", d, dh, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, work, size)
+
+
+@pytest.mark.parametrize("bad", [dict(type=3), dict(type=-1), dict(activation=3), dict(activation=-1), dict(rows=-1),
+                                 dict(rows=1 << 31), dict(features=0), dict(features=1 << 31), dict(hidden=0), dict(hidden=-1),
+                                 dict(rows=1 << 30, features=1 << 11), dict(hidden=1 << 30, features=1 << 11)])
+def test_refuses(bad):
+    for f in (forward, backward):
+        ok, message = f(desc(**bad))
+        assert not ok and b"invalid gated linear contract" in message
+    lib = bfhip.hip_lib()
+    assert lib.bfhip_gated_linear_workspace(desc(**bad)) == 0 and lib.bfhip_gated_linear_backward_workspace(desc(**bad)) == 0
+
+
+def test_refuses_one_of_two():
+    for bad in (dict(gate=None), dict(up=None)):
+        assert b"contract" in forward(desc(), **bad)[1]
+    for bad in (dict(dw_gate=None), dict(dw_up=None), dict(dx=None, dw_gate=None, dw_up=None)):
+        assert b"contract" in backward(desc(), **bad)[1]
+
+
+@pytest.mark.parametrize("bad", [mat(None), mat(stride=255), mat(stride=-512), mat(stride=1 << 41)])
+def test_refuses_matrices(bad):
+    for name in ("x", "w_gate", "w_up", "h", "gate", "up"):
+        ok, message = forward(desc(), **{name: bad})
+        assert not ok and b"invalid gated linear matrices" in message, name
+    for name in ("dh", "x", "w_gate", "w_up", "gate", "up", "dx", "dw_gate", "dw_up"):
+        ok, message = backward(desc(), **{name: bad})
+        assert not ok and b"invalid gated linear matrices" in message, name
+    assert b"matrices" in forward(desc(), x=None)[1] and b"matrices" in backward(desc(), x=None)[1]
+
+
+def test_refuses_weights_of_two_strides():
+    for f in (forward, backward):
+        assert b"one stride" in f(desc(), w_up=mat(stride=520))[1]
+
+
+def test_refuses_workspaces():
+    lib = bfhip.hip_lib()
+    for f, size, d in ((forward, lib.bfhip_gated_linear_workspace, desc(rows=300, features=4096)),
+                       (backward, lib.bfhip_gated_linear_backward_workspace, desc())):
+        need = size(d)
+        assert need > 0
+        wide = {n: mat(stride=4096) for n in ("x", "w_gate", "w_up")}
+        for bad in (dict(size=need - 1), dict(work=None), dict(work=C.c_void_p(4104))):
+            ok, message = f(d, **wide, **bad)
+            assert not ok and b"workspace" in message
+
+
+def test_nothing_to_do():
+    none = mat(None)
+    assert forward(desc(rows=0), x=none, h=none, gate=none, up=none, work=None, size=0)[0]
+    assert backward(desc(rows=0), dh=none, x=none, gate=none, up=none, dx=none, dw_gate=None, dw_up=None, work=None, size=0)[0]
+
+
+def test_workspaces_are_bounded():
+    rng, lib = random.Random(1), bfhip.hip_lib()
+    log = lambda most: int(most ** rng.random())
+    some = 0
+    for _ in range(5000):
+        d = desc(type=rng.randint(0, 2), rows=log(1 << 20), features=log(1 << 15), hidden=log(1 << 16))
+        need = lib.bfhip_gated_linear_workspace(d)
+        assert need <= 256 << 20
+        some += need > 0
+        size = 4 if d.type == 0 else 2
+        products = 2 * ((d.rows * (d.hidden + 7) // 8 * 8 * size + 255) // 256 * 256)
+        rest = lib.bfhip_gated_linear_backward_workspace(d) - products
+        assert rest <= (256 << 20) + 16 * d.rows * size + 8192
+    assert some > 300
+
+
+def test_python_refuses():
+    x, w = torch.zeros((4, 8)), torch.zeros((6, 8))
+    for args, named in (((x, w, w), {}), ((x, w, w[:3]), {}), ((x, w.half(), w), {}), ((x[0], w, w), {}),
+                        ((x, w, w), dict(activation="tanh")), ((x, w.T.contiguous().T, w), {}), ((x.double(), w, w), {})):
+        with pytest.raises(bfhip.BfHipError):
+            bfhip.gated_linear(*args, **named)
+    with pytest.raises(bfhip.BfHipError):
+        bfhip.gated_linear_backward(torch.zeros((4, 5)), x, w, w, torch.zeros((4, 6)), torch.zeros((4, 6)))

@@ -1,0 +1,266 @@
+"""The gated linear (bfhip_gated_linear) and its gradients against 64-bit
+formulas."""
+
+import math
+
+import pytest
+import torch
+
+import bfhip
+import decoder_ref as ref
+from transformer_ref import check
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def gen(device, seed=0):
+    return torch.Generator(device).manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(shape, generator=g, device=g.device) * scale).to(dtype)
+
+
+def inputs(device, dtype, rows, features, hidden, seed=1):
+    g = gen(device, seed)
+    return dict(x=randn(g, rows, features, dtype=dtype),
+                w_gate=randn(g, hidden, features, dtype=dtype, scale=1.5 * features ** -0.5),
+                w_up=randn(g, hidden, features, dtype=dtype, scale=features ** -0.5)), randn(g, rows, hidden, dtype=dtype)
+
+
+def run(call, dh, activation):
+    h, gate, up = bfhip.gated_linear(**call, activation=activation, save=True)
+    return dict(h=h, gate=gate, up=up), dict(zip(("dx", "dw_gate", "dw_up"),
+                                                 bfhip.gated_linear_backward(dh, **call, gate=gate, up=up, activation=activation)))
+
+
+def check_finite(name, got, value, bound):
+    """Within the bound where the type holds the value, infinite beyond."""
+    most = torch.finfo(got.dtype).max
+    held = value.abs() + bound <= most
+    check(name, got[held], value[held], bound[held])
+    # (what rounds to the type's next number past its largest is infinite)
+    over = value.abs() - bound > most * (1 + torch.finfo(got.dtype).eps)
+    assert torch.equal(got[over].double(), value[over].sign() * math.inf), name
+
+
+def compare(call, dh, activation):
+    forward, back = run(call, dh, activation)
+    for name, (value, bound) in ref.gated_linear(**call, activation=activation).items():
+        check_finite(name, forward[name], value, bound)
+    assert torch.equal(bfhip.gated_linear(**call, activation=activation), forward["h"])
+    want = ref.gated_linear_backward(dh, **call, gate=forward["gate"], up=forward["up"], activation=activation)
+    for name, (value, bound) in want.items():
+        check_finite(name, back[name], value, bound)
+    return forward, back
+
+
+# (rows, features, hidden): one of each, sizes that no chunk, tile or step divides,
+# fewer and more rows than tiles of each size, long and short contractions.
+SIZES = [(1, 1, 1), (3, 5, 2), (1, 512, 300), (16, 1024, 128), (17, 64, 129), (65, 96, 40), (100, 771, 257), (130, 128, 500),
+         (257, 264, 136), (5, 4096, 64), (1000, 40, 24), (2100, 33, 65), (600, 1000, 2056)]
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gated_linear(device, dtype, size):
+    compare(*inputs(device, dtype, *size), "silu")
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_activations(device, dtype, activation):
+    """Over their whole range: products from -30 to 30, and far ones."""
+    call, dh = inputs(device, dtype, 200, 64, 128)
+    call["x"] *= 5
+    call["x"][::7] *= 0.01
+    call["x"][5] *= 40
+    compare(call, dh, activation)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_large_tiles(device, dtype):
+    """Results of more tiles than CUs, whole and ragged."""
+    compare(*inputs(device, dtype, 4096, 256, 2048), "silu")
+    compare(*inputs(device, dtype, 4100, 520, 2056), "gelu")
+    compare(*inputs(device, dtype, 3001, 515, 2051), "relu")
+
+
+def test_large_tiles_f32(device):
+    compare(*inputs(device, F32, 2050, 260, 1100), "gelu")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rows_of_any_alignment(device, dtype):
+    """Views into wider tensors, on and off 16 bytes; the weights' views of one."""
+    call, dh = inputs(device, dtype, 70, 72, 136)
+    want, grads = run(call, dh, "silu")
+
+    def inside(t, left, right):
+        wide = torch.full((t.shape[0], t.shape[1] + left + right), math.nan, dtype=dtype, device=device)
+        view = wide[:, left:left + t.shape[1]]
+        view.copy_(t)
+        return view
+    for left, right in ((8, 8), (1, 2), (0, 3)):
+        moved = {n: inside(t, left, right) for n, t in call.items()}
+        got, back = run(moved, inside(dh, left, right), "silu")
+        for a, b in ((want, got), (grads, back)):
+            for n in a:
+                assert torch.equal(a[n], b[n]), (n, left)
+    both = torch.stack([call["w_gate"], call["w_up"]], 1)
+    got, back = run(dict(call, w_gate=both[:, 0], w_up=both[:, 1]), dh, "silu")
+    assert torch.equal(got["h"], want["h"]) and torch.equal(back["dx"], grads["dx"])
+
+
+def test_results_only_where_they_belong(device):
+    for dtype in (F32, F16, BF16):
+        call, _ = inputs(device, dtype, 70, 72, 133)
+        wide = torch.full((74, 150), math.nan, dtype=dtype, device=device)
+        out = wide[2:72, 3:136]
+        want = bfhip.gated_linear(**call)
+        bfhip.gated_linear(**call, out=out)
+        assert torch.equal(out, want)
+        out.fill_(math.nan)
+        assert torch.isnan(wide).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rows_do_not_depend_on_others(device, dtype):
+    """Infinities and NaN in one row of x stay in that row."""
+    call, dh = inputs(device, dtype, 150, 200, 72)
+    want, _ = run(call, dh, "silu")
+    for value in (math.inf, math.nan):
+        x = call["x"].clone()
+        x[33, 7] = value
+        h = bfhip.gated_linear(x, call["w_gate"], call["w_up"])
+        keep = torch.arange(150, device=device) != 33
+        assert torch.equal(h[keep], want["h"][keep]) and not torch.isfinite(h[33]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_no_rows(device, dtype):
+    call, dh = inputs(device, dtype, 0, 24, 40)
+    forward, back = run(call, dh, "silu")
+    assert forward["h"].shape == (0, 40) and back["dx"].shape == (0, 24)
+    assert (back["dw_gate"] == 0).all() and (back["dw_up"] == 0).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -11, 1.0, 2.0 ** 9])
+def test_fp16_gradients_of_any_size(device, size):
+    """Of a loss that is a mean, and of one that is scaled up: dg of 2^-40 and of
+    2^20 in fp16."""
+    call, dh = inputs(device, F16, 300, 128, 264)
+    dh = (dh * size).to(F16)
+    call["w_up"] *= 16 if size > 1 else 2 ** -6 if size < 2.0 ** -19 else 1
+    call["w_gate"] *= 2 ** -4 if size > 1 else 1
+    h, gate, up = bfhip.gated_linear(**call, save=True)
+    back = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up)
+    want = ref.gated_linear_backward(dh, **call, gate=gate, up=up, activation="silu")
+    for got, name in zip(back, ("dx", "dw_gate", "dw_up")):
+        check_finite(name, got, *want[name])
+
+
+def test_fp16_gradients_that_are_zero_or_infinite(device):
+    call, dh = inputs(device, F16, 64, 64, 64)
+    h, gate, up = bfhip.gated_linear(**call, save=True)
+    for t in bfhip.gated_linear_backward(torch.zeros_like(dh), **call, gate=gate, up=up):
+        assert (t == 0).all()
+    want = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up)
+    dh[5, 6] = math.inf  # reaches row 5 of dx and row 6 of the weights' gradients alone
+    got = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up)
+    rows = torch.arange(64, device=device)
+    assert torch.equal(got[0][rows != 5], want[0][rows != 5]) and not torch.isfinite(got[0][5]).any()
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a[rows != 6], b[rows != 6])
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_gradients_by_differences(device, activation):
+    """sum(dh h) in fp32, by central differences of steps of 2^-6: off by the
+    third derivative's share (2^-12 / 6 of it, at most 2 of each slope here) and by
+    the roundings of h, 2^-24 sqrt(terms) over the step."""
+    call, dh = inputs(device, F32, 20, 24, 32)
+    h, gate, up = bfhip.gated_linear(**call, activation=activation, save=True)
+    grads = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up, activation=activation)
+    step = 2.0 ** -6
+    for name, grad in zip(("x", "w_gate", "w_up"), grads):
+        for seed in range(3):
+            way = randn(gen(device, seed), *call[name].shape)
+            way /= way.norm()
+            at = lambda s: (bfhip.gated_linear(**dict(call, **{name: call[name] + s * way}), activation=activation).double()
+                            * dh.double()).sum()
+            slope, want = (at(step) - at(-step)) / (2 * step), (grad.double() * way.double()).sum()
+            assert abs(slope - want) <= 2e-3 * grad.double().norm(), (name, slope, want)
+
+
+def test_equal_calls_give_equal_bits(device):
+    for dtype, size in ((BF16, (300, 512, 256)), (F16, (40, 4096, 128)), (F32, (300, 200, 128))):
+        call, dh = inputs(device, dtype, *size)
+        first = run(call, dh, "gelu")
+        for _ in range(3):
+            again = run(call, dh, "gelu")
+            for a, b in zip(first, again):
+                assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_in_a_graph(device):
+    """Forward and backward captured, replayed on other inputs, with eager work
+    in between."""
+    for dtype, size in ((F16, (64, 2048, 128)), (BF16, (500, 136, 264)), (F32, (3, 512, 64))):
+        call, dh = inputs(device, dtype, *size)
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            run(call, dh, "silu")
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = run(call, dh, "silu")
+        for seed in (5, 6, 7):
+            other, odh = inputs(device, dtype, *size, seed=seed)
+            for n in call:
+                call[n].copy_(other[n])
+            dh.copy_(odh * 2.0 ** -seed)
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(results, run(call, dh, "silu")):
+                assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_calls_on_two_streams(device):
+    calls = [inputs(device, F16, 200, 1024, 256, seed=s) for s in (1, 2)]
+    want = [run(*c, "silu") for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for (call, dh), s in zip(calls, streams):
+            h, gate, up = bfhip.gated_linear(**call, save=True, stream=s)
+            got.append((h, bfhip.gated_linear_backward(dh, **call, gate=gate, up=up, stream=s)))
+    torch.cuda.synchronize()
+    for (h, back), (f, b) in zip(got, want):
+        assert torch.equal(h, f["h"]) and all(torch.equal(x, b[n]) for x, n in zip(back, b))
+
+
+def test_a_block(device):
+    """A feed-forward block with the norm before it, both directions, as a
+    program trains it: norm, gated linear, and a plain linear behind them."""
+    g = gen(device, 3)
+    x, gamma = randn(g, 90, 64), 1 + randn(g, 64, scale=0.1)
+    wg, wu, wd = (randn(g, *s, scale=0.2) for s in ((160, 64), (160, 64), (64, 160)))
+    dy = randn(g, 90, 64)
+    y, mean, rstd = bfhip.layer_norm(x, gamma, stats=True)
+    h, gate, up = bfhip.gated_linear(y, wg, wu, save=True)
+    dh = dy @ wd
+    d_in, dwg, dwu = bfhip.gated_linear_backward(dh, y, wg, wu, gate, up)
+    dx, dgamma, _ = bfhip.layer_norm_backward(d_in, x, mean, rstd, gamma)
+    leaves = [t.double().cpu().requires_grad_() for t in (x, gamma, wg, wu)]
+    X, G, A, B = leaves
+    n = torch.nn.functional.layer_norm(X, (64,), G)
+    p = n @ A.T
+    loss = ((p * torch.sigmoid(p)) * (n @ B.T) @ wd.double().cpu().T * dy.double().cpu()).sum()
+    loss.backward()
+    for name, got, leaf in zip(("dx", "dgamma", "dwg", "dwu"), (dx, dgamma, dwg, dwu), leaves):
+        # sums of at most 160 x 64 x 90 fp32 roundings of random sign: 2^-24 * 1000
+        scale = leaf.grad.abs().max()
+        assert (got.double().cpu() - leaf.grad).abs().max() <= 6e-5 * scale, name
