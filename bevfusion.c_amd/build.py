@@ -32,11 +32,13 @@ HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     # Packed-fp32 VALU forms are kept out of the generated code.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    # MFMA results in VGPRs: epilogues and softmax read them without
-    # v_accvgpr_read copies.
-    "-mllvm", "-amdgpu-mfma-vgpr-form",
     f"-I{INCLUDE}", f"-I{CSRC}",
 ]
+# MFMA results in VGPRs: epilogues and softmax read them without
+# v_accvgpr_read copies.  Not for kernels whose accumulators are all of the 256
+# accumulation registers.
+VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+ACCUMULATION_REGISTERS = {"gated_large.hip"}
 
 
 def _run(cmd, quiet_packed=True):
@@ -81,7 +83,8 @@ def _kernel_resources(text: str) -> dict:
 def _compile_hip(src: pathlib.Path):
     OBJ.mkdir(exist_ok=True)
     obj = OBJ / (src.stem + ".o")
-    text = _run([HIPCC, *HIP_FLAGS, "-Rpass-analysis=kernel-resource-usage", "-c", str(src),
+    form = [] if src.name in ACCUMULATION_REGISTERS else VGPR_FORM
+    text = _run([HIPCC, *HIP_FLAGS, *form, "-Rpass-analysis=kernel-resource-usage", "-c", str(src),
                  "-o", str(obj)])
     return obj, _kernel_resources(text)
 

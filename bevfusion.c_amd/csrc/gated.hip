@@ -1,394 +1,53 @@
 // The gated linear of a feed-forward block, forward and backward
-// (include/bfhip_transformer.h).
-//
-// Three products share one tiled kernel, which multiplies a tile of m x n
-// results over a contraction axis k:
-//   forward        h = act(x Wg^T) * (x Wu^T)   m rows,   n hidden,   k features
-//   inputs' grad.  dx = dg Wg + du Wu           m rows,   n features, k hidden, twice
-//   weights' grad. dWg = dg^T x, dWu = du^T x   m hidden, n features, k rows
-// An operand whose k is contiguous in memory (x and W forward, dg and du in dx)
-// lies in LDS as rows of BK elements; one whose k is the row (W in dx, both in
-// dW) as BK rows, and is read transposed.
+// (include/bfhip_transformer.h): small tiles, the gradients of the two products, and
+// the entry points.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
-#include "attention.h"
+#include "gated.h"
 
 using namespace bfhip;
 
 namespace {
 
-enum Form { kForward, kInputs, kWeights };
-
-struct GatedOperand {
-    const char *gate, *up;  // one matrix each, or the same
-    long long stride;       // bytes
-};
-
-struct GatedArgs {
-    GatedOperand m_op, n_op;
-    int m, n, k;     // of the result, and of the contraction (of one of its two halves)
-    char *out[3];    // forward: h, gate, up; inputs: dx; weights: dWg, dWu
-    long long out_stride[3];  // bytes
-    const int *shift;         // fp16 gradients were multiplied by 2^shift
-    int activation;
-    int tiles_m, tiles_n;
-    int parts, per;  // of the contraction's steps
-    float *partial;  // parts > 1: accumulators, [part][tile][wave][block][lane][4]
-};
-
-// ---------------------------------------------------------------- activations
-template <class E>
-__device__ __forceinline__ float exp_of(float v) {
-    if constexpr (E::kSize == 4) return expf(v);
-    else return __expf(v);
-}
-template <class E>
-__device__ __forceinline__ float over(float a, float b) {
-    if constexpr (E::kSize == 4) return a / b;
-    else return a * __builtin_amdgcn_rcpf(b);
-}
-
-// act(g); erfc keeps gelu's relative precision where it is small.
-template <class E>
-__device__ __forceinline__ float activate(int kind, float g) {
-    if (kind == BFHIP_SILU) return over<E>(g, 1.f + exp_of<E>(-g));
-    if (kind == BFHIP_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);
-    return g > 0.f ? g : g == g ? 0.f : g;
-}
-
-// act(g) and its derivative.
-template <class E>
-__device__ __forceinline__ float2 slope(int kind, float g) {
-    if (kind == BFHIP_SILU) {
-        const float s = over<E>(1.f, 1.f + exp_of<E>(-g)), rest = over<E>(1.f, 1.f + exp_of<E>(g));
-        return make_float2(g * s, s * fmaf(g, rest, 1.f));
-    }
-    if (kind == BFHIP_GELU) {
-        const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-        return make_float2(g * cdf, fmaf(g * 0.39894228040143268f, exp_of<E>(-0.5f * g * g), cdf));
-    }
-    return make_float2(g > 0.f ? g : g == g ? 0.f : g, g > 0.f ? 1.f : 0.f);
-}
-
-// ------------------------------------------------------------------- tiles
-// One operand's tile of OUTER (m or n) x BK (k) elements in LDS.  DMA: rows start
-// on 16 bytes and hold whole chunks of 16 bytes.
-template <class E, int OUTER, int BK, int THREADS, bool COL, bool DMA>
-struct GatedTile {
-    using T = std::conditional_t<COL, AttnTile<E, OUTER>, AttnTile<E, BK>>;
-    static constexpr int kRows = COL ? BK : OUTER, kWords = 16 / E::kSize;
-    static constexpr int kBytes = kRows * T::kRow, kIssue = kRows * T::kChunks / THREADS;
-    static_assert(kRows * T::kChunks % THREADS == 0, "whole chunks per thread");
-    typedef uint32_t Chunk __attribute__((ext_vector_type(4)));
-
-    // PAIR > 0: outer rows are PAIR / 2 of the gate's, PAIR / 2 of the up's in turn.
-    template <int PAIR>
-    __device__ __forceinline__ static int source(int r) { return PAIR ? r / PAIR * (PAIR / 2) + r % (PAIR / 2) : r; }
-
-    // Rows that the threads' j-th chunks span; chunk j of a thread is chunk 0 moved
-    // by j times as many (a multiple of the swizzle's period).
-    static constexpr int kSpan = THREADS / T::kChunks;
-    static_assert(kSpan % 16 == 0 && THREADS % T::kChunks == 0, "chunks repeat with the swizzle");
-    uint32_t off;  // DMA: bytes of chunk 0 from the tile's first row
-    int row, first;  // its row in the matrix, and its first element along the row
-    Chunk held[DMA ? 1 : kIssue];
-    const char *base_a, *base_b;
-    long long stride;
-    int wave, left, thread;
-
-    // Row of the matrix at which the span j begins.
-    template <int PAIR>
-    __device__ __forceinline__ static constexpr int span_row(int j) { return source<PAIR>(j * kSpan); }
-
-    // The tile from `outer0` on, of `count` outer elements in all.
-    template <int PAIR>
-    __device__ __forceinline__ void init(const GatedOperand &op, bool up, int outer0, int count) {
-        static_assert(!PAIR || PAIR % (2 * kSpan) == 0 || kSpan % PAIR == 0, "a span is of one matrix or of whole pairs");
-        thread = threadIdx.x;
-        wave = __builtin_amdgcn_readfirstlane(thread / kWave);
-        stride = op.stride;
-        left = count - outer0;
-        const long long at = COL ? (long long)outer0 * E::kSize : outer0 * op.stride;
-        base_a = (PAIR || !up ? op.gate : op.up) + at;
-        base_b = op.up + at;
-        const int r = thread / T::kChunks, c = (thread % T::kChunks) ^ T::swizzle(r);
-        row = source<PAIR>(r);
-        first = c * kWords;
-        off = (uint32_t)row * (uint32_t)stride + 16u * c;
-    }
-    // Whether the wave's j-th chunks are the second matrix's.
-    template <int PAIR>
-    __device__ __forceinline__ bool second(int j) const {
-        if constexpr (PAIR == 0) return false;
-        else return (j * kSpan + wave * kWave / T::kChunks) % PAIR >= PAIR / 2;
-    }
-    // Fetches the tile from k0 on, of k elements in all, out of the matrix at `a` (with
-    // PAIR, the up's rows out of that at `b`).
-    template <int PAIR>
-    __device__ __forceinline__ void fetch(const char *a, const char *b, int k0, int k, char *lds) {
-        const long long at = COL ? k0 * stride : (long long)k0 * E::kSize;
-        const int rows = COL ? k - k0 : left, length = COL ? left : k - k0;  // what there is of the tile
-        if constexpr (DMA) {
-            const __amdgpu_buffer_rsrc_t ra = buffer_rsrc(a + at, kDmaOutOfRange - 1), rb = buffer_rsrc(b + at, kDmaOutOfRange - 1);
-#pragma unroll
-            for (int j = 0; j < kIssue; ++j) {
-                const bool in = row + span_row<PAIR>(j) < rows && first < length;
-                dma16(second<PAIR>(j) ? rb : ra, reinterpret_cast<bf16 *>(lds + (j * THREADS + wave * kWave) * 16),
-                      in ? off + (uint32_t)span_row<PAIR>(j) * (uint32_t)stride : kDmaOutOfRange);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kIssue; ++j) {
-                const int r = row + span_row<PAIR>(j), n = r < rows ? length - first : 0;
-                const char *p = (second<PAIR>(j) ? b : a) + at + r * stride + first * E::kSize;
-                Chunk v = {0, 0, 0, 0};
-                if (n >= kWords) {
-                    __builtin_memcpy(&v, p, 16);
-                } else if (n > 0) {
-                    typedef typename E::Word Row __attribute__((ext_vector_type(kWords)));
-                    Row w = __builtin_bit_cast(Row, v);
-#pragma unroll
-                    for (int e = 0; e < kWords; ++e)
-                        if (e < n) w[e] = ((const typename E::Word *)p)[e];
-                    v = __builtin_bit_cast(Chunk, w);
-                }
-                held[j] = v;
-            }
-        }
-    }
-    __device__ __forceinline__ void put(char *lds) const {
-        if constexpr (!DMA)
-#pragma unroll
-            for (int j = 0; j < kIssue; ++j) *reinterpret_cast<Chunk *>(lds + (j * THREADS + thread) * 16) = held[j];
-    }
-    // Where in the tile the lane reads the fragments of the outer elements from o0
-    // on (a multiple of 64).
-    __device__ __forceinline__ static uint32_t lane_at(int o0, int lane) {
-        const int c16 = lane & 15, g = lane >> 4;
-        if constexpr (!COL) {
-            return (o0 + c16) * T::kRow + 16 * ((E::kSize == 2 ? g : 2 * g) ^ T::swizzle(c16));
-        } else if constexpr (E::kSize == 2) {
-            // (see col_frag: here the lane's k are neighbours)
-            const int r = 8 * g + (c16 >> 2);
-            return r * T::kRow + 16 * ((o0 / 8 + ((c16 & 3) >> 1)) ^ T::swizzle(r)) + 8 * (c16 & 1);
-        } else {
-            return 8 * g * T::kRow + 16 * ((o0 / 4 + (c16 >> 2)) ^ (8 * (g & 1))) + 4 * (c16 & 3);
-        }
-    }
-    // Fragment i of 16 outer elements, k 32 kk ..+31: lane l holds outer element l & 15,
-    // k 8 (l >> 4) ..+7.  Tiles start on 512 bytes and the swizzle is an exclusive or
-    // of address bits, so that every fragment is one exclusive or away from the first.
-    __device__ __forceinline__ static typename E::Frag frag(const char *lds, uint32_t at, int i, int kk) {
-        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)(lds) + at;
-        if constexpr (!COL) {
-            const uint32_t p = (base ^ 64u * kk) + i * 16 * T::kRow;
-            if constexpr (E::kSize == 2) {
-                return *(__attribute__((address_space(3))) const bf16x8 *)p;
-            } else {
-                static_assert(E::kSize == 2 || BK == 32, "one step of 32");
-                const f32x4 a = *(__attribute__((address_space(3))) const f32x4 *)p;
-                const f32x4 b = *(__attribute__((address_space(3))) const f32x4 *)(p ^ 16u);
-                return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-        } else if constexpr (E::kSize == 2) {
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s16x4 *Ptr;
-            // Four rows on, the swizzle differs in chunk bit 3.
-            const uint32_t p = (base ^ 32u * i) + 32 * kk * T::kRow, q = (base ^ 32u * i ^ 128u) + (32 * kk + 4) * T::kRow;
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)q);
-            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-        } else {
-            f32x8 v;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[e] = *(__attribute__((address_space(3))) const float *)((base ^ (64u * i ^ 16u * e)) + (32 * kk + e) * T::kRow);
-            return v;
-        }
-    }
-};
-
-// BM x BN results by WM x WN waves.
-template <class E, Form F, int BM_, int BN_, int WM_, int WN_, bool DMA_>
-struct GatedShape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = 128 / E::kSize;
-    static constexpr bool DMA = DMA_;
-    static constexpr int kThreads = WM * WN * kWave, kM = BM / WM, kN = BN / WN, kMB = kM / 16, kNB = kN / 16;
-    using MTile = GatedTile<E, BM, BK, kThreads, F == kWeights, DMA>;
-    using NTile = GatedTile<E, BN, BK, kThreads, F != kForward, DMA>;
-    static constexpr int kPair = F == kForward ? kN : 0;  // gate and up columns of a wave
-    static constexpr int kCols = F == kForward ? BN / 2 : BN;
-    static constexpr int kStage = MTile::kBytes + NTile::kBytes;
-};
-
-struct TileAt {
-    int tm, tn;
-};
-
-// Tiles are dealt to the XCDs in runs, each of which walks groups of eight rows
-// of tiles column by column, so that what runs together on an XCD's L2 shares
-// its operands' panels.
-__device__ __forceinline__ TileAt tile_at(int id, int tiles_m, int tiles_n) {
-    constexpr int kGroup = 8;
-    id = xcd_swizzle(id, tiles_m * tiles_n);
-    const int group = id / (kGroup * tiles_n), first = group * kGroup, rows = min(kGroup, tiles_m - first);
-    const int in = id - group * kGroup * tiles_n;
-    return TileAt{first + in % rows, in / rows};
-}
-
-// Four neighbouring results of a row, of which `n` exist.
-template <class E>
-__device__ __forceinline__ void put4(char *row, int at, int n, const float *v) {
-    typename E::Word *p = (typename E::Word *)row + at;
-    if (n >= 4) {
-        Words<E, 4> w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w.put(e, v[e]);
-        w.store(p);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < n) p[e] = E::put(v[e]);
-    }
-}
-
-// A lane holds row m (of its block of 16) and four neighbouring columns.
-template <class E, Form F, class S>
-__device__ __forceinline__ void gated_store(const GatedArgs &a, const f32x4 (&acc)[S::kNB][S::kMB], TileAt at, int wave, int lane) {
-    const int wm = wave / S::WN, wn = wave % S::WN, l16 = lane & 15, g = lane >> 4;
-    const int tiles = F == kWeights ? a.tiles_m / 2 : a.tiles_m;
-    const bool up = F == kWeights && at.tm >= tiles;
-    const int m0 = (up ? at.tm - tiles : at.tm) * S::BM + wm * S::kM, n0 = at.tn * S::kCols + wn * (S::kPair ? S::kN / 2 : S::kN);
-    const int shift = F != kForward && a.shift ? -*a.shift : 0;
-#pragma unroll
-    for (int j = 0; j < S::kMB; ++j) {
-        const int m = m0 + 16 * j + l16;
-        if (m >= a.m) continue;
-        if constexpr (F == kForward) {
-#pragma unroll
-            for (int i = 0; i < S::kNB / 2; ++i) {
-                const int n = n0 + 16 * i + 4 * g;
-                if (n >= a.n) continue;
-                const f32x4 gate = acc[i][j], up4 = acc[i + S::kNB / 2][j];
-                float h[4], p[4], q[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[e] = gate[e];
-                    q[e] = up4[e];
-                    h[e] = activate<E>(a.activation, gate[e]) * up4[e];
-                }
-                put4<E>(a.out[0] + m * a.out_stride[0], n, a.n - n, h);
-                if (a.out[1]) {
-                    put4<E>(a.out[1] + m * a.out_stride[1], n, a.n - n, p);
-                    put4<E>(a.out[2] + m * a.out_stride[2], n, a.n - n, q);
-                }
-            }
-        } else {
-            char *const row = (up ? a.out[1] : a.out[0]) + m * (up ? a.out_stride[1] : a.out_stride[0]);
-#pragma unroll
-            for (int i = 0; i < S::kNB; ++i) {
-                const int n = n0 + 16 * i + 4 * g;
-                if (n >= a.n) continue;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = std::is_same_v<E, ElemF16> ? ldexpf(acc[i][j][e], shift) : acc[i][j][e];
-                put4<E>(row, n, a.n - n, v);
-            }
-        }
-    }
-}
-
+// Small tiles: two workgroups share a CU and cover each other's waits.
 template <class E, Form F, class S>
 __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a) {
-    __shared__ __attribute__((aligned(512))) char smem[2 * S::kStage];
+    __shared__ __attribute__((aligned(512))) char smem[gated_lds<E, F, S>(2 * S::kStage)];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int wm = wave / S::WN, wn = wave % S::WN;
-    const int tiles = a.tiles_m * a.tiles_n, part = blockIdx.x / tiles;
-    const TileAt at = tile_at(blockIdx.x % tiles, a.tiles_m, a.tiles_n);
-    const int half = F == kWeights ? a.tiles_m / 2 : a.tiles_m;
-    const bool up = F == kWeights && at.tm >= half;
-    typename S::MTile mt;
-    typename S::NTile nt;
-    mt.template init<0>(a.m_op, up, (up ? at.tm - half : at.tm) * S::BM, a.m);
-    nt.template init<S::kPair>(a.n_op, up, at.tn * S::kCols, a.n);
-    // The contraction's steps: for the inputs' gradient the gate's, then the up's.
-    const int each = (a.k + S::BK - 1) / S::BK, steps = F == kInputs ? 2 * each : each;
-    const int begin = part * a.per, end = min(steps, begin + a.per);
-    const auto fetch = [&](int t) {
-        const bool second = F == kInputs && t >= each;
-        const int k0 = (second ? t - each : t) * S::BK;
-        char *const to = smem + (t & 1) * S::kStage;
-        mt.template fetch<0>(second ? mt.base_b : mt.base_a, mt.base_b, k0, a.k, to);
-        nt.template fetch<S::kPair>(second ? nt.base_b : nt.base_a, nt.base_b, k0, a.k, to + S::MTile::kBytes);
-    };
-    f32x4 acc[S::kNB][S::kMB];
+    GatedWork<E, F, S> w;
+    w.init(a, wave, lane);
+    f32x4 acc[S::kMB][S::kNB];
 #pragma unroll
-    for (int i = 0; i < S::kNB; ++i)
+    for (int j = 0; j < S::kMB; ++j)
 #pragma unroll
-        for (int j = 0; j < S::kMB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const auto put = [&](int t) {
-        char *const to = smem + (t & 1) * S::kStage;
-        mt.put(to);
-        nt.put(to + S::MTile::kBytes);
-    };
-    const uint32_t m_at = S::MTile::lane_at(wm * S::kM, lane), n_at = S::NTile::lane_at(wn * S::kN, lane);
-    if (begin < end) {
-        fetch(begin);
-        put(begin);
+        for (int i = 0; i < S::kNB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (w.begin < w.end) {
+        w.fetch(w.begin, smem + (w.begin & 1) * S::kStage);
+        w.put(smem + (w.begin & 1) * S::kStage);
     }
-    for (int t = begin; t < end; ++t) {
+    for (int t = w.begin; t < w.end; ++t) {
         if constexpr (S::DMA) wait_vmcnt<0>();
         lds_barrier();  // this tile is there, and the one before has been read
-        if (t + 1 < end) fetch(t + 1);
+        char *const next = smem + (~t & 1) * S::kStage;
+        if (t + 1 < w.end) w.fetch(t + 1, next);
         const char *const ml = smem + (t & 1) * S::kStage, *const nl = ml + S::MTile::kBytes;
 #pragma unroll
         for (int kk = 0; kk < S::BK / 32; ++kk) {
             typename E::Frag nf[S::kNB], mf[S::kMB];
 #pragma unroll
-            for (int i = 0; i < S::kNB; ++i) nf[i] = S::NTile::frag(nl, n_at, i, kk);
+            for (int i = 0; i < S::kNB; ++i) nf[i] = S::NTile::frag(nl, w.n_at, i, kk);
 #pragma unroll
-            for (int j = 0; j < S::kMB; ++j) mf[j] = S::MTile::frag(ml, m_at, j, kk);
+            for (int j = 0; j < S::kMB; ++j) mf[j] = S::MTile::frag(ml, w.m_at, j, kk);
 #pragma unroll
             for (int i = 0; i < S::kNB; ++i)
 #pragma unroll
-                for (int j = 0; j < S::kMB; ++j) acc[i][j] = E::mfma(nf[i], mf[j], acc[i][j]);
+                for (int j = 0; j < S::kMB; ++j) acc[j][i] = E::mfma(nf[i], mf[j], acc[j][i]);
         }
-        if (t + 1 < end) put(t + 1);
+        if (t + 1 < w.end) w.put(next);
     }
-    if (a.parts > 1) {
-        f32x4 *to = reinterpret_cast<f32x4 *>(a.partial) +
-                    (((size_t)part * tiles + blockIdx.x % tiles) * S::WM * S::WN + wave) * S::kNB * S::kMB * kWave + lane;
-#pragma unroll
-        for (int i = 0; i < S::kNB; ++i)
-#pragma unroll
-            for (int j = 0; j < S::kMB; ++j) to[(i * S::kMB + j) * kWave] = acc[i][j];
-        return;
-    }
-    gated_store<E, F, S>(a, acc, at, wave, lane);
-}
-
-// Adds up the parts' accumulators in order and stores the results.
-template <class E, Form F, class S>
-__global__ __launch_bounds__(S::kThreads) void gated_join_kernel(GatedArgs a) {
-    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int tiles = a.tiles_m * a.tiles_n;
-    const TileAt at = tile_at(blockIdx.x, a.tiles_m, a.tiles_n);
-    const f32x4 *from = reinterpret_cast<const f32x4 *>(a.partial) + ((size_t)blockIdx.x * S::WM * S::WN + wave) * S::kNB * S::kMB * kWave + lane;
-    const size_t step = (size_t)tiles * S::WM * S::WN * S::kNB * S::kMB * kWave;
-    f32x4 acc[S::kNB][S::kMB];
-#pragma unroll
-    for (int i = 0; i < S::kNB; ++i)
-#pragma unroll
-        for (int j = 0; j < S::kMB; ++j) acc[i][j] = from[(i * S::kMB + j) * kWave];
-    for (int p = 1; p < a.parts; ++p) {
-        from += step;
-#pragma unroll
-        for (int i = 0; i < S::kNB; ++i)
-#pragma unroll
-            for (int j = 0; j < S::kMB; ++j) acc[i][j] += from[(i * S::kMB + j) * kWave];
-    }
-    gated_store<E, F, S>(a, acc, at, wave, lane);
+    lds_barrier();  // the last tile has been read
+    w.store(a, acc, smem, wave, lane);
 }
 
 // ------------------------------------------------- gradients of the two products
@@ -398,7 +57,7 @@ struct SlopeArgs {
     char *dg, *du;
     long long stride;  // elements between the rows of dg and du
     long long rows;
-    int hidden, activation;
+    int hidden;
     float *most;  // fp16: the workgroups' largest |dg| and |du|
     int *shift;
 };
@@ -406,7 +65,7 @@ struct SlopeArgs {
 constexpr int kSlopeThreads = 256, kMostGroups = 1024;
 
 // dg and du of eight neighbouring elements; those past the row's end are zero.
-template <class E>
+template <class E, int kActivation>
 __device__ __forceinline__ void slope8(const SlopeArgs &a, long long r, int c, float (&dg)[8], float (&du)[8]) {
     using Word = typename E::Word;
     const Word *dh = (const Word *)(a.dh + r * a.dh_stride) + c, *gate = (const Word *)(a.gate + r * a.gate_stride) + c;
@@ -427,27 +86,46 @@ __device__ __forceinline__ void slope8(const SlopeArgs &a, long long r, int c, f
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float2 s = slope<E>(a.activation, g.get(e));
+        const float2 s = slope<E, kActivation>(g.get(e));
         dg[e] = d.get(e) * u.get(e) * s.y;
         du[e] = d.get(e) * s.x;
     }
 }
 
+// Threads walk the chunks of eight elements in the rows' order (`per` a row):
+// f(chunk, row, first element).
+template <class G>
+__device__ __forceinline__ void each_chunk(long long rows, int per, G f) {
+    const long long step = (long long)gridDim.x * kSlopeThreads, first = (long long)blockIdx.x * kSlopeThreads + threadIdx.x;
+    const long long step_r = step / per;
+    const int step_c = (int)(step % per);
+    long long r = first / per;
+    int c = (int)(first % per);
+    for (long long i = first; r < rows; i += step) {
+        f(i, r, 8 * c);
+        r += step_r;
+        c += step_c;
+        if (c >= per) {
+            c -= per;
+            ++r;
+        }
+    }
+}
+
 // Largest finite |dg| and |du| of a workgroup's share.
+template <int kActivation>
 __global__ __launch_bounds__(kSlopeThreads) void gated_most_kernel(SlopeArgs a) {
     __shared__ float part[kSlopeThreads / kWave];
-    const int per = (a.hidden + 7) / 8;
-    const long long n = a.rows * per;
     float most = 0.f;
-    for (long long i = (long long)blockIdx.x * kSlopeThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kSlopeThreads) {
+    each_chunk(a.rows, (a.hidden + 7) / 8, [&](long long, long long r, int c) {
         float dg[8], du[8];
-        slope8<ElemF16>(a, i / per, (int)(i % per) * 8, dg, du);
+        slope8<ElemF16, kActivation>(a, r, c, dg, du);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             most = fmaxf(most, __builtin_isinf(dg[e]) ? 0.f : fabsf(dg[e]));
             most = fmaxf(most, __builtin_isinf(du[e]) ? 0.f : fabsf(du[e]));
         }
-    }
+    });
     most = group_max<kWave>(most);
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = most;
     __syncthreads();
@@ -459,7 +137,7 @@ __global__ __launch_bounds__(kSlopeThreads) void gated_most_kernel(SlopeArgs a) 
 
 // dg and du, rounded to the type; fp16's times a power of two that takes the
 // largest of them to 2^14 or just above.
-template <class E>
+template <class E, int kActivation>
 __global__ __launch_bounds__(kSlopeThreads) void gated_slope_kernel(SlopeArgs a, int groups) {
     int shift = 0;
     if constexpr (std::is_same_v<E, ElemF16>) {
@@ -474,13 +152,9 @@ __global__ __launch_bounds__(kSlopeThreads) void gated_slope_kernel(SlopeArgs a,
         if (most > 0.f) shift = 14 - ilogbf(most);
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.shift = shift;
     }
-    const int per = (int)(a.stride / 8);
-    const long long n = a.rows * per;
-    for (long long i = (long long)blockIdx.x * kSlopeThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kSlopeThreads) {
-        const long long r = i / per;
-        const int c = (int)(i - r * per) * 8;
+    each_chunk(a.rows, (int)(a.stride / 8), [&](long long i, long long r, int c) {
         float dg[8], du[8];
-        slope8<E>(a, r, c, dg, du);
+        slope8<E, kActivation>(a, r, c, dg, du);
         Words<E, 8> x, y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -489,7 +163,7 @@ __global__ __launch_bounds__(kSlopeThreads) void gated_slope_kernel(SlopeArgs a,
         }
         x.store((typename E::Word *)a.dg + i * 8);
         y.store((typename E::Word *)a.du + i * 8);
-    }
+    });
 }
 
 // ------------------------------------------------------------------ the host
@@ -508,8 +182,8 @@ bool bad_matrix(const bfhip_matrix *x, long long rows, long long length) {
 }
 
 struct GatedPlan {
-    bool big;
-    int tiles_m, tiles_n, parts, per;
+    bool large;
+    int tiles_m, tiles_n, whole, parts, per;
     size_t bytes;  // of the parts' sums
 };
 
@@ -520,36 +194,39 @@ bool chunks(const bfhip_matrix *x, long long rows, long long length, int size) {
            (rows <= 1 || x->stride < 1 << 21);
 }
 
-// Tiles, and where they are fewer than CUs the contraction's parts, of eight steps
-// or more, as many as fill the CUs twice.
+// Tiles, dealt in rounds of as many as the chip holds at once.  Those of the last
+// round are split along the contraction, in parts of eight steps or more, where
+// that fills it better.
 template <class S>
-void plan_tiles(GatedPlan &p, Form f, long long m, long long n, long long k) {
+void plan_tiles(GatedPlan &p, Form f, long long m, long long n, long long k, int round) {
     p.tiles_m = (int)((m + S::BM - 1) / S::BM * (f == kWeights ? 2 : 1));
     p.tiles_n = (int)((n + S::kCols - 1) / S::kCols);
     const long long steps = (k + S::BK - 1) / S::BK * (f == kInputs ? 2 : 1), tiles = (long long)p.tiles_m * p.tiles_n;
-    const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float);
-    long long parts = p.big ? 1 : std::min({512 / std::max(1ll, tiles), steps / 8, kPartBytes / std::max(1ll, tiles * tile_bytes)});
-    if (parts < 2) parts = 1;
-    p.per = (int)((steps + parts - 1) / std::max(1ll, parts));
-    if (p.per < 1) p.per = 1;
-    p.parts = (int)std::max(1ll, (steps + p.per - 1) / p.per);
-    p.bytes = p.parts > 1 ? (size_t)p.parts * tiles * tile_bytes : 0;
+    const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % round;
+    p.whole = (int)std::min(tiles, 0x7fffffffll);
+    p.parts = 1;
+    if (!rest) return;
+    const long long parts = std::min({round / rest, steps / 8, kPartBytes / (rest * tile_bytes)});
+    if (parts < 2) return;
+    p.per = (int)((steps + parts - 1) / parts);
+    p.parts = (int)((steps + p.per - 1) / p.per);
+    p.whole = (int)(tiles - rest);
+    p.bytes = (size_t)(p.parts * rest * tile_bytes);
 }
 
-// The shapes: large tiles where there are enough of them to fill the chip, and
-// only for matrices that are copied in whole chunks.
+// The shapes: large tiles, one per CU, where there are enough of them to fill the
+// chip, and only for matrices that are copied in whole chunks; small ones, two
+// per CU.
 template <class E, Form F, bool DMA>
 using SmallShape = GatedShape<E, F, 128, 128, 2, E::kSize == 4 ? 4 : 2, DMA>;
-template <class E, Form F>
-using BigShape = GatedShape<E, F, 256, 256, 2, 4, true>;
 
 template <class E, Form F>
 GatedPlan gated_plan(long long m, long long n, long long k, bool dma) {
     GatedPlan p{};
     const long long cols = F == kForward ? 128 : 256;
-    p.big = dma && E::kSize == 2 && (m + 255) / 256 * ((n + cols - 1) / cols) * (F == kWeights ? 2 : 1) >= 192;
-    if (p.big) plan_tiles<BigShape<ElemBf16, F>>(p, F, m, n, k);
-    else plan_tiles<SmallShape<E, F, true>>(p, F, m, n, k);
+    p.large = dma && E::kSize == 2 && (m + 255) / 256 * ((n + cols - 1) / cols) * (F == kWeights ? 2 : 1) >= 192;
+    if (p.large) plan_tiles<LargeShape<ElemBf16, F>>(p, F, m, n, k, 256);
+    else plan_tiles<SmallShape<E, F, true>>(p, F, m, n, k, 512);
     return p;
 }
 
@@ -557,24 +234,21 @@ template <class E, Form F>
 int gated_launch(GatedArgs a, const GatedPlan &p, bool dma, hipStream_t s) {
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
+    a.whole = p.whole;
     a.parts = p.parts;
     a.per = p.per;
-    const long long tiles = (long long)p.tiles_m * p.tiles_n, grid = tiles * p.parts;
-    if (grid > 0x7fffffff || !launch_fits(grid, 512)) return 0;
-    const auto run = [&](auto shape) {
-        using S = decltype(shape);
-        hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
-    };
+    const long long split = (long long)p.tiles_m * p.tiles_n - p.whole, grid = p.whole + split * p.parts;
+    if (!launch_fits(grid, 512)) return 0;
     if constexpr (E::kSize == 2) {
-        if (p.big) {
-            run(BigShape<E, F>{});
+        if (p.large) {
+            launch_gated_large<E, F>(a, grid, s);
             return 1;
         }
     }
-    using Join = SmallShape<E, F, true>;
-    if (dma) run(Join{});
-    else run(SmallShape<E, F, false>{});
-    if (p.parts > 1) hipLaunchKernelGGL((gated_join_kernel<E, F, Join>), dim3((unsigned)tiles), dim3(Join::kThreads), 0, s, a);
+    using S = SmallShape<E, F, true>;
+    if (dma) hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
+    else hipLaunchKernelGGL((gated_product_kernel<E, F, SmallShape<E, F, false>>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
+    if (split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(split * S::kMB)), dim3(S::kThreads), 0, s, a);
     return 1;
 }
 
@@ -692,7 +366,6 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     e.stride = stride;
     e.rows = d->rows;
     e.hidden = (int)d->hidden;
-    e.activation = d->activation;
     e.most = (float *)(work + 2 * p.slopes + p.parts);
     e.shift = (int *)(e.most + kMostGroups);
     const long long groups = std::min<long long>(kMostGroups, (d->rows * (stride / 8) + kSlopeThreads - 1) / kSlopeThreads);
@@ -703,8 +376,11 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     with_element(d->type, [&](auto el) {
         using E = decltype(el);
         if (d->rows) {
-            if (d->type == BFHIP_F16) hipLaunchKernelGGL(gated_most_kernel, dim3((unsigned)groups), dim3(kSlopeThreads), 0, s, e);
-            hipLaunchKernelGGL(gated_slope_kernel<E>, dim3((unsigned)grid), dim3(kSlopeThreads), 0, s, e, (int)groups);
+            with_activation(d->activation, [&](auto kind) {
+                constexpr int A = decltype(kind)::value;
+                if (d->type == BFHIP_F16) hipLaunchKernelGGL(gated_most_kernel<A>, dim3((unsigned)groups), dim3(kSlopeThreads), 0, s, e);
+                hipLaunchKernelGGL((gated_slope_kernel<E, A>), dim3((unsigned)grid), dim3(kSlopeThreads), 0, s, e, (int)groups);
+            });
         }
         GatedArgs a{};
         a.activation = d->activation;
