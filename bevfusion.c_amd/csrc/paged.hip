@@ -29,12 +29,12 @@ struct PagedArgs {
     int sequences, heads, kv_heads, dim, page_size, table_pages, reach;
     float scale2;
     int flip;
-    int target;        // parts that the keys of one head are split into, about; 0: no split
-    int least;         // tiles of a part, at least
-    long long slots;   // of the grid
-    float *part_out;   // [slot][kv_heads][kRows][padded dim]
-    float2 *part_stat; // [slot][kv_heads][kRows]
-    int2 *info;        // [sequences]: first slot, parts of each row tile
+    int shares;        // workgroups of a key head
+    int least;         // units of a share, at least
+    int piece;         // units of a row tile beside its key tiles
+    float *part_out;   // [2 shares][kv_heads][kRows][padded dim]
+    float2 *part_stat; // [2 shares][kv_heads][kRows]
+    long long *info;   // [sequences + 1]: first unit of each sequence that has some; units of a share
 };
 
 // Keys of sequence b.
@@ -78,17 +78,24 @@ __global__ __launch_bounds__(256) void cache_append_kernel(PagedArgs a, AttnRows
 
 // ---------------------------------------------------------------- attention
 // How the work is dealt.  Lengths are on the device alone, so every workgroup
-// works the deal out for itself: sequence b has row tiles (16 rows, token * group
-// + head in group) and key tiles; with `per` = all sequences' (row tiles x key
-// tiles) / target, each of its row tiles is split into ceil(key tiles / per)
-// parts, and the slots are counted through the sequences in order.  A
-// sequence without new tokens has none.
+// works the deal out for itself.  Sequence b has row tiles (16 rows, token * group +
+// head in group) and key tiles; a row tile takes units of time, one per key tile and
+// `piece` for its queries' way in and its results' way out.  Units, row tile after row
+// tile, sequence after sequence, are dealt in equal shares, one per workgroup
+// that the chip holds at once, whatever the lengths are.  So a share has whole row
+// tiles and at most one that an earlier share began and one that it leaves to a
+// later one: two places for sums that are to be joined.  (A sequence without new
+// tokens has no units.)
 struct SequenceWork {
-    int start, queries, keys, row_tiles, tiles;
+    int start, queries, keys, row_tiles, tiles, piece;
+    __device__ __forceinline__ int cost() const { return tiles + piece; }
+    __device__ __forceinline__ long long units() const { return (long long)row_tiles * cost(); }
+    // Key tiles up to unit x of a row tile.
+    __device__ __forceinline__ int tile(int x) const { return (int)((long long)x * tiles / cost()); }
 };
 
 __device__ __forceinline__ SequenceWork sequence_work(const PagedArgs &a, int b) {
-    SequenceWork w{0, 0, 0, 0, 0};
+    SequenceWork w{0, 0, 0, 0, 0, a.piece};
     if (b >= a.sequences) return w;
     const long long s = clamp_start(a.starts, b, a.tokens), e = clamp_start(a.starts, b + 1, a.tokens);
     w.start = (int)s;
@@ -100,58 +107,58 @@ __device__ __forceinline__ SequenceWork sequence_work(const PagedArgs &a, int b)
     return w;
 }
 
-struct PagedSlot {
-    int sequence;  // -1: none
-    SequenceWork work;
-    int row_tile, part, parts;
-};
+// The sequences from the one that a share begins in, 64 at a time, a lane each.
+struct Sequences {
+    int first, at;           // the lanes' first sequence, and the lane in turn
+    SequenceWork lane_work;  // of the lane's sequence
+    long long lane_upto;     // units up to its end
 
-__device__ __forceinline__ PagedSlot find_part(const PagedArgs &a, int slot) {
-    const int lane = threadIdx.x % kWave;
-    int per = 0x7fffffff;
-    if (a.target) {
-        long long total = 0;
-        for (int b = lane; b < a.sequences; b += kWave) {
-            const SequenceWork w = sequence_work(a, b);
-            total += (long long)w.row_tiles * w.tiles;
-        }
-#pragma unroll
-        for (int o = 1; o < kWave; o *= 2) total += __shfl_xor(total, o);
-        const long long share = (total + a.target - 1) / a.target;
-        per = (int)max((long long)a.least, min(share, 0x7fffffffll));
-    }
-    PagedSlot s{-1, {}, 0, 0, 1};
-    int before = 0;
-    for (int first = 0; first < a.sequences; first += kWave) {
-        const SequenceWork w = sequence_work(a, first + lane);
-        const int parts = w.tiles > per ? (w.tiles + per - 1) / per : 1, own = w.row_tiles * parts;
-        int upto = own;
+    // Units of the sequences before the lanes' in `before`.
+    __device__ __forceinline__ void load(const PagedArgs &a, int b, long long before) {
+        const int lane = threadIdx.x % kWave;
+        first = b;
+        lane_work = sequence_work(a, b + lane);
+        lane_upto = lane_work.units();
 #pragma unroll
         for (int o = 1; o < kWave; o *= 2) {
-            const int x = __shfl_up(upto, o);
-            if (lane >= o) upto += x;
+            const long long x = __shfl_up(lane_upto, o);
+            if (lane >= o) lane_upto += x;
         }
-        upto += before;
-        const unsigned long long at = __ballot(slot < upto);
-        if (at) {
-            const int l = (int)__builtin_ctzll(at);
-            s.sequence = first + l;
-            s.work.start = __builtin_amdgcn_readlane(w.start, l);
-            s.work.queries = __builtin_amdgcn_readlane(w.queries, l);
-            s.work.keys = __builtin_amdgcn_readlane(w.keys, l);
-            s.work.tiles = __builtin_amdgcn_readlane(w.tiles, l);
-            s.work.row_tiles = __builtin_amdgcn_readlane(w.row_tiles, l);
-            s.parts = __builtin_amdgcn_readlane(parts, l);
-            const int in = slot - (__builtin_amdgcn_readlane(upto, l) - s.work.row_tiles * s.parts);
-            s.row_tile = in / s.parts;
-            s.part = in - s.row_tile * s.parts;
-            // (starts that descend can make the sums above too large for an int)
-            if (in < 0 || s.row_tile >= s.work.row_tiles) s.sequence = -1;
-            return s;
-        }
-        before = __builtin_amdgcn_readlane(upto, kWave - 1);
+        lane_upto += before;
     }
-    return s;
+    __device__ __forceinline__ static long long read(long long v, int lane) {
+        return (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) |
+                           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
+    }
+    __device__ __forceinline__ SequenceWork work() const {
+        return SequenceWork{__builtin_amdgcn_readlane(lane_work.start, at), __builtin_amdgcn_readlane(lane_work.queries, at),
+                            __builtin_amdgcn_readlane(lane_work.keys, at), __builtin_amdgcn_readlane(lane_work.row_tiles, at),
+                            __builtin_amdgcn_readlane(lane_work.tiles, at), lane_work.piece};
+    }
+    __device__ __forceinline__ long long upto() const { return read(lane_upto, at); }
+    // Turns to the sequence that holds `unit`, from the lanes' on; false if none does.
+    __device__ __forceinline__ bool seek(const PagedArgs &a, long long unit) {
+        for (;;) {
+            const unsigned long long in = __ballot(unit < lane_upto);
+            if (in) {
+                at = (int)__builtin_ctzll(in);
+                return true;
+            }
+            if (first + kWave >= a.sequences) return false;
+            load(a, first + kWave, read(lane_upto, kWave - 1));
+        }
+    }
+};
+
+__device__ __forceinline__ long long share_units(const PagedArgs &a) {
+    if (a.shares == 1) return 0x7fffffffffffffffll;
+    long long total = 0;
+    for (int b = threadIdx.x % kWave; b < a.sequences; b += kWave) total += sequence_work(a, b).units();
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) total += __shfl_xor(total, o);
+    total = Sequences::read(total, 0);
+    const long long share = (total + a.shares - 1) / a.shares;
+    return share > a.least ? share : a.least;
 }
 
 // What a lane reads in place of a row that is not there.
@@ -173,177 +180,203 @@ struct PagedTile {
     static constexpr int kIssue = kKeys * T::kChunks / kWave;  // copies of one of the two
 };
 
-// Bound by reading the keys and values once.  A workgroup has a part of a
-// sequence's keys for one key head, whose whole group of query heads shares each
-// tile.  Each wave walks tiles of its own, 32 keys at a time, through its own
-// two LDS buffers, two tiles in flight, without a barrier; the waves' sums are
-// joined at the end.  Rows of a tile may lie in different pages, so every lane
-// copies from an address of its own: lane r knows the page of row r, loaded a
-// tile ahead.
+// Bound by reading the keys and values once.  A workgroup has a share of the units
+// of one key head, whose whole group of query heads shares each tile.  Each wave
+// walks tiles of its own, 32 keys at a time, through its own two LDS buffers, two
+// tiles in flight, without a barrier; the waves' sums are joined at a row tile's
+// end.  Rows of a tile may lie in different pages, so every lane copies from an
+// address of its own: lane r knows the page of row r, loaded a tile ahead.
 template <class E, int DIM, bool BIAS>
-__global__ __launch_bounds__(256, 1) void paged_attention_kernel(PagedArgs a) {
+struct PagedWalk {
     using P = PagedTile<E, DIM>;
     using T = typename P::T;
-    constexpr int kKB = DIM / 32, kDB = DIM / 16, kWaves = P::kWaves;
+    static constexpr int kKB = DIM / 32, kDB = DIM / 16, kWaves = P::kWaves;
+    const PagedArgs &a;
+    char *smem;
+    int kv, share, lane, wave;
+
+    // Row tile `row_tile` of sequence b, its units x0 .. x1.
+    __device__ __forceinline__ void piece(int b, const SequenceWork &s, int row_tile, int x0, int x1) {
+        float2(*const stat)[kRows] = reinterpret_cast<float2(*)[kRows]>(smem + kWaves * 2 * P::kStage);
+        const int l16 = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads;
+        const bool whole = x0 == 0 && x1 == s.cost();
+        const int t0 = s.tile(x0), t1 = s.tile(x1);
+        const int q_start = s.start, k_len = s.keys, rows = s.queries * group;
+        const int offset = k_len - s.queries, first = row_tile * kRows;
+
+        const int row = first + l16, token = row / group, head = kv * group + row % group;
+        const bool live = row < rows;
+        typename E::Frag qf[kKB];
+        {
+            const char *q = a.q.at((long long)q_start + token, head);
+#pragma unroll
+            for (int kk = 0; kk < kKB; ++kk) {
+                const int d = 32 * kk + 8 * g;
+                qf[kk] = typename E::Frag{};
+                if (live && d < a.dim) qf[kk] = signed_frag<E>(load_frag<E>(q + d * E::kSize), a.flip);
+            }
+        }
+        const int limit = min(k_len, token + offset + 1);  // keys that the lane's row sees
+        const int last = min(k_len, (min(first + kRows, rows) - 1) / group + 1 + offset);
+        const int full = min(k_len, first / group + offset + 1);
+        const int end = min(last > 0 ? (last + kKeys - 1) / kKeys : 0, t1);
+
+        char *const mine = smem + wave * 2 * P::kStage;
+        const int *const table = a.table + b * a.table_stride;
+        // The page of row lane % 32 of tile t.
+        const auto page = [&](int t) {
+            const int j = t * kKeys + lane % kKeys;
+            return t < end && j < last ? table[j / a.page_size] : -1;
+        };
+        const auto issue = [&](int t, int ids, int buffer) {
+            const int in = (t * kKeys + lane % kKeys) % a.page_size;
+            char *const to = mine + buffer * P::kStage;
+#pragma unroll
+            for (int i = 0; i < P::kIssue; ++i) {
+                const int id = i * kWave + lane, r = id / T::kChunks;
+                const int c = 16 * ((id % T::kChunks) ^ T::swizzle(r));
+                const int pg = __shfl(ids, r), at = __shfl(in, r);
+                const bool there = pg >= 0 && pg < a.pages && c < a.dim * E::kSize;
+                dma16_from(there ? a.k.at(pg, at, kv) + c : (const char *)no_row, to + i * kWave * 16);
+                dma16_from(there ? a.v.at(pg, at, kv) + c : (const char *)no_row, to + kKeys * T::kRow + i * kWave * 16);
+            }
+        };
+        Running<1, kDB> run;
+        run.clear();
+        int t = t0 + wave;
+        int ids = page(t);
+        uint32_t there = 0;  // keys of the tile that have a page
+        if (t < end) {
+            there = (uint32_t)__ballot(ids >= 0 && ids < a.pages);
+            issue(t, ids, 0);
+        }
+        ids = page(t + kWaves);
+        for (int buffer = 0; t < end; t += kWaves, buffer ^= 1) {
+            uint32_t next_there = 0;
+            if (t + kWaves < end) {
+                const int now = ids;
+                ids = page(t + 2 * kWaves);
+                next_there = (uint32_t)__ballot(now >= 0 && now < a.pages);
+                issue(t + kWaves, now, buffer ^ 1);
+                wait_vmcnt<(2 * P::kIssue > 63 ? 63 : 2 * P::kIssue)>();  // this tile's, not the next one's
+            } else {
+                wait_vmcnt<0>();
+            }
+            asm volatile("" ::: "memory");
+            const char *const kt = mine + buffer * P::kStage, *const vt = kt + kKeys * T::kRow;
+            const int j0 = t * kKeys;
+            f32x4 sc[2][1];
+#pragma unroll
+            for (int jb = 0; jb < 2; ++jb) {
+                sc[jb][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < kKB; ++kk) sc[jb][0] = E::mfma(row_frag<E, DIM>(kt, 16 * jb, kk, lane), qf[kk], sc[jb][0]);
+            }
+            if constexpr (BIAS) {
+#pragma unroll
+                for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int far = min(max(j0 + 16 * jb + 4 * g + e - (token + offset), -a.reach), a.reach) + a.reach;
+                        const float bias = live ? a.bias[(size_t)head * (2 * a.reach + 1) + far] : 0.f;
+                        sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, base2_bias(bias));
+                    }
+            }
+            if (j0 + kKeys > full || there != ~0u) {
+#pragma unroll
+                for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = 16 * jb + 4 * g + e;
+                        sc[jb][0][e] = j0 + j < limit && (there >> j & 1) ? sc[jb][0][e] : -INFINITY;
+                    }
+            }
+            there = next_there;
+            run.template take<2>(sc, BIAS ? 1.f : a.scale2);
+            const typename E::Frag pf = to_frag<E>(sc[0][0], sc[1][0]);
+            typename E::Frag vf[kDB];
+            col_frags_in_flight<E, DIM>(vt, lane, vf);
+#pragma unroll
+            for (int db = 0; db < kDB; ++db) run.o[0][db] = E::mfma(vf[db], pf, run.o[0][db]);
+            // The next round's copy goes into the buffer just read.
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+            asm volatile("" ::: "memory");
+        }
+        // The waves' sums at their common maximum, added in order.
+        run.finish();
+        if (g == 0) stat[wave][l16] = make_float2(run.m[0], run.l[0]);
+        __syncthreads();
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stat[w][l16].x);
+        const float at = top == -INFINITY ? 0.f : top;
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) total += stat[w][l16].y * exp2_raw(stat[w][l16].x - at);
+        const float fade = exp2_raw(run.m[0] - at);
+        float *const sums = reinterpret_cast<float *>(smem);  // [wave][16][DIM + 4]
+#pragma unroll
+        for (int db = 0; db < kDB; ++db)
+            *reinterpret_cast<f32x4 *>(sums + (wave * 16 + l16) * (DIM + 4) + 16 * db + 4 * g) = run.o[0][db] * fade;
+        __syncthreads();
+        const float inv = inverse(total);
+        const size_t part_row = ((size_t)(2 * share + (x0 == 0)) * a.kv_heads + kv) * kRows + l16;
+#pragma unroll
+        for (int d0 = 0; d0 < kDB; d0 += kWaves) {
+            const int d = 16 * (d0 + wave) + 4 * g;
+            if (d0 + wave >= kDB) break;
+            f32x4 v = *reinterpret_cast<const f32x4 *>(sums + l16 * (DIM + 4) + d);
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) v += *reinterpret_cast<const f32x4 *>(sums + (w * 16 + l16) * (DIM + 4) + d);
+            if (!live) continue;
+            if (!whole) {
+                *reinterpret_cast<f32x4 *>(a.part_out + part_row * DIM + d) = v;
+            } else if (d < a.dim) {
+                Words<E, 4> w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.put(e, v[e] * inv);
+                w.store(reinterpret_cast<typename E::Word *>(a.out.at((long long)q_start + token, head)) + d);
+            }
+        }
+        if (wave == 0 && g == 0 && live) {
+            if (!whole) a.part_stat[part_row] = make_float2(top, total);
+            else if (a.lse) a.lse[(size_t)head * a.tokens + q_start + token] = natural_lse(top, total);
+        }
+    }
+};
+
+template <class E, int DIM, bool BIAS>
+__global__ __launch_bounds__(256, 1) void paged_attention_kernel(PagedArgs a) {
+    using Walk = PagedWalk<E, DIM, BIAS>;
     // One LDS object: with two the compiler waits for every copy in flight
     // before any LDS read.
-    __shared__ __attribute__((aligned(16))) char smem[kWaves * (2 * P::kStage + kRows * sizeof(float2))];
-    float2(*const stat)[kRows] = reinterpret_cast<float2(*)[kRows]>(smem + kWaves * 2 * P::kStage);
-    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int l16 = lane & 15, g = lane >> 4, group = a.heads / a.kv_heads;
-    const int kv = blockIdx.x % a.kv_heads, slot = blockIdx.x / a.kv_heads;
-    const PagedSlot s = find_part(a, slot);
-    if (s.sequence < 0) return;
-    if (a.info && kv == 0 && s.row_tile == 0 && s.part == 0 && threadIdx.x == 0) a.info[s.sequence] = make_int2(slot, s.parts);
-    const int q_start = s.work.start, k_len = s.work.keys, rows = s.work.queries * group;
-    const int offset = k_len - s.work.queries, first = s.row_tile * kRows;
-    const int per = (s.work.tiles + s.parts - 1) / s.parts, begin = s.part * per;
-
-    const int row = first + l16, token = row / group, head = kv * group + row % group;
-    const bool live = row < rows;
-    typename E::Frag qf[kKB];
-    {
-        const char *q = a.q.at((long long)q_start + token, head);
-#pragma unroll
-        for (int kk = 0; kk < kKB; ++kk) {
-            const int d = 32 * kk + 8 * g;
-            qf[kk] = typename E::Frag{};
-            if (live && d < a.dim) qf[kk] = signed_frag<E>(load_frag<E>(q + d * E::kSize), a.flip);
-        }
-    }
-    const int limit = min(k_len, token + offset + 1);  // keys that the lane's row sees
-    const int last = min(k_len, (min(first + kRows, rows) - 1) / group + 1 + offset);
-    const int full = min(k_len, first / group + offset + 1);
-    const int tiles = last > 0 ? (last + kKeys - 1) / kKeys : 0, end = min(tiles, begin + per);
-
-    char *const mine = smem + wave * 2 * P::kStage;
-    const int *const table = a.table + s.sequence * a.table_stride;
-    // The page of row lane % 32 of tile t.
-    const auto page = [&](int t) {
-        const int j = t * kKeys + lane % kKeys;
-        return t < end && j < last ? table[j / a.page_size] : -1;
-    };
-    const auto issue = [&](int t, int ids, int buffer) {
-        const int in = (t * kKeys + lane % kKeys) % a.page_size;
-        char *const to = mine + buffer * P::kStage;
-#pragma unroll
-        for (int i = 0; i < P::kIssue; ++i) {
-            const int id = i * kWave + lane, r = id / T::kChunks;
-            const int c = 16 * ((id % T::kChunks) ^ T::swizzle(r));
-            const int pg = __shfl(ids, r), at = __shfl(in, r);
-            const bool there = pg >= 0 && pg < a.pages && c < a.dim * E::kSize;
-            dma16_from(there ? a.k.at(pg, at, kv) + c : (const char *)no_row, to + i * kWave * 16);
-            dma16_from(there ? a.v.at(pg, at, kv) + c : (const char *)no_row, to + kKeys * T::kRow + i * kWave * 16);
-        }
-    };
-    Running<1, kDB> run;
-    run.clear();
-    int t = begin + wave;
-    int ids = page(t);
-    uint32_t there = 0;  // keys of the tile that have a page
-    if (t < end) {
-        there = (uint32_t)__ballot(ids >= 0 && ids < a.pages);
-        issue(t, ids, 0);
-    }
-    ids = page(t + kWaves);
-    for (int buffer = 0; t < end; t += kWaves, buffer ^= 1) {
-        uint32_t next_there = 0;
-        if (t + kWaves < end) {
-            const int now = ids;
-            ids = page(t + 2 * kWaves);
-            next_there = (uint32_t)__ballot(now >= 0 && now < a.pages);
-            issue(t + kWaves, now, buffer ^ 1);
-            wait_vmcnt<(2 * P::kIssue > 63 ? 63 : 2 * P::kIssue)>();  // this tile's, not the next one's
-        } else {
-            wait_vmcnt<0>();
-        }
-        asm volatile("" ::: "memory");
-        const char *const kt = mine + buffer * P::kStage, *const vt = kt + kKeys * T::kRow;
-        const int j0 = t * kKeys;
-        f32x4 sc[2][1];
-#pragma unroll
-        for (int jb = 0; jb < 2; ++jb) {
-            sc[jb][0] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kk = 0; kk < kKB; ++kk) sc[jb][0] = E::mfma(row_frag<E, DIM>(kt, 16 * jb, kk, lane), qf[kk], sc[jb][0]);
-        }
-        if constexpr (BIAS) {
-#pragma unroll
-            for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int far = min(max(j0 + 16 * jb + 4 * g + e - (token + offset), -a.reach), a.reach) + a.reach;
-                    const float b = live ? a.bias[(size_t)head * (2 * a.reach + 1) + far] : 0.f;
-                    sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, base2_bias(b));
-                }
-        }
-        if (j0 + kKeys > full || there != ~0u) {
-#pragma unroll
-            for (int jb = 0; jb < 2; ++jb)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = 16 * jb + 4 * g + e;
-                    sc[jb][0][e] = j0 + j < limit && (there >> j & 1) ? sc[jb][0][e] : -INFINITY;
-                }
-        }
-        there = next_there;
-        run.template take<2>(sc, BIAS ? 1.f : a.scale2);
-        const typename E::Frag pf = to_frag<E>(sc[0][0], sc[1][0]);
-        typename E::Frag vf[kDB];
-        col_frags_in_flight<E, DIM>(vt, lane, vf);
-#pragma unroll
-        for (int db = 0; db < kDB; ++db) run.o[0][db] = E::mfma(vf[db], pf, run.o[0][db]);
-        // The next round's copy goes into the buffer just read.
-        __builtin_amdgcn_s_waitcnt(0xC07F);
-        asm volatile("" ::: "memory");
-    }
-    // The waves' sums at their common maximum, added in order.
-    run.finish();
-    if (g == 0) stat[wave][l16] = make_float2(run.m[0], run.l[0]);
-    __syncthreads();
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stat[w][l16].x);
-    const float at = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += stat[w][l16].y * exp2_raw(stat[w][l16].x - at);
-    const float fade = exp2_raw(run.m[0] - at);
-    float *const sums = reinterpret_cast<float *>(smem);  // [wave][16][DIM + 4]
-#pragma unroll
-    for (int db = 0; db < kDB; ++db)
-        *reinterpret_cast<f32x4 *>(sums + (wave * 16 + l16) * (DIM + 4) + 16 * db + 4 * g) = run.o[0][db] * fade;
-    __syncthreads();
-    const float inv = inverse(total);
-    const size_t part_row = ((size_t)slot * a.kv_heads + kv) * kRows + l16;
-#pragma unroll
-    for (int b = 0; b < kDB; b += kWaves) {
-        const int d = 16 * (b + wave) + 4 * g;
-        if (b + wave >= kDB) break;
-        f32x4 v = *reinterpret_cast<const f32x4 *>(sums + l16 * (DIM + 4) + d);
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) v += *reinterpret_cast<const f32x4 *>(sums + (w * 16 + l16) * (DIM + 4) + d);
-        if (!live) continue;
-        if (s.parts > 1) {
-            *reinterpret_cast<f32x4 *>(a.part_out + part_row * DIM + d) = v;
-        } else if (d < a.dim) {
-            Words<E, 4> w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.put(e, v[e] * inv);
-            w.store(reinterpret_cast<typename E::Word *>(a.out.at((long long)q_start + token, head)) + d);
-        }
-    }
-    if (wave == 0 && g == 0 && live) {
-        if (s.parts > 1) a.part_stat[part_row] = make_float2(top, total);
-        else if (a.lse) a.lse[(size_t)head * a.tokens + q_start + token] = natural_lse(top, total);
+    __shared__ __attribute__((aligned(16))) char smem[Walk::kWaves * (2 * Walk::P::kStage + kRows * sizeof(float2))];
+    Walk walk{a, smem, (int)blockIdx.x % a.kv_heads, (int)blockIdx.x / a.kv_heads, (int)threadIdx.x % kWave,
+              __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)};
+    const long long units = share_units(a);
+    long long u = walk.share * units;
+    const long long end = a.shares == 1 ? units : u + units;
+    const bool writes = a.info && walk.kv == 0 && threadIdx.x == 0;
+    if (writes && walk.share == 0) a.info[a.sequences] = units;
+    Sequences at;
+    at.load(a, 0, 0);
+    while (u < end && at.seek(a, u)) {
+        const SequenceWork s = at.work();
+        const long long begin = at.upto() - s.units(), in = u - begin;
+        const int row_tile = (int)(in / s.cost()), x0 = (int)(in - (long long)row_tile * s.cost());
+        const int x1 = (int)min((long long)s.cost(), x0 + (end - u));
+        if (writes && in == 0) a.info[at.first + at.at] = begin;
+        walk.piece(at.first + at.at, s, row_tile, x0, x1);
+        u += x1 - x0;
+        __syncthreads();  // the sums have been read
     }
 }
 
 // Joins the parts' sums of each query and head: DIM / 4 threads, four elements
-// each, times four shares of the parts, which are added up in order at the end.
+// each, times eight (or fewer) of the parts, which are added up in order at the end.
 template <class E, int DIM>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
-    constexpr int kShares = 4, kPer = 256 * 4 / DIM / kShares;
+    constexpr int kShares = 8, kPer = 256 * 4 / DIM / kShares;
     __shared__ float2 stat_part[kShares][kPer];
     __shared__ __attribute__((aligned(16))) float sums[kShares][kPer][DIM];
     const int q = threadIdx.x / (DIM / 4), share = q % kShares, i = q / kShares, d = threadIdx.x % (DIM / 4) * 4;
@@ -352,27 +385,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     const int head = blockIdx.x % per_token * kPer + i, group = a.heads / a.kv_heads;
     const int sequence = find_token(a.starts, a.sequences, a.tokens, token);
     if (sequence < 0) return;
-    const int2 info = a.info[sequence];
-    const int parts = info.y;
-    if (parts <= 1) return;  // written by the kernel before
-    int start, length;
-    sequence_rows(a.starts, sequence, a.tokens, start, length);
-    const int kv = min(head, a.heads - 1) / group, row = (token - start) * group + min(head, a.heads - 1) % group;
-    const long long slot = info.x + (long long)(row / kRows) * parts;
-    // (where starts descend, a row's sequence need not be one that was dealt)
-    if (info.x < 0 || slot + parts > a.slots) return;
-    const size_t step = (size_t)a.kv_heads * kRows, at_row = (slot * a.kv_heads + kv) * kRows + row % kRows;
-    const float2 *const stat = a.part_stat + at_row;
-    const float *const out = a.part_out + at_row * DIM + d;
+    const SequenceWork s = sequence_work(a, sequence);
+    const int kv = min(head, a.heads - 1) / group, row = (token - s.start) * group + min(head, a.heads - 1) % group;
+    // Shares that have units of the row's tile: the first in their second place, the
+    // others in their first.  (Where starts descend, a row's sequence need not be one
+    // that was dealt: any place within the workspace will do then.)
+    const long long units = a.info[a.sequences], begin = a.info[sequence] + (long long)(row / kRows) * s.cost();
+    const long long from = begin / units, to = (begin + s.cost() - 1) / units;
+    if (from == to || from < 0 || to >= a.shares) return;  // (one share has written the result)
+    const int parts = (int)(to - from) + 1;
+    const size_t step = (size_t)a.kv_heads * kRows, place = (size_t)kv * kRows + row % kRows;
     float m = -INFINITY, l = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = share; p < parts; p += kShares) {
-        const float2 ml = stat[p * step];
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(out + p * step * DIM);
-        const float to = fmaxf(m, ml.x), at = to == -INFINITY ? 0.f : to;
+        const size_t at_row = (2 * (size_t)(from + p) + (p == 0)) * step + place;
+        const float2 ml = a.part_stat[at_row];
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(a.part_out + at_row * DIM + d);
+        const float top = fmaxf(m, ml.x), at = top == -INFINITY ? 0.f : top;
         const float old = exp2_raw(m - at), now = exp2_raw(ml.x - at);
-        m = to;
+        m = top;
         l = l * old + ml.y * now;
         v = v * old + x * now;
     }
@@ -465,35 +497,26 @@ PagedArgs paged_args(const bfhip_paged_desc *d, const bfhip_pages *k, const bfhi
 }
 
 struct PagedPlan {
-    int dim, target, least;
-    long long slots;
+    int dim, shares, least, piece;
+    size_t bytes;
 };
 
-// About 1536 workgroups read keys, whatever the lengths are; row tiles beyond the
-// first of a sequence bring slots of their own.  Where a cache holds no two
-// parts nothing is split, and neither where the parts' sums would take more than
-// kPartBytes: so many queries fill the chip by themselves.
-constexpr long long kPartBytes = 1ll << 30;
-
-long long paged_bytes(const bfhip_paged_desc *d, long long slots, int dim) {
-    return slots * d->kv_heads * kRows * (long long)(dim * sizeof(float) + sizeof(float2)) + d->sequences * (long long)sizeof(int2);
-}
-
+// Shares of a key head: as many as make the workgroups that the chip holds at once,
+// two per CU (one for long fp32 rows).  Heads of 128, 32 on 8, bf16, with three
+// times as many: one sequence of 131071 keys 131 us and 118 so, 64 of 2048 124 and 108.
 PagedPlan paged_plan(const bfhip_paged_desc *d) {
     PagedPlan p{};
-    const int size = d->type == BFHIP_F32 ? 4 : 2, group = d->heads / d->kv_heads;
+    const int size = d->type == BFHIP_F32 ? 4 : 2;
     p.dim = d->head_dim <= 32 ? 32 : d->head_dim <= 64 ? 64 : 128;
     if (!d->sequences || !d->tokens) return p;
     p.least = size * p.dim <= 128 ? 4 : 2;
-    const long long row_tiles = d->tokens * group / kRows + std::min<long long>(d->sequences, d->tokens);
-    p.slots = row_tiles;
-    const long long capacity = ((long long)d->table_pages * d->page_size + kKeys - 1) / kKeys;
-    const int target = std::max(1, 1536 / d->kv_heads);
-    // sum of row tiles x ceil(key tiles / per) <= target + row tiles
-    if (capacity > p.least && paged_bytes(d, row_tiles + target, p.dim) <= kPartBytes) {
-        p.target = target;
-        p.slots += target;
-    }
+    // A row tile's beginning and end take about as long as 64 KiB of keys and values
+    // (3 tokens for each of 100 sequences of 3 to 1500 keys, 12 heads of 64: 45 us, 82
+    // where they are not counted and a share of short sequences has many of them).
+    p.piece = (64 << 10) / (2 * kKeys * size * p.dim);
+    p.shares = std::max(1, (size * p.dim > 256 ? 256 : 512) / d->kv_heads);
+    const size_t rows = (size_t)2 * p.shares * d->kv_heads * kRows;
+    if (p.shares > 1) p.bytes = rows * (p.dim * sizeof(float) + sizeof(float2)) + ((size_t)d->sequences + 1) * sizeof(long long);
     return p;
 }
 
@@ -524,8 +547,7 @@ extern "C" int bfhip_cache_append(const bfhip_paged_desc *d, const bfhip_rows *k
 
 extern "C" size_t bfhip_paged_attention_workspace(const bfhip_paged_desc *d) {
     if (bad_paged(d) || bad_paged_queries(d)) return 0;
-    const PagedPlan p = paged_plan(d);
-    return p.target ? (size_t)paged_bytes(d, p.slots, p.dim) : 0;
+    return paged_plan(d).bytes;
 }
 
 extern "C" int bfhip_paged_attention(const bfhip_paged_desc *d, const bfhip_rows *q, const bfhip_pages *k_pages,
@@ -538,12 +560,12 @@ extern "C" int bfhip_paged_attention(const bfhip_paged_desc *d, const bfhip_rows
     if (bad_rows(q, d->tokens, d->head_dim, size) || bad_result(out, d->tokens, d->heads, d->head_dim, size))
         return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
     const PagedPlan p = paged_plan(d);
-    const size_t need = p.target ? (size_t)paged_bytes(d, p.slots, p.dim) : 0;
+    const size_t need = p.bytes;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "paged attention workspace too small or not 16-byte aligned");
     if (!d->sequences || !d->tokens) return 1;
-    const long long grid = p.slots * d->kv_heads, joins = p.target ? ((long long)d->heads * p.dim + 255) / 256 * d->tokens : 0;
-    if (!launch_fits(grid, 256) || !launch_fits(joins, 256)) return fail(error, cap, "paged attention has too many rows");
+    const long long grid = (long long)p.shares * d->kv_heads, per_token = (d->heads * p.dim + 127) / 128, joins = need ? per_token * d->tokens : 0;
+    if (d->tokens * (d->heads / d->kv_heads) > 1 << 30 || !launch_fits(grid, 256) || !launch_fits(joins, 256)) return fail(error, cap, "paged attention has too many rows");
     PagedArgs a = paged_args(d, k_pages, v_pages);
     a.q = attn_rows(q, d->tokens, d->head_dim, size);
     a.out = attn_rows(out, d->tokens, d->head_dim, size);
@@ -551,14 +573,14 @@ extern "C" int bfhip_paged_attention(const bfhip_paged_desc *d, const bfhip_rows
     // Scores are compared before they are scaled: see bfhip_attention_forward.
     a.flip = d->scale < 0.f;
     a.scale2 = d->scale == 0.f ? __FLT_DENORM_MIN__ : __builtin_fabsf(d->scale * kLog2E);
-    a.target = p.target;
+    a.shares = p.shares;
     a.least = p.least;
-    a.slots = p.slots;
+    a.piece = p.piece;
     if (need) {
-        const size_t rows = (size_t)p.slots * d->kv_heads * kRows;
+        const size_t rows = (size_t)2 * p.shares * d->kv_heads * kRows;
         a.part_out = (float *)workspace;
         a.part_stat = (float2 *)(a.part_out + rows * p.dim);
-        a.info = (int2 *)(a.part_stat + rows);
+        a.info = (long long *)(a.part_stat + rows);
     }
     hipStream_t s = (hipStream_t)stream;
     with_element(d->type, [&](auto e) {

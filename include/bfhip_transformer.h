@@ -289,7 +289,8 @@ int bfhip_cache_append(const bfhip_paged_desc *desc, const bfhip_rows *k, const 
  * position and what pages hold past a length reach no result, but a NaN or
  * infinity in the value of a token reaches the queries of the same sequence in
  * the same call that stand before it.
- * The workspace holds the sums of split keys (at most 1 GiB). */
+ * The workspace holds sums of keys that are shared out (at most 16 MiB) and eight
+ * bytes per sequence.  tokens * heads / kv_heads at most 2^30. */
 size_t bfhip_paged_attention_workspace(const bfhip_paged_desc *desc);
 
 int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
