@@ -50,6 +50,115 @@ __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a)
     w.store(a, acc, smem, wave, lane);
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 16 MB rows: bound by reading both weights once, so these go from memory to the
+// matrix cores without LDS.  A workgroup has 16 HB hidden elements; its waves take
+// turns along the features, 64 at a time (a line of a 16-bit row), and their sums are
+// added in order at the end.  The lanes of rows that are not there load nothing.
+constexpr int kFewRows = 32, kFewWaves = 8, kFewDeep = 64;
+
+template <class E, int MB, int HB>
+__global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a) {
+    constexpr int kSum = 2 * HB * MB * kWave;
+    __shared__ f32x4 sums[kFewWaves][kSum];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), waves = blockDim.x / kWave;
+    const int l16 = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16 * HB;
+    using Word = typename E::Word;
+    using Frag = typename E::Frag;
+    const Word *w[2][HB], *x[MB];
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+        const long long r = min(n0 + 16 * b + l16, a.n - 1);  // (rows past the last one give results that are not stored)
+        w[0][b] = (const Word *)(a.n_op.gate + r * a.n_op.stride);
+        w[1][b] = (const Word *)(a.n_op.up + r * a.n_op.stride);
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b) x[b] = (const Word *)(a.m_op.gate + (long long)min(16 * b + l16, a.m - 1) * a.m_op.stride);
+    f32x4 acc[2][HB][MB];
+#pragma unroll
+    for (int b = 0; b < HB; ++b)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[0][b][m] = acc[1][b][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto load = [&](const Word *row, int k) {
+        Frag f;
+        __builtin_memcpy(&f, row + k, sizeof f);
+        return f;
+    };
+    const auto multiply = [&](int k, auto fetch) {
+        // Lane group g's k of both products are 16 neighbours: any order will do that
+        // both operands have.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = k + 16 * g + 8 * h;
+            Frag xf[MB];
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                xf[m] = Frag{};
+                if (16 * m + l16 < a.m) xf[m] = fetch(x[m], at);
+            }
+#pragma unroll
+            for (int b = 0; b < HB; ++b) {
+                const Frag gate = fetch(w[0][b], at), up = fetch(w[1][b], at);
+#pragma unroll
+                for (int m = 0; m < MB; ++m) {
+                    acc[0][b][m] = E::mfma(gate, xf[m], acc[0][b][m]);
+                    acc[1][b][m] = E::mfma(up, xf[m], acc[1][b][m]);
+                }
+            }
+        }
+    };
+    int k = wave * kFewDeep;
+#pragma unroll 4
+    for (; k + kFewDeep <= a.k; k += waves * kFewDeep) multiply(k, load);
+    if (k < a.k)
+        multiply(k, [&](const Word *row, int at) {
+            Words<E, 8> f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f.w[e] = at + e < a.k ? row[at + e] : (Word)0.f;
+            return __builtin_bit_cast(Frag, f.w);
+        });
+#pragma unroll
+    for (int b = 0; b < HB; ++b)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sums[wave][((b * MB + m) * 2 + u) * kWave + lane] = acc[u][b][m];
+    __syncthreads();
+    for (int i = threadIdx.x; i < HB * MB * kWave; i += blockDim.x) {
+        const int block = i / kWave, row = 16 * (block % MB) + (i & 15), n = n0 + 16 * (block / MB) + 4 * (i % kWave / 16);
+        if (row >= a.m || n >= a.n) continue;
+        const int at = block * 2 * kWave + i % kWave;
+        f32x4 gate = sums[0][at], up = sums[0][at + kWave];
+        for (int v = 1; v < waves; ++v) {
+            gate += sums[v][at];
+            up += sums[v][at + kWave];
+        }
+        f32x4 h;
+        with_activation(a.activation, [&](auto kind) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = activate<E, decltype(kind)::value>(gate[e]) * up[e];
+        });
+        const auto put = [&](int o, const f32x4 &v) {
+            Word *p = (Word *)(a.out[o] + row * a.out_stride[o]) + n;
+            Words<E, 4> w4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w4.put(e, v[e]);
+            if (n + 4 <= a.n) {
+                w4.store(p);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.n) p[e] = w4.w[e];
+            }
+        };
+        put(0, h);
+        if (a.out[1]) {
+            put(1, gate);
+            put(2, up);
+        }
+    }
+}
+
 // ------------------------------------------------- gradients of the two products
 struct SlopeArgs {
     const char *dh, *gate, *up;
@@ -252,6 +361,21 @@ int gated_launch(GatedArgs a, const GatedPlan &p, bool dma, hipStream_t s) {
     return 1;
 }
 
+// Few rows.  Eight waves a workgroup where workgroups of four would leave CUs idle.
+template <class E>
+int gated_few_launch(const GatedArgs &a, hipStream_t s) {
+    const auto run = [&](auto rows, auto cols) {
+        constexpr int MB = decltype(rows)::value, HB = decltype(cols)::value;
+        const long long grid = ((long long)a.n + 16 * HB - 1) / (16 * HB);
+        if (!launch_fits(grid, kFewWaves * kWave)) return 0;
+        const int waves = grid < 512 ? kFewWaves : 4;
+        hipLaunchKernelGGL((gated_few_kernel<E, MB, HB>), dim3((unsigned)grid), dim3(waves * kWave), 0, s, a);
+        return 1;
+    };
+    if (a.m <= 16) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+    return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+}
+
 // dg and du: rows of whole 16-byte chunks.
 long long slope_stride(const bfhip_gated_desc *d) { return (d->hidden + 7) / 8 * 8; }
 
@@ -286,7 +410,7 @@ GatedOperand operand(const bfhip_matrix *gate, const bfhip_matrix *up, long long
 }  // namespace
 
 extern "C" size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *d) {
-    if (bad_gated(d) || !d->rows) return 0;
+    if (bad_gated(d) || d->rows <= kFewRows) return 0;
     size_t n = 0;
     with_element(d->type, [&](auto e) { n = part_bytes<decltype(e), kForward>(d->rows, d->hidden, d->features); });
     return n;
@@ -325,7 +449,8 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
     int ok = 1;
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
-        ok = gated_launch<E, kForward>(a, gated_plan<E, kForward>(d->rows, d->hidden, d->features, dma), dma, (hipStream_t)stream);
+        if (d->rows <= kFewRows) ok = gated_few_launch<E>(a, (hipStream_t)stream);
+        else ok = gated_launch<E, kForward>(a, gated_plan<E, kForward>(d->rows, d->hidden, d->features, dma), dma, (hipStream_t)stream);
     });
     if (!ok) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
