@@ -266,8 +266,8 @@ TRANSFORMER_SIGNATURES = {
     "bfhip_paged_attention_workspace": (_sz, [_pagedp]),
     "bfhip_paged_attention": (_i, [_pagedp, _rowsp, _pagesp, _pagesp, _rowsp, _vp, _vp, _sz, _vp,
                                    C.c_char_p, _sz]),
-    "bfhip_gated_linear_workspace": (_sz, [_gatedp]),
-    "bfhip_gated_linear_backward_workspace": (_sz, [_gatedp]),
+    "bfhip_gated_linear_workspace": (_sz, [_gatedp] + [_matrixp] * 3),
+    "bfhip_gated_linear_backward_workspace": (_sz, [_gatedp] + [_matrixp] * 3),
     "bfhip_gated_linear": (_i, [_gatedp] + [_matrixp] * 6 + [_vp, _sz, _vp, C.c_char_p, _sz]),
     "bfhip_gated_linear_backward": (_i, [_gatedp] + [_matrixp] * 9 + [_vp, _sz, _vp, C.c_char_p,
                                                                        _sz]),
@@ -913,7 +913,7 @@ def gated_linear(x, w_gate, w_up, activation="silu", out=None, save=False, strea
     with _place(stream, x, w_gate, w_up, out) as queue:
         h = x.new_empty(shape) if out is None else out
         kept = [x.new_empty(shape) for _ in range(2)] if save else [None, None]
-        size = lib.bfhip_gated_linear_workspace(desc)
+        size = lib.bfhip_gated_linear_workspace(desc, *given)
         work, pw = _scratch(size, x)
         err = _err()
         _check(lib.bfhip_gated_linear(
@@ -931,7 +931,7 @@ def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation="silu", stre
     more = [_gated_matrix(n, t, shape, x) for n, t in (("dh", dh), ("gate", gate), ("up", up))]
     with _place(stream, x, dh, w_gate, w_up, gate, up) as queue:
         grads = [t.new_empty(t.shape) for t in (x, w_gate, w_up)]
-        size = lib.bfhip_gated_linear_backward_workspace(desc)
+        size = lib.bfhip_gated_linear_backward_workspace(desc, *given)
         work, pw = _scratch(size, x)
         err = _err()
         _check(lib.bfhip_gated_linear_backward(

@@ -101,15 +101,14 @@ __device__ __forceinline__ void copy16(Resource r, const char *lds, uint32_t vof
                  : "memory", "m0");
 }
 
-// One operand's tile of OUTER (m or n) x BK (k) elements in LDS.  DMA: rows start
-// on 16 bytes and hold whole chunks of 16 bytes.
-template <class E, int OUTER, int BK, int THREADS, bool COL, bool DMA>
+// One operand's tile of OUTER (m or n) x BK (k) elements in LDS, copied in chunks of 16
+// bytes: rows start on 16 bytes and hold whole chunks.
+template <class E, int OUTER, int BK, int THREADS, bool COL>
 struct GatedTile {
     using T = std::conditional_t<COL, AttnTile<E, OUTER>, AttnTile<E, BK>>;
-    static constexpr int kRows = COL ? BK : OUTER, kWords = 16 / E::kSize;
+    static constexpr int kOuter = OUTER, kRows = COL ? BK : OUTER, kWords = 16 / E::kSize;
     static constexpr int kBytes = kRows * T::kRow, kIssue = kRows * T::kChunks / THREADS;
     static_assert(kRows * T::kChunks % THREADS == 0, "whole chunks per thread");
-    typedef uint32_t Chunk __attribute__((ext_vector_type(4)));
 
     // PAIR > 0: outer rows are PAIR / 2 of the gate's, PAIR / 2 of the up's in turn.
     template <int PAIR>
@@ -120,9 +119,8 @@ struct GatedTile {
     // (or of half of it: then every other chunk is at the other half's place).
     static constexpr int kSpan = THREADS / T::kChunks, kPlaces = kSpan % 16 ? 2 : 1;
     static_assert(kSpan % 8 == 0 && THREADS % T::kChunks == 0, "chunks repeat with the swizzle");
-    uint32_t off[kPlaces];  // DMA: bytes of chunk 0 from the tile's first row
+    uint32_t off[kPlaces];    // bytes of chunk 0 from the tile's first row
     int row, first[kPlaces];  // its row in the matrix, and its first element along the row
-    Chunk held[DMA ? 1 : kIssue];
     const char *base_a, *base_b;
     long long stride;
     int wave, left, thread;
@@ -160,42 +158,18 @@ struct GatedTile {
     // Fetches the tile from k0 on, of k elements in all, out of the matrix at `a` (with
     // PAIR, the up's rows out of that at `b`).
     template <int PAIR>
-    __device__ __forceinline__ void fetch(const char *a, const char *b, int k0, int k, char *lds) {
+    __device__ __forceinline__ void fetch(const char *a, const char *b, int k0, int k, const char *lds) const {
         const long long at = COL ? k0 * stride : (long long)k0 * E::kSize;
         const int rows = COL ? k - k0 : left, length = COL ? left : k - k0;  // what there is of the tile
-        if constexpr (DMA) {
-            const Resource ra = resource(a + at), rb = resource(b + at);
+        const Resource ra = resource(a + at), rb = resource(b + at);
 #pragma unroll
-            for (int j = 0; j < kIssue; ++j) {
-                const bool in = row + span_row<PAIR>(j) < rows && first[j % kPlaces] < length;
-                copy16(second<PAIR>(j) ? rb : ra, lds + (j * THREADS + wave * kWave) * 16,
-                       in ? off[j % kPlaces] + (uint32_t)span_row<PAIR>(j) * (uint32_t)stride : kDmaOutOfRange);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < kIssue; ++j) {
-                const int r = row + span_row<PAIR>(j), n = r < rows ? length - first[j % kPlaces] : 0;
-                const char *p = (second<PAIR>(j) ? b : a) + at + r * stride + first[j % kPlaces] * E::kSize;
-                Chunk v = {0, 0, 0, 0};
-                if (n >= kWords) {
-                    __builtin_memcpy(&v, p, 16);
-                } else if (n > 0) {
-                    typedef typename E::Word Row __attribute__((ext_vector_type(kWords)));
-                    Row w = __builtin_bit_cast(Row, v);
-#pragma unroll
-                    for (int e = 0; e < kWords; ++e)
-                        if (e < n) w[e] = ((const typename E::Word *)p)[e];
-                    v = __builtin_bit_cast(Chunk, w);
-                }
-                held[j] = v;
-            }
+        for (int j = 0; j < kIssue; ++j) {
+            const bool in = row + span_row<PAIR>(j) < rows && first[j % kPlaces] < length;
+            copy16(second<PAIR>(j) ? rb : ra, lds + (j * THREADS + wave * kWave) * 16,
+                   in ? off[j % kPlaces] + (uint32_t)span_row<PAIR>(j) * (uint32_t)stride : kDmaOutOfRange);
         }
     }
-    __device__ __forceinline__ void put(char *lds) const {
-        if constexpr (!DMA)
-#pragma unroll
-            for (int j = 0; j < kIssue; ++j) *reinterpret_cast<Chunk *>(lds + (j * THREADS + thread) * 16) = held[j];
-    }
+
     // Where in the tile the lane reads the fragments of the outer elements from o0
     // on (a multiple of 64).
     __device__ __forceinline__ static uint32_t lane_at(int o0, int lane) {
@@ -243,13 +217,12 @@ struct GatedTile {
 };
 
 // BM x BN results by WM x WN waves, BK of the contraction at a time.
-template <class E, Form F, int BM_, int BN_, int WM_, int WN_, bool DMA_, int BK_ = 128 / E::kSize>
+template <class E, Form F, int BM_, int BN_, int WM_, int WN_>
 struct GatedShape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = BK_;
-    static constexpr bool DMA = DMA_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = 128 / E::kSize;
     static constexpr int kThreads = WM * WN * kWave, kM = BM / WM, kN = BN / WN, kMB = kM / 16, kNB = kN / 16;
-    using MTile = GatedTile<E, BM, BK, kThreads, F == kWeights, DMA>;
-    using NTile = GatedTile<E, BN, BK, kThreads, F != kForward, DMA>;
+    using MTile = GatedTile<E, BM, BK, kThreads, F == kWeights>;
+    using NTile = GatedTile<E, BN, BK, kThreads, F != kForward>;
     static constexpr int kPair = F == kForward ? kN : 0;  // gate and up columns of a wave
     static constexpr int kCols = F == kForward ? BN / 2 : BN;
     static constexpr int kStage = MTile::kBytes + NTile::kBytes;
@@ -369,15 +342,12 @@ struct GatedWork {
         begin = split < 0 ? 0 : split % a.parts * a.per;
         end = split < 0 ? steps : min(steps, begin + a.per);
     }
-    __device__ __forceinline__ void fetch(int t, char *to) {
+    // Past the last step the tiles are empty: zeros, without a read.
+    __device__ __forceinline__ void fetch(int t, const char *to) const {
         const bool second = F == kInputs && t >= each;
-        const int k0 = (second ? t - each : t) * S::BK;
+        const int k0 = t < end ? (second ? t - each : t) * S::BK : k;
         mt.template fetch<0>(second ? mt.base_b : mt.base_a, mt.base_b, k0, k, to);
         nt.template fetch<S::kPair>(second ? nt.base_b : nt.base_a, nt.base_b, k0, k, to + S::MTile::kBytes);
-    }
-    __device__ __forceinline__ void put(char *to) const {
-        mt.put(to);
-        nt.put(to + S::MTile::kBytes);
     }
     // Hands the accumulators to the results, by way of `smem`, or to the parts' sums.
     // No copy into LDS may be in flight and no wave may still read its tiles.
@@ -435,7 +405,7 @@ __global__ __launch_bounds__(S::kThreads) void gated_join_kernel(GatedArgs a) {
 
 // A product by large tiles (gated_large.hip).
 template <class E, Form F>
-using LargeShape = GatedShape<E, F, 256, 256, 2, 2, true>;
+using LargeShape = GatedShape<E, F, 256, 256, 2, 2>;
 template <class E, Form F>
 __attribute__((visibility("hidden"))) void launch_gated_large(const GatedArgs &a, long long grid, hipStream_t s);
 

@@ -10,11 +10,17 @@ using namespace bfhip;
 
 namespace {
 
-// Small tiles: two workgroups share a CU and cover each other's waits.
+// Small tiles, where there are too few large ones: four stages in LDS, three of them in
+// flight while one is multiplied.
+constexpr int kStages = 4;
+
 template <class E, Form F, class S>
 __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a) {
-    __shared__ __attribute__((aligned(512))) char smem[gated_lds<E, F, S>(2 * S::kStage)];
+    static_assert((kStages & (kStages - 1)) == 0, "stages by a mask");
+    constexpr int kCopies = S::MTile::kIssue + S::NTile::kIssue;
+    __shared__ __attribute__((aligned(512))) char smem[gated_lds<E, F, S>(kStages * S::kStage)];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const auto stage = [&](int t) { return smem + (t & (kStages - 1)) * S::kStage; };
     GatedWork<E, F, S> w;
     w.init(a, wave, lane);
     f32x4 acc[S::kMB][S::kNB];
@@ -22,16 +28,13 @@ __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a)
     for (int j = 0; j < S::kMB; ++j)
 #pragma unroll
         for (int i = 0; i < S::kNB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (w.begin < w.end) {
-        w.fetch(w.begin, smem + (w.begin & 1) * S::kStage);
-        w.put(smem + (w.begin & 1) * S::kStage);
-    }
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) w.fetch(w.begin + s, stage(w.begin + s));
     for (int t = w.begin; t < w.end; ++t) {
-        if constexpr (S::DMA) wait_vmcnt<0>();
+        wait_vmcnt<(kStages - 2) * kCopies>();
         lds_barrier();  // this tile is there, and the one before has been read
-        char *const next = smem + (~t & 1) * S::kStage;
-        if (t + 1 < w.end) w.fetch(t + 1, next);
-        const char *const ml = smem + (t & 1) * S::kStage, *const nl = ml + S::MTile::kBytes;
+        w.fetch(t + kStages - 1, stage(t + kStages - 1));
+        const char *const ml = stage(t), *const nl = ml + S::MTile::kBytes;
 #pragma unroll
         for (int kk = 0; kk < S::BK / 32; ++kk) {
             typename E::Frag nf[S::kNB], mf[S::kMB];
@@ -44,9 +47,9 @@ __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a)
 #pragma unroll
                 for (int j = 0; j < S::kMB; ++j) acc[j][i] = E::mfma(nf[i], mf[j], acc[j][i]);
         }
-        if (t + 1 < w.end) w.put(next);
     }
-    lds_barrier();  // the last tile has been read
+    wait_vmcnt<0>();
+    lds_barrier();  // no copy and no read of a tile is left
     w.store(a, acc, smem, wave, lane);
 }
 
@@ -159,6 +162,56 @@ __global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a
     }
 }
 
+// -------------------------------------------------------------------- alignment
+constexpr int kChunkThreads = 256;
+
+// Threads walk the chunks of eight elements in the rows' order (`per` a row):
+// f(chunk, row, first element).
+template <class G>
+__device__ __forceinline__ void each_chunk(long long rows, int per, G f) {
+    const long long step = (long long)gridDim.x * kChunkThreads, first = (long long)blockIdx.x * kChunkThreads + threadIdx.x;
+    const long long step_r = step / per;
+    const int step_c = (int)(step % per);
+    long long r = first / per;
+    int c = (int)(first % per);
+    for (long long i = first; r < rows; i += step) {
+        f(i, r, 8 * c);
+        r += step_r;
+        c += step_c;
+        if (c >= per) {
+            c -= per;
+            ++r;
+        }
+    }
+}
+
+// Rows of any alignment into rows of whole chunks, their ends filled with zeros.
+struct PadArgs {
+    const char *from[3];
+    char *to[3];
+    long long stride[3];  // bytes
+    long long rows[3];
+    int length;
+};
+
+template <class E>
+__global__ __launch_bounds__(kChunkThreads) void gated_pad_kernel(PadArgs a) {
+    using Word = typename E::Word;
+    const int i = blockIdx.y, per = (a.length + 7) / 8;
+    if (!a.from[i]) return;
+    each_chunk(a.rows[i], per, [&](long long chunk, long long r, int c) {
+        const Word *row = (const Word *)(a.from[i] + r * a.stride[i]) + c;
+        Words<E, 8> v;
+        if (c + 8 <= a.length) {
+            v = Words<E, 8>::load(row);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.w[e] = c + e < a.length ? row[e] : (Word)0.f;
+        }
+        v.store((Word *)a.to[i] + chunk * 8);
+    });
+}
+
 // ------------------------------------------------- gradients of the two products
 struct SlopeArgs {
     const char *dh, *gate, *up;
@@ -171,7 +224,7 @@ struct SlopeArgs {
     int *shift;
 };
 
-constexpr int kSlopeThreads = 256, kMostGroups = 1024;
+constexpr int kMostGroups = 1024;
 
 // dg and du of eight neighbouring elements; those past the row's end are zero.
 template <class E, int kActivation>
@@ -201,30 +254,10 @@ __device__ __forceinline__ void slope8(const SlopeArgs &a, long long r, int c, f
     }
 }
 
-// Threads walk the chunks of eight elements in the rows' order (`per` a row):
-// f(chunk, row, first element).
-template <class G>
-__device__ __forceinline__ void each_chunk(long long rows, int per, G f) {
-    const long long step = (long long)gridDim.x * kSlopeThreads, first = (long long)blockIdx.x * kSlopeThreads + threadIdx.x;
-    const long long step_r = step / per;
-    const int step_c = (int)(step % per);
-    long long r = first / per;
-    int c = (int)(first % per);
-    for (long long i = first; r < rows; i += step) {
-        f(i, r, 8 * c);
-        r += step_r;
-        c += step_c;
-        if (c >= per) {
-            c -= per;
-            ++r;
-        }
-    }
-}
-
 // Largest finite |dg| and |du| of a workgroup's share.
 template <int kActivation>
-__global__ __launch_bounds__(kSlopeThreads) void gated_most_kernel(SlopeArgs a) {
-    __shared__ float part[kSlopeThreads / kWave];
+__global__ __launch_bounds__(kChunkThreads) void gated_most_kernel(SlopeArgs a) {
+    __shared__ float part[kChunkThreads / kWave];
     float most = 0.f;
     each_chunk(a.rows, (a.hidden + 7) / 8, [&](long long, long long r, int c) {
         float dg[8], du[8];
@@ -239,7 +272,7 @@ __global__ __launch_bounds__(kSlopeThreads) void gated_most_kernel(SlopeArgs a) 
     if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = most;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kSlopeThreads / kWave; ++w) most = fmaxf(most, part[w]);
+        for (int w = 1; w < kChunkThreads / kWave; ++w) most = fmaxf(most, part[w]);
         a.most[blockIdx.x] = most;
     }
 }
@@ -247,17 +280,17 @@ __global__ __launch_bounds__(kSlopeThreads) void gated_most_kernel(SlopeArgs a) 
 // dg and du, rounded to the type; fp16's times a power of two that takes the
 // largest of them to 2^14 or just above.
 template <class E, int kActivation>
-__global__ __launch_bounds__(kSlopeThreads) void gated_slope_kernel(SlopeArgs a, int groups) {
+__global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a, int groups) {
     int shift = 0;
     if constexpr (std::is_same_v<E, ElemF16>) {
-        __shared__ float part[kSlopeThreads / kWave];
+        __shared__ float part[kChunkThreads / kWave];
         float most = 0.f;
-        for (int i = threadIdx.x; i < groups; i += kSlopeThreads) most = fmaxf(most, a.most[i]);
+        for (int i = threadIdx.x; i < groups; i += kChunkThreads) most = fmaxf(most, a.most[i]);
         most = group_max<kWave>(most);
         if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = most;
         __syncthreads();
         most = part[0];
-        for (int w = 1; w < kSlopeThreads / kWave; ++w) most = fmaxf(most, part[w]);
+        for (int w = 1; w < kChunkThreads / kWave; ++w) most = fmaxf(most, part[w]);
         if (most > 0.f) shift = 14 - ilogbf(most);
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.shift = shift;
     }
@@ -279,9 +312,10 @@ __global__ __launch_bounds__(kSlopeThreads) void gated_slope_kernel(SlopeArgs a,
 constexpr long long kPartBytes = 256ll << 20;
 
 bool bad_gated(const bfhip_gated_desc *d) {
-    const long long most = 0x7fffffff, elements = 1ll << 40;
+    // (tiles past the last row are counted in an int, and a tile's rows in 32-bit offsets)
+    const long long most_rows = 0x7fff0000, most = 1 << 20, elements = 1ll << 40;
     return !d || d->type < BFHIP_F32 || d->type > BFHIP_BF16 || d->activation < BFHIP_SILU || d->activation > BFHIP_RELU ||
-           d->rows < 0 || d->rows > most || d->features < 1 || d->features > most || d->hidden < 1 || d->hidden > most ||
+           d->rows < 0 || d->rows > most_rows || d->features < 1 || d->features > most || d->hidden < 1 || d->hidden > most ||
            d->rows * d->features > elements || d->rows * d->hidden > elements || d->features * d->hidden > elements;
 }
 
@@ -290,57 +324,65 @@ bool bad_matrix(const bfhip_matrix *x, long long rows, long long length) {
     return !x || (rows && !x->data) || (rows > 1 && (x->stride < length || x->stride > 1ll << 40));
 }
 
+// Whether a matrix can be copied to LDS in chunks of 16 bytes.
+bool chunked(const bfhip_matrix *x, long long rows, long long length, int size) {
+    const long long words = 16 / size;
+    return ((uintptr_t)x->data & 15) == 0 && length % words == 0 && (rows <= 1 || (x->stride % words == 0 && x->stride < 1 << 21));
+}
+
 struct GatedPlan {
     bool large;
     int tiles_m, tiles_n, whole, parts, per;
     size_t bytes;  // of the parts' sums
+    double time;   // an estimate, in us
 };
 
-// Whether a matrix can be copied to LDS in chunks of 16 bytes.
-bool chunks(const bfhip_matrix *x, long long rows, long long length, int size) {
-    const long long words = 16 / size;
-    return ((uintptr_t)x->data & 15) == 0 && length % words == 0 && (rows <= 1 || x->stride % words == 0) &&
-           (rows <= 1 || x->stride < 1 << 21);
-}
-
-// Tiles, dealt in rounds of as many as the chip holds at once.  Those of the last
-// round are split along the contraction, in parts of eight steps or more, where
-// that fills it better.
+// Tiles, dealt in rounds of one per CU.  Those of the last round are split along the
+// contraction, in parts of four steps or more, where that fills it better.  A step
+// takes `step` us.
 template <class S>
-void plan_tiles(GatedPlan &p, Form f, long long m, long long n, long long k, int round) {
+GatedPlan plan_tiles(Form f, long long m, long long n, long long k, double step) {
+    constexpr int kRound = 256;
+    GatedPlan p{};
     p.tiles_m = (int)((m + S::BM - 1) / S::BM * (f == kWeights ? 2 : 1));
     p.tiles_n = (int)((n + S::kCols - 1) / S::kCols);
     const long long steps = (k + S::BK - 1) / S::BK * (f == kInputs ? 2 : 1), tiles = (long long)p.tiles_m * p.tiles_n;
-    const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % round;
+    const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % kRound;
     p.whole = (int)std::min(tiles, 0x7fffffffll);
     p.parts = 1;
-    if (!rest) return;
-    const long long parts = std::min({round / rest, steps / 8, kPartBytes / (rest * tile_bytes)});
-    if (parts < 2) return;
+    p.time = (double)((tiles + kRound - 1) / kRound) * (steps * step + 5);
+    if (!rest) return p;
+    const long long parts = std::min({kRound / rest, steps / 4, kPartBytes / (rest * tile_bytes)});
+    if (parts < 2) return p;
     p.per = (int)((steps + parts - 1) / parts);
+    const double split = (double)(tiles / kRound) * (steps * step + 5) + p.per * step + 10 + (double)(parts * rest * tile_bytes) / 2.4e6;
+    if (split > p.time) return p;
+    p.time = split;
     p.parts = (int)((steps + p.per - 1) / p.per);
     p.whole = (int)(tiles - rest);
     p.bytes = (size_t)(p.parts * rest * tile_bytes);
-}
-
-// The shapes: large tiles, one per CU, where there are enough of them to fill the
-// chip, and only for matrices that are copied in whole chunks; small ones, two
-// per CU.
-template <class E, Form F, bool DMA>
-using SmallShape = GatedShape<E, F, 128, 128, 2, E::kSize == 4 ? 4 : 2, DMA>;
-
-template <class E, Form F>
-GatedPlan gated_plan(long long m, long long n, long long k, bool dma) {
-    GatedPlan p{};
-    const long long cols = F == kForward ? 128 : 256;
-    p.large = dma && E::kSize == 2 && (m + 255) / 256 * ((n + cols - 1) / cols) * (F == kWeights ? 2 : 1) >= 192;
-    if (p.large) plan_tiles<LargeShape<ElemBf16, F>>(p, F, m, n, k, 256);
-    else plan_tiles<SmallShape<E, F, true>>(p, F, m, n, k, 512);
     return p;
 }
 
 template <class E, Form F>
-int gated_launch(GatedArgs a, const GatedPlan &p, bool dma, hipStream_t s) {
+using SmallShape = GatedShape<E, F, 128, 128, 2, E::kSize == 4 ? 4 : 2>;
+
+// Large tiles or small ones, whichever are estimated to take less time.  A step of
+// 64 of a large tile takes 1.1 us, of a small one 0.45 (fp32: of 32, 1.7).
+template <class E, Form F>
+GatedPlan gated_plan(long long m, long long n, long long k) {
+    GatedPlan p = plan_tiles<SmallShape<E, F>>(F, m, n, k, E::kSize == 4 ? 1.7 : 0.45);
+    if constexpr (E::kSize == 2) {
+        GatedPlan l = plan_tiles<LargeShape<E, F>>(F, m, n, k, 1.1);
+        l.large = true;
+        if (l.time < p.time) return l;
+    }
+    return p;
+}
+
+template <class E, Form F>
+int gated_launch(GatedArgs a, hipStream_t s) {
+    const GatedPlan p = gated_plan<E, F>(a.m, a.n, a.k);
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
     a.whole = p.whole;
@@ -354,9 +396,8 @@ int gated_launch(GatedArgs a, const GatedPlan &p, bool dma, hipStream_t s) {
             return 1;
         }
     }
-    using S = SmallShape<E, F, true>;
-    if (dma) hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
-    else hipLaunchKernelGGL((gated_product_kernel<E, F, SmallShape<E, F, false>>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
+    using S = SmallShape<E, F>;
+    hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
     if (split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(split * S::kMB)), dim3(S::kThreads), 0, s, a);
     return 1;
 }
@@ -381,15 +422,45 @@ long long slope_stride(const bfhip_gated_desc *d) { return (d->hidden + 7) / 8 *
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Bytes of a product's parts, whichever way its matrices are copied.
-template <class E, Form F>
-size_t part_bytes(long long m, long long n, long long k) {
-    return std::max(gated_plan<E, F>(m, n, k, true).bytes, gated_plan<E, F>(m, n, k, false).bytes);
-}
+// Where x and the weights lie for the products: as they are, or in the workspace in
+// rows of whole chunks.
+struct Aligned {
+    bfhip_matrix x, gate, up;
+    size_t bytes;
+    PadArgs pad;
+
+    Aligned(const bfhip_gated_desc *d, const bfhip_matrix *x_, const bfhip_matrix *gate_, const bfhip_matrix *up_, char *work)
+        : x(*x_), gate(*gate_), up(*up_), bytes(0), pad{} {
+        const int size = d->type == BFHIP_F32 ? 4 : 2;
+        const long long length = (d->features + 7) / 8 * 8;
+        pad.length = (int)d->features;
+        int i = 0;
+        const auto move = [&](bfhip_matrix &m, long long rows) {
+            pad.from[i] = (const char *)m.data;
+            pad.to[i] = work + bytes;
+            pad.stride[i] = rows > 1 ? m.stride * size : 0;
+            pad.rows[i++] = rows;
+            m = bfhip_matrix{work + bytes, length};
+            bytes += up256((size_t)rows * length * size);
+        };
+        if (!chunked(x_, d->rows, d->features, size)) move(x, d->rows);
+        if (!chunked(gate_, d->hidden, d->features, size) || !chunked(up_, d->hidden, d->features, size)) {
+            move(gate, d->hidden);  // (both: they have one stride)
+            move(up, d->hidden);
+        }
+    }
+    template <class E>
+    void launch(hipStream_t s) const {
+        if (!bytes) return;
+        const long long most = std::max({pad.rows[0], pad.rows[1], pad.rows[2]}) * ((pad.length + 7) / 8);
+        const unsigned grid = (unsigned)std::min<long long>(4096, (most + kChunkThreads - 1) / kChunkThreads);
+        if (grid) hipLaunchKernelGGL(gated_pad_kernel<E>, dim3(grid, 3), dim3(kChunkThreads), 0, s, pad);
+    }
+};
 
 struct BackwardBytes {
     size_t slopes, parts;  // of each of dg and du, and of the larger of the products' parts
-    size_t all() const { return 2 * slopes + parts + (kMostGroups + 64) * sizeof(float); }
+    size_t all() const { return 2 * slopes + parts + up256((kMostGroups + 64) * sizeof(float)); }
 };
 
 BackwardBytes backward_bytes(const bfhip_gated_desc *d) {
@@ -397,10 +468,21 @@ BackwardBytes backward_bytes(const bfhip_gated_desc *d) {
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
         b.slopes = up256((size_t)d->rows * slope_stride(d) * E::kSize);
-        b.parts = up256(std::max(part_bytes<E, kInputs>(d->rows, d->features, d->hidden),
-                                 part_bytes<E, kWeights>(d->hidden, d->features, d->rows)));
+        b.parts = up256(std::max(gated_plan<E, kInputs>(d->rows, d->features, d->hidden).bytes,
+                                 gated_plan<E, kWeights>(d->hidden, d->features, d->rows).bytes));
     });
     return b;
+}
+
+size_t forward_parts(const bfhip_gated_desc *d) {
+    size_t n = 0;
+    with_element(d->type, [&](auto e) { n = gated_plan<decltype(e), kForward>(d->rows, d->hidden, d->features).bytes; });
+    return up256(n);
+}
+
+bool bad_inputs(const bfhip_gated_desc *d, const bfhip_matrix *x, const bfhip_matrix *w_gate, const bfhip_matrix *w_up) {
+    return bad_matrix(x, d->rows, d->features) || bad_matrix(w_gate, d->hidden, d->features) ||
+           bad_matrix(w_up, d->hidden, d->features) || (d->hidden > 1 && w_gate->stride != w_up->stride);
 }
 
 GatedOperand operand(const bfhip_matrix *gate, const bfhip_matrix *up, long long rows, int size) {
@@ -409,11 +491,10 @@ GatedOperand operand(const bfhip_matrix *gate, const bfhip_matrix *up, long long
 
 }  // namespace
 
-extern "C" size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *d) {
-    if (bad_gated(d) || d->rows <= kFewRows) return 0;
-    size_t n = 0;
-    with_element(d->type, [&](auto e) { n = part_bytes<decltype(e), kForward>(d->rows, d->hidden, d->features); });
-    return n;
+extern "C" size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *d, const bfhip_matrix *x, const bfhip_matrix *w_gate,
+                                               const bfhip_matrix *w_up) {
+    if (bad_gated(d) || bad_inputs(d, x, w_gate, w_up) || d->rows <= kFewRows) return 0;
+    return Aligned(d, x, w_gate, w_up, nullptr).bytes + forward_parts(d);
 }
 
 extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix *x, const bfhip_matrix *w_gate,
@@ -421,19 +502,19 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
                                   const bfhip_matrix *up, void *workspace, size_t workspace_bytes, void *stream, char *error,
                                   size_t cap) {
     if (bad_gated(d) || !gate != !up) return fail(error, cap, "invalid gated linear contract");
-    if (bad_matrix(x, d->rows, d->features) || bad_matrix(w_gate, d->hidden, d->features) ||
-        bad_matrix(w_up, d->hidden, d->features) || bad_matrix(h, d->rows, d->hidden) ||
+    if (bad_inputs(d, x, w_gate, w_up) || bad_matrix(h, d->rows, d->hidden) ||
         (gate && (bad_matrix(gate, d->rows, d->hidden) || bad_matrix(up, d->rows, d->hidden))))
-        return fail(error, cap, "invalid gated linear matrices: strides of at least a row");
-    if (d->hidden > 1 && w_gate->stride != w_up->stride) return fail(error, cap, "invalid gated linear matrices: the weights need one stride");
+        return fail(error, cap, "invalid gated linear matrices: strides of at least a row, one stride for both weights");
     if (!d->rows) return 1;
-    const size_t need = bfhip_gated_linear_workspace(d);
+    const size_t need = bfhip_gated_linear_workspace(d, x, w_gate, w_up);
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
     const int size = d->type == BFHIP_F32 ? 4 : 2;
+    const bool few = d->rows <= kFewRows;
+    const Aligned in(d, x, w_gate, w_up, (char *)workspace);
     GatedArgs a{};
-    a.m_op = operand(x, x, d->rows, size);
-    a.n_op = operand(w_gate, w_up, d->hidden, size);
+    a.m_op = few ? operand(x, x, d->rows, size) : operand(&in.x, &in.x, d->rows, size);
+    a.n_op = few ? operand(w_gate, w_up, d->hidden, size) : operand(&in.gate, &in.up, d->hidden, size);
     a.m = (int)d->rows;
     a.n = (int)d->hidden;
     a.k = (int)d->features;
@@ -443,22 +524,26 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
         a.out_stride[i] = d->rows > 1 ? out[i]->stride * size : 0;
     }
     a.activation = d->activation;
-    a.partial = (float *)workspace;
-    const bool dma = chunks(x, d->rows, d->features, size) && chunks(w_gate, d->hidden, d->features, size) &&
-                     chunks(w_up, d->hidden, d->features, size);
+    a.partial = (float *)((char *)workspace + in.bytes);
+    hipStream_t s = (hipStream_t)stream;
     int ok = 1;
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
-        if (d->rows <= kFewRows) ok = gated_few_launch<E>(a, (hipStream_t)stream);
-        else ok = gated_launch<E, kForward>(a, gated_plan<E, kForward>(d->rows, d->hidden, d->features, dma), dma, (hipStream_t)stream);
+        if (few) {
+            ok = gated_few_launch<E>(a, s);
+            return;
+        }
+        in.launch<E>(s);
+        ok = gated_launch<E, kForward>(a, s);
     });
     if (!ok) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
 }
 
-extern "C" size_t bfhip_gated_linear_backward_workspace(const bfhip_gated_desc *d) {
-    if (bad_gated(d)) return 0;
-    return backward_bytes(d).all();
+extern "C" size_t bfhip_gated_linear_backward_workspace(const bfhip_gated_desc *d, const bfhip_matrix *x,
+                                                        const bfhip_matrix *w_gate, const bfhip_matrix *w_up) {
+    if (bad_gated(d) || bad_inputs(d, x, w_gate, w_up)) return 0;
+    return Aligned(d, x, w_gate, w_up, nullptr).bytes + backward_bytes(d).all();
 }
 
 extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhip_matrix *dh, const bfhip_matrix *x,
@@ -467,19 +552,18 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
                                            const bfhip_matrix *dw_up, void *workspace, size_t workspace_bytes, void *stream,
                                            char *error, size_t cap) {
     if (bad_gated(d) || !dw_gate != !dw_up || (!dx && !dw_gate)) return fail(error, cap, "invalid gated linear contract");
-    if (bad_matrix(dh, d->rows, d->hidden) || bad_matrix(gate, d->rows, d->hidden) || bad_matrix(up, d->rows, d->hidden) ||
-        bad_matrix(x, d->rows, d->features) || bad_matrix(w_gate, d->hidden, d->features) || bad_matrix(w_up, d->hidden, d->features) ||
-        (dx && bad_matrix(dx, d->rows, d->features)) ||
+    if (bad_inputs(d, x, w_gate, w_up) || bad_matrix(dh, d->rows, d->hidden) || bad_matrix(gate, d->rows, d->hidden) ||
+        bad_matrix(up, d->rows, d->hidden) || (dx && bad_matrix(dx, d->rows, d->features)) ||
         (dw_gate && (bad_matrix(dw_gate, d->hidden, d->features) || bad_matrix(dw_up, d->hidden, d->features))))
-        return fail(error, cap, "invalid gated linear matrices: strides of at least a row");
-    if (d->hidden > 1 && w_gate->stride != w_up->stride) return fail(error, cap, "invalid gated linear matrices: the weights need one stride");
+        return fail(error, cap, "invalid gated linear matrices: strides of at least a row, one stride for both weights");
     if (!d->rows && !dw_gate) return 1;
-    const BackwardBytes p = backward_bytes(d);
-    const size_t need = p.all();
+    const size_t need = bfhip_gated_linear_backward_workspace(d, x, w_gate, w_up);
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
         return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
     const int size = d->type == BFHIP_F32 ? 4 : 2;
+    const BackwardBytes p = backward_bytes(d);
     char *work = (char *)workspace;
+    const Aligned in(d, x, w_gate, w_up, work + p.all());
     const long long stride = slope_stride(d);
     SlopeArgs e{};
     const auto step = [&](const bfhip_matrix *t, long long rows) { return rows > 1 ? t->stride * size : 0; };
@@ -493,38 +577,37 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     e.hidden = (int)d->hidden;
     e.most = (float *)(work + 2 * p.slopes + p.parts);
     e.shift = (int *)(e.most + kMostGroups);
-    const long long groups = std::min<long long>(kMostGroups, (d->rows * (stride / 8) + kSlopeThreads - 1) / kSlopeThreads);
-    const long long grid = std::min<long long>(8192, (d->rows * (stride / 8) + kSlopeThreads - 1) / kSlopeThreads);
+    const long long groups = std::min<long long>(kMostGroups, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
+    const long long grid = std::min<long long>(8192, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
     const bfhip_matrix slopes_g{e.dg, stride}, slopes_u{e.du, stride};
     hipStream_t s = (hipStream_t)stream;
     int ok = 1;
     with_element(d->type, [&](auto el) {
         using E = decltype(el);
         if (d->rows) {
+            in.launch<E>(s);
             with_activation(d->activation, [&](auto kind) {
                 constexpr int A = decltype(kind)::value;
-                if (d->type == BFHIP_F16) hipLaunchKernelGGL(gated_most_kernel<A>, dim3((unsigned)groups), dim3(kSlopeThreads), 0, s, e);
-                hipLaunchKernelGGL((gated_slope_kernel<E, A>), dim3((unsigned)grid), dim3(kSlopeThreads), 0, s, e, (int)groups);
+                if (d->type == BFHIP_F16) hipLaunchKernelGGL(gated_most_kernel<A>, dim3((unsigned)groups), dim3(kChunkThreads), 0, s, e);
+                hipLaunchKernelGGL((gated_slope_kernel<E, A>), dim3((unsigned)grid), dim3(kChunkThreads), 0, s, e, (int)groups);
             });
         }
         GatedArgs a{};
         a.activation = d->activation;
         a.shift = d->type == BFHIP_F16 && d->rows ? e.shift : nullptr;
         a.partial = (float *)(work + 2 * p.slopes);
+        a.m_op = operand(&slopes_g, &slopes_u, 2, size);
         if (dx && d->rows) {
-            a.m_op = operand(&slopes_g, &slopes_u, 2, size);
-            a.n_op = operand(w_gate, w_up, d->hidden, size);
+            a.n_op = operand(&in.gate, &in.up, d->hidden, size);
             a.m = (int)d->rows;
             a.n = (int)d->features;
             a.k = (int)d->hidden;
             a.out[0] = (char *)dx->data;
             a.out_stride[0] = step(dx, d->rows);
-            const bool dma = stride < 1 << 21 && chunks(w_gate, d->hidden, d->features, size) && chunks(w_up, d->hidden, d->features, size);
-            ok = gated_launch<E, kInputs>(a, gated_plan<E, kInputs>(a.m, a.n, a.k, dma), dma, s) && ok;
+            ok = gated_launch<E, kInputs>(a, s) && ok;
         }
         if (dw_gate) {
-            a.m_op = operand(&slopes_g, &slopes_u, 2, size);
-            a.n_op = operand(x, x, d->rows, size);
+            a.n_op = operand(&in.x, &in.x, d->rows, size);
             a.m = (int)d->hidden;
             a.n = (int)d->features;
             a.k = (int)d->rows;
@@ -532,8 +615,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             a.out[1] = (char *)dw_up->data;
             a.out_stride[0] = step(dw_gate, d->hidden);
             a.out_stride[1] = step(dw_up, d->hidden);
-            const bool dma = stride < 1 << 21 && chunks(x, d->rows, d->features, size);
-            ok = gated_launch<E, kWeights>(a, gated_plan<E, kWeights>(a.m, a.n, a.k, dma), dma, s) && ok;
+            ok = gated_launch<E, kWeights>(a, s) && ok;
         }
     });
     if (!ok) return fail(error, cap, "gated linear has too many rows");

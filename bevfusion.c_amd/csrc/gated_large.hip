@@ -33,9 +33,9 @@ struct GatedStream {
         const long long at = there ? (COL ? k0 * tile.stride : (long long)k0 * E::kSize) : 0;
         int size = 0;
         if (rest > 0) {
-            // To the end of the last row that there is.
-            if (COL) size = (min(rest, BK) - 1) * (int)tile.stride + tile.left * E::kSize;
-            else size = (tile.left - 1) * (int)tile.stride + rest * E::kSize;
+            // To the end of the last row that there is, in whole chunks.
+            const int length = ((COL ? tile.left : rest) + Tile::kWords - 1) / Tile::kWords * 16;
+            size = (min(COL ? rest : tile.left, COL ? BK : Tile::kOuter) - 1) * (int)tile.stride + length;
         }
         a = resource(base_a + at);
         a[2] = (uint32_t)__builtin_amdgcn_readfirstlane(size);
@@ -64,7 +64,7 @@ template <class E, Form F, class S>
 struct LargeLoop {
     using Frag = typename E::Frag;
     static constexpr int kN = S::kNB, kM = S::kMB, kTile = S::MTile::kBytes, kCopy = S::kThreads * 16;
-    static_assert(S::DMA && S::WM * S::WN == 4 && S::BK == 64 && kN == 8 && kM == 8 && S::MTile::kIssue == 8 && S::NTile::kIssue == 8 &&
+    static_assert(S::WM * S::WN == 4 && S::BK == 64 && kN == 8 && kM == 8 && S::MTile::kIssue == 8 && S::NTile::kIssue == 8 &&
                       kTile == S::NTile::kBytes,
                   "a copy and two reads per block of products");
     GatedWork<E, F, S> w;

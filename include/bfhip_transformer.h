@@ -316,9 +316,11 @@ int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
  *
  * Matrices: row r at element r * <name>.stride (at least the row's length, of no
  * account where there is at most one row), the elements of a row contiguous.
- * Any alignment will do; pointers and strides on 16 bytes, and rows of whole 16
- * bytes, are faster.  Wg and Wu have one stride.  Results overlap nothing.  Sizes 0 .. 2^31 - 1 each, features and hidden at least 1, no
- * matrix of more than 2^40 elements.  The workspace holds dg and du and, where
+ * Any alignment will do; x and weights whose pointers, strides and rows are
+ * multiples of 16 bytes (and strides below 2 Mi elements) need no copy.  Wg and Wu
+ * have one stride.  Results overlap nothing.  rows at most 0x7fff0000, features and
+ * hidden 1 .. 2^20, no matrix of more than 2^40 elements.  The workspace holds dg and du, copies of x
+ * and the weights where they need them (more than 32 rows, or backward), and, where
  * results are few beside the sums' lengths, parts of sums (at most 256 MiB). */
 enum { BFHIP_SILU = 0, BFHIP_GELU = 1, BFHIP_RELU = 2 };
 
@@ -335,8 +337,10 @@ typedef struct {
     long long hidden;
 } bfhip_gated_desc;
 
-size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *desc);
-size_t bfhip_gated_linear_backward_workspace(const bfhip_gated_desc *desc);
+size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *desc, const bfhip_matrix *x,
+                                    const bfhip_matrix *w_gate, const bfhip_matrix *w_up);
+size_t bfhip_gated_linear_backward_workspace(const bfhip_gated_desc *desc, const bfhip_matrix *x,
+                                             const bfhip_matrix *w_gate, const bfhip_matrix *w_up);
 
 int bfhip_gated_linear(const bfhip_gated_desc *desc, const bfhip_matrix *x,
                        const bfhip_matrix *w_gate, const bfhip_matrix *w_up,

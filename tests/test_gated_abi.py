@@ -39,15 +39,19 @@ def backward(d, dh=mat(), x=mat(), w_gate=mat(), w_up=mat(), gate=mat(), up=mat(
     return call("bfhip_gated_linear_backward", d, dh, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, work, size)
 
 
+def workspaces(d, x=mat(), w_gate=mat(), w_up=mat()):
+    lib = bfhip.hip_lib()
+    return [f(d, x, w_gate, w_up) for f in (lib.bfhip_gated_linear_workspace, lib.bfhip_gated_linear_backward_workspace)]
+
+
 @pytest.mark.parametrize("bad", [dict(type=3), dict(type=-1), dict(activation=3), dict(activation=-1), dict(rows=-1),
-                                 dict(rows=1 << 31), dict(features=0), dict(features=1 << 31), dict(hidden=0), dict(hidden=-1),
+                                 dict(rows=0x7fff0001), dict(features=0), dict(features=(1 << 20) + 1), dict(hidden=(1 << 20) + 1), dict(hidden=0), dict(hidden=-1),
                                  dict(rows=1 << 30, features=1 << 11), dict(hidden=1 << 30, features=1 << 11)])
 def test_refuses(bad):
     for f in (forward, backward):
         ok, message = f(desc(**bad))
         assert not ok and b"invalid gated linear contract" in message
-    lib = bfhip.hip_lib()
-    assert lib.bfhip_gated_linear_workspace(desc(**bad)) == 0 and lib.bfhip_gated_linear_backward_workspace(desc(**bad)) == 0
+    assert not any(workspaces(desc(**bad)))
 
 
 def test_refuses_one_of_two():
@@ -74,14 +78,13 @@ def test_refuses_weights_of_two_strides():
 
 
 def test_refuses_workspaces():
-    lib = bfhip.hip_lib()
-    for f, size, d in ((forward, lib.bfhip_gated_linear_workspace, desc(rows=300, features=4096)),
-                       (backward, lib.bfhip_gated_linear_backward_workspace, desc())):
-        need = size(d)
+    wide = {n: mat(stride=4096) for n in ("x", "w_gate", "w_up")}
+    d = desc(rows=300, features=4096)
+    for f, need in zip((forward, backward), workspaces(d, **wide)):
         assert need > 0
-        wide = {n: mat(stride=4096) for n in ("x", "w_gate", "w_up")}
+        named = dict(wide, dx=mat(stride=4096), dw_gate=mat(stride=4096), dw_up=mat(stride=4096)) if f is backward else wide
         for bad in (dict(size=need - 1), dict(work=None), dict(work=C.c_void_p(4104))):
-            ok, message = f(d, **wide, **bad)
+            ok, message = f(d, **named, **bad)
             assert not ok and b"workspace" in message
 
 
@@ -92,19 +95,30 @@ def test_nothing_to_do():
 
 
 def test_workspaces_are_bounded():
-    rng, lib = random.Random(1), bfhip.hip_lib()
+    rng = random.Random(1)
     log = lambda most: int(most ** rng.random())
     some = 0
     for _ in range(5000):
         d = desc(type=rng.randint(0, 2), rows=log(1 << 20), features=log(1 << 15), hidden=log(1 << 16))
-        need = lib.bfhip_gated_linear_workspace(d)
-        assert need <= 256 << 20
-        some += need > 0
-        size = 4 if d.type == 0 else 2
-        products = 2 * ((d.rows * (d.hidden + 7) // 8 * 8 * size + 255) // 256 * 256)
-        rest = lib.bfhip_gated_linear_backward_workspace(d) - products
-        assert rest <= (256 << 20) + 16 * d.rows * size + 8192
+        size, up = (4 if d.type == 0 else 2), lambda n: (n + 7) // 8 * 8
+        at, stride = rng.choice(((4096, up(d.features)), (4096, d.features), (4098 if size == 2 else 4100, up(d.features))))
+        x = mat(at, stride)
+        copied = at % 16 or d.features % (16 // size) or stride % (16 // size)
+        copies = (d.rows + 2 * d.hidden) * up(d.features) * size + 1024 if copied else 0
+        one, two = workspaces(d, x, x, x)
+        assert one <= (256 << 20) + (copies if d.rows > 32 else 0)
+        assert two <= (256 << 20) + copies + 2 * (d.rows * up(d.hidden) * size + 256) + 8192
+        some += one > 0
     assert some > 300
+
+
+def test_workspace_holds_copies_where_they_are_needed():
+    d = desc(rows=100)
+    whole = workspaces(d)
+    off = mat(4098, 512)
+    for named, bytes_ in ((dict(x=off), 100 * 512), (dict(w_up=off), 2 * 512 * 512), (dict(x=mat(stride=300)), 100 * 512)):
+        for a, b in zip(whole, workspaces(d, **named)):
+            assert a + bytes_ <= b <= a + bytes_ + 768
 
 
 def test_python_refuses():

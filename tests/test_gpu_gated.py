@@ -87,6 +87,26 @@ def test_large_tiles(device, dtype):
     compare(*inputs(device, dtype, 3001, 515, 2051), "relu")
 
 
+def test_rows_past_4_gib(device):
+    """Rows of zeros but for the first and last ones; results of rows in the
+    middle are zeros."""
+    rows, features, hidden = 600_000, 4096, 128
+    call, dh = inputs(device, BF16, 400, features, hidden)
+    ends = torch.cat([torch.arange(200), torch.arange(rows - 200, rows)]).to(device)
+    x, dy = (torch.zeros((rows, t.shape[1]), dtype=BF16, device=device) for t in (call["x"], dh))
+    x[ends], dy[ends] = call["x"], dh
+    far = dict(call, x=x)
+    forward, back = run(far, dy, "silu")
+    for name, (value, bound) in ref.gated_linear(**call, activation="silu").items():
+        check(name, forward[name][ends], value, bound)
+        assert not forward[name][200:-200].any()
+    want = ref.gated_linear_backward(dh, **call, gate=forward["gate"][ends], up=forward["up"][ends], activation="silu")
+    check("dx", back["dx"][ends], *want["dx"])
+    assert not back["dx"][200:-200].any()
+    for name in ("dw_gate", "dw_up"):  # (a sum of more terms, all but 400 of them zero)
+        check(name, back[name], *want[name])
+
+
 def test_large_tiles_f32(device):
     compare(*inputs(device, F32, 2050, 260, 1100), "gelu")
 
