@@ -766,69 +766,72 @@ def rotary_backward(dq, dk, positions, frequencies, interleaved=False, amplitude
 
 def _rotary(q, k, positions, frequencies, interleaved, amplitude, out, stream, inverse):
     torch = _torch()
-    code, given = _type_code(q), [q] if k is None else [q, k]
-    rows = [_head_rows(n, t, q) for n, t in zip("qk", given)]
+    code, rq, rk, to_q, to_k, kv_heads = _type_code(q), _head_rows("q", q, q), None, None, None, 0
     tokens, heads, dim = q.shape
-    if any(t.shape[0] != tokens for t in given):
-        raise BfHipError("q and k must have the same tokens")
+    if k is not None:
+        rk, kv_heads = _head_rows("k", k, q), k.shape[1]
+        if k.shape[0] != tokens:
+            raise BfHipError("q and k must have the same tokens")
+    half = frequencies.numel()
     pp = _expect("positions", positions, q, (tokens,), torch.int32)
-    pf = _expect("frequencies", frequencies, q, (frequencies.numel(),), torch.float64)
-    wanted = [None] * len(given) if out is None else [out] if torch.is_tensor(out) else list(out)
-    if len(wanted) != len(given):
-        raise BfHipError("out must hold a tensor for each of q and k")
-    desc = RotaryDesc(code, dim, 2 * frequencies.numel(), int(interleaved), inverse, heads,
-                      0 if k is None else k.shape[1], amplitude, tokens, pp, pf)
-    with _place(stream, *given, positions, frequencies, *wanted) as queue:
-        results = [t.new_empty(t.shape) if o is None else o for t, o in zip(given, wanted)]
-        if any(o.shape != t.shape for o, t in zip(results, given)):
-            raise BfHipError("out must have the shapes of q and k")
-        to = [_head_rows("out", o, q) for o in results]
-        if k is None:
-            rows.append(None)
-            to.append(None)
+    pf = _expect("frequencies", frequencies, q, (half,), torch.float64)
+    if out is not None:
+        to_q, to_k = (out, None) if torch.is_tensor(out) else out if len(out) == 2 else (None, None)
+        if (to_q is None or (to_k is None) != (k is None) or to_q.shape != q.shape
+                or (k is not None and to_k.shape != k.shape)):
+            raise BfHipError("out must hold a tensor of its shape for each of q and k")
+    desc = RotaryDesc(code, dim, 2 * half, interleaved, inverse, heads, kv_heads, amplitude, tokens,
+                      pp, pf)
+    with _place(stream, q, k, positions, frequencies, to_q, to_k) as queue:
+        if to_q is None:
+            to_q = q.new_empty((tokens, heads, dim))
+            ro, rp = Rows(to_q.data_ptr(), heads * dim, dim), None
+            if k is not None:
+                to_k = q.new_empty((tokens, kv_heads, dim))
+                rp = Rows(to_k.data_ptr(), kv_heads * dim, dim)
+        else:
+            ro, rp = _head_rows("out", to_q, q), to_k
+            if k is not None:
+                rp = _head_rows("out", to_k, q)
         err = _err()
-        _check(hip_lib().bfhip_rotary(desc, rows[0], to[0], rows[1], to[1], queue, err, 512),
-               err, "bfhip_rotary")
-    return results[0] if k is None else tuple(results)
+        _check(hip_lib().bfhip_rotary(desc, rq, ro, rk, rp, queue, err, 512), err, "bfhip_rotary")
+    return to_q if k is None else (to_q, to_k)
 
 
-def _page_pool(what, t, like):
+def _page_pool(what, t, like, dim):
     """[pages, page_size, kv_heads, head_dim] with contiguous heads -> Pages."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != 4 or (stride[3] != 1 and shape[3] > 1):
-        raise BfHipError(f"{what} must be [pages, page_size, kv_heads, head_dim] with contiguous "
-                         "heads")
-    if t.dtype != like.dtype or t.device != like.device or shape[3] != like.shape[-1]:
-        raise BfHipError(f"{what} must be {like.dtype} of head_dim {like.shape[-1]} on "
-                         f"{like.device}")
-    return Pages(t.data_ptr(), *stride[:3])
+    if (len(shape) != 4 or shape[3] != dim or (stride[3] != 1 and dim > 1)
+            or t.dtype != like.dtype or t.device != like.device):
+        raise BfHipError(f"{what} must be a {like.dtype} [pages, page_size, kv_heads, {dim}] tensor "
+                         f"with contiguous heads on {like.device}")
+    return Pages(t.data_ptr(), stride[0], stride[1], stride[2])
 
 
 def _paged_desc(like, heads, k_pages, v_pages, page_table, starts, lengths, scale, bias):
-    torch = _torch()
-    code = _type_code(like)
-    pools = [_page_pool("k_pages", k_pages, like), _page_pool("v_pages", v_pages, like)]
-    if k_pages.shape != v_pages.shape:
+    int32, dim = _torch().int32, like.shape[2]
+    pools = (_page_pool("k_pages", k_pages, like, dim), _page_pool("v_pages", v_pages, like, dim))
+    shape = k_pages.shape
+    if shape != v_pages.shape:
         raise BfHipError("k_pages and v_pages must have one shape")
-    pages, size, kv_heads, dim = k_pages.shape
     n = starts.numel() - 1
     if n < 0:
         raise BfHipError("starts must hold one entry more than there are sequences")
-    if (page_table.dim() != 2 or page_table.shape[0] != n or page_table.dtype != torch.int32
-            or page_table.device != like.device
-            or (page_table.stride(1) != 1 and page_table.shape[1] > 1)):
+    table, strides = page_table.shape, page_table.stride()
+    if (len(table) != 2 or table[0] != n or page_table.dtype != int32
+            or page_table.device != like.device or (strides[1] != 1 and table[1] > 1)):
         raise BfHipError(f"page_table must be an int32 [{n}, pages of a sequence] tensor with "
                          f"contiguous rows on {like.device}")
-    ps = _expect("starts", starts, like, (n + 1,), torch.int32)
-    pl = _expect("lengths", lengths, like, (n,), torch.int32)
     reach, pb = 0, None
     if bias is not None:
         if bias.dim() != 2 or bias.shape[1] % 2 == 0:
             raise BfHipError("bias must be [heads, 2 * reach + 1]")
         reach = bias.shape[1] // 2
-        pb = _expect("bias", bias, like, (heads, 2 * reach + 1), torch.float32)
-    return PagedDesc(code, n, heads, kv_heads, dim, size, page_table.shape[1], reach, scale,
-                     like.shape[0], pages, page_table.stride(0), ps, pl, page_table.data_ptr(),
+        pb = _expect("bias", bias, like, (heads, 2 * reach + 1), _torch().float32)
+    return PagedDesc(_type_code(like), n, heads, shape[2], dim, shape[1], table[1], reach, scale,
+                     like.shape[0], shape[0], strides[0],
+                     _expect("starts", starts, like, (n + 1,), int32),
+                     _expect("lengths", lengths, like, (n,), int32), page_table.data_ptr(),
                      pb), pools
 
 
@@ -858,20 +861,24 @@ def paged_attention(q, k_pages, v_pages, page_table, starts, lengths, scale=None
     written."""
     torch = _torch()
     rq = _head_rows("q", q, q)
-    if not q.shape[2]:
+    tokens, heads, dim = q.shape
+    if not dim:
         raise BfHipError("heads must have elements")
-    scale = q.shape[2] ** -0.5 if scale is None else scale
-    desc, pools = _paged_desc(q, q.shape[1], k_pages, v_pages, page_table, starts, lengths, scale,
+    scale = dim ** -0.5 if scale is None else scale
+    desc, pools = _paged_desc(q, heads, k_pages, v_pages, page_table, starts, lengths, scale,
                               bias)
     lib = hip_lib()
     with _place(stream, q, k_pages, v_pages, page_table, starts, lengths, bias, out) as queue:
-        o = q.new_empty(q.shape) if out is None else out
-        if o.shape != q.shape:
-            raise BfHipError("out must have the shape of q")
-        ro = _head_rows("out", o, q)
+        if out is None:
+            o = q.new_empty((tokens, heads, dim))
+            ro = Rows(o.data_ptr(), heads * dim, dim)
+        else:
+            o, ro = out, _head_rows("out", out, q)
+            if o.shape != q.shape:
+                raise BfHipError("out must have the shape of q")
         stat, pl = None, None
         if lse:
-            stat = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+            stat = q.new_empty((heads, tokens), dtype=torch.float32)
             pl = stat.data_ptr()
         size = lib.bfhip_paged_attention_workspace(desc)
         work, pw = _scratch(size, q)

@@ -339,9 +339,9 @@ struct GatedPlan {
 
 // Tiles, dealt in rounds of one per CU.  Those of the last round are split along the
 // contraction, in parts of four steps or more, where that fills it better.  A step
-// takes `step` us.
+// takes `step` us, the way into a tile and out of it `ends`.
 template <class S>
-GatedPlan plan_tiles(Form f, long long m, long long n, long long k, double step) {
+GatedPlan plan_tiles(Form f, long long m, long long n, long long k, double step, double ends) {
     constexpr int kRound = 256;
     GatedPlan p{};
     p.tiles_m = (int)((m + S::BM - 1) / S::BM * (f == kWeights ? 2 : 1));
@@ -350,12 +350,12 @@ GatedPlan plan_tiles(Form f, long long m, long long n, long long k, double step)
     const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % kRound;
     p.whole = (int)std::min(tiles, 0x7fffffffll);
     p.parts = 1;
-    p.time = (double)((tiles + kRound - 1) / kRound) * (steps * step + 5);
+    p.time = (double)((tiles + kRound - 1) / kRound) * (steps * step + ends);
     if (!rest) return p;
     const long long parts = std::min({kRound / rest, steps / 4, kPartBytes / (rest * tile_bytes)});
     if (parts < 2) return p;
     p.per = (int)((steps + parts - 1) / parts);
-    const double split = (double)(tiles / kRound) * (steps * step + 5) + p.per * step + 10 + (double)(parts * rest * tile_bytes) / 2.4e6;
+    const double split = (double)(tiles / kRound) * (steps * step + ends) + p.per * step + ends + 6 + (double)(parts * rest * tile_bytes) / 2.4e6;
     if (split > p.time) return p;
     p.time = split;
     p.parts = (int)((steps + p.per - 1) / p.per);
@@ -368,12 +368,12 @@ template <class E, Form F>
 using SmallShape = GatedShape<E, F, 128, 128, 2, E::kSize == 4 ? 4 : 2>;
 
 // Large tiles or small ones, whichever are estimated to take less time.  A step of
-// 64 of a large tile takes 1.1 us, of a small one 0.45 (fp32: of 32, 1.7).
+// 64 of a large tile takes 1.45 us, of a small one 0.6 (fp32: of 32, 1.7).
 template <class E, Form F>
 GatedPlan gated_plan(long long m, long long n, long long k) {
-    GatedPlan p = plan_tiles<SmallShape<E, F>>(F, m, n, k, E::kSize == 4 ? 1.7 : 0.45);
+    GatedPlan p = plan_tiles<SmallShape<E, F>>(F, m, n, k, E::kSize == 4 ? 1.7 : 0.6, 6);
     if constexpr (E::kSize == 2) {
-        GatedPlan l = plan_tiles<LargeShape<E, F>>(F, m, n, k, 1.1);
+        GatedPlan l = plan_tiles<LargeShape<E, F>>(F, m, n, k, 1.45, 10);
         l.large = true;
         if (l.time < p.time) return l;
     }
