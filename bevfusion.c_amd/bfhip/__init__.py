@@ -888,12 +888,12 @@ def paged_attention(q, k_pages, v_pages, page_table, starts, lengths, scale=None
     return (o, stat) if lse else o
 
 
-def _gated_matrix(what, t, shape, like):
-    stride = t.stride()
-    if t.shape != shape or t.dtype != like.dtype or t.device != like.device \
+def _gated_matrix(what, t, shape, like, dtype=None):
+    stride, dtype = t.stride(), dtype or like.dtype
+    if t.shape != shape or t.dtype != dtype or t.device != like.device \
             or (stride[1] != 1 and shape[1] > 1):
-        raise BfHipError(f"{what} must be a {like.dtype} {list(shape)} tensor with contiguous rows "
-                         f"on {like.device}")
+        raise BfHipError(f"{what} must be a {dtype} {list(shape)} tensor with contiguous rows on "
+                         f"{like.device}")
     return Matrix(t.data_ptr(), stride[0])
 
 
@@ -914,12 +914,14 @@ def gated_linear(x, w_gate, w_up, activation="silu", out=None, save=False, strea
     """act(x @ w_gate^T) * (x @ w_up^T) (bfhip_gated_linear): x [rows, features],
     the weights [hidden, features] of one stride (views of one tensor will do),
     all with contiguous rows; activation silu, gelu or relu.  Returns h [rows,
-    hidden], or (h, gate, up) with `save`, which gated_linear_backward takes."""
+    hidden], or (h, gate, up) with `save`, the products in fp32, which
+    gated_linear_backward takes."""
     desc, given = _gated_desc(x, w_gate, w_up, activation)
     shape, lib = (x.shape[0], w_gate.shape[0]), hip_lib()
     with _place(stream, x, w_gate, w_up, out) as queue:
         h = x.new_empty(shape) if out is None else out
-        kept = [x.new_empty(shape) for _ in range(2)] if save else [None, None]
+        kept = ([x.new_empty(shape, dtype=_torch().float32) for _ in range(2)] if save
+                else [None, None])
         size = lib.bfhip_gated_linear_workspace(desc, *given)
         work, pw = _scratch(size, x)
         err = _err()
@@ -935,7 +937,8 @@ def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation="silu", stre
     (dx, dw_gate, dw_up)."""
     desc, given = _gated_desc(x, w_gate, w_up, activation)
     shape, lib = (x.shape[0], w_gate.shape[0]), hip_lib()
-    more = [_gated_matrix(n, t, shape, x) for n, t in (("dh", dh), ("gate", gate), ("up", up))]
+    more = [_gated_matrix("dh", dh, shape, x)]
+    more += [_gated_matrix(n, t, shape, x, _torch().float32) for n, t in (("gate", gate), ("up", up))]
     with _place(stream, x, dh, w_gate, w_up, gate, up) as queue:
         grads = [t.new_empty(t.shape) for t in (x, w_gate, w_up)]
         size = lib.bfhip_gated_linear_backward_workspace(desc, *given)

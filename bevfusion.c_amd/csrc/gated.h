@@ -27,7 +27,7 @@ struct GatedOperand {
 struct GatedArgs {
     GatedOperand m_op, n_op;
     int m, n, k;     // of the result, and of the contraction (of one of its two halves)
-    char *out[3];    // forward: h, gate, up; inputs: dx; weights: dWg, dWu
+    char *out[3];    // forward: h, and gate and up in fp32; inputs: dx; weights: dWg, dWu
     long long out_stride[3];  // bytes
     const int *shift;         // fp16 gradients were multiplied by 2^shift
     int activation;
@@ -276,8 +276,6 @@ struct GatedStore {
     static constexpr int kRow = S::kN + 4, kCols = S::kPair ? S::kN / 2 : S::kN, kRounds = S::kMB > 1 ? 2 : 1;
     static constexpr int kColumns = S::kMB / kRounds;                  // block columns of a round
     static constexpr int kFloats = 16 * kColumns * kRow;               // of a wave
-    using W = Words<E, 8>;
-    using Word = typename E::Word;
     int m0, n0, shift;
     char *out;
     long long stride;
@@ -296,9 +294,10 @@ struct GatedStore {
         for (int i = 0; i < S::kNB; ++i)
             *reinterpret_cast<f32x4 *>(mine + (16 * column + (lane & 15)) * kRow + 16 * i + 4 * (lane >> 4)) = acc[i];
     }
+    template <class T>
     __device__ __forceinline__ static void put(char *row, int n, int count, const float (&v)[8]) {
-        Word *p = (Word *)row + n;
-        W w;
+        typename T::Word *p = (typename T::Word *)row + n;
+        Words<T, 8> w;
 #pragma unroll
         for (int e = 0; e < 8; ++e) w.put(e, v[e]);
         if (count >= 8) {
@@ -314,10 +313,10 @@ struct GatedStore {
         float h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[e] = activate<E, kActivation>(g[e]) * u[e];
-        put(a.out[0] + m * a.out_stride[0], n, a.n - n, h);
+        put<E>(a.out[0] + m * a.out_stride[0], n, a.n - n, h);
         if (a.out[1]) {
-            put(a.out[1] + m * a.out_stride[1], n, a.n - n, g);
-            put(a.out[2] + m * a.out_stride[2], n, a.n - n, u);
+            put<ElemF32>(a.out[1] + m * a.out_stride[1], n, a.n - n, g);
+            put<ElemF32>(a.out[2] + m * a.out_stride[2], n, a.n - n, u);
         }
     }
     // Stores the rows from block column `first` on that lie in `mine`.
@@ -334,7 +333,7 @@ struct GatedStore {
                 if constexpr (std::is_same_v<E, ElemF16>)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], shift);
-                put(out + m * stride, n, a.n - n, v);
+                put<E>(out + m * stride, n, a.n - n, v);
             }
         }
     }

@@ -141,9 +141,10 @@ __global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[e] = activate<E, decltype(kind)::value>(gate[e]) * up[e];
         });
-        const auto put = [&](int o, const f32x4 &v) {
-            Word *p = (Word *)(a.out[o] + row * a.out_stride[o]) + n;
-            Words<E, 4> w4;
+        const auto put = [&](auto type, int o, const f32x4 &v) {
+            using T = decltype(type);
+            typename T::Word *p = (typename T::Word *)(a.out[o] + row * a.out_stride[o]) + n;
+            Words<T, 4> w4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) w4.put(e, v[e]);
             if (n + 4 <= a.n) {
@@ -154,10 +155,10 @@ __global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a
                     if (n + e < a.n) p[e] = w4.w[e];
             }
         };
-        put(0, h);
+        put(E{}, 0, h);
         if (a.out[1]) {
-            put(1, gate);
-            put(2, up);
+            put(ElemF32{}, 1, gate);
+            put(ElemF32{}, 2, up);
         }
     }
 }
@@ -230,20 +231,21 @@ constexpr int kMostGroups = 1024;
 template <class E, int kActivation>
 __device__ __forceinline__ void slope8(const SlopeArgs &a, long long r, int c, float (&dg)[8], float (&du)[8]) {
     using Word = typename E::Word;
-    const Word *dh = (const Word *)(a.dh + r * a.dh_stride) + c, *gate = (const Word *)(a.gate + r * a.gate_stride) + c;
-    const Word *up = (const Word *)(a.up + r * a.up_stride) + c;
-    Words<E, 8> d, g, u;
+    const Word *dh = (const Word *)(a.dh + r * a.dh_stride) + c;
+    const float *gate = (const float *)(a.gate + r * a.gate_stride) + c, *up = (const float *)(a.up + r * a.up_stride) + c;
+    Words<E, 8> d;
+    Words<ElemF32, 8> g, u;
     if (c + 8 <= a.hidden) {
         d = Words<E, 8>::load(dh);
-        g = Words<E, 8>::load(gate);
-        u = Words<E, 8>::load(up);
+        g = Words<ElemF32, 8>::load(gate);
+        u = Words<ElemF32, 8>::load(up);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool in = c + e < a.hidden;
             d.w[e] = in ? dh[e] : (Word)0.f;
-            g.w[e] = in ? gate[e] : (Word)0.f;
-            u.w[e] = in ? up[e] : (Word)0.f;
+            g.w[e] = in ? gate[e] : 0.f;
+            u.w[e] = in ? up[e] : 0.f;
         }
     }
 #pragma unroll
@@ -521,7 +523,7 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
     const bfhip_matrix *out[3] = {h, gate, up};
     for (int i = 0; i < (gate ? 3 : 1); ++i) {
         a.out[i] = (char *)out[i]->data;
-        a.out_stride[i] = d->rows > 1 ? out[i]->stride * size : 0;
+        a.out_stride[i] = d->rows > 1 ? out[i]->stride * (i ? (int)sizeof(float) : size) : 0;
     }
     a.activation = d->activation;
     a.partial = (float *)((char *)workspace + in.bytes);
@@ -566,10 +568,10 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     const Aligned in(d, x, w_gate, w_up, work + p.all());
     const long long stride = slope_stride(d);
     SlopeArgs e{};
-    const auto step = [&](const bfhip_matrix *t, long long rows) { return rows > 1 ? t->stride * size : 0; };
-    e.dh = (const char *)dh->data; e.dh_stride = step(dh, d->rows);
-    e.gate = (const char *)gate->data; e.gate_stride = step(gate, d->rows);
-    e.up = (const char *)up->data; e.up_stride = step(up, d->rows);
+    const auto step = [&](const bfhip_matrix *t, long long rows, int bytes) { return rows > 1 ? t->stride * bytes : 0; };
+    e.dh = (const char *)dh->data; e.dh_stride = step(dh, d->rows, size);
+    e.gate = (const char *)gate->data; e.gate_stride = step(gate, d->rows, sizeof(float));
+    e.up = (const char *)up->data; e.up_stride = step(up, d->rows, sizeof(float));
     e.dg = work;
     e.du = work + p.slopes;
     e.stride = stride;
@@ -603,7 +605,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             a.n = (int)d->features;
             a.k = (int)d->hidden;
             a.out[0] = (char *)dx->data;
-            a.out_stride[0] = step(dx, d->rows);
+            a.out_stride[0] = step(dx, d->rows, size);
             ok = gated_launch<E, kInputs>(a, s) && ok;
         }
         if (dw_gate) {
@@ -613,8 +615,8 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             a.k = (int)d->rows;
             a.out[0] = (char *)dw_gate->data;
             a.out[1] = (char *)dw_up->data;
-            a.out_stride[0] = step(dw_gate, d->hidden);
-            a.out_stride[1] = step(dw_up, d->hidden);
+            a.out_stride[0] = step(dw_gate, d->hidden, size);
+            a.out_stride[1] = step(dw_up, d->hidden, size);
             ok = gated_launch<E, kWeights>(a, s) && ok;
         }
     });

@@ -302,8 +302,9 @@ int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
  * h = act(x Wg^T) * (x Wu^T), both products, the activation and their product
  * in one kernel: x [rows, features], Wg and Wu [hidden, features], h [rows,
  * hidden].  act: silu, v / (1 + e^-v); gelu, v (1 + erf(v / sqrt 2)) / 2; relu,
- * max(v, 0).  gate and up (both or neither NULL): the two products, rounded to
- * the type, which the backward pass takes.
+ * max(v, 0).  gate and up (both or neither NULL): the two products in fp32,
+ * which the backward pass takes (in 16 bits they would double the error of its
+ * gradients).
  *
  * Backward, with g = gate, u = up and dh the gradient of h:
  *   dg = dh * u * act'(g),  du = dh * act(g)

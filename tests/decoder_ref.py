@@ -77,8 +77,8 @@ def gated_linear(x, w_gate, w_up, activation):
     e_a = U * e_a + 1.13 * e_g  # (no slope is larger)
     y = a * u
     out = a.abs() * e_u + (u.abs() + e_u) * e_a + 2 * U * y.abs()
-    return dict(h=(y, SLACK * out + h * y.abs() + t + 1e-30), gate=(g, SLACK * e_g + h * g.abs() + t + 1e-30),
-                up=(u, SLACK * e_u + h * u.abs() + t + 1e-30))
+    return dict(h=(y, SLACK * out + h * y.abs() + t + 1e-30), gate=(g, SLACK * e_g + U * g.abs() + 1e-30),
+                up=(u, SLACK * e_u + U * u.abs() + 1e-30))
 
 
 def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation):
