@@ -54,11 +54,11 @@ __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a)
 }
 
 // ------------------------------------------------------------------ few rows
-// Up to 16 MB rows: bound by reading both weights once, so these go from memory to the
-// matrix cores without LDS.  A workgroup has 16 HB hidden elements; its waves take
+// Up to 16 MB rows: bound by reading both weights once (one row of 4096 -> 11008, bf16:
+// 37 us, 4.9 TB/s), so these go from memory to the matrix cores without LDS.  A workgroup has 16 HB hidden elements; its waves take
 // turns along the features, 64 at a time (a line of a 16-bit row), and their sums are
 // added in order at the end.  The lanes of rows that are not there load nothing.
-constexpr int kFewRows = 32, kFewWaves = 8, kFewDeep = 64;
+constexpr int kFewWaves = 8, kFewDeep = 64;
 
 template <class E, int MB, int HB>
 __global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a) {
@@ -82,44 +82,68 @@ __global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a
     for (int b = 0; b < HB; ++b)
 #pragma unroll
         for (int m = 0; m < MB; ++m) acc[0][b][m] = acc[1][b][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const auto load = [&](const Word *row, int k) {
+    // The fragments of 64 features.  Lane group g's k of the two products are 16
+    // neighbours: any order will do that both operands have.
+    struct Step {
+        Frag x[2][MB], w[2][2][HB];
+    };
+    const auto fetch = [&](Step &f, int k, auto load) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = k + 16 * g + 8 * h;
+#pragma unroll
+            for (int b = 0; b < HB; ++b) {
+                f.w[h][0][b] = load(w[0][b], at);
+                f.w[h][1][b] = load(w[1][b], at);
+            }
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                f.x[h][m] = Frag{};
+                if (16 * m + l16 < a.m) f.x[h][m] = load(x[m], at);
+            }
+        }
+    };
+    const auto multiply = [&](const Step &f) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int b = 0; b < HB; ++b)
+#pragma unroll
+                for (int m = 0; m < MB; ++m) {
+                    acc[0][b][m] = E::mfma(f.w[h][0][b], f.x[h][m], acc[0][b][m]);
+                    acc[1][b][m] = E::mfma(f.w[h][1][b], f.x[h][m], acc[1][b][m]);
+                }
+    };
+    const auto whole = [&](const Word *row, int k) {
         Frag f;
         __builtin_memcpy(&f, row + k, sizeof f);
         return f;
     };
-    const auto multiply = [&](int k, auto fetch) {
-        // Lane group g's k of both products are 16 neighbours: any order will do that
-        // both operands have.
+    const auto ragged = [&](const Word *row, int k) {
+        Words<E, 8> f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = k + 16 * g + 8 * h;
-            Frag xf[MB];
-#pragma unroll
-            for (int m = 0; m < MB; ++m) {
-                xf[m] = Frag{};
-                if (16 * m + l16 < a.m) xf[m] = fetch(x[m], at);
-            }
-#pragma unroll
-            for (int b = 0; b < HB; ++b) {
-                const Frag gate = fetch(w[0][b], at), up = fetch(w[1][b], at);
-#pragma unroll
-                for (int m = 0; m < MB; ++m) {
-                    acc[0][b][m] = E::mfma(gate, xf[m], acc[0][b][m]);
-                    acc[1][b][m] = E::mfma(up, xf[m], acc[1][b][m]);
-                }
-            }
-        }
+        for (int e = 0; e < 8; ++e) f.w[e] = k + e < a.k ? row[k + e] : (Word)0.f;
+        return __builtin_bit_cast(Frag, f.w);
     };
-    int k = wave * kFewDeep;
-#pragma unroll 4
-    for (; k + kFewDeep <= a.k; k += waves * kFewDeep) multiply(k, load);
-    if (k < a.k)
-        multiply(k, [&](const Word *row, int at) {
-            Words<E, 8> f;
+    // kAhead steps' loads are in flight.
+    constexpr int kAhead = E::kSize == 4 ? 2 : 4;
+    const int stride = waves * kFewDeep, steps = a.k / kFewDeep;  // whole ones, the waves' in turn
+    Step ring[kAhead];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f.w[e] = at + e < a.k ? row[at + e] : (Word)0.f;
-            return __builtin_bit_cast(Frag, f.w);
-        });
+    for (int s = 0; s < kAhead; ++s)
+        if (wave + s * waves < steps) fetch(ring[s], wave * kFewDeep + s * stride, whole);
+    for (int s = wave; s < steps; s += kAhead * waves) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int now = s + i * waves, next = now + kAhead * waves;
+            if (now < steps) multiply(ring[i]);
+            if (next < steps) fetch(ring[i], next * kFewDeep, whole);
+        }
+    }
+    if (steps * kFewDeep < a.k && steps % waves == wave) {
+        fetch(ring[0], steps * kFewDeep, ragged);
+        multiply(ring[0]);
+    }
 #pragma unroll
     for (int b = 0; b < HB; ++b)
 #pragma unroll
@@ -382,8 +406,16 @@ GatedPlan gated_plan(long long m, long long n, long long k) {
     return p;
 }
 
+// Whether a launch holds a product's workgroups.
 template <class E, Form F>
-int gated_launch(GatedArgs a, hipStream_t s) {
+bool gated_fits(long long m, long long n, long long k) {
+    const GatedPlan p = gated_plan<E, F>(m, n, k);
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    return tiles <= 0x7fffffff && launch_fits(p.whole + (tiles - p.whole) * p.parts, 512);
+}
+
+template <class E, Form F>
+void gated_launch(GatedArgs a, hipStream_t s) {
     const GatedPlan p = gated_plan<E, F>(a.m, a.n, a.k);
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
@@ -391,32 +423,36 @@ int gated_launch(GatedArgs a, hipStream_t s) {
     a.parts = p.parts;
     a.per = p.per;
     const long long split = (long long)p.tiles_m * p.tiles_n - p.whole, grid = p.whole + split * p.parts;
-    if (!launch_fits(grid, 512)) return 0;
     if constexpr (E::kSize == 2) {
         if (p.large) {
             launch_gated_large<E, F>(a, grid, s);
-            return 1;
+            return;
         }
     }
     using S = SmallShape<E, F>;
     hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
     if (split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(split * S::kMB)), dim3(S::kThreads), 0, s, a);
-    return 1;
+}
+
+// Whether a forward pass goes by the kernel for few rows: up to 16, or up to 32 where the
+// tiles' two launches (16-bit, weights up to 48 MiB) or their products of 128 rows
+// (fp32) take longer.  17 rows, us: 4096 -> 11008 bf16 59 (tiles 43), fp32 158 (264); 2048 ->
+// 5632 bf16 16 (22).
+bool few_rows(const bfhip_gated_desc *d) {
+    return d->rows <= 16 || (d->rows <= 32 && (d->type == BFHIP_F32 || 4 * d->features * d->hidden <= 48 << 20));
 }
 
 // Few rows.  Eight waves a workgroup where workgroups of four would leave CUs idle.
 template <class E>
-int gated_few_launch(const GatedArgs &a, hipStream_t s) {
+void gated_few_launch(const GatedArgs &a, hipStream_t s) {
     const auto run = [&](auto rows, auto cols) {
         constexpr int MB = decltype(rows)::value, HB = decltype(cols)::value;
         const long long grid = ((long long)a.n + 16 * HB - 1) / (16 * HB);
-        if (!launch_fits(grid, kFewWaves * kWave)) return 0;
         const int waves = grid < 512 ? kFewWaves : 4;
         hipLaunchKernelGGL((gated_few_kernel<E, MB, HB>), dim3((unsigned)grid), dim3(waves * kWave), 0, s, a);
-        return 1;
     };
-    if (a.m <= 16) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-    return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+    if (a.m <= 16) run(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+    else run(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
 }
 
 // dg and du: rows of whole 16-byte chunks.
@@ -495,7 +531,7 @@ GatedOperand operand(const bfhip_matrix *gate, const bfhip_matrix *up, long long
 
 extern "C" size_t bfhip_gated_linear_workspace(const bfhip_gated_desc *d, const bfhip_matrix *x, const bfhip_matrix *w_gate,
                                                const bfhip_matrix *w_up) {
-    if (bad_gated(d) || bad_inputs(d, x, w_gate, w_up) || d->rows <= kFewRows) return 0;
+    if (bad_gated(d) || bad_inputs(d, x, w_gate, w_up) || few_rows(d)) return 0;
     return Aligned(d, x, w_gate, w_up, nullptr).bytes + forward_parts(d);
 }
 
@@ -512,7 +548,7 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
     const int size = d->type == BFHIP_F32 ? 4 : 2;
-    const bool few = d->rows <= kFewRows;
+    const bool few = few_rows(d);
     const Aligned in(d, x, w_gate, w_up, (char *)workspace);
     GatedArgs a{};
     a.m_op = few ? operand(x, x, d->rows, size) : operand(&in.x, &in.x, d->rows, size);
@@ -528,17 +564,19 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
     a.activation = d->activation;
     a.partial = (float *)((char *)workspace + in.bytes);
     hipStream_t s = (hipStream_t)stream;
-    int ok = 1;
+    bool fits = true;
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
         if (few) {
-            ok = gated_few_launch<E>(a, s);
+            gated_few_launch<E>(a, s);
             return;
         }
+        fits = gated_fits<E, kForward>(a.m, a.n, a.k);
+        if (!fits) return;
         in.launch<E>(s);
-        ok = gated_launch<E, kForward>(a, s);
+        gated_launch<E, kForward>(a, s);
     });
-    if (!ok) return fail(error, cap, "gated linear has too many rows");
+    if (!fits) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
 }
 
@@ -583,9 +621,12 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     const long long grid = std::min<long long>(8192, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
     const bfhip_matrix slopes_g{e.dg, stride}, slopes_u{e.du, stride};
     hipStream_t s = (hipStream_t)stream;
-    int ok = 1;
+    bool fits = true;
     with_element(d->type, [&](auto el) {
         using E = decltype(el);
+        fits = (!dx || gated_fits<E, kInputs>(d->rows, d->features, d->hidden)) &&
+               (!dw_gate || gated_fits<E, kWeights>(d->hidden, d->features, d->rows));
+        if (!fits) return;
         if (d->rows) {
             in.launch<E>(s);
             with_activation(d->activation, [&](auto kind) {
@@ -606,7 +647,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             a.k = (int)d->hidden;
             a.out[0] = (char *)dx->data;
             a.out_stride[0] = step(dx, d->rows, size);
-            ok = gated_launch<E, kInputs>(a, s) && ok;
+            gated_launch<E, kInputs>(a, s);
         }
         if (dw_gate) {
             a.n_op = operand(&in.x, &in.x, d->rows, size);
@@ -617,9 +658,9 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             a.out[1] = (char *)dw_up->data;
             a.out_stride[0] = step(dw_gate, d->hidden, size);
             a.out_stride[1] = step(dw_up, d->hidden, size);
-            ok = gated_launch<E, kWeights>(a, s) && ok;
+            gated_launch<E, kWeights>(a, s);
         }
     });
-    if (!ok) return fail(error, cap, "gated linear has too many rows");
+    if (!fits) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
 }

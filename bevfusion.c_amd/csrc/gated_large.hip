@@ -16,11 +16,10 @@ struct GatedStream {
     Resource a, b;                  // of the step's tile (b: the up's rows)
     uint32_t off[Tile::kPlaces];    // the lane's offsets
     uint32_t span[Tile::kIssue];    // bytes from copy 0 to copy J
-    const char *other;              // inputs' gradient: the second matrix
     const Tile &tile;
     int k;
 
-    __device__ __forceinline__ GatedStream(const Tile &t, int k_) : other(t.base_b), tile(t), k(k_) {
+    __device__ __forceinline__ GatedStream(const Tile &t, int k_) : tile(t), k(k_) {
 #pragma unroll
         for (int j = 0; j < Tile::kIssue; ++j)
             span[j] = (uint32_t)__builtin_amdgcn_readfirstlane((int)(Tile::template span_row<PAIR>(j) * (int)t.stride));

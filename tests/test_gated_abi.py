@@ -88,6 +88,15 @@ def test_refuses_workspaces():
             assert not ok and b"workspace" in message
 
 
+def test_refuses_what_no_launch_holds():
+    d = desc(rows=0x7fff0000, features=8, hidden=500)
+    x = mat(stride=512)
+    assert b"too many" in forward(d, x=x, w_gate=x, w_up=x)[1]
+    d = desc(rows=0x7fff0000, features=500, hidden=8)
+    for named in (dict(), dict(dw_gate=None, dw_up=None)):
+        assert b"too many" in backward(d, **dict(dict.fromkeys(("x", "w_gate", "w_up"), x), **named))[1]
+
+
 def test_nothing_to_do():
     none = mat(None)
     assert forward(desc(rows=0), x=none, h=none, gate=none, up=none, work=None, size=0)[0]
@@ -106,7 +115,7 @@ def test_workspaces_are_bounded():
         copied = at % 16 or d.features % (16 // size) or stride % (16 // size)
         copies = (d.rows + 2 * d.hidden) * up(d.features) * size + 1024 if copied else 0
         one, two = workspaces(d, x, x, x)
-        assert one <= (256 << 20) + (copies if d.rows > 32 else 0)
+        assert one <= (256 << 20) + (copies if d.rows > 16 else 0)
         assert two <= (256 << 20) + copies + 2 * (d.rows * up(d.hidden) * size + 256) + 8192
         some += one > 0
     assert some > 300

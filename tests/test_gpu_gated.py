@@ -68,6 +68,20 @@ def test_gated_linear(device, dtype, size):
     compare(*inputs(device, dtype, *size), "silu")
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [2, 16, 17, 31, 32, 33])
+def test_few_rows(device, dtype, rows):
+    """Features that leave waves without a step, with one, with many and a rest;
+    hidden elements that end inside a block."""
+    for features, hidden in ((63, 33), (64, 16), (500, 40), (4096, 100), (3003, 4100)):
+        call, dh = inputs(device, dtype, rows, features, hidden)
+        forward = dict(zip(("h", "gate", "up"), bfhip.gated_linear(**call, activation="gelu", save=True)))
+        for name, (value, bound) in ref.gated_linear(**call, activation="gelu").items():
+            check(name, forward[name], value, bound)
+    call, dh = inputs(device, dtype, rows, 2816, 4480)  # (weights of more than 48 MiB)
+    check("h", bfhip.gated_linear(**call), *ref.gated_linear(**call, activation="silu")["h"])
+
+
 @pytest.mark.parametrize("activation", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_activations(device, dtype, activation):
