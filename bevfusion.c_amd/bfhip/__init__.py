@@ -736,6 +736,18 @@ def attention_backward(dout, q, k, v, out, lse, q_starts, k_starts, causal=False
     return tuple(grads)
 
 
+def _rows_like(t):
+    """A tensor of the shape of t [tokens, heads, head_dim] for a result, and its
+    Rows."""
+    torch = _torch()
+    o = torch.empty_like(t)  # (in t's order of strides, without gaps)
+    strides = o.stride()
+    if strides[2] != 1:
+        o = t.new_empty(t.shape)
+        strides = o.stride()
+    return o, Rows(o.data_ptr(), strides[0], strides[1])
+
+
 def rotary_frequencies(part, base=10000.0, factor=1.0, length=0, low=1.0, high=4.0, device="cuda"):
     """Radians per position of rotary's part / 2 pairs (bfhip_rotary_frequencies):
     fp64 on `device`.  Contexts `factor` times as long as the trained ones divide
@@ -784,11 +796,10 @@ def _rotary(q, k, positions, frequencies, interleaved, amplitude, out, stream, i
                       pp, pf)
     with _place(stream, q, k, positions, frequencies, to_q, to_k) as queue:
         if to_q is None:
-            to_q = q.new_empty((tokens, heads, dim))
-            ro, rp = Rows(to_q.data_ptr(), heads * dim, dim), None
+            to_q, ro = _rows_like(q)
+            rp = None
             if k is not None:
-                to_k = q.new_empty((tokens, kv_heads, dim))
-                rp = Rows(to_k.data_ptr(), kv_heads * dim, dim)
+                to_k, rp = _rows_like(k)
         else:
             ro, rp = _head_rows("out", to_q, q), to_k
             if k is not None:
@@ -870,8 +881,7 @@ def paged_attention(q, k_pages, v_pages, page_table, starts, lengths, scale=None
     lib = hip_lib()
     with _place(stream, q, k_pages, v_pages, page_table, starts, lengths, bias, out) as queue:
         if out is None:
-            o = q.new_empty((tokens, heads, dim))
-            ro = Rows(o.data_ptr(), heads * dim, dim)
+            o, ro = _rows_like(q)
         else:
             o, ro = out, _head_rows("out", out, q)
             if o.shape != q.shape:

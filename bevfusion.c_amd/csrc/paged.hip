@@ -12,6 +12,7 @@ namespace {
 
 constexpr int kKeys = 32;   // keys per tile
 constexpr int kRows = 16;   // rows (token, head in group) per tile
+constexpr int kFine = 16;   // units of time per key tile
 
 struct PagedPool {
     char *data;
@@ -30,8 +31,8 @@ struct PagedArgs {
     float scale2;
     int flip;
     int shares;        // workgroups of a key head
-    int least;         // units of a share, at least
-    int piece;         // units of a row tile beside its key tiles
+    int least;         // key tiles' time of a share, at least
+    int piece;         // key tiles that a row tile's beginning and end take the time of
     float *part_out;   // [2 shares][kv_heads][kRows][padded dim]
     float2 *part_stat; // [2 shares][kv_heads][kRows]
     long long *info;   // [sequences + 1]: first unit of each sequence that has some; units of a share
@@ -79,8 +80,8 @@ __global__ __launch_bounds__(256) void cache_append_kernel(PagedArgs a, AttnRows
 // ---------------------------------------------------------------- attention
 // How the work is dealt.  Lengths are on the device alone, so every workgroup
 // works the deal out for itself.  Sequence b has row tiles (16 rows, token * group +
-// head in group) and key tiles; a row tile takes units of time, one per key tile and
-// `piece` for its queries' way in and its results' way out.  Units, row tile after row
+// head in group) and key tiles; a row tile takes kFine units of time for each of its key
+// tiles and `piece` tiles' for its queries' way in and its results' way out.  Units, row tile after row
 // tile, sequence after sequence, are dealt in equal shares, one per workgroup
 // that the chip holds at once, whatever the lengths are.  So a share has whole row
 // tiles and at most one that an earlier share began and one that it leaves to a
@@ -88,23 +89,20 @@ __global__ __launch_bounds__(256) void cache_append_kernel(PagedArgs a, AttnRows
 // tokens has no units.)
 struct SequenceWork {
     int start, queries, keys, row_tiles, tiles, piece;
-    __device__ __forceinline__ int cost() const { return tiles + piece; }
+    __device__ __forceinline__ int cost() const { return (tiles + piece) * kFine; }  // below 2^31: tiles of 32 keys
     __device__ __forceinline__ long long units() const { return (long long)row_tiles * cost(); }
     // Key tiles up to unit x of a row tile.
     __device__ __forceinline__ int tile(int x) const { return (int)((long long)x * tiles / cost()); }
 };
 
+// (All loads come before the first use, so that they wait together.)
 __device__ __forceinline__ SequenceWork sequence_work(const PagedArgs &a, int b) {
-    SequenceWork w{0, 0, 0, 0, 0, a.piece};
-    if (b >= a.sequences) return w;
-    const long long s = clamp_start(a.starts, b, a.tokens), e = clamp_start(a.starts, b + 1, a.tokens);
-    w.start = (int)s;
-    w.queries = (int)(e > s ? e - s : 0);
-    if (!w.queries) return w;
-    w.keys = cache_length(a, b);
-    w.row_tiles = (int)(((long long)w.queries * (a.heads / a.kv_heads) + kRows - 1) / kRows);
-    w.tiles = (w.keys + kKeys - 1) / kKeys;
-    return w;
+    if (b >= a.sequences) return SequenceWork{0, 0, 0, 0, 0, a.piece};
+    const int first = a.starts[b], next = a.starts[b + 1], length = a.lengths[b];
+    const long long s = min(max((long long)first, 0ll), a.tokens), e = min(max((long long)next, 0ll), a.tokens);
+    const int queries = (int)(e > s ? e - s : 0), keys = queries ? min(max(length, 0), a.table_pages * a.page_size) : 0;
+    return SequenceWork{(int)s, queries, keys, (int)(((long long)queries * (a.heads / a.kv_heads) + kRows - 1) / kRows),
+                        (keys + kKeys - 1) / kKeys, a.piece};
 }
 
 // The sequences from the one that a share begins in, 64 at a time, a lane each.
@@ -150,15 +148,19 @@ struct Sequences {
     }
 };
 
-__device__ __forceinline__ long long share_units(const PagedArgs &a) {
+// Units of a share; `at` holds the first sequences.
+__device__ __forceinline__ long long share_units(const PagedArgs &a, const Sequences &at) {
     if (a.shares == 1) return 0x7fffffffffffffffll;
-    long long total = 0;
-    for (int b = threadIdx.x % kWave; b < a.sequences; b += kWave) total += sequence_work(a, b).units();
+    long long total = Sequences::read(at.lane_upto, kWave - 1);
+    if (a.sequences > kWave) {
+        long long rest = 0;
+        for (int b = kWave + threadIdx.x % kWave; b < a.sequences; b += kWave) rest += sequence_work(a, b).units();
 #pragma unroll
-    for (int o = 1; o < kWave; o *= 2) total += __shfl_xor(total, o);
-    total = Sequences::read(total, 0);
+        for (int o = 1; o < kWave; o *= 2) rest += __shfl_xor(rest, o);
+        total += Sequences::read(rest, 0);
+    }
     const long long share = (total + a.shares - 1) / a.shares;
-    return share > a.least ? share : a.least;
+    return share > a.least * kFine ? share : a.least * kFine;
 }
 
 // What a lane reads in place of a row that is not there.
@@ -353,13 +355,13 @@ __global__ __launch_bounds__(256, 1) void paged_attention_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) char smem[Walk::kWaves * (2 * Walk::P::kStage + kRows * sizeof(float2))];
     Walk walk{a, smem, (int)blockIdx.x % a.kv_heads, (int)blockIdx.x / a.kv_heads, (int)threadIdx.x % kWave,
               __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)};
-    const long long units = share_units(a);
+    Sequences at;
+    at.load(a, 0, 0);
+    const long long units = share_units(a, at);
     long long u = walk.share * units;
     const long long end = a.shares == 1 ? units : u + units;
     const bool writes = a.info && walk.kv == 0 && threadIdx.x == 0;
     if (writes && walk.share == 0) a.info[a.sequences] = units;
-    Sequences at;
-    at.load(a, 0, 0);
     while (u < end && at.seek(a, u)) {
         const SequenceWork s = at.work();
         const long long begin = at.upto() - s.units(), in = u - begin;
@@ -385,12 +387,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     const int head = blockIdx.x % per_token * kPer + i, group = a.heads / a.kv_heads;
     const int sequence = find_token(a.starts, a.sequences, a.tokens, token);
     if (sequence < 0) return;
+    const long long units = a.info[a.sequences], first = a.info[sequence];
     const SequenceWork s = sequence_work(a, sequence);
     const int kv = min(head, a.heads - 1) / group, row = (token - s.start) * group + min(head, a.heads - 1) % group;
     // Shares that have units of the row's tile: the first in their second place, the
     // others in their first.  (Where starts descend, a row's sequence need not be one
     // that was dealt: any place within the workspace will do then.)
-    const long long units = a.info[a.sequences], begin = a.info[sequence] + (long long)(row / kRows) * s.cost();
+    const long long begin = first + (long long)(row / kRows) * s.cost();
     const long long from = begin / units, to = (begin + s.cost() - 1) / units;
     if (from == to || from < 0 || to >= a.shares) return;  // (one share has written the result)
     const int parts = (int)(to - from) + 1;
