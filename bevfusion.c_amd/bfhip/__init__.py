@@ -898,26 +898,37 @@ def paged_attention(q, k_pages, v_pages, page_table, starts, lengths, scale=None
     return (o, stat) if lse else o
 
 
-def _gated_matrix(what, t, shape, like, dtype=None):
-    stride, dtype = t.stride(), dtype or like.dtype
-    if t.shape != shape or t.dtype != dtype or t.device != like.device \
-            or (stride[1] != 1 and shape[1] > 1):
-        raise BfHipError(f"{what} must be a {dtype} {list(shape)} tensor with contiguous rows on "
-                         f"{like.device}")
+def _gated_matrix(what, t, rows, length, dtype, device):
+    """[rows, length] with contiguous rows -> Matrix."""
+    shape, stride = t.shape, t.stride()
+    if (len(shape) != 2 or shape[0] != rows or shape[1] != length or t.dtype != dtype
+            or t.device != device or (stride[1] != 1 and length > 1)):
+        raise BfHipError(f"{what} must be a {dtype} {[rows, length]} tensor with contiguous rows "
+                         f"on {device}")
     return Matrix(t.data_ptr(), stride[0])
 
 
 def _gated_desc(x, w_gate, w_up, activation):
-    code = _type_code(x)
+    code, kind = _type_code(x), ACTIVATIONS.get(activation)
     if x.dim() != 2 or w_gate.dim() != 2:
         raise BfHipError("x must be [rows, features], the weights [hidden, features]")
-    if activation not in ACTIVATIONS:
+    if kind is None:
         raise BfHipError(f"activation must be one of {', '.join(ACTIVATIONS)}")
-    (rows, features), hidden = x.shape, w_gate.shape[0]
-    return GatedDesc(code, ACTIVATIONS[activation], rows, features, hidden), \
-        [_gated_matrix("x", x, (rows, features), x),
-         _gated_matrix("w_gate", w_gate, (hidden, features), x),
-         _gated_matrix("w_up", w_up, (hidden, features), x)]
+    (rows, features), hidden, dtype, device = x.shape, w_gate.shape[0], x.dtype, x.device
+    return GatedDesc(code, kind, rows, features, hidden), (
+        _gated_matrix("x", x, rows, features, dtype, device),
+        _gated_matrix("w_gate", w_gate, hidden, features, dtype, device),
+        _gated_matrix("w_up", w_up, hidden, features, dtype, device)), rows, hidden, dtype, device
+
+
+def _matrix_like(t):
+    """A tensor of the shape of t [rows, length] for a result, and its Matrix."""
+    o = _torch().empty_like(t)  # (contiguous rows, without gaps)
+    strides = o.stride()
+    if strides[1] != 1:
+        o = t.new_empty(t.shape)
+        strides = o.stride()
+    return o, Matrix(o.data_ptr(), strides[0])
 
 
 def gated_linear(x, w_gate, w_up, activation="silu", out=None, save=False, stream=None):
@@ -926,38 +937,45 @@ def gated_linear(x, w_gate, w_up, activation="silu", out=None, save=False, strea
     all with contiguous rows; activation silu, gelu or relu.  Returns h [rows,
     hidden], or (h, gate, up) with `save`, the products in fp32, which
     gated_linear_backward takes."""
-    desc, given = _gated_desc(x, w_gate, w_up, activation)
-    shape, lib = (x.shape[0], w_gate.shape[0]), hip_lib()
+    desc, given, rows, hidden, dtype, device = _gated_desc(x, w_gate, w_up, activation)
+    lib, gate, up, mg, mu = hip_lib(), None, None, None, None
     with _place(stream, x, w_gate, w_up, out) as queue:
-        h = x.new_empty(shape) if out is None else out
-        kept = ([x.new_empty(shape, dtype=_torch().float32) for _ in range(2)] if save
-                else [None, None])
+        if out is None:
+            out = x.new_empty((rows, hidden))
+            mh = Matrix(out.data_ptr(), hidden)
+        else:
+            mh = _gated_matrix("out", out, rows, hidden, dtype, device)
+        if save:
+            gate = x.new_empty((rows, hidden), dtype=_torch().float32)
+            mg = Matrix(gate.data_ptr(), hidden)
+            up, mu = _matrix_like(gate)
         size = lib.bfhip_gated_linear_workspace(desc, *given)
         work, pw = _scratch(size, x)
         err = _err()
-        _check(lib.bfhip_gated_linear(
-            desc, *given, _gated_matrix("out", h, shape, x),
-            *(t if t is None else Matrix(t.data_ptr(), shape[1]) for t in kept), pw, size, queue,
-            err, 512), err, "bfhip_gated_linear")
-    return (h, *kept) if save else h
+        _check(lib.bfhip_gated_linear(desc, *given, mh, mg, mu, pw, size, queue, err, 512), err,
+               "bfhip_gated_linear")
+    return (out, gate, up) if save else out
 
 
 def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation="silu", stream=None):
     """Gradients of gated_linear (bfhip_gated_linear_backward) from that of h:
     (dx, dw_gate, dw_up)."""
-    desc, given = _gated_desc(x, w_gate, w_up, activation)
-    shape, lib = (x.shape[0], w_gate.shape[0]), hip_lib()
-    more = [_gated_matrix("dh", dh, shape, x)]
-    more += [_gated_matrix(n, t, shape, x, _torch().float32) for n, t in (("gate", gate), ("up", up))]
+    desc, given, rows, hidden, dtype, device = _gated_desc(x, w_gate, w_up, activation)
+    lib, float32 = hip_lib(), _torch().float32
+    md = _gated_matrix("dh", dh, rows, hidden, dtype, device)
+    mg = _gated_matrix("gate", gate, rows, hidden, float32, device)
+    mu = _gated_matrix("up", up, rows, hidden, float32, device)
     with _place(stream, x, dh, w_gate, w_up, gate, up) as queue:
-        grads = [t.new_empty(t.shape) for t in (x, w_gate, w_up)]
+        dx, mx = _matrix_like(x)
+        dw_gate, mwg = _matrix_like(w_gate)
+        dw_up, mwu = _matrix_like(w_gate)
         size = lib.bfhip_gated_linear_backward_workspace(desc, *given)
         work, pw = _scratch(size, x)
         err = _err()
-        _check(lib.bfhip_gated_linear_backward(
-            desc, more[0], *given, *more[1:], *(Matrix(t.data_ptr(), t.shape[1]) for t in grads),
-            pw, size, queue, err, 512), err, "bfhip_gated_linear_backward")
-    return tuple(grads)
+        _check(lib.bfhip_gated_linear_backward(desc, md, *given, mg, mu, mx, mwg, mwu, pw, size,
+                                               queue, err, 512),
+               err, "bfhip_gated_linear_backward")
+    return dx, dw_gate, dw_up
 
 
 def window_map(batches, height, width, shift, device, stream=None):

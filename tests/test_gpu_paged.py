@@ -234,6 +234,36 @@ def test_paged_attention_biases_that_mask(device):
     check("out", out, *ref.paged_attention(table=table, **call)["out"])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_paged_of_nothing(device, dtype):
+    """No pages, tables without entries, no sequences, no tokens."""
+    i32 = dict(dtype=torch.int32, device=device)
+    q = randn(gen(device), 3, 4, 64, dtype=dtype)
+    pages = torch.empty((0, 16, 2, 64), dtype=dtype, device=device)
+    some = randn(gen(device, 1), 2, 16, 2, 64, dtype=dtype)
+    one = dict(starts=starts_of(device, [1, 2]), lengths=torch.tensor([5, 30], **i32))
+    for pool, table in ((pages, torch.zeros((2, 2), **i32)), (some, torch.zeros((2, 0), **i32)), (pages, torch.zeros((2, 0), **i32))):
+        out, lse = bfhip.paged_attention(q, pool, pool, table, lse=True, **one)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        before = pool.clone()
+        bfhip.cache_append(q[:, :2], q[:, 2:], pool, pool, table, **one)
+        assert torch.equal(pool, before)
+    none = dict(starts=torch.zeros(1, **i32), lengths=torch.zeros(0, **i32))
+    out = torch.full_like(q, 3.0)
+    bfhip.paged_attention(q, some, some, torch.zeros((0, 2), **i32), out=out, **none)
+    assert (out == 3).all()
+    empty = dict(starts=starts_of(device, [0, 0]), lengths=one["lengths"])
+    assert bfhip.paged_attention(q[:0], some, some, torch.zeros((2, 2), **i32), **empty).shape == (0, 4, 64)
+
+
+def test_paged_sequences_that_share_pages(device):
+    """A common beginning, and one page twice in a sequence."""
+    call, table = inputs(device, (BF16, 8, 2, 64, 16, [1, 1, 2], [700, 90, 320], None))
+    table[1, :5] = table[0, :5]
+    table[2, 3:9] = table[2, 2]
+    compare(call, table)
+
+
 # ------------------------------------------------------------------- append
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("size", [1, 5, 16, 64])
