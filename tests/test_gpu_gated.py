@@ -101,6 +101,18 @@ def test_large_tiles(device, dtype):
     compare(*inputs(device, dtype, 3001, 515, 2051), "relu")
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_large_tiles_of_every_product(device, dtype):
+    """All three products by large tiles whose last ones have few rows, few
+    columns and few terms, in matrices with NaN behind every row and the last."""
+    sizes = dict(x=(4100, 2808), w_gate=(2810, 2808), w_up=(2810, 2808))
+    call, dh = inputs(device, dtype, 4100, 2808, 2810)
+    wide = {n: torch.full((rows + 256, length + 64), math.nan, dtype=dtype, device=device) for n, (rows, length) in sizes.items()}
+    views = {n: wide[n][:rows, :length].copy_(call[n]) for n, (rows, length) in sizes.items()}
+    compare(views, dh, "silu")
+    compare(*inputs(device, dtype, 4100, 2805, 2810), "relu")
+
+
 def test_rows_past_4_gib(device):
     """Rows of zeros but for the first and last ones; results of rows in the
     middle are zeros."""
