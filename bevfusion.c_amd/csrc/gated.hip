@@ -10,17 +10,20 @@ using namespace bfhip;
 
 namespace {
 
-// Small tiles, where there are too few large ones: four stages in LDS, three of them in
-// flight while one is multiplied.
-constexpr int kStages = 4;
+// Small and low tiles, where there are too few large ones: two stages in LDS, one of
+// them in flight while the other is multiplied, so that two workgroups of small tiles
+// or three of low ones share a CU and cover each other's waits, ways in and ways out.
+// (With four stages a workgroup is alone there and no faster for it.  Forward, 999 rows
+// of 776 -> 2056, fp16, 264 tiles: 17 us, 26 with four; gradient of 5632 x 2048 weights,
+// 512 rows, bf16: 36 and 57.)
+constexpr int kStages = 2;
 
 template <class E, Form F, class S>
 __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a) {
-    static_assert((kStages & (kStages - 1)) == 0, "stages by a mask");
     constexpr int kCopies = S::MTile::kIssue + S::NTile::kIssue;
     __shared__ __attribute__((aligned(512))) char smem[gated_lds<E, F, S>(kStages * S::kStage)];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const auto stage = [&](int t) { return smem + (t & (kStages - 1)) * S::kStage; };
+    const auto stage = [&](int t) { return smem + t % kStages * S::kStage; };
     GatedWork<E, F, S> w;
     w.init(a, wave, lane);
     f32x4 acc[S::kMB][S::kNB];
@@ -356,53 +359,72 @@ bool chunked(const bfhip_matrix *x, long long rows, long long length, int size) 
     return ((uintptr_t)x->data & 15) == 0 && length % words == 0 && (rows <= 1 || (x->stride % words == 0 && x->stride < 1 << 21));
 }
 
+enum GatedTiles { kSmall, kLow, kLarge };
+
 struct GatedPlan {
-    bool large;
+    GatedTiles kind;
     int tiles_m, tiles_n, whole, parts, per;
     size_t bytes;  // of the parts' sums
     double time;   // an estimate, in us
 };
 
-// Tiles, dealt in rounds of one per CU.  Those of the last round are split along the
-// contraction, in parts of four steps or more, where that fills it better.  A step
-// takes `step` us, the way into a tile and out of it `ends`.
+// Times in us that fit what products of 100 random sizes took to a tenth or so.
+struct GatedTimes {
+    int resident;  // workgroups that a CU holds at once
+    double step;   // of the contraction, where a CU always has one to multiply
+    double alone;  // a step where it waits for its tiles
+    double ends;   // the way into a tile and out of it
+};
+
+// Tiles in rounds of as many workgroups as the chip holds; those of the last round may
+// be split along the contraction, whichever number of parts is estimated to take least.
 template <class S>
-GatedPlan plan_tiles(Form f, long long m, long long n, long long k, double step, double ends) {
-    constexpr int kRound = 256;
-    GatedPlan p{};
-    p.tiles_m = (int)((m + S::BM - 1) / S::BM * (f == kWeights ? 2 : 1));
-    p.tiles_n = (int)((n + S::kCols - 1) / S::kCols);
-    const long long steps = (k + S::BK - 1) / S::BK * (f == kInputs ? 2 : 1), tiles = (long long)p.tiles_m * p.tiles_n;
-    const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % kRound;
-    p.whole = (int)std::min(tiles, 0x7fffffffll);
-    p.parts = 1;
-    p.time = (double)((tiles + kRound - 1) / kRound) * (steps * step + ends);
-    if (!rest) return p;
-    const long long parts = std::min({kRound / rest, steps / 4, kPartBytes / (rest * tile_bytes)});
-    if (parts < 2) return p;
-    p.per = (int)((steps + parts - 1) / parts);
-    const double split = (double)(tiles / kRound) * (steps * step + ends) + p.per * step + ends + 6 + (double)(parts * rest * tile_bytes) / 2.4e6;
-    if (split > p.time) return p;
-    p.time = split;
-    p.parts = (int)((steps + p.per - 1) / p.per);
-    p.whole = (int)(tiles - rest);
-    p.bytes = (size_t)(p.parts * rest * tile_bytes);
-    return p;
+GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long long k, const GatedTimes &c) {
+    constexpr int kCus = 256;
+    GatedPlan best{};
+    best.kind = kind;
+    best.tiles_m = (int)((m + S::BM - 1) / S::BM * (f == kWeights ? 2 : 1));
+    best.tiles_n = (int)((n + S::kCols - 1) / S::kCols);
+    const long long steps = (k + S::BK - 1) / S::BK * (f == kInputs ? 2 : 1), tiles = (long long)best.tiles_m * best.tiles_n;
+    const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % (kCus * c.resident);
+    const auto time = [&](long long groups, long long each) {
+        const long long turns = (groups + kCus - 1) / kCus, rounds = (turns + c.resident - 1) / c.resident;
+        return groups ? std::max(turns * (each * c.step + c.ends), rounds * each * c.alone + c.ends) : 0;
+    };
+    best.whole = (int)std::min(tiles, 0x7fffffffll);
+    best.parts = 1;
+    best.time = time(tiles, steps);
+    for (const int p : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+        const long long per = (steps + p - 1) / p, parts = per ? (steps + per - 1) / per : 0, bytes = parts * rest * tile_bytes;
+        if (!rest || steps < 2 * p || bytes > kPartBytes) break;
+        // (the launch that joins the parts: 1.8 us, 0.17 a part, 4.2 TB/s)
+        const double t = time(tiles - rest, steps) + time(rest * parts, per) + 1.8 + 0.17 * parts + bytes / 4.2e6;
+        if (t >= best.time) continue;
+        best.time = t;
+        best.whole = (int)(tiles - rest);
+        best.parts = (int)parts;
+        best.per = (int)per;
+        best.bytes = (size_t)bytes;
+    }
+    return best;
 }
 
 template <class E, Form F>
-using SmallShape = GatedShape<E, F, 128, 128, 2, E::kSize == 4 ? 4 : 2>;
+using SmallShape = GatedShape<E, F, 128, 128, 2, 2>;
+template <class E, Form F>
+using LowShape = GatedShape<E, F, 64, 128, 1, 4>;
 
-// Large tiles or small ones, whichever are estimated to take less time.  A step of
-// 64 of a large tile takes 1.45 us, of a small one 0.6 (fp32: of 32, 1.7).
+// Large tiles (16-bit), small ones or low ones (where rows of m are contiguous along k),
+// whichever are estimated to take the least time.
 template <class E, Form F>
 GatedPlan gated_plan(long long m, long long n, long long k) {
-    GatedPlan p = plan_tiles<SmallShape<E, F>>(F, m, n, k, E::kSize == 4 ? 1.7 : 0.6, 6);
-    if constexpr (E::kSize == 2) {
-        GatedPlan l = plan_tiles<LargeShape<E, F>>(F, m, n, k, 1.45, 10);
-        l.large = true;
-        if (l.time < p.time) return l;
-    }
+    constexpr bool kHalf = E::kSize == 2;
+    GatedPlan p = plan_tiles<SmallShape<E, F>>(kSmall, F, m, n, k, kHalf ? GatedTimes{2, 0.46, 0.62, 1.6} : GatedTimes{2, 1.93, 2.1, 0.5});
+    const auto take = [&](const GatedPlan &q) {
+        if (q.time < p.time) p = q;
+    };
+    if constexpr (F != kWeights) take(plan_tiles<LowShape<E, F>>(kLow, F, m, n, k, kHalf ? GatedTimes{3, 0.34, 0.48, 0.75} : GatedTimes{3, 1.0, 1.15, 0.2}));
+    if constexpr (kHalf) take(plan_tiles<LargeShape<E, F>>(kLarge, F, m, n, k, GatedTimes{1, 1.13, 1.13, 7.1}));
     return p;
 }
 
@@ -423,23 +445,32 @@ void gated_launch(GatedArgs a, hipStream_t s) {
     a.parts = p.parts;
     a.per = p.per;
     const long long split = (long long)p.tiles_m * p.tiles_n - p.whole, grid = p.whole + split * p.parts;
+    const auto run = [&](auto shape) {
+        using S = decltype(shape);
+        hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
+        if (split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(split * S::kMB)), dim3(S::kThreads), 0, s, a);
+    };
     if constexpr (E::kSize == 2) {
-        if (p.large) {
+        if (p.kind == kLarge) {
             launch_gated_large<E, F>(a, grid, s);
             return;
         }
     }
-    using S = SmallShape<E, F>;
-    hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
-    if (split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(split * S::kMB)), dim3(S::kThreads), 0, s, a);
+    if constexpr (F != kWeights) {
+        if (p.kind == kLow) {
+            run(LowShape<E, F>{});
+            return;
+        }
+    }
+    run(SmallShape<E, F>{});
 }
 
 // Whether a forward pass goes by the kernel for few rows: up to 16, or up to 32 where the
-// tiles' two launches (16-bit, weights up to 48 MiB) or their products of 128 rows
-// (fp32) take longer.  17 rows, us: 4096 -> 11008 bf16 59 (tiles 43), fp32 158 (264); 2048 ->
-// 5632 bf16 16 (22).
+// weights are small.  17 rows, few or tiles, us: 1024 -> 4096 bf16 9.1 and 12.5, 2048 -> 5632
+// 15.4 and 16.3, 4096 -> 11008 43 and 43; 512 -> 2048 fp32 10.8 and 16.6, 1024 -> 4096 20 and
+// 20, 2048 -> 5632 45 and 39.
 bool few_rows(const bfhip_gated_desc *d) {
-    return d->rows <= 16 || (d->rows <= 32 && (d->type == BFHIP_F32 || 4 * d->features * d->hidden <= 48 << 20));
+    return d->rows <= 16 || (d->rows <= 32 && d->features * d->hidden <= (d->type == BFHIP_F32 ? 4 : 12) << 20);
 }
 
 // Few rows.  Eight waves a workgroup where workgroups of four would leave CUs idle.
