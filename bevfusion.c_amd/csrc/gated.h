@@ -349,9 +349,9 @@ struct GatedWork {
     uint32_t m_at, n_at;  // where the lane reads its fragments
     int k;
 
-    __device__ __forceinline__ void init(const GatedArgs &a, int wave, int lane) {
-        split = (int)blockIdx.x - a.whole;
-        const int tile = split < 0 ? (int)blockIdx.x : a.whole + split / a.parts;
+    __device__ __forceinline__ void init(const GatedArgs &a, int block, int wave, int lane) {
+        split = block - a.whole;
+        const int tile = split < 0 ? block : a.whole + split / a.parts;
         at = tile_at(tile, a.whole, a.tiles_m, a.tiles_n);
         const int half = F == kWeights ? a.tiles_m / 2 : a.tiles_m;
         const bool up = F == kWeights && at.tm >= half;
@@ -406,11 +406,13 @@ constexpr int gated_lds(int tiles) {
 // Adds up the parts' accumulators of a split tile in order and stores the results,
 // a block column per workgroup.
 template <class E, Form F, class S>
-__global__ __launch_bounds__(S::kThreads) void gated_join_kernel(GatedArgs a) {
+constexpr int kJoinFloats = S::WM * S::WN * 16 * GatedStore<E, F, S>::kRow;
+
+template <class E, Form F, class S>
+__device__ __forceinline__ void gated_join(const GatedArgs &a, int block, float *smem) {
     using Out = GatedStore<E, F, S>;
-    __shared__ __attribute__((aligned(16))) float smem[S::WM * S::WN * 16 * Out::kRow];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int tile = blockIdx.x / S::kMB, j = blockIdx.x % S::kMB;
+    const int tile = block / S::kMB, j = block % S::kMB;
     constexpr size_t kBlocks = (size_t)S::kNB * S::kMB * kWave, kStep = kBlocks * S::WM * S::WN;
     const f32x4 *from = reinterpret_cast<const f32x4 *>(a.partial) + (size_t)tile * a.parts * kStep + wave * kBlocks + j * S::kNB * kWave + lane;
     f32x4 acc[S::kNB];
@@ -425,6 +427,12 @@ __global__ __launch_bounds__(S::kThreads) void gated_join_kernel(GatedArgs a) {
     float *const mine = smem + wave * 16 * Out::kRow;
     Out::lay(mine, acc, 0, lane);
     out.rows(a, mine, j, 1, lane);
+}
+
+template <class E, Form F, class S>
+__global__ __launch_bounds__(S::kThreads) void gated_join_kernel(GatedArgs a) {
+    __shared__ __attribute__((aligned(16))) float smem[kJoinFloats<E, F, S>];
+    gated_join<E, F, S>(a, blockIdx.x, smem);
 }
 
 // A product by large tiles (gated_large.hip).

@@ -19,13 +19,15 @@ namespace {
 constexpr int kStages = 2;
 
 template <class E, Form F, class S>
-__global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a) {
+constexpr int kProductLds = gated_lds<E, F, S>(kStages * S::kStage);
+
+template <class E, Form F, class S>
+__device__ __forceinline__ void gated_product(const GatedArgs &a, int block, char *smem) {
     constexpr int kCopies = S::MTile::kIssue + S::NTile::kIssue;
-    __shared__ __attribute__((aligned(512))) char smem[gated_lds<E, F, S>(kStages * S::kStage)];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const auto stage = [&](int t) { return smem + t % kStages * S::kStage; };
     GatedWork<E, F, S> w;
-    w.init(a, wave, lane);
+    w.init(a, block, wave, lane);
     f32x4 acc[S::kMB][S::kNB];
 #pragma unroll
     for (int j = 0; j < S::kMB; ++j)
@@ -54,6 +56,36 @@ __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a)
     wait_vmcnt<0>();
     lds_barrier();  // no copy and no read of a tile is left
     w.store(a, acc, smem, wave, lane);
+}
+
+template <class E, Form F, class S>
+__global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a) {
+    __shared__ __attribute__((aligned(512))) char smem[kProductLds<E, F, S>];
+    gated_product<E, F, S>(a, blockIdx.x, smem);
+}
+
+template <class E, Form F>
+using SmallShape = GatedShape<E, F, 128, 128, 2, 2>;
+template <class E, Form F>
+using LowShape = GatedShape<E, F, 64, 128, 1, 4>;
+
+// Both gradients in one launch, the inputs' in the first `first` workgroups: neither
+// fills the chip by itself.  (The whole backward pass with them in one launch and in two,
+// bf16: 1024 rows of 512 -> 2048 31 and 39 us, 64 rows 14 and 18.)
+template <class E, class S, class W = SmallShape<E, kWeights>>
+__global__ __launch_bounds__(S::kThreads) void gated_gradients_kernel(GatedArgs inputs, GatedArgs weights, int first) {
+    static_assert(S::kThreads == W::kThreads, "one workgroup's size");
+    __shared__ __attribute__((aligned(512))) char smem[std::max(kProductLds<E, kInputs, S>, kProductLds<E, kWeights, W>)];
+    const int block = blockIdx.x;
+    if (block < first) gated_product<E, kInputs, S>(inputs, block, smem);
+    else gated_product<E, kWeights, W>(weights, block - first, smem);
+}
+template <class E, class S, class W = SmallShape<E, kWeights>>
+__global__ __launch_bounds__(S::kThreads) void gated_gradients_join_kernel(GatedArgs inputs, GatedArgs weights, int first) {
+    __shared__ __attribute__((aligned(16))) float smem[std::max(kJoinFloats<E, kInputs, S>, kJoinFloats<E, kWeights, W>)];
+    const int block = blockIdx.x;
+    if (block < first) gated_join<E, kInputs, S>(inputs, block, smem);
+    else gated_join<E, kWeights, W>(weights, block - first, smem);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -193,11 +225,11 @@ __global__ __launch_bounds__(kFewWaves *kWave) void gated_few_kernel(GatedArgs a
 // -------------------------------------------------------------------- alignment
 constexpr int kChunkThreads = 256;
 
-// Threads walk the chunks of eight elements in the rows' order (`per` a row):
-// f(chunk, row, first element).
+// The threads of `blocks` workgroups walk the chunks of eight elements in the rows' order
+// (`per` a row): f(chunk, row, first element).
 template <class G>
-__device__ __forceinline__ void each_chunk(long long rows, int per, G f) {
-    const long long step = (long long)gridDim.x * kChunkThreads, first = (long long)blockIdx.x * kChunkThreads + threadIdx.x;
+__device__ __forceinline__ void each_chunk(int block, int blocks, long long rows, int per, G f) {
+    const long long step = (long long)blocks * kChunkThreads, first = (long long)block * kChunkThreads + threadIdx.x;
     const long long step_r = step / per;
     const int step_c = (int)(step % per);
     long long r = first / per;
@@ -220,14 +252,17 @@ struct PadArgs {
     long long stride[3];  // bytes
     long long rows[3];
     int length;
+    int blocks;  // workgroups of each of the three
 };
 
+// The copies of workgroup `block`; false if it is none of theirs.
 template <class E>
-__global__ __launch_bounds__(kChunkThreads) void gated_pad_kernel(PadArgs a) {
+__device__ __forceinline__ bool gated_pad(const PadArgs &a, int block) {
     using Word = typename E::Word;
-    const int i = blockIdx.y, per = (a.length + 7) / 8;
-    if (!a.from[i]) return;
-    each_chunk(a.rows[i], per, [&](long long chunk, long long r, int c) {
+    if (block >= 3 * a.blocks) return false;
+    const int i = block / a.blocks, per = (a.length + 7) / 8;
+    if (!a.from[i]) return true;
+    each_chunk(block % a.blocks, a.blocks, a.rows[i], per, [&](long long chunk, long long r, int c) {
         const Word *row = (const Word *)(a.from[i] + r * a.stride[i]) + c;
         Words<E, 8> v;
         if (c + 8 <= a.length) {
@@ -238,6 +273,12 @@ __global__ __launch_bounds__(kChunkThreads) void gated_pad_kernel(PadArgs a) {
         }
         v.store((Word *)a.to[i] + chunk * 8);
     });
+    return true;
+}
+
+template <class E>
+__global__ __launch_bounds__(kChunkThreads) void gated_pad_kernel(PadArgs a) {
+    gated_pad<E>(a, blockIdx.x);
 }
 
 // ------------------------------------------------- gradients of the two products
@@ -283,12 +324,15 @@ __device__ __forceinline__ void slope8(const SlopeArgs &a, long long r, int c, f
     }
 }
 
-// Largest finite |dg| and |du| of a workgroup's share.
+// Largest finite |dg| and |du| of a workgroup's share.  (The first workgroups copy x and
+// the weights, as the next kernel's do for other types.)
 template <int kActivation>
-__global__ __launch_bounds__(kChunkThreads) void gated_most_kernel(SlopeArgs a) {
+__global__ __launch_bounds__(kChunkThreads) void gated_most_kernel(SlopeArgs a, PadArgs pad) {
+    if (gated_pad<ElemF16>(pad, blockIdx.x)) return;
+    const int block = blockIdx.x - 3 * pad.blocks, blocks = gridDim.x - 3 * pad.blocks;
     __shared__ float part[kChunkThreads / kWave];
     float most = 0.f;
-    each_chunk(a.rows, (a.hidden + 7) / 8, [&](long long, long long r, int c) {
+    each_chunk(block, blocks, a.rows, (a.hidden + 7) / 8, [&](long long, long long r, int c) {
         float dg[8], du[8];
         slope8<ElemF16, kActivation>(a, r, c, dg, du);
 #pragma unroll
@@ -302,14 +346,16 @@ __global__ __launch_bounds__(kChunkThreads) void gated_most_kernel(SlopeArgs a) 
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kChunkThreads / kWave; ++w) most = fmaxf(most, part[w]);
-        a.most[blockIdx.x] = most;
+        a.most[block] = most;
     }
 }
 
 // dg and du, rounded to the type; fp16's times a power of two that takes the
 // largest of them to 2^14 or just above.
 template <class E, int kActivation>
-__global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a, int groups) {
+__global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a, int groups, PadArgs pad) {
+    if (gated_pad<E>(pad, blockIdx.x)) return;
+    const int block = blockIdx.x - 3 * pad.blocks, blocks = gridDim.x - 3 * pad.blocks;
     int shift = 0;
     if constexpr (std::is_same_v<E, ElemF16>) {
         __shared__ float part[kChunkThreads / kWave];
@@ -321,9 +367,9 @@ __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a,
         most = part[0];
         for (int w = 1; w < kChunkThreads / kWave; ++w) most = fmaxf(most, part[w]);
         if (most > 0.f) shift = 14 - ilogbf(most);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *a.shift = shift;
+        if (block == 0 && threadIdx.x == 0) *a.shift = shift;
     }
-    each_chunk(a.rows, (int)(a.stride / 8), [&](long long i, long long r, int c) {
+    each_chunk(block, blocks, a.rows, (int)(a.stride / 8), [&](long long i, long long r, int c) {
         float dg[8], du[8];
         slope8<E, kActivation>(a, r, c, dg, du);
         Words<E, 8> x, y;
@@ -338,7 +384,7 @@ __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a,
 }
 
 // ------------------------------------------------------------------ the host
-constexpr long long kPartBytes = 256ll << 20;
+constexpr long long kPartBytes = 128ll << 20;  // of one product's sums
 
 bool bad_gated(const bfhip_gated_desc *d) {
     // (tiles past the last row are counted in an int, and a tile's rows in 32-bit offsets)
@@ -409,11 +455,6 @@ GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long lon
     return best;
 }
 
-template <class E, Form F>
-using SmallShape = GatedShape<E, F, 128, 128, 2, 2>;
-template <class E, Form F>
-using LowShape = GatedShape<E, F, 64, 128, 1, 4>;
-
 // Large tiles (16-bit), small ones or low ones (where rows of m are contiguous along k),
 // whichever are estimated to take the least time.
 template <class E, Form F>
@@ -429,30 +470,37 @@ GatedPlan gated_plan(long long m, long long n, long long k) {
 }
 
 // Whether a launch holds a product's workgroups.
-template <class E, Form F>
-bool gated_fits(long long m, long long n, long long k) {
-    const GatedPlan p = gated_plan<E, F>(m, n, k);
+bool gated_fits(const GatedPlan &p) {
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     return tiles <= 0x7fffffff && launch_fits(p.whole + (tiles - p.whole) * p.parts, 512);
 }
 
-template <class E, Form F>
-void gated_launch(GatedArgs a, hipStream_t s) {
-    const GatedPlan p = gated_plan<E, F>(a.m, a.n, a.k);
+// A product's workgroups, and of those the tiles that are split.
+struct GatedGrid {
+    long long groups, split;
+};
+
+GatedGrid gated_deal(GatedArgs &a, const GatedPlan &p) {
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
     a.whole = p.whole;
     a.parts = p.parts;
     a.per = p.per;
-    const long long split = (long long)p.tiles_m * p.tiles_n - p.whole, grid = p.whole + split * p.parts;
+    const long long split = (long long)p.tiles_m * p.tiles_n - p.whole;
+    return {p.whole + split * p.parts, split};
+}
+
+template <class E, Form F>
+void gated_launch(GatedArgs a, const GatedPlan &p, hipStream_t s) {
+    const GatedGrid g = gated_deal(a, p);
     const auto run = [&](auto shape) {
         using S = decltype(shape);
-        hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, s, a);
-        if (split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(split * S::kMB)), dim3(S::kThreads), 0, s, a);
+        hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)g.groups), dim3(S::kThreads), 0, s, a);
+        if (g.split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(g.split * S::kMB)), dim3(S::kThreads), 0, s, a);
     };
     if constexpr (E::kSize == 2) {
         if (p.kind == kLarge) {
-            launch_gated_large<E, F>(a, grid, s);
+            launch_gated_large<E, F>(a, g.groups, s);
             return;
         }
     }
@@ -463,6 +511,20 @@ void gated_launch(GatedArgs a, hipStream_t s) {
         }
     }
     run(SmallShape<E, F>{});
+}
+
+// Both gradients, none of them by large tiles.
+template <class E>
+void gated_gradients(GatedArgs inputs, const GatedPlan &pi, GatedArgs weights, const GatedPlan &pw, hipStream_t s) {
+    const GatedGrid gi = gated_deal(inputs, pi), gw = gated_deal(weights, pw);
+    const auto run = [&](auto shape) {
+        using S = decltype(shape);
+        hipLaunchKernelGGL((gated_gradients_kernel<E, S>), dim3((unsigned)(gi.groups + gw.groups)), dim3(S::kThreads), 0, s, inputs, weights, (int)gi.groups);
+        const long long ji = gi.split * S::kMB, jw = gw.split * SmallShape<E, kWeights>::kMB;
+        if (ji + jw) hipLaunchKernelGGL((gated_gradients_join_kernel<E, S>), dim3((unsigned)(ji + jw)), dim3(S::kThreads), 0, s, inputs, weights, (int)ji);
+    };
+    if (pi.kind == kLow) run(LowShape<E, kInputs>{});
+    else run(SmallShape<E, kInputs>{});
 }
 
 // Whether a forward pass goes by the kernel for few rows: up to 16, or up to 32 where the
@@ -517,28 +579,25 @@ struct Aligned {
             move(gate, d->hidden);  // (both: they have one stride)
             move(up, d->hidden);
         }
-    }
-    template <class E>
-    void launch(hipStream_t s) const {
-        if (!bytes) return;
         const long long most = std::max({pad.rows[0], pad.rows[1], pad.rows[2]}) * ((pad.length + 7) / 8);
-        const unsigned grid = (unsigned)std::min<long long>(4096, (most + kChunkThreads - 1) / kChunkThreads);
-        if (grid) hipLaunchKernelGGL(gated_pad_kernel<E>, dim3(grid, 3), dim3(kChunkThreads), 0, s, pad);
+        pad.blocks = (int)std::min<long long>(4096, (most + kChunkThreads - 1) / kChunkThreads);
     }
 };
 
-struct BackwardBytes {
-    size_t slopes, parts;  // of each of dg and du, and of the larger of the products' parts
+struct BackwardPlan {
+    GatedPlan inputs, weights;
+    size_t slopes, parts;  // bytes of each of dg and du, and of the two products' parts
     size_t all() const { return 2 * slopes + parts + up256((kMostGroups + 64) * sizeof(float)); }
 };
 
-BackwardBytes backward_bytes(const bfhip_gated_desc *d) {
-    BackwardBytes b{};
+BackwardPlan backward_plan(const bfhip_gated_desc *d) {
+    BackwardPlan b{};
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
+        b.inputs = gated_plan<E, kInputs>(d->rows, d->features, d->hidden);
+        b.weights = gated_plan<E, kWeights>(d->hidden, d->features, d->rows);
         b.slopes = up256((size_t)d->rows * slope_stride(d) * E::kSize);
-        b.parts = up256(std::max(gated_plan<E, kInputs>(d->rows, d->features, d->hidden).bytes,
-                                 gated_plan<E, kWeights>(d->hidden, d->features, d->rows).bytes));
+        b.parts = up256(b.inputs.bytes) + up256(b.weights.bytes);
     });
     return b;
 }
@@ -602,10 +661,11 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
             gated_few_launch<E>(a, s);
             return;
         }
-        fits = gated_fits<E, kForward>(a.m, a.n, a.k);
+        const GatedPlan p = gated_plan<E, kForward>(a.m, a.n, a.k);
+        fits = gated_fits(p);
         if (!fits) return;
-        in.launch<E>(s);
-        gated_launch<E, kForward>(a, s);
+        if (in.pad.blocks) hipLaunchKernelGGL(gated_pad_kernel<E>, dim3((unsigned)(3 * in.pad.blocks)), dim3(kChunkThreads), 0, s, in.pad);
+        gated_launch<E, kForward>(a, p, s);
     });
     if (!fits) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
@@ -614,7 +674,7 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
 extern "C" size_t bfhip_gated_linear_backward_workspace(const bfhip_gated_desc *d, const bfhip_matrix *x,
                                                         const bfhip_matrix *w_gate, const bfhip_matrix *w_up) {
     if (bad_gated(d) || bad_inputs(d, x, w_gate, w_up)) return 0;
-    return Aligned(d, x, w_gate, w_up, nullptr).bytes + backward_bytes(d).all();
+    return Aligned(d, x, w_gate, w_up, nullptr).bytes + backward_plan(d).all();
 }
 
 extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhip_matrix *dh, const bfhip_matrix *x,
@@ -632,7 +692,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
         return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
     const int size = d->type == BFHIP_F32 ? 4 : 2;
-    const BackwardBytes p = backward_bytes(d);
+    const BackwardPlan p = backward_plan(d);
     char *work = (char *)workspace;
     const Aligned in(d, x, w_gate, w_up, work + p.all());
     const long long stride = slope_stride(d);
@@ -652,46 +712,51 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     const long long grid = std::min<long long>(8192, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
     const bfhip_matrix slopes_g{e.dg, stride}, slopes_u{e.du, stride};
     hipStream_t s = (hipStream_t)stream;
-    bool fits = true;
+    if ((dx && !gated_fits(p.inputs)) || (dw_gate && !gated_fits(p.weights))) return fail(error, cap, "gated linear has too many rows");
     with_element(d->type, [&](auto el) {
         using E = decltype(el);
-        fits = (!dx || gated_fits<E, kInputs>(d->rows, d->features, d->hidden)) &&
-               (!dw_gate || gated_fits<E, kWeights>(d->hidden, d->features, d->rows));
-        if (!fits) return;
         if (d->rows) {
-            in.launch<E>(s);
+            const int pads = 3 * in.pad.blocks;
             with_activation(d->activation, [&](auto kind) {
                 constexpr int A = decltype(kind)::value;
-                if (d->type == BFHIP_F16) hipLaunchKernelGGL(gated_most_kernel<A>, dim3((unsigned)groups), dim3(kChunkThreads), 0, s, e);
-                hipLaunchKernelGGL((gated_slope_kernel<E, A>), dim3((unsigned)grid), dim3(kChunkThreads), 0, s, e, (int)groups);
+                PadArgs pad = in.pad;
+                if (d->type == BFHIP_F16) {
+                    hipLaunchKernelGGL(gated_most_kernel<A>, dim3((unsigned)(groups + pads)), dim3(kChunkThreads), 0, s, e, pad);
+                    pad.blocks = 0;
+                }
+                hipLaunchKernelGGL((gated_slope_kernel<E, A>), dim3((unsigned)(grid + 3 * pad.blocks)), dim3(kChunkThreads), 0, s, e, (int)groups, pad);
             });
         }
         GatedArgs a{};
-        a.activation = d->activation;
         a.shift = d->type == BFHIP_F16 && d->rows ? e.shift : nullptr;
-        a.partial = (float *)(work + 2 * p.slopes);
         a.m_op = operand(&slopes_g, &slopes_u, 2, size);
-        if (dx && d->rows) {
+        GatedArgs b = a;
+        a.partial = (float *)(work + 2 * p.slopes);
+        b.partial = (float *)(work + 2 * p.slopes + up256(p.inputs.bytes));
+        if (dx) {
             a.n_op = operand(&in.gate, &in.up, d->hidden, size);
             a.m = (int)d->rows;
             a.n = (int)d->features;
             a.k = (int)d->hidden;
             a.out[0] = (char *)dx->data;
             a.out_stride[0] = step(dx, d->rows, size);
-            gated_launch<E, kInputs>(a, s);
         }
         if (dw_gate) {
-            a.n_op = operand(&in.x, &in.x, d->rows, size);
-            a.m = (int)d->hidden;
-            a.n = (int)d->features;
-            a.k = (int)d->rows;
-            a.out[0] = (char *)dw_gate->data;
-            a.out[1] = (char *)dw_up->data;
-            a.out_stride[0] = step(dw_gate, d->hidden, size);
-            a.out_stride[1] = step(dw_up, d->hidden, size);
-            gated_launch<E, kWeights>(a, s);
+            b.n_op = operand(&in.x, &in.x, d->rows, size);
+            b.m = (int)d->hidden;
+            b.n = (int)d->features;
+            b.k = (int)d->rows;
+            b.out[0] = (char *)dw_gate->data;
+            b.out[1] = (char *)dw_up->data;
+            b.out_stride[0] = step(dw_gate, d->hidden, size);
+            b.out_stride[1] = step(dw_up, d->hidden, size);
+        }
+        if (dx && dw_gate && d->rows && p.inputs.kind != kLarge && p.weights.kind != kLarge) {
+            gated_gradients<E>(a, p.inputs, b, p.weights, s);
+        } else {
+            if (dx && d->rows) gated_launch<E, kInputs>(a, p.inputs, s);
+            if (dw_gate) gated_launch<E, kWeights>(b, p.weights, s);
         }
     });
-    if (!fits) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
 }

@@ -134,7 +134,7 @@ struct LargeLoop {
         block<I>(n1, m1, s, to);
     }
     __device__ __forceinline__ void run(const GatedArgs &a, int wave, int lane) {
-        w.init(a, wave, lane);
+        w.init(a, blockIdx.x, wave, lane);
         GatedStream<E, typename S::MTile, 0, F == kWeights, S::BK> ms(w.mt, w.k);
         GatedStream<E, typename S::NTile, S::kPair, F != kForward, S::BK> ns(w.nt, w.k);
         // Past the last step the tiles are empty: zeros, without a read.
