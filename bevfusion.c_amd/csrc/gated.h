@@ -30,6 +30,7 @@ struct GatedArgs {
     char *out[3];    // forward: h, and gate and up in fp32; inputs: dx; weights: dWg, dWu
     long long out_stride[3];  // bytes
     const int *shift;         // fp16 gradients were multiplied by 2^shift
+    long long low;            // bytes from dg and du to what their rounding left; 0: that is not taken
     int activation;
     int tiles_m, tiles_n;
     // Tiles from `whole` on are split into `parts` of `per` of the contraction's
@@ -348,6 +349,7 @@ struct GatedWork {
     typename S::NTile nt;
     uint32_t m_at, n_at;  // where the lane reads its fragments
     int k;
+    long long low;
 
     __device__ __forceinline__ void init(const GatedArgs &a, int block, int wave, int lane) {
         split = block - a.whole;
@@ -359,18 +361,21 @@ struct GatedWork {
         nt.template init<S::kPair>(a.n_op, up, at.tn * S::kCols, a.n);
         m_at = S::MTile::lane_at(wave / S::WN * S::kM, lane);
         n_at = S::NTile::lane_at(wave % S::WN * S::kN, lane);
-        // For the inputs' gradient the gate's steps, then the up's.
+        // For the inputs' gradient the gate's steps, then the up's.  With `low` each step is
+        // followed by that of what the rounding left, on the same tile of n.
         k = a.k;
+        low = F == kForward ? 0 : a.low;
         each = (k + S::BK - 1) / S::BK;
-        const int steps = F == kInputs ? 2 * each : each;
+        const int steps = (F == kInputs ? 2 : 1) * (low ? 2 : 1) * each;
         begin = split < 0 ? 0 : split % a.parts * a.per;
         end = split < 0 ? steps : min(steps, begin + a.per);
     }
     // Past the last step the tiles are empty: zeros, without a read.
     __device__ __forceinline__ void fetch(int t, const char *to) const {
-        const bool second = F == kInputs && t >= each;
-        const int k0 = t < end ? (second ? t - each : t) * S::BK : k;
-        mt.template fetch<0>(second ? mt.base_b : mt.base_a, mt.base_b, k0, k, to);
+        const int i = low ? t / 2 : t;
+        const bool second = F == kInputs && i >= each;
+        const int k0 = t < end ? (second ? i - each : i) * S::BK : k;
+        mt.template fetch<0>((second ? mt.base_b : mt.base_a) + (t & 1 ? low : 0), mt.base_b, k0, k, to);
         nt.template fetch<S::kPair>(second ? nt.base_b : nt.base_a, nt.base_b, k0, k, to + S::MTile::kBytes);
     }
     // Hands the accumulators to the results, by way of `smem`, or to the parts' sums.

@@ -286,6 +286,7 @@ struct SlopeArgs {
     const char *dh, *gate, *up;
     long long dh_stride, gate_stride, up_stride;  // bytes
     char *dg, *du;
+    long long low;     // bytes from dg and du to what their rounding leaves, 0: nowhere
     long long stride;  // elements between the rows of dg and du
     long long rows;
     int hidden;
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(kChunkThreads) void gated_most_kernel(SlopeArgs a, 
 }
 
 // dg and du, rounded to the type; fp16's times a power of two that takes the
-// largest of them to 2^14 or just above.
+// largest of them to 2^14 or just above.  With `low` what the rounding left as well.
 template <class E, int kActivation>
 __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a, int groups, PadArgs pad) {
     if (gated_pad<E>(pad, blockIdx.x)) return;
@@ -375,11 +376,23 @@ __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a,
         Words<E, 8> x, y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x.put(e, shift ? ldexpf(dg[e], shift) : dg[e]);
-            y.put(e, shift ? ldexpf(du[e], shift) : du[e]);
+            dg[e] = shift ? ldexpf(dg[e], shift) : dg[e];
+            du[e] = shift ? ldexpf(du[e], shift) : du[e];
+            x.put(e, dg[e]);
+            y.put(e, du[e]);
         }
         x.store((typename E::Word *)a.dg + i * 8);
         y.store((typename E::Word *)a.du + i * 8);
+        if (E::kSize == 2 && a.low) {
+            const auto left = [](float v, float rounded) { return fabsf(rounded) < INFINITY ? v - rounded : 0.f; };
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x.put(e, left(dg[e], x.get(e)));
+                y.put(e, left(du[e], y.get(e)));
+            }
+            x.store((typename E::Word *)(a.dg + a.low) + i * 8);
+            y.store((typename E::Word *)(a.du + a.low) + i * 8);
+        }
     });
 }
 
@@ -425,13 +438,13 @@ struct GatedTimes {
 // Tiles in rounds of as many workgroups as the chip holds; those of the last round may
 // be split along the contraction, whichever number of parts is estimated to take least.
 template <class S>
-GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long long k, const GatedTimes &c) {
+GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long long k, int passes, const GatedTimes &c) {
     constexpr int kCus = 256;
     GatedPlan best{};
     best.kind = kind;
     best.tiles_m = (int)((m + S::BM - 1) / S::BM * (f == kWeights ? 2 : 1));
     best.tiles_n = (int)((n + S::kCols - 1) / S::kCols);
-    const long long steps = (k + S::BK - 1) / S::BK * (f == kInputs ? 2 : 1), tiles = (long long)best.tiles_m * best.tiles_n;
+    const long long steps = (k + S::BK - 1) / S::BK * passes * (f == kInputs ? 2 : 1), tiles = (long long)best.tiles_m * best.tiles_n;
     const long long tile_bytes = (long long)S::BM * S::BN * sizeof(float), rest = tiles % (kCus * c.resident);
     const auto time = [&](long long groups, long long each) {
         const long long turns = (groups + kCus - 1) / kCus, rounds = (turns + c.resident - 1) / c.resident;
@@ -456,16 +469,19 @@ GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long lon
 }
 
 // Large tiles (16-bit), small ones or low ones (where rows of m are contiguous along k),
-// whichever are estimated to take the least time.
+// whichever are estimated to take the least time.  passes: 2 where what the rounding of
+// the slopes left is taken too (not by large tiles), 1 otherwise.
 template <class E, Form F>
-GatedPlan gated_plan(long long m, long long n, long long k) {
+GatedPlan gated_plan(long long m, long long n, long long k, int passes = 1) {
     constexpr bool kHalf = E::kSize == 2;
-    GatedPlan p = plan_tiles<SmallShape<E, F>>(kSmall, F, m, n, k, kHalf ? GatedTimes{2, 0.46, 0.62, 1.6} : GatedTimes{2, 1.93, 2.1, 0.5});
+    GatedPlan p = plan_tiles<SmallShape<E, F>>(kSmall, F, m, n, k, passes, kHalf ? GatedTimes{2, 0.46, 0.62, 1.6} : GatedTimes{2, 1.93, 2.1, 0.5});
     const auto take = [&](const GatedPlan &q) {
         if (q.time < p.time) p = q;
     };
-    if constexpr (F != kWeights) take(plan_tiles<LowShape<E, F>>(kLow, F, m, n, k, kHalf ? GatedTimes{3, 0.34, 0.48, 0.75} : GatedTimes{3, 1.0, 1.15, 0.2}));
-    if constexpr (kHalf) take(plan_tiles<LargeShape<E, F>>(kLarge, F, m, n, k, GatedTimes{1, 1.13, 1.13, 7.1}));
+    if constexpr (F != kWeights) take(plan_tiles<LowShape<E, F>>(kLow, F, m, n, k, passes, kHalf ? GatedTimes{3, 0.34, 0.48, 0.75} : GatedTimes{3, 1.0, 1.15, 0.2}));
+    if constexpr (kHalf) {
+        if (passes == 1) take(plan_tiles<LargeShape<E, F>>(kLarge, F, m, n, k, 1, GatedTimes{1, 1.13, 1.13, 7.1}));
+    }
     return p;
 }
 
@@ -584,19 +600,31 @@ struct Aligned {
     }
 };
 
+// Up to this many slopes (rows * hidden) enter the products in two parts, rounded and what
+// the rounding left.  Of many slopes the roundings average out to about the error that
+// the results' own rounding has; of few one or two large ones can make it more.  (So few
+// products are bound by their launches and the weights: the backward pass of 16 rows of 1024 ->
+// 1024 bf16 13.8 us, 12.1 without; one row of 4096 -> 11008 117 and 106.)
+constexpr long long kFewSlopes = 1 << 14;
+
 struct BackwardPlan {
     GatedPlan inputs, weights;
-    size_t slopes, parts;  // bytes of each of dg and du, and of the two products' parts
-    size_t all() const { return 2 * slopes + parts + up256((kMostGroups + 64) * sizeof(float)); }
+    size_t slope, slopes;  // bytes of dg, and of all that is kept of dg and du
+    size_t parts;          // of the two products' parts
+    long long low;         // from dg and du to what their rounding left, or 0
+    size_t all() const { return slopes + parts + up256((kMostGroups + 64) * sizeof(float)); }
 };
 
 BackwardPlan backward_plan(const bfhip_gated_desc *d) {
     BackwardPlan b{};
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
-        b.inputs = gated_plan<E, kInputs>(d->rows, d->features, d->hidden);
-        b.weights = gated_plan<E, kWeights>(d->hidden, d->features, d->rows);
-        b.slopes = up256((size_t)d->rows * slope_stride(d) * E::kSize);
+        const int passes = E::kSize == 2 && d->rows * d->hidden <= kFewSlopes ? 2 : 1;
+        b.inputs = gated_plan<E, kInputs>(d->rows, d->features, d->hidden, passes);
+        b.weights = gated_plan<E, kWeights>(d->hidden, d->features, d->rows, passes);
+        b.slope = up256((size_t)d->rows * slope_stride(d) * E::kSize);
+        b.slopes = 2 * passes * b.slope;
+        b.low = passes > 1 ? 2 * b.slope : 0;
         b.parts = up256(b.inputs.bytes) + up256(b.weights.bytes);
     });
     return b;
@@ -702,11 +730,12 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     e.gate = (const char *)gate->data; e.gate_stride = step(gate, d->rows, sizeof(float));
     e.up = (const char *)up->data; e.up_stride = step(up, d->rows, sizeof(float));
     e.dg = work;
-    e.du = work + p.slopes;
+    e.du = work + p.slope;
+    e.low = p.low;
     e.stride = stride;
     e.rows = d->rows;
     e.hidden = (int)d->hidden;
-    e.most = (float *)(work + 2 * p.slopes + p.parts);
+    e.most = (float *)(work + p.slopes + p.parts);
     e.shift = (int *)(e.most + kMostGroups);
     const long long groups = std::min<long long>(kMostGroups, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
     const long long grid = std::min<long long>(8192, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
@@ -730,9 +759,10 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
         GatedArgs a{};
         a.shift = d->type == BFHIP_F16 && d->rows ? e.shift : nullptr;
         a.m_op = operand(&slopes_g, &slopes_u, 2, size);
+        a.low = p.low;
         GatedArgs b = a;
-        a.partial = (float *)(work + 2 * p.slopes);
-        b.partial = (float *)(work + 2 * p.slopes + up256(p.inputs.bytes));
+        a.partial = (float *)(work + p.slopes);
+        b.partial = (float *)(work + p.slopes + up256(p.inputs.bytes));
         if (dx) {
             a.n_op = operand(&in.gate, &in.up, d->hidden, size);
             a.m = (int)d->rows;

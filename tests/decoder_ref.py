@@ -81,11 +81,14 @@ def gated_linear(x, w_gate, w_up, activation):
                 up=(u, SLACK * e_u + U * u.abs() + 1e-30))
 
 
-def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation):
-    """Dict of (value, bound) for dx, dw_gate and dw_up."""
+def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation, left=False):
+    """Dict of (value, bound) for dx, dw_gate and dw_up.  left: what the slopes'
+    rounding left is taken too (few slopes), which leaves a rounding of that, and
+    twice as many terms."""
     h, t, (rows, hidden) = half(x.dtype), tiny(x.dtype), gate.shape
     dtype = x.dtype
     hp = 0.0 if dtype == torch.float32 else h  # rounding on the way into the matrix cores
+    hp, terms = (hp * hp, 2) if left else (hp, 1)
     dh, x, wg, wu, g, u = (v.double() for v in (dh, x, w_gate, w_up, gate, up))
     a, d, e_a, e_d = _activation(activation, g, dtype)
     dg, du = dh * u * d, dh * a
@@ -97,9 +100,9 @@ def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation):
         most = max(dg.abs().max(), du.abs().max()) * 2.0 ** (-25 - 14)
         e_g, e_u = e_g + most, e_u + most
     res = {}
-    k = 2 * hidden + 16
+    k = terms * 2 * hidden + 16
     res["dx"] = dg @ wg + du @ wu, (e_g + k * U * dg.abs()) @ wg.abs() + (e_u + k * U * du.abs()) @ wu.abs()
-    xa, k = x.abs().contiguous(), rows + 16
+    xa, k = x.abs().contiguous(), terms * rows + 16
     for name, v, e in (("dw_gate", dg, e_g), ("dw_up", du, e_u)):
         res[name] = v.T.contiguous() @ x, (e + k * U * v.abs()).T.contiguous() @ xa
     return {n: (v, SLACK * b + h * v.abs() + t + 1e-30) for n, (v, b) in res.items()}

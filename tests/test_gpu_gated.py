@@ -94,6 +94,34 @@ def test_activations(device, dtype, activation):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("size", [(1, 300, 70), (1, 4096, 1000), (7, 64, 2300), (16, 520, 1024), (70, 40, 234), (16384, 24, 1)], ids=str)
+def test_few_slopes(device, dtype, size):
+    """Up to 16384 slopes reach the gradients with twice the type's precision."""
+    rows, features, hidden = size
+    assert rows * hidden <= 1 << 14
+    call, dh = inputs(device, dtype, rows, features, hidden)
+    call["x"][:, 0] = 0  # (a column whose gradients are zeros)
+    forward, back = run(call, dh, "gelu")
+    want = ref.gated_linear_backward(dh, **call, gate=forward["gate"], up=forward["up"], activation="gelu", left=True)
+    for name, (value, bound) in want.items():
+        check_finite(name, back[name], value, bound)
+    assert not back["dw_gate"][:, 0].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_few_slopes_that_are_infinite(device, dtype):
+    """What the rounding of an infinite slope left is nothing, not NaN."""
+    call, dh = inputs(device, dtype, 4, 64, 96)
+    h, gate, up = bfhip.gated_linear(**call, save=True)
+    gate[1], up[1, 5], call["x"][1] = 40.0, math.inf, 1.0
+    dh[1] = 1.0
+    dx, dw_gate, dw_up = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up)
+    rest = torch.arange(96, device=device) != 5
+    assert (dw_gate[5] == math.inf).all() and dw_gate[rest].isfinite().all() and dw_up.isfinite().all()
+    assert (dx[1].abs() == math.inf).all() and dx[[0, 2, 3]].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
 def test_large_tiles(device, dtype):
     """Results of more tiles than CUs, whole and ragged."""
     compare(*inputs(device, dtype, 4096, 256, 2048), "silu")
