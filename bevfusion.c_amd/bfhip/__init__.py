@@ -332,8 +332,11 @@ def hip_lib():
     return _hip_lib
 
 
+_ErrorText = C.c_char * 512
+
+
 def _err():
-    return C.create_string_buffer(512)
+    return _ErrorText()
 
 
 def _check(ok, err, what):
@@ -809,41 +812,50 @@ def _rotary(q, k, positions, frequencies, interleaved, amplitude, out, stream, i
     return to_q if k is None else (to_q, to_k)
 
 
-def _page_pool(what, t, like, dim):
+def _page_pool(what, t, shape, dtype, device):
     """[pages, page_size, kv_heads, head_dim] with contiguous heads -> Pages."""
-    shape, stride = t.shape, t.stride()
-    if (len(shape) != 4 or shape[3] != dim or (stride[3] != 1 and dim > 1)
-            or t.dtype != like.dtype or t.device != like.device):
-        raise BfHipError(f"{what} must be a {like.dtype} [pages, page_size, kv_heads, {dim}] tensor "
-                         f"with contiguous heads on {like.device}")
+    stride = t.stride()
+    if (t.shape != shape or t.dtype != dtype or t.device != device
+            or (stride[3] != 1 and shape[3] > 1)):
+        raise BfHipError(f"{what} must be a {dtype} {list(shape)} tensor with contiguous heads on "
+                         f"{device}")
     return Pages(t.data_ptr(), stride[0], stride[1], stride[2])
 
 
+def _ints(what, t, n, dtype, device):
+    """Address of `t`, n contiguous whole numbers."""
+    if t.dtype != dtype or t.device != device or t.shape != (n,) or not t.is_contiguous():
+        raise BfHipError(f"{what} must be a contiguous {dtype} [{n}] tensor on {device}")
+    return t.data_ptr()
+
+
 def _paged_desc(like, heads, k_pages, v_pages, page_table, starts, lengths, scale, bias):
-    int32, dim = _torch().int32, like.shape[2]
-    pools = (_page_pool("k_pages", k_pages, like, dim), _page_pool("v_pages", v_pages, like, dim))
-    shape = k_pages.shape
-    if shape != v_pages.shape:
+    code, int32, (tokens, _, dim) = _type_code(like), _torch().int32, like.shape
+    dtype, device, shape = like.dtype, like.device, k_pages.shape
+    if len(shape) != 4 or shape[3] != dim:
+        raise BfHipError(f"k_pages must be [pages, page_size, kv_heads, {dim}]")
+    if v_pages.shape != shape:
         raise BfHipError("k_pages and v_pages must have one shape")
+    pools = (_page_pool("k_pages", k_pages, shape, dtype, device),
+             _page_pool("v_pages", v_pages, shape, dtype, device))
     n = starts.numel() - 1
     if n < 0:
         raise BfHipError("starts must hold one entry more than there are sequences")
     table, strides = page_table.shape, page_table.stride()
     if (len(table) != 2 or table[0] != n or page_table.dtype != int32
-            or page_table.device != like.device or (strides[1] != 1 and table[1] > 1)):
+            or page_table.device != device or (strides[1] != 1 and table[1] > 1)):
         raise BfHipError(f"page_table must be an int32 [{n}, pages of a sequence] tensor with "
-                         f"contiguous rows on {like.device}")
+                         f"contiguous rows on {device}")
     reach, pb = 0, None
     if bias is not None:
         if bias.dim() != 2 or bias.shape[1] % 2 == 0:
             raise BfHipError("bias must be [heads, 2 * reach + 1]")
         reach = bias.shape[1] // 2
         pb = _expect("bias", bias, like, (heads, 2 * reach + 1), _torch().float32)
-    return PagedDesc(_type_code(like), n, heads, shape[2], dim, shape[1], table[1], reach, scale,
-                     like.shape[0], shape[0], strides[0],
-                     _expect("starts", starts, like, (n + 1,), int32),
-                     _expect("lengths", lengths, like, (n,), int32), page_table.data_ptr(),
-                     pb), pools
+    pages, page_size, kv_heads, _ = shape
+    return PagedDesc(code, n, heads, kv_heads, dim, page_size, table[1], reach, scale, tokens, pages,
+                     strides[0], _ints("starts", starts, n + 1, int32, device),
+                     _ints("lengths", lengths, n, int32, device), page_table.data_ptr(), pb), pools
 
 
 def cache_append(k, v, k_pages, v_pages, page_table, starts, lengths, stream=None):
@@ -853,10 +865,10 @@ def cache_append(k, v, k_pages, v_pages, page_table, starts, lengths, stream=Non
     [sequences + 1], the sequences' new tokens; lengths int32 [sequences], their
     keys with the new tokens, which stand at the end."""
     rows = [_head_rows("k", k, k), _head_rows("v", v, k)]
-    if k.shape != v.shape or k.shape[1] != k_pages.shape[2]:
+    shape = k.shape
+    desc, pools = _paged_desc(k, shape[1], k_pages, v_pages, page_table, starts, lengths, 1.0, None)
+    if v.shape != shape or shape[1] != desc.kv_heads:
         raise BfHipError("k and v must have one shape, with the pages' heads")
-    desc, pools = _paged_desc(k, k.shape[1], k_pages, v_pages, page_table, starts, lengths, 1.0,
-                              None)
     with _place(stream, k, v, k_pages, v_pages, page_table, starts, lengths) as queue:
         err = _err()
         _check(hip_lib().bfhip_cache_append(desc, *rows, *pools, queue, err, 512), err,

@@ -148,3 +148,8 @@ def test_python_refuses():
     for k2, v2 in ((k, k[:3]), (k[:, :1], k[:, :1]), (k[0], k[0])):
         with pytest.raises(bfhip.BfHipError):
             bfhip.cache_append(k2, v2, **good)
+    for bad in (dict(k_pages=pages[0, 0], v_pages=pages[0, 0]), dict(page_table=table[0]), dict(starts=starts[:0])):
+        with pytest.raises(bfhip.BfHipError):
+            bfhip.cache_append(k, k, **dict(good, **bad))
+        with pytest.raises(bfhip.BfHipError):
+            bfhip.paged_attention(k, **dict(good, **bad))
