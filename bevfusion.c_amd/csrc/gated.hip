@@ -10,22 +10,24 @@ using namespace bfhip;
 
 namespace {
 
-// Small and low tiles, where there are too few large ones: two stages in LDS, one of
-// them in flight while the other is multiplied, so that two workgroups of small tiles
-// or three of low ones share a CU and cover each other's waits, ways in and ways out.
-// (With four stages a workgroup is alone there and no faster for it.  Forward, 999 rows
-// of 776 -> 2056, fp16, 264 tiles: 17 us, 26 with four; gradient of 5632 x 2048 weights,
-// 512 rows, bf16: 36 and 57.)
-constexpr int kStages = 2;
+// Small and low tiles, where there are too few large ones.  `kStages` steps' tiles lie in
+// LDS; while one is multiplied the others are on their way.  Small ones have two: two
+// workgroups then share a CU and cover each other's waits, ways in and ways out.  (With
+// four a workgroup is alone there: forward, 999 rows of 776 -> 2056 fp16, 264 tiles: 17
+// us, 26 with four; gradient of 5632 x 2048 weights by 512 rows bf16: 36 and 60.)  With
+// four they are `deep` ones, for tiles that are no more than the CUs and stream weights from
+// memory (128 rows of 4096 -> 11008 bf16: 53 us, 65 with two).  Low ones have three, and share
+// a CU by twos (64 rows of 4096 -> 11008 bf16: 44 us, 59 with two stages).
+constexpr int kSmallStages = 2, kDeepStages = 4, kLowStages = 3;
 
-template <class E, Form F, class S>
+template <class E, Form F, class S, int kStages>
 constexpr int kProductLds = gated_lds<E, F, S>(kStages * S::kStage);
 
-template <class E, Form F, class S>
+template <class E, Form F, class S, int kStages>
 __device__ __forceinline__ void gated_product(const GatedArgs &a, int block, char *smem) {
     constexpr int kCopies = S::MTile::kIssue + S::NTile::kIssue;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const auto stage = [&](int t) { return smem + t % kStages * S::kStage; };
+    const auto stage = [&](int t) { return smem + (uint32_t)t % kStages * S::kStage; };
     GatedWork<E, F, S> w;
     w.init(a, block, wave, lane);
     f32x4 acc[S::kMB][S::kNB];
@@ -58,10 +60,10 @@ __device__ __forceinline__ void gated_product(const GatedArgs &a, int block, cha
     w.store(a, acc, smem, wave, lane);
 }
 
-template <class E, Form F, class S>
+template <class E, Form F, class S, int kStages>
 __global__ __launch_bounds__(S::kThreads) void gated_product_kernel(GatedArgs a) {
-    __shared__ __attribute__((aligned(512))) char smem[kProductLds<E, F, S>];
-    gated_product<E, F, S>(a, blockIdx.x, smem);
+    __shared__ __attribute__((aligned(512))) char smem[kProductLds<E, F, S, kStages>];
+    gated_product<E, F, S, kStages>(a, blockIdx.x, smem);
 }
 
 template <class E, Form F>
@@ -72,13 +74,13 @@ using LowShape = GatedShape<E, F, 64, 128, 1, 4>;
 // Both gradients in one launch, the inputs' in the first `first` workgroups: neither
 // fills the chip by itself.  (The whole backward pass with them in one launch and in two,
 // bf16: 1024 rows of 512 -> 2048 31 and 39 us, 64 rows 14 and 18.)
-template <class E, class S, class W = SmallShape<E, kWeights>>
+template <class E, class S, int kStages, class W = SmallShape<E, kWeights>>
 __global__ __launch_bounds__(S::kThreads) void gated_gradients_kernel(GatedArgs inputs, GatedArgs weights, int first) {
     static_assert(S::kThreads == W::kThreads, "one workgroup's size");
-    __shared__ __attribute__((aligned(512))) char smem[std::max(kProductLds<E, kInputs, S>, kProductLds<E, kWeights, W>)];
+    __shared__ __attribute__((aligned(512))) char smem[std::max(kProductLds<E, kInputs, S, kStages>, kProductLds<E, kWeights, W, kSmallStages>)];
     const int block = blockIdx.x;
-    if (block < first) gated_product<E, kInputs, S>(inputs, block, smem);
-    else gated_product<E, kWeights, W>(weights, block - first, smem);
+    if (block < first) gated_product<E, kInputs, S, kStages>(inputs, block, smem);
+    else gated_product<E, kWeights, W, kSmallStages>(weights, block - first, smem);
 }
 template <class E, class S, class W = SmallShape<E, kWeights>>
 __global__ __launch_bounds__(S::kThreads) void gated_gradients_join_kernel(GatedArgs inputs, GatedArgs weights, int first) {
@@ -418,7 +420,7 @@ bool chunked(const bfhip_matrix *x, long long rows, long long length, int size) 
     return ((uintptr_t)x->data & 15) == 0 && length % words == 0 && (rows <= 1 || (x->stride % words == 0 && x->stride < 1 << 21));
 }
 
-enum GatedTiles { kSmall, kLow, kLarge };
+enum GatedTiles { kSmall, kDeep, kLow, kLarge };
 
 struct GatedPlan {
     GatedTiles kind;
@@ -437,8 +439,9 @@ struct GatedTimes {
 
 // Tiles in rounds of as many workgroups as the chip holds; those of the last round may
 // be split along the contraction, whichever number of parts is estimated to take least.
+// `least`: the time that the operands' way from memory takes at least, in us.
 template <class S>
-GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long long k, int passes, const GatedTimes &c) {
+GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long long k, int passes, double least, const GatedTimes &c) {
     constexpr int kCus = 256;
     GatedPlan best{};
     best.kind = kind;
@@ -452,12 +455,12 @@ GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long lon
     };
     best.whole = (int)std::min(tiles, 0x7fffffffll);
     best.parts = 1;
-    best.time = time(tiles, steps);
+    best.time = std::max(time(tiles, steps), least);
     for (const int p : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
         const long long per = (steps + p - 1) / p, parts = per ? (steps + per - 1) / per : 0, bytes = parts * rest * tile_bytes;
         if (!rest || steps < 2 * p || bytes > kPartBytes) break;
-        // (the launch that joins the parts: 1.8 us, 0.17 a part, 4.2 TB/s)
-        const double t = time(tiles - rest, steps) + time(rest * parts, per) + 1.8 + 0.17 * parts + bytes / 4.2e6;
+        // (the launch that joins the parts: 4 us with the host's time for it, 0.17 a part, 4.2 TB/s)
+        const double t = std::max(time(tiles - rest, steps) + time(rest * parts, per), least) + 4 + 0.17 * parts + bytes / 4.2e6;
         if (t >= best.time) continue;
         best.time = t;
         best.whole = (int)(tiles - rest);
@@ -468,21 +471,26 @@ GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long lon
     return best;
 }
 
-// Large tiles (16-bit), small ones or low ones (where rows of m are contiguous along k),
-// whichever are estimated to take the least time.  passes: 2 where what the rounding of
-// the slopes left is taken too (not by large tiles), 1 otherwise.
+// Large, small, deep or low tiles (deep and large ones of 16-bit types, deep and low ones
+// where rows of m are contiguous along k), whichever are estimated to take the least
+// time.  passes: 2 where what the rounding of the slopes left is taken too (not by large
+// tiles), 1 otherwise.
 template <class E, Form F>
-GatedPlan gated_plan(long long m, long long n, long long k, int passes = 1) {
+GatedPlan gated_plan(long long m, long long n, long long k, int passes = 1, bool large = true) {
     constexpr bool kHalf = E::kSize == 2;
-    GatedPlan p = plan_tiles<SmallShape<E, F>>(kSmall, F, m, n, k, passes, kHalf ? GatedTimes{2, 0.46, 0.62, 1.6} : GatedTimes{2, 1.93, 2.1, 0.5});
-    const auto take = [&](const GatedPlan &q) {
-        if (q.time < p.time) p = q;
+    const double least = (double)k * ((F == kForward ? 1 : 2) * m + (F == kWeights ? 1 : 2) * n) * E::kSize / 4.8e6;
+    GatedPlan best{};
+    const auto take = [&](auto shape, GatedTiles kind, const GatedTimes &c) {
+        const GatedPlan p = plan_tiles<decltype(shape)>(kind, F, m, n, k, passes, least, c);
+        if (!best.parts || p.time < best.time) best = p;
     };
-    if constexpr (F != kWeights) take(plan_tiles<LowShape<E, F>>(kLow, F, m, n, k, passes, kHalf ? GatedTimes{3, 0.34, 0.48, 0.75} : GatedTimes{3, 1.0, 1.15, 0.2}));
+    take(SmallShape<E, F>{}, kSmall, kHalf ? GatedTimes{2, 0.56, 0.74, 1.4} : GatedTimes{2, 1.9, 2.17, 1.95});
+    if constexpr (F != kWeights) take(LowShape<E, F>{}, kLow, kHalf ? GatedTimes{2, 0.41, 0.45, 1.0} : GatedTimes{2, 1.06, 1.22, 1.45});
+    if constexpr (kHalf && F != kWeights) take(SmallShape<E, F>{}, kDeep, GatedTimes{1, 0.64, 0.64, 3.0});
     if constexpr (kHalf) {
-        if (passes == 1) take(plan_tiles<LargeShape<E, F>>(kLarge, F, m, n, k, 1, GatedTimes{1, 1.13, 1.13, 7.1}));
+        if (large && passes == 1) take(LargeShape<E, F>{}, kLarge, GatedTimes{1, 1.18, 1.18, 6.8});
     }
-    return p;
+    return best;
 }
 
 // Whether a launch holds a product's workgroups.
@@ -506,12 +514,15 @@ GatedGrid gated_deal(GatedArgs &a, const GatedPlan &p) {
     return {p.whole + split * p.parts, split};
 }
 
+template <int kStages>
+using Stages = std::integral_constant<int, kStages>;
+
 template <class E, Form F>
 void gated_launch(GatedArgs a, const GatedPlan &p, hipStream_t s) {
     const GatedGrid g = gated_deal(a, p);
-    const auto run = [&](auto shape) {
+    const auto run = [&](auto shape, auto stages) {
         using S = decltype(shape);
-        hipLaunchKernelGGL((gated_product_kernel<E, F, S>), dim3((unsigned)g.groups), dim3(S::kThreads), 0, s, a);
+        hipLaunchKernelGGL((gated_product_kernel<E, F, S, decltype(stages)::value>), dim3((unsigned)g.groups), dim3(S::kThreads), 0, s, a);
         if (g.split) hipLaunchKernelGGL((gated_join_kernel<E, F, S>), dim3((unsigned)(g.split * S::kMB)), dim3(S::kThreads), 0, s, a);
     };
     if constexpr (E::kSize == 2) {
@@ -519,28 +530,34 @@ void gated_launch(GatedArgs a, const GatedPlan &p, hipStream_t s) {
             launch_gated_large<E, F>(a, g.groups, s);
             return;
         }
+        if constexpr (F != kWeights) {
+            if (p.kind == kDeep) {
+                run(SmallShape<E, F>{}, Stages<kDeepStages>{});
+                return;
+            }
+        }
     }
     if constexpr (F != kWeights) {
         if (p.kind == kLow) {
-            run(LowShape<E, F>{});
+            run(LowShape<E, F>{}, Stages<kLowStages>{});
             return;
         }
     }
-    run(SmallShape<E, F>{});
+    run(SmallShape<E, F>{}, Stages<kSmallStages>{});
 }
 
-// Both gradients, none of them by large tiles.
+// Both gradients, none of them by large tiles (deep ones share CUs here: they are small).
 template <class E>
 void gated_gradients(GatedArgs inputs, const GatedPlan &pi, GatedArgs weights, const GatedPlan &pw, hipStream_t s) {
     const GatedGrid gi = gated_deal(inputs, pi), gw = gated_deal(weights, pw);
-    const auto run = [&](auto shape) {
+    const auto run = [&](auto shape, auto stages) {
         using S = decltype(shape);
-        hipLaunchKernelGGL((gated_gradients_kernel<E, S>), dim3((unsigned)(gi.groups + gw.groups)), dim3(S::kThreads), 0, s, inputs, weights, (int)gi.groups);
+        hipLaunchKernelGGL((gated_gradients_kernel<E, S, decltype(stages)::value>), dim3((unsigned)(gi.groups + gw.groups)), dim3(S::kThreads), 0, s, inputs, weights, (int)gi.groups);
         const long long ji = gi.split * S::kMB, jw = gw.split * SmallShape<E, kWeights>::kMB;
         if (ji + jw) hipLaunchKernelGGL((gated_gradients_join_kernel<E, S>), dim3((unsigned)(ji + jw)), dim3(S::kThreads), 0, s, inputs, weights, (int)ji);
     };
-    if (pi.kind == kLow) run(LowShape<E, kInputs>{});
-    else run(SmallShape<E, kInputs>{});
+    if (pi.kind == kLow) run(LowShape<E, kInputs>{}, Stages<kLowStages>{});
+    else run(SmallShape<E, kInputs>{}, Stages<kSmallStages>{});
 }
 
 // Whether a forward pass goes by the kernel for few rows: up to 16, or up to 32 where the
@@ -609,6 +626,7 @@ constexpr long long kFewSlopes = 1 << 14;
 
 struct BackwardPlan {
     GatedPlan inputs, weights;
+    bool together;  // in one launch, where both are wanted
     size_t slope, slopes;  // bytes of dg, and of all that is kept of dg and du
     size_t parts;          // of the two products' parts
     long long low;         // from dg and du to what their rounding left, or 0
@@ -620,8 +638,16 @@ BackwardPlan backward_plan(const bfhip_gated_desc *d) {
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
         const int passes = E::kSize == 2 && d->rows * d->hidden <= kFewSlopes ? 2 : 1;
-        b.inputs = gated_plan<E, kInputs>(d->rows, d->features, d->hidden, passes);
-        b.weights = gated_plan<E, kWeights>(d->hidden, d->features, d->rows, passes);
+        const auto plan = [&](bool large) {
+            b.inputs = gated_plan<E, kInputs>(d->rows, d->features, d->hidden, passes, large);
+            b.weights = gated_plan<E, kWeights>(d->hidden, d->features, d->rows, passes, large);
+            return b.inputs.time + b.weights.time;
+        };
+        // (one launch takes about 6 us less than two: see gated_gradients_kernel)
+        const double one = plan(false) - 6;
+        b.together = true;
+        if (plan(true) < one) b.together = b.inputs.kind != kLarge && b.weights.kind != kLarge;
+        else plan(false);
         b.slope = up256((size_t)d->rows * slope_stride(d) * E::kSize);
         b.slopes = 2 * passes * b.slope;
         b.low = passes > 1 ? 2 * b.slope : 0;
@@ -781,7 +807,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             b.out_stride[0] = step(dw_gate, d->hidden, size);
             b.out_stride[1] = step(dw_up, d->hidden, size);
         }
-        if (dx && dw_gate && d->rows && p.inputs.kind != kLarge && p.weights.kind != kLarge) {
+        if (dx && dw_gate && d->rows && p.together) {
             gated_gradients<E>(a, p.inputs, b, p.weights, s);
         } else {
             if (dx && d->rows) gated_launch<E, kInputs>(a, p.inputs, s);
