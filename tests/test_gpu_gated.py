@@ -212,6 +212,31 @@ def test_rows_do_not_depend_on_others(device, dtype):
         assert torch.equal(h[keep], want["h"][keep]) and not torch.isfinite(h[33]).all()
 
 
+@pytest.mark.parametrize("size", [(128, 4096, 1100), (999, 771, 2055), (5, 64, 300), (2100, 33, 65), (4100, 2808, 2810)], ids=str)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_one_gradient(device, dtype, size):
+    """The inputs' gradient alone or the weights' alone: the same bits, nothing else
+    written, in a workspace of the stated size."""
+    call, dh = inputs(device, dtype, *size)
+    h, gate, up = bfhip.gated_linear(**call, save=True)
+    want = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up)
+    lib, error = bfhip.hip_lib(), bfhip._err()
+    matrix = lambda t: bfhip.Matrix(t.data_ptr(), t.stride(0))
+    desc = bfhip.GatedDesc(bfhip._type_code(dh), 0, *size)
+    given = [matrix(call[n]) for n in ("x", "w_gate", "w_up")]
+    bytes_ = lib.bfhip_gated_linear_backward_workspace(desc, *given)
+    for wanted in ((True, False, False), (False, True, True), (True, True, True)):
+        got = [torch.full_like(t, 7) if w else None for t, w in zip(want, wanted)]
+        work = torch.full((bytes_ + 256,), 0xa5, dtype=torch.uint8, device=device)
+        ok = lib.bfhip_gated_linear_backward(desc, matrix(dh), *given, matrix(gate), matrix(up),
+                                             *(t if t is None else matrix(t) for t in got), work.data_ptr(), bytes_,
+                                             torch.cuda.current_stream().cuda_stream, error, 512)
+        assert ok, error.value
+        assert (work[bytes_:] == 0xa5).all()
+        for t, g in zip(want, got):
+            assert g is None or torch.equal(g, t)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_no_rows(device, dtype):
     call, dh = inputs(device, dtype, 0, 24, 40)
