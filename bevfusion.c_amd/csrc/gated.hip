@@ -474,6 +474,12 @@ GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long lon
     return best;
 }
 
+// Whether a launch holds a product's workgroups.
+bool gated_fits(const GatedPlan &p) {
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    return tiles <= 0x7fffffff && launch_fits(p.whole + (tiles - p.whole) * p.parts, 512);
+}
+
 // Large, small, deep or low tiles (deep and large ones of 16-bit types, deep and low ones
 // where rows of m are contiguous along k), whichever are estimated to take the least
 // time.  passes: 2 where what the rounding of the slopes left is taken too (not by large
@@ -485,7 +491,8 @@ GatedPlan gated_plan(long long m, long long n, long long k, int passes = 1, bool
     GatedPlan best{};
     const auto take = [&](auto shape, GatedTiles kind, const GatedTimes &c) {
         const GatedPlan p = plan_tiles<decltype(shape)>(kind, F, m, n, k, passes, least, c);
-        if (!best.parts || p.time < best.time) best = p;
+        // (a launch that holds its tiles before one that does not)
+        if (!best.parts || gated_fits(p) > gated_fits(best) || (gated_fits(p) == gated_fits(best) && p.time < best.time)) best = p;
     };
     take(SmallShape<E, F>{}, kSmall, kHalf ? GatedTimes{2, 0.56, 0.74, 1.4} : GatedTimes{2, 1.9, 2.17, 1.95});
     if constexpr (F != kWeights) take(LowShape<E, F>{}, kLow, kHalf ? GatedTimes{2, 0.41, 0.45, 1.0} : GatedTimes{2, 1.06, 1.22, 1.45});
@@ -494,12 +501,6 @@ GatedPlan gated_plan(long long m, long long n, long long k, int passes = 1, bool
         if (large && passes == 1) take(LargeShape<E, F>{}, kLarge, GatedTimes{1, 1.18, 1.18, 6.8});
     }
     return best;
-}
-
-// Whether a launch holds a product's workgroups.
-bool gated_fits(const GatedPlan &p) {
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    return tiles <= 0x7fffffff && launch_fits(p.whole + (tiles - p.whole) * p.parts, 512);
 }
 
 // A product's workgroups, and of those the tiles that are split.

@@ -321,9 +321,10 @@ int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
  * Any alignment will do; x and weights whose pointers, strides and rows are
  * multiples of 16 bytes (and strides below 2 Mi elements) need no copy.  Wg and Wu
  * have one stride.  Results overlap nothing.  rows at most 0x7fff0000, features and
- * hidden 1 .. 2^20, no matrix of more than 2^40 elements.  The workspace holds dg and du, copies of x
- * and the weights where they need them (more than 16 rows, or backward), and, where
- * results are few beside the sums' lengths, parts of sums (at most 256 MiB). */
+ * hidden 1 .. 2^20, no matrix of more than 2^40 elements.  The workspace holds dg and
+ * du (and what their rounding left), copies of x and the weights where they need them
+ * (more than 16 rows, or backward), and, where results are few beside the sums'
+ * lengths, parts of sums (at most 256 MiB). */
 enum { BFHIP_SILU = 0, BFHIP_GELU = 1, BFHIP_RELU = 2 };
 
 typedef struct {
