@@ -748,7 +748,7 @@ def _rows_like(t):
     if strides[2] != 1:
         o = t.new_empty(t.shape)
         strides = o.stride()
-    return o, Rows(o.data_ptr(), strides[0], strides[1])
+    return o, Rows(o.data_ptr(), strides[0], strides[1] if t.shape[1] > 1 else 0)
 
 
 def rotary_frequencies(part, base=10000.0, factor=1.0, length=0, low=1.0, high=4.0, device="cuda"):

@@ -377,3 +377,16 @@ def test_two_calls_on_two_streams(device):
         got = [bfhip.paged_attention(page_table=t, stream=s, **c) for (c, t), s in zip(calls, streams)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_paged_strides_of_no_account(device):
+    """One token of one head: its strides are of no account."""
+    call, table = inputs(device, (BF16, 1, 1, 64, 16, [1], [70], None))
+    want = bfhip.paged_attention(page_table=table, **call)
+    for strides in ((0, 0, 1), (64, 1, 1), (5, 7, 1)):
+        q = call["q"].as_strided((1, 1, 64), strides)
+        assert torch.equal(bfhip.paged_attention(page_table=table, **dict(call, q=q)), want)
+        pools = [call[n].clone() for n in ("k_pages", "v_pages")]
+        bfhip.cache_append(q, q, *pools, table, call["starts"], call["lengths"])
+        page, row = table[0, 69 // 16], 69 % 16
+        assert all(torch.equal(p[page, row], q[0]) for p in pools)
