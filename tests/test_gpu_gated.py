@@ -363,3 +363,25 @@ def test_a_block(device):
         # sums of at most 160 x 64 x 90 fp32 roundings of random sign: 2^-24 * 1000
         scale = leaf.grad.abs().max()
         assert (got.double().cpu() - leaf.grad).abs().max() <= 6e-5 * scale, name
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_strides_of_no_account(device, rows):
+    """One row of any stride, one feature of any, weights that are views of one."""
+    call, dh = inputs(device, BF16, rows, 1, 96)
+    want, grads = run(call, dh, "silu")
+    wide = {n: t.repeat_interleave(3, 1)[:, ::3] for n, t in call.items()}
+    if rows == 1:
+        wide["x"] = wide["x"].as_strided((1, 1), (0, 5))
+    got, back = run(wide, dh, "silu")
+    for a, b in ((want, got), (grads, back)):
+        assert all(torch.equal(a[n], b[n]) for n in a)
+    call, dh = inputs(device, BF16, rows, 72, 96)
+    want, grads = run(call, dh, "silu")
+    fused = torch.cat([call["w_gate"], call["w_up"]], 1)
+    views = dict(x=call["x"], w_gate=fused[:, :72], w_up=fused[:, 72:])
+    if rows == 1:
+        views["x"] = call["x"].as_strided((1, 72), (0, 1))
+    got, back = run(views, dh, "silu")
+    for a, b in ((want, got), (grads, back)):
+        assert all(torch.equal(a[n], b[n]) for n in a)

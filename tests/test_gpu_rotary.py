@@ -162,3 +162,16 @@ def test_rotary_in_a_graph_and_on_a_stream(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, bfhip.rotary(q, k, positions, freq)))
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_rotary_of_broadcast_rows(device, tokens):
+    """Rows that share memory, and strides that are of no account."""
+    q, _, positions, freq = inputs(device, BF16, tokens, 4, 2, 64, 64)
+    for x in (q[:, :1].expand(-1, 4, -1), q[:1].expand(tokens, -1, -1), q[:1, :1].expand(tokens, 3, -1), q[:, :1],
+              q.as_strided((tokens, 1, 64), (q.stride(0), 0, 1)), q[:1].as_strided((1, 4, 64), (0, 64, 1))):
+        at = positions[:x.shape[0]]
+        want = bfhip.rotary(x.contiguous(), None, at, freq)
+        assert torch.equal(bfhip.rotary(x, None, at, freq), want)
+        for got in bfhip.rotary(x, x, at, freq):
+            assert torch.equal(got, want)
