@@ -671,8 +671,11 @@ bool bad_inputs(const bfhip_gated_desc *d, const bfhip_matrix *x, const bfhip_ma
            bad_matrix(w_up, d->hidden, d->features) || (d->hidden > 1 && w_gate->stride != w_up->stride);
 }
 
-GatedOperand operand(const bfhip_matrix *gate, const bfhip_matrix *up, long long rows, int size) {
-    return GatedOperand{(const char *)gate->data, (const char *)up->data, rows > 1 ? gate->stride * size : 0};
+// A single row, whose stride is of no account, takes that of a matrix without gaps, so that
+// a tile's further rows lie past its end as the last rows of other matrices do.
+GatedOperand operand(const bfhip_matrix *gate, const bfhip_matrix *up, long long rows, long long length, int size) {
+    const long long stride = rows > 1 ? gate->stride : (length + 7) / 8 * 8;
+    return GatedOperand{(const char *)gate->data, (const char *)up->data, stride * size};
 }
 
 }  // namespace
@@ -699,8 +702,8 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
     const bool few = few_rows(d);
     const Aligned in(d, x, w_gate, w_up, (char *)workspace);
     GatedArgs a{};
-    a.m_op = few ? operand(x, x, d->rows, size) : operand(&in.x, &in.x, d->rows, size);
-    a.n_op = few ? operand(w_gate, w_up, d->hidden, size) : operand(&in.gate, &in.up, d->hidden, size);
+    a.m_op = few ? operand(x, x, d->rows, d->features, size) : operand(&in.x, &in.x, d->rows, d->features, size);
+    a.n_op = few ? operand(w_gate, w_up, d->hidden, d->features, size) : operand(&in.gate, &in.up, d->hidden, d->features, size);
     a.m = (int)d->rows;
     a.n = (int)d->hidden;
     a.k = (int)d->features;
@@ -788,13 +791,13 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
         }
         GatedArgs a{};
         a.shift = d->type == BFHIP_F16 && d->rows ? e.shift : nullptr;
-        a.m_op = operand(&slopes_g, &slopes_u, 2, size);
+        a.m_op = operand(&slopes_g, &slopes_u, d->rows, stride, size);
         a.low = p.low;
         GatedArgs b = a;
         a.partial = (float *)(work + p.slopes);
         b.partial = (float *)(work + p.slopes + up256(p.inputs.bytes));
         if (dx) {
-            a.n_op = operand(&in.gate, &in.up, d->hidden, size);
+            a.n_op = operand(&in.gate, &in.up, d->hidden, d->features, size);
             a.m = (int)d->rows;
             a.n = (int)d->features;
             a.k = (int)d->hidden;
@@ -802,7 +805,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
             a.out_stride[0] = step(dx, d->rows, size);
         }
         if (dw_gate) {
-            b.n_op = operand(&in.x, &in.x, d->rows, size);
+            b.n_op = operand(&in.x, &in.x, d->rows, d->features, size);
             b.m = (int)d->hidden;
             b.n = (int)d->features;
             b.k = (int)d->rows;

@@ -385,3 +385,21 @@ def test_strides_of_no_account(device, rows):
     got, back = run(views, dh, "silu")
     for a, b in ((want, got), (grads, back)):
         assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_infinite_weight_of_a_single_hidden_element(device, dtype):
+    """dx = dg Wg + du Wu has one term each: an infinite weight makes its feature's
+    gradients infinite, with the slope's sign, and no others."""
+    rows, features = 65536, 4096
+    g = gen(device, 4)
+    x = torch.ones((rows, features), dtype=dtype, device=device)
+    w_gate, w_up = (randn(g, 1, features, dtype=dtype) for _ in range(2))
+    w_gate[0, 7], w_gate[0, 3000] = math.inf, -math.inf
+    gate, up = torch.ones((rows, 1), device=device), torch.full((rows, 1), 0.5, device=device)
+    dh = torch.where(randn(g, rows, 1) > 0, 1.0, -1.0).to(dtype)
+    dx, _, _ = bfhip.gated_linear_backward(dh, x, w_gate, w_up, gate, up)
+    assert torch.equal(dx[:, 7:8], dh * math.inf) and torch.equal(dx[:, 3000:3001], -dh * math.inf)
+    rest = torch.ones(features, dtype=torch.bool, device=device)
+    rest[[7, 3000]] = False
+    assert dx[:, rest].isfinite().all()
