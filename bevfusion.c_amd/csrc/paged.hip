@@ -378,14 +378,15 @@ __global__ __launch_bounds__(256, 1) void paged_attention_kernel(PagedArgs a) {
 
 // Joins the parts' sums of each query and head: DIM / 4 threads, four elements
 // each, times eight (or fewer) of the parts, which are added up in order at the end.
+// The launch's tokens begin at first_token.
 template <class E, int DIM>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int first_token) {
     constexpr int kShares = 8, kPer = 256 * 4 / DIM / kShares;
     __shared__ float2 stat_part[kShares][kPer];
     __shared__ __attribute__((aligned(16))) float sums[kShares][kPer][DIM];
     const int q = threadIdx.x / (DIM / 4), share = q % kShares, i = q / kShares, d = threadIdx.x % (DIM / 4) * 4;
     // A workgroup's rows are neighbouring heads of one token.
-    const int per_token = (a.heads + kPer - 1) / kPer, token = blockIdx.x / per_token;
+    const int per_token = (a.heads + kPer - 1) / kPer, token = first_token + blockIdx.x / per_token;
     const int head = blockIdx.x % per_token * kPer + i, group = a.heads / a.kv_heads;
     const int sequence = find_token(a.starts, a.sequences, a.tokens, token);
     if (sequence < 0) return;
@@ -397,7 +398,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     // that was dealt: any place within the workspace will do then.)
     const long long begin = first + (long long)(row / kRows) * s.cost();
     const long long from = begin / units, to = (begin + s.cost() - 1) / units;
-    if (from == to || from < 0 || to >= a.shares) return;  // (one share has written the result)
+    // (One share has written the result.  Heads of a workgroup may end here apart, for
+    // they can lie in different row tiles: a head has whole waves, and the barrier
+    // waits for those that have not ended.)
+    static_assert(kShares * (DIM / 4) % kWave == 0, "whole waves per head");
+    if (from == to || from < 0 || to >= a.shares) return;
     const int parts = (int)(to - from) + 1;
     const size_t step = (size_t)a.kv_heads * kRows, place = (size_t)kv * kRows + row % kRows;
     float m = -INFINITY, l = 0.f;
@@ -565,13 +570,14 @@ extern "C" int bfhip_paged_attention(const bfhip_paged_desc *d, const bfhip_rows
     const int size = d->type == BFHIP_F32 ? 4 : 2;
     if (bad_rows(q, d->tokens, d->head_dim, size) || bad_result(out, d->tokens, d->heads, d->head_dim, size))
         return fail(error, cap, "invalid attention rows: pointers and strides in steps of 16 bytes, token strides of at least head_dim, no results on one another");
+    if (d->tokens * (d->heads / d->kv_heads) > 1 << 30) return fail(error, cap, "paged attention has too many rows");
     const PagedPlan p = paged_plan(d);
     const size_t need = p.bytes;
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "paged attention workspace too small or not 16-byte aligned");
     if (!d->sequences || !d->tokens) return 1;
-    const long long grid = (long long)p.shares * d->kv_heads, per_token = (d->heads * p.dim + 127) / 128, joins = need ? per_token * d->tokens : 0;
-    if (d->tokens * (d->heads / d->kv_heads) > 1 << 30 || !launch_fits(grid, 256) || !launch_fits(joins, 256)) return fail(error, cap, "paged attention has too many rows");
+    const long long grid = (long long)p.shares * d->kv_heads, per_token = (d->heads * p.dim + 127) / 128;
+    const long long at_once = (1ll << 23) / per_token;  // tokens that a launch joins: it holds 2^24 - 1 workgroups
     PagedArgs a = paged_args(d, k_pages, v_pages);
     a.q = attn_rows(q, d->tokens, d->head_dim, size);
     a.out = attn_rows(out, d->tokens, d->head_dim, size);
@@ -596,7 +602,8 @@ extern "C" int bfhip_paged_attention(const bfhip_paged_desc *d, const bfhip_rows
             constexpr int kThreads = PagedTile<E, DIM>::kThreads;
             if (d->bias) hipLaunchKernelGGL((paged_attention_kernel<E, DIM, true>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
             else hipLaunchKernelGGL((paged_attention_kernel<E, DIM, false>), dim3((unsigned)grid), dim3(kThreads), 0, s, a);
-            if (joins) hipLaunchKernelGGL((paged_join_kernel<E, DIM>), dim3((unsigned)joins), dim3(256), 0, s, a);
+            for (long long t = 0; need && t < d->tokens; t += at_once)
+                hipLaunchKernelGGL((paged_join_kernel<E, DIM>), dim3((unsigned)(per_token * std::min(at_once, d->tokens - t))), dim3(256), 0, s, a, (int)t);
         });
     });
     return launch_ok(error, cap, "paged attention launch");

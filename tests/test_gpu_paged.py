@@ -390,3 +390,20 @@ def test_paged_strides_of_no_account(device):
         bfhip.cache_append(q, q, *pools, table, call["starts"], call["lengths"])
         page, row = table[0, 69 // 16], 69 % 16
         assert all(torch.equal(p[page, row], q[0]) for p in pools)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,n", [(128, 128, 8, 5250), (32, 16, 128, 2650)])
+def test_paged_attention_of_more_tokens_than_one_launch_joins(device, heads, kv_heads, dim, n):
+    """Sequences of new tokens alone, whose number times heads times the padded dim
+    / 128 is more than the workgroups of a launch; all sequences have the same
+    queries and pages."""
+    new = 100 if dim == 8 else 200
+    assert n * new * heads * max(dim, 32) // 128 >= 1 << 24
+    call, table = inputs(device, (F16, heads, kv_heads, dim, 16, [new], [new], None))
+    value, bound = ref.paged_attention(table=table, **call)["out"]
+    many = dict(call, q=call["q"].repeat(n, 1, 1), starts=torch.arange(n + 1, dtype=torch.int32, device=device) * new,
+                lengths=call["lengths"].repeat(n))
+    out = bfhip.paged_attention(page_table=table.repeat(n, 1), **many).view(n, *value.shape)
+    for part in range(0, n, 50):  # (all of them: a share's border falls into any sequence)
+        share = ((out[part:part + 50].double() - value).abs() / bound).max()
+        assert share <= 1, (part, share)

@@ -113,6 +113,18 @@ def test_paged_attention_refuses_what_no_launch_holds():
     assert b"too many" in attend(desc(tokens=0x7ffff000, heads=64, kv_heads=1), out=row(token=4096))[1]
 
 
+@pytest.mark.parametrize("heads,kv_heads,most", [(32, 32, 0x7ffff000), (32, 8, 1 << 28), (3, 1, (1 << 30) // 3)])
+def test_paged_attention_takes_as_many_rows_as_stated(heads, kv_heads, most):
+    """tokens * heads / kv_heads up to 2^30 (and tokens as in any call), whatever
+    the heads' number and size are."""
+    most = min(most, (1 << 30) * kv_heads // heads)
+    for dim in (8, 128):
+        wide = row(token=heads * dim, head=dim)
+        good, more = (desc(tokens=n, heads=heads, kv_heads=kv_heads, head_dim=dim) for n in (most, most + 1))
+        assert b"workspace" in attend(good, q=wide, out=wide, work=None)[1]
+        assert b"too many" in attend(more, q=wide, out=wide, work=None)[1]
+
+
 def test_paged_nothing_to_do():
     for change in (dict(tokens=0), dict(sequences=0)):
         assert append(desc(**change))[0] and attend(desc(**change))[0]
