@@ -183,8 +183,8 @@ struct PagedTile {
     static constexpr int kIssue = kKeys * T::kChunks / kWave;  // copies of one of the two
 };
 
-// Bound by reading the keys and values once (131071 keys, 32 heads on 8 of 128, bf16: 103
-// us, 5.2 TB/s, and 5 us for the join).  A workgroup has a share of the units
+// Bound by reading the keys and values once (131071 keys, 32 heads on 8 of 128, bf16: 107
+// us, 5.0 TB/s, and 5 us for the join).  A workgroup has a share of the units
 // of one key head, whose whole group of query heads shares each tile.  Each wave
 // walks tiles of its own, 32 keys at a time, through its own two LDS buffers, two
 // tiles in flight, without a barrier; the waves' sums are joined at a row tile's
@@ -246,65 +246,92 @@ struct PagedWalk {
             }
         };
         Running<1, kDB> run;
-        run.clear();
-        int t = t0 + wave;
-        int ids = page(t);
-        uint32_t there = 0;  // keys of the tile that have a page
-        if (t < end) {
-            there = (uint32_t)__ballot(ids >= 0 && ids < a.pages);
-            issue(t, ids, 0);
-        }
-        ids = page(t + kWaves);
-        for (int buffer = 0; t < end; t += kWaves, buffer ^= 1) {
-            uint32_t next_there = 0;
-            if (t + kWaves < end) {
-                const int now = ids;
-                ids = page(t + 2 * kWaves);
-                next_there = (uint32_t)__ballot(now >= 0 && now < a.pages);
-                issue(t + kWaves, now, buffer ^ 1);
-                wait_vmcnt<(2 * P::kIssue > 63 ? 63 : 2 * P::kIssue)>();  // this tile's, not the next one's
-            } else {
-                wait_vmcnt<0>();
+        // Probabilities meet the values rounded to the type and with what their rounding
+        // left, or it would add as much again to the results' error as their own rounding
+        // has: bf16, random values, 0.0023 of the results' norm, 0.0017 with it.  (One
+        // sequence of 131071 keys 113 us, 109 without; 48 mixed ones 110 and 107; 3 tokens
+        // for each of 100 50.6 and 50.1.)  An infinite value would meet parts of both signs:
+        // sums that are not finite are found again without what was left.
+        for (bool left_too = E::kSize == 2;; left_too = false) {
+            int t = t0 + wave;
+            run.clear();
+            int ids = page(t);
+            uint32_t there = 0;  // keys of the tile that have a page
+            if (t < end) {
+                there = (uint32_t)__ballot(ids >= 0 && ids < a.pages);
+                issue(t, ids, 0);
             }
-            asm volatile("" ::: "memory");
-            const char *const kt = mine + buffer * P::kStage, *const vt = kt + kKeys * T::kRow;
-            const int j0 = t * kKeys;
-            f32x4 sc[2][1];
+            ids = page(t + kWaves);
+            for (int buffer = 0; t < end; t += kWaves, buffer ^= 1) {
+                uint32_t next_there = 0;
+                if (t + kWaves < end) {
+                    const int now = ids;
+                    ids = page(t + 2 * kWaves);
+                    next_there = (uint32_t)__ballot(now >= 0 && now < a.pages);
+                    issue(t + kWaves, now, buffer ^ 1);
+                    wait_vmcnt<(2 * P::kIssue > 63 ? 63 : 2 * P::kIssue)>();  // this tile's, not the next one's
+                } else {
+                    wait_vmcnt<0>();
+                }
+                asm volatile("" ::: "memory");
+                const char *const kt = mine + buffer * P::kStage, *const vt = kt + kKeys * T::kRow;
+                const int j0 = t * kKeys;
+                f32x4 sc[2][1];
 #pragma unroll
-            for (int jb = 0; jb < 2; ++jb) {
-                sc[jb][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int jb = 0; jb < 2; ++jb) {
+                    sc[jb][0] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kk = 0; kk < kKB; ++kk) sc[jb][0] = E::mfma(row_frag<E, DIM>(kt, 16 * jb, kk, lane), qf[kk], sc[jb][0]);
-            }
-            if constexpr (BIAS) {
+                    for (int kk = 0; kk < kKB; ++kk) sc[jb][0] = E::mfma(row_frag<E, DIM>(kt, 16 * jb, kk, lane), qf[kk], sc[jb][0]);
+                }
+                if constexpr (BIAS) {
 #pragma unroll
-                for (int jb = 0; jb < 2; ++jb)
+                    for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int far = min(max(j0 + 16 * jb + 4 * g + e - (token + offset), -a.reach), a.reach) + a.reach;
+                            const float bias = live ? a.bias[(size_t)head * (2 * a.reach + 1) + far] : 0.f;
+                            sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, base2_bias(bias));
+                        }
+                }
+                if (j0 + kKeys > full || there != ~0u) {
+#pragma unroll
+                    for (int jb = 0; jb < 2; ++jb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = 16 * jb + 4 * g + e;
+                            sc[jb][0][e] = j0 + j < limit && (there >> j & 1) ? sc[jb][0][e] : -INFINITY;
+                        }
+                }
+                there = next_there;
+                run.template take<2>(sc, BIAS ? 1.f : a.scale2);
+                const typename E::Frag pf = to_frag<E>(sc[0][0], sc[1][0]);
+                typename E::Frag vf[kDB];
+                col_frags_in_flight<E, DIM>(vt, lane, vf);
+#pragma unroll
+                for (int db = 0; db < kDB; ++db) run.o[0][db] = E::mfma(vf[db], pf, run.o[0][db]);
+                if (left_too) {  // (probabilities are at most 2^8 or NaN)
+                    typedef typename E::Word Words8 __attribute__((ext_vector_type(8)));
+                    const f32x8 taken = __builtin_convertvector(__builtin_bit_cast(Words8, pf), f32x8);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int far = min(max(j0 + 16 * jb + 4 * g + e - (token + offset), -a.reach), a.reach) + a.reach;
-                        const float bias = live ? a.bias[(size_t)head * (2 * a.reach + 1) + far] : 0.f;
-                        sc[jb][0][e] = fmaf(sc[jb][0][e], a.scale2, base2_bias(bias));
+                        sc[0][0][e] -= taken[e];
+                        sc[1][0][e] -= taken[e + 4];
                     }
+                    const typename E::Frag left = to_frag<E>(sc[0][0], sc[1][0]);
+#pragma unroll
+                    for (int db = 0; db < kDB; ++db) run.o[0][db] = E::mfma(vf[db], left, run.o[0][db]);
+                }
+                // The next round's copy goes into the buffer just read.
+                __builtin_amdgcn_s_waitcnt(0xC07F);
+                asm volatile("" ::: "memory");
             }
-            if (j0 + kKeys > full || there != ~0u) {
+            if (!left_too) break;
+            float none = 0.f;
 #pragma unroll
-                for (int jb = 0; jb < 2; ++jb)
+            for (int db = 0; db < kDB; ++db)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = 16 * jb + 4 * g + e;
-                        sc[jb][0][e] = j0 + j < limit && (there >> j & 1) ? sc[jb][0][e] : -INFINITY;
-                    }
-            }
-            there = next_there;
-            run.template take<2>(sc, BIAS ? 1.f : a.scale2);
-            const typename E::Frag pf = to_frag<E>(sc[0][0], sc[1][0]);
-            typename E::Frag vf[kDB];
-            col_frags_in_flight<E, DIM>(vt, lane, vf);
-#pragma unroll
-            for (int db = 0; db < kDB; ++db) run.o[0][db] = E::mfma(vf[db], pf, run.o[0][db]);
-            // The next round's copy goes into the buffer just read.
-            __builtin_amdgcn_s_waitcnt(0xC07F);
-            asm volatile("" ::: "memory");
+                for (int e = 0; e < 4; ++e) none = fmaf(run.o[0][db][e], 0.f, none);
+            if (!__any(none != 0.f)) break;
         }
         // The waves' sums at their common maximum, added in order.
         run.finish();
@@ -512,9 +539,10 @@ struct PagedPlan {
 };
 
 // Shares of a key head: as many as make the workgroups that the chip holds at once,
-// two per CU (one for long fp32 rows).  Heads of 128, 32 on 8, bf16: one sequence of 131071
-// keys 108 us, 48 of 1 to 16384 107 (with three times as many, cut at whole tiles, 131 and
-// 129).
+// two per CU (one for long fp32 rows; there is room for four of 16-bit heads of up to 32,
+// which get two all the same).  Heads of 128, 32 on 8, bf16, with probabilities rounded once:
+// one sequence of 131071 keys 108 us, 48 of 1 to 16384 107 (with three times as many, cut at
+// whole tiles, 131 and 129).
 PagedPlan paged_plan(const bfhip_paged_desc *d) {
     PagedPlan p{};
     const int size = d->type == BFHIP_F32 ? 4 : 2;

@@ -281,9 +281,10 @@ int bfhip_cache_append(const bfhip_paged_desc *desc, const bfhip_rows *k, const 
 
 /* Attention of the new tokens over the cache, causal: token i of n stands at
  * position lengths[b] - n + i and sees the keys up to its own.  Scores, bias,
- * softmax, roundings, out and lse ([heads, tokens] or NULL) are those of
+ * softmax, out and lse ([heads, tokens] or NULL) are those of
  * bfhip_attention_forward, and so is what is said there of rows without keys and
- * of rows outside every sequence.  Made for few tokens per sequence: a key head's
+ * of rows outside every sequence; but probabilities meet the values with what their
+ * rounding left, as if they had twice the type's precision.  Made for few tokens per sequence: a key head's
  * keys are read once for each 16 rows (token, head of its group); the work is
  * split over the keys as the lengths on the device say.  Keys past a query's
  * position and what pages hold past a length reach no result, but a NaN or

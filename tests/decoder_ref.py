@@ -43,11 +43,12 @@ def gathered(pages, table, lengths):
     return torch.cat(rows) if rows else pages.new_zeros((0, *pages.shape[2:])), starts
 
 
-def paged_attention(q, k_pages, v_pages, table, starts, lengths, scale, bias=None):
-    """Dict of (value, bound) for out and lse."""
+def paged_attention(q, k_pages, v_pages, table, starts, lengths, scale, bias=None, left=False):
+    """Dict of (value, bound) for out and lse.  left: probabilities are multiplied
+    with twice the type's precision."""
     k, k_starts = gathered(k_pages, table, lengths)
     v, _ = gathered(v_pages, table, lengths)
-    both = ref.attention(q, k, v, starts, k_starts, True, scale, bias)
+    both = ref.attention(q, k, v, starts, k_starts, True, scale, bias, left=left)
     return {n: both[n] for n in ("out", "lse")}
 
 

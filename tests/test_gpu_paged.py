@@ -407,3 +407,33 @@ def test_paged_attention_of_more_tokens_than_one_launch_joins(device, heads, kv_
     for part in range(0, n, 50):  # (all of them: a share's border falls into any sequence)
         share = ((out[part:part + 50].double() - value).abs() / bound).max()
         assert share <= 1, (part, share)
+
+
+@pytest.mark.parametrize("case", [(BF16, 8, 8, 64, 16, [4] * 40, [4 + 3 * i for i in range(40)], None),
+                                  (F16, 8, 2, 128, 16, [1] * 8, [3, 9, 40, 100, 300, 1000, 5000, 20000], None),
+                                  (BF16, 16, 2, 32, 7, [1, 20], [700, 200], 30), (F16, 4, 4, 40, 5, [2] * 20, [25] * 20, None)], ids=lambda c: str(c)[:60])
+def test_probabilities_have_twice_the_precision(device, case):
+    """No rounding of a 16-bit type comes between the scores and the results but
+    the results' own."""
+    call, table = inputs(device, case)
+    out = bfhip.paged_attention(page_table=table, **call)
+    check("out", out, *ref.paged_attention(table=table, left=True, **call)["out"])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dim", [24, 64, 128])
+def test_infinite_values(device, dtype, dim):
+    """An infinite value makes its element's results infinite and nothing else, of
+    keys that lie in one share and in many."""
+    call, table = inputs(device, (dtype, 8, 2, dim, 16, [1] * 5, [5, 40, 300, 20000, 33], None))
+    want = bfhip.paged_attention(page_table=table, **call)
+    for b, j, d, value in ((0, 2, 1, math.inf), (1, 35, dim - 1, -math.inf), (2, 0, 5, math.inf), (3, 17000, 9, -math.inf)):
+        call["v_pages"][table[b, j // 16].long(), j % 16, 1, d] = value
+        want[b, 4:, d] = value
+    got = bfhip.paged_attention(page_table=table, **call)
+    assert torch.equal(got.isinf(), want.isinf()) and not got.isnan().any()
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    assert torch.equal(got[:, :4], want[:, :4]) and torch.equal(got[4], want[4])
+    value, bound = ref.paged_attention(table=table, **dict(call, v_pages=call["v_pages"].nan_to_num(0, 0, 0)))["out"]
+    keep = ~want.isinf()
+    check("others", got[keep], value[keep], bound[keep])

@@ -89,12 +89,15 @@ def position_bias_backward(dbias, buckets, count):
     return total, n * U * size
 
 
-def attention(q, k, v, q_starts, k_starts, causal, scale, bias=None, dout=None):
+def attention(q, k, v, q_starts, k_starts, causal, scale, bias=None, dout=None, left=False):
     """Dict of (value, bound) for out, lse (-inf where no key is seen) and, with
-    dout, dq, dk, dv and dbias.  Rows outside every sequence: zero, bound 0."""
+    dout, dq, dk, dv and dbias.  Rows outside every sequence: zero, bound 0.
+    left: what the probabilities' rounding left is taken too (not with dout)."""
+    assert not left or dout is None
     h = half(q.dtype)
     t = tiny(q.dtype)
     hp = 0.0 if q.dtype == torch.float32 else h  # rounding on the way into the matrix cores
+    hp = hp * hp if left else hp
     heads, kv_heads, dim, dev = q.shape[1], k.shape[1], q.shape[2], q.device
     zeros = lambda *shape: torch.zeros(shape, dtype=torch.float64, device=dev)
     res = {n: (zeros(*x.shape), zeros(*x.shape)) for n, x in
