@@ -252,6 +252,7 @@ struct PagedWalk {
         // sequence of 131071 keys 113 us, 109 without; 48 mixed ones 110 and 107; 3 tokens
         // for each of 100 50.6 and 50.1.)  An infinite value would meet parts of both signs:
         // sums that are not finite are found again without what was left.
+        f32x4 finite[kDB];
         for (bool left_too = E::kSize == 2;; left_too = false) {
             int t = t0 + wave;
             run.clear();
@@ -325,12 +326,22 @@ struct PagedWalk {
                 __builtin_amdgcn_s_waitcnt(0xC07F);
                 asm volatile("" ::: "memory");
             }
-            if (!left_too) break;
+            if (E::kSize == 4) break;
+            if (!left_too) {
+#pragma unroll
+                for (int db = 0; db < kDB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        run.o[0][db][e] = fabsf(finite[db][e]) < INFINITY ? finite[db][e] : run.o[0][db][e];
+                break;
+            }
             float none = 0.f;
 #pragma unroll
-            for (int db = 0; db < kDB; ++db)
+            for (int db = 0; db < kDB; ++db) {
+                finite[db] = run.o[0][db];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) none = fmaf(run.o[0][db][e], 0.f, none);
+                for (int e = 0; e < 4; ++e) none = fmaf(finite[db][e], 0.f, none);
+            }
             if (!__any(none != 0.f)) break;
         }
         // The waves' sums at their common maximum, added in order.

@@ -430,10 +430,4 @@ def test_infinite_values(device, dtype, dim):
     for b, j, d, value in ((0, 2, 1, math.inf), (1, 35, dim - 1, -math.inf), (2, 0, 5, math.inf), (3, 17000, 9, -math.inf)):
         call["v_pages"][table[b, j // 16].long(), j % 16, 1, d] = value
         want[b, 4:, d] = value
-    got = bfhip.paged_attention(page_table=table, **call)
-    assert torch.equal(got.isinf(), want.isinf()) and not got.isnan().any()
-    assert torch.equal(got[want.isinf()], want[want.isinf()])
-    assert torch.equal(got[:, :4], want[:, :4]) and torch.equal(got[4], want[4])
-    value, bound = ref.paged_attention(table=table, **dict(call, v_pages=call["v_pages"].nan_to_num(0, 0, 0)))["out"]
-    keep = ~want.isinf()
-    check("others", got[keep], value[keep], bound[keep])
+    assert torch.equal(bfhip.paged_attention(page_table=table, **call), want)
