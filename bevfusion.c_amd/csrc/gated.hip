@@ -355,8 +355,26 @@ __global__ __launch_bounds__(kChunkThreads) void gated_most_kernel(SlopeArgs a, 
     }
 }
 
+// The type's word next to v on zero's side.
+template <class E>
+__device__ __forceinline__ typename E::Word toward_zero(float v) {
+    if constexpr (std::is_same_v<E, ElemF16>) return __builtin_bit_cast(_Float16, __builtin_amdgcn_cvt_pkrtz(v, 0.f)[0]);
+    else return __builtin_bit_cast(typename E::Word, (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16));
+}
+
+// What that left of v, rounded to nearest: off by 2^-16 of v (bf16) or 2^-22 (fp16), and in
+// fp16 by 2^-24.  It has v's sign and is nothing only where `taken` is, so that the two
+// agree on what an infinite weight makes of them.
+template <class E>
+__device__ __forceinline__ typename E::Word left_of(float v, typename E::Word taken) {
+    constexpr float least = std::is_same_v<E, ElemF16> ? 0x1p-24f : 0x1p-126f;
+    const float most = E::get(taken), left = E::get(E::put(fabsf(most) < INFINITY ? v - most : 0.f));
+    return E::put(left == 0.f && most != 0.f ? copysignf(least, v) : left);
+}
+
 // dg and du, rounded to the type; fp16's times a power of two that takes the
-// largest of them to 2^14 or just above.  With `low` what the rounding left as well.
+// largest of them to 2^14 or just above.  With `low` in two parts of one sign (then fp16's
+// largest comes to 2^15, so that 2^-24 is as little of it).
 // Bound by memory (8192 rows of 5632, bf16: 135 us, 4.8 TB/s).
 template <class E, int kActivation>
 __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a, int groups, PadArgs pad) {
@@ -372,7 +390,7 @@ __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a,
         __syncthreads();
         most = part[0];
         for (int w = 1; w < kChunkThreads / kWave; ++w) most = fmaxf(most, part[w]);
-        if (most > 0.f) shift = 14 - ilogbf(most);
+        if (most > 0.f) shift = (a.low ? 15 : 14) - ilogbf(most);
         if (block == 0 && threadIdx.x == 0) *a.shift = shift;
     }
     each_chunk(block, blocks, a.rows, (int)(a.stride / 8), [&](long long i, long long r, int c) {
@@ -386,18 +404,22 @@ __global__ __launch_bounds__(kChunkThreads) void gated_slope_kernel(SlopeArgs a,
             x.put(e, dg[e]);
             y.put(e, du[e]);
         }
+        if constexpr (E::kSize == 2) {
+            if (a.low) {
+                Words<E, 8> left_x, left_y;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x.w[e] = toward_zero<E>(dg[e]);
+                    y.w[e] = toward_zero<E>(du[e]);
+                    left_x.w[e] = left_of<E>(dg[e], x.w[e]);
+                    left_y.w[e] = left_of<E>(du[e], y.w[e]);
+                }
+                left_x.store((typename E::Word *)(a.dg + a.low) + i * 8);
+                left_y.store((typename E::Word *)(a.du + a.low) + i * 8);
+            }
+        }
         x.store((typename E::Word *)a.dg + i * 8);
         y.store((typename E::Word *)a.du + i * 8);
-        if (E::kSize == 2 && a.low) {
-            const auto left = [](float v, float rounded) { return fabsf(rounded) < INFINITY ? v - rounded : 0.f; };
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x.put(e, left(dg[e], x.get(e)));
-                y.put(e, left(du[e], y.get(e)));
-            }
-            x.store((typename E::Word *)(a.dg + a.low) + i * 8);
-            y.store((typename E::Word *)(a.du + a.low) + i * 8);
-        }
     });
 }
 
@@ -621,8 +643,8 @@ struct Aligned {
     }
 };
 
-// Up to this many slopes (rows * hidden) enter the products in two parts, rounded and what
-// the rounding left.  Of many slopes the roundings average out to about the error that
+// Up to this many slopes (rows * hidden) enter the products in two parts, the type's word
+// next to them on zero's side and what that left.  Of many slopes the roundings average out to about the error that
 // the results' own rounding has; of few one or two large ones can make it more.  (So few
 // products are bound by their launches and the weights: the backward pass of 16 rows of 1024 ->
 // 1024 bf16 13.8 us, 12.1 without; one row of 4096 -> 11008 117 and 106.)

@@ -313,8 +313,8 @@ int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
  * dx, or dWg and dWu together, may be NULL where they are not wanted.  dg and du
  * are rounded to the type where they enter the matrix cores (up to 16384 of each enter
  * with what the rounding left, as if they had twice the precision); fp16's are
- * multiplied by a power of two on the way (their largest comes near 2^14), so that
- * they may be of any size.  A result beyond the type's range is infinite.
+ * multiplied by a power of two on the way (their largest comes near 2^14 or 2^15), so
+ * that they may be of any size.  A result beyond the type's range is infinite.
  * relu'(0) = 0.
  *
  * Matrices: row r at element r * <name>.stride (at least the row's length, of no

@@ -403,3 +403,30 @@ def test_infinite_weight_of_a_single_hidden_element(device, dtype):
     rest = torch.ones(features, dtype=torch.bool, device=device)
     rest[[7, 3000]] = False
     assert dx[:, rest].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [(7, 72, 300), (130, 520, 100), (1, 4096, 1000)], ids=str)
+def test_infinite_operands_of_few_slopes(device, dtype, size):
+    """An infinite weight makes its feature's gradients infinite, an infinite x its
+    column's, with the slopes' signs; others are within the bound of slopes that
+    are rounded once."""
+    rows, features, hidden = size
+    assert rows * hidden <= 1 << 14
+    call, dh = inputs(device, dtype, *size)
+    g = gen(device, 9)
+    gate, up = 0.5 + torch.rand((rows, hidden), generator=g, device=device), 0.5 + torch.rand((rows, hidden), generator=g, device=device)
+    dh = torch.where(dh > 0, dh + 0.5, dh - 0.5).to(dtype)
+    want = {n: v.clone() for n, (v, _) in ref.gated_linear_backward(dh, **call, gate=gate, up=up, activation="silu").items()}
+    for w, h, f, value in (("w_gate", 3, 9, math.inf), ("w_up", hidden - 1, 70, -math.inf)):
+        call[w][h, f] = value
+        want["dx"][:, f] = dh[:, h].double().sign() * value
+    call["x"][rows - 1, 5] = -math.inf
+    want["dw_gate"][:, 5] = want["dw_up"][:, 5] = -dh[rows - 1].double().sign() * math.inf
+    finite = {n: t.nan_to_num(0, 0, 0) for n, t in call.items()}
+    bounds = ref.gated_linear_backward(dh, **finite, gate=gate, up=up, activation="silu")
+    got = bfhip.gated_linear_backward(dh, **call, gate=gate, up=up)
+    for t, name in zip(got, ("dx", "dw_gate", "dw_up")):
+        far = want[name].isinf()
+        assert far.any() and torch.equal(t[far].double(), want[name][far]), name
+        check(name, t[~far], bounds[name][0][~far], bounds[name][1][~far])
