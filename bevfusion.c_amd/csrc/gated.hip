@@ -496,7 +496,7 @@ GatedPlan plan_tiles(GatedTiles kind, Form f, long long m, long long n, long lon
     return best;
 }
 
-// Whether a launch holds a product's workgroups.
+// Whether a launch holds a product's workgroups, and with another product's beside them.
 bool gated_fits(const GatedPlan &p) {
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     return tiles <= 0x7fffffff && launch_fits(p.whole + (tiles - p.whole) * p.parts, 512);
@@ -644,10 +644,13 @@ struct Aligned {
 };
 
 // Up to this many slopes (rows * hidden) enter the products in two parts, the type's word
-// next to them on zero's side and what that left.  Of many slopes the roundings average out to about the error that
-// the results' own rounding has; of few one or two large ones can make it more.  (So few
-// products are bound by their launches and the weights: the backward pass of 16 rows of 1024 ->
-// 1024 bf16 13.8 us, 12.1 without; one row of 4096 -> 11008 117 and 106.)
+// next to them on zero's side and what that left.  Of many slopes the roundings average out to
+// about the error that the results' own rounding has (together 0.0023 of the gradients' norm in
+// bf16, 0.0017 in two parts); of few one or two large ones can make it more.  So few products
+// are bound by their launches and the weights: the backward pass of 16 rows of 1024 -> 1024 bf16
+// 14.3 us, 11.7 without; one row of 4096 -> 11008 104 and 90.  Many would pay for it: a training
+// step of 999 rows of 771 -> 2055 fp16 93 us instead of 75, of 8192 rows of 2048 -> 5632 bf16
+// 1980 instead of 1060.
 constexpr long long kFewSlopes = 1 << 14;
 
 struct BackwardPlan {
@@ -671,8 +674,9 @@ BackwardPlan backward_plan(const bfhip_gated_desc *d) {
         };
         // (one launch takes about 6 us less than two: see gated_gradients_kernel)
         const double one = plan(false) - 6;
+        const bool held = gated_fits(b.inputs) && gated_fits(b.weights);
         b.together = true;
-        if (plan(true) < one) b.together = b.inputs.kind != kLarge && b.weights.kind != kLarge;
+        if (plan(true) < one || !held) b.together = b.inputs.kind != kLarge && b.weights.kind != kLarge;
         else plan(false);
         b.slope = up256((size_t)d->rows * slope_stride(d) * E::kSize);
         b.slopes = 2 * passes * b.slope;
@@ -717,12 +721,15 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
         (gate && (bad_matrix(gate, d->rows, d->hidden) || bad_matrix(up, d->rows, d->hidden))))
         return fail(error, cap, "invalid gated linear matrices: strides of at least a row, one stride for both weights");
     if (!d->rows) return 1;
-    const size_t need = bfhip_gated_linear_workspace(d, x, w_gate, w_up);
+    const bool few = few_rows(d);
+    GatedPlan p{};
+    if (!few) with_element(d->type, [&](auto e) { p = gated_plan<decltype(e), kForward>(d->rows, d->hidden, d->features); });
+    if (!few && !gated_fits(p)) return fail(error, cap, "gated linear has too many rows");
+    const Aligned in(d, x, w_gate, w_up, (char *)workspace);
+    const size_t need = few ? 0 : in.bytes + up256(p.bytes);
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need))
         return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
     const int size = d->type == BFHIP_F32 ? 4 : 2;
-    const bool few = few_rows(d);
-    const Aligned in(d, x, w_gate, w_up, (char *)workspace);
     GatedArgs a{};
     a.m_op = few ? operand(x, x, d->rows, d->features, size) : operand(&in.x, &in.x, d->rows, d->features, size);
     a.n_op = few ? operand(w_gate, w_up, d->hidden, d->features, size) : operand(&in.gate, &in.up, d->hidden, d->features, size);
@@ -737,20 +744,15 @@ extern "C" int bfhip_gated_linear(const bfhip_gated_desc *d, const bfhip_matrix 
     a.activation = d->activation;
     a.partial = (float *)((char *)workspace + in.bytes);
     hipStream_t s = (hipStream_t)stream;
-    bool fits = true;
     with_element(d->type, [&](auto e) {
         using E = decltype(e);
         if (few) {
             gated_few_launch<E>(a, s);
             return;
         }
-        const GatedPlan p = gated_plan<E, kForward>(a.m, a.n, a.k);
-        fits = gated_fits(p);
-        if (!fits) return;
         if (in.pad.blocks) hipLaunchKernelGGL(gated_pad_kernel<E>, dim3((unsigned)(3 * in.pad.blocks)), dim3(kChunkThreads), 0, s, in.pad);
         gated_launch<E, kForward>(a, p, s);
     });
-    if (!fits) return fail(error, cap, "gated linear has too many rows");
     return launch_ok(error, cap, "gated linear launch");
 }
 
@@ -771,13 +773,13 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
         (dw_gate && (bad_matrix(dw_gate, d->hidden, d->features) || bad_matrix(dw_up, d->hidden, d->features))))
         return fail(error, cap, "invalid gated linear matrices: strides of at least a row, one stride for both weights");
     if (!d->rows && !dw_gate) return 1;
-    const size_t need = bfhip_gated_linear_backward_workspace(d, x, w_gate, w_up);
-    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
-        return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
-    const int size = d->type == BFHIP_F32 ? 4 : 2;
     const BackwardPlan p = backward_plan(d);
+    if ((dx && !gated_fits(p.inputs)) || (dw_gate && !gated_fits(p.weights))) return fail(error, cap, "gated linear has too many rows");
     char *work = (char *)workspace;
     const Aligned in(d, x, w_gate, w_up, work + p.all());
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < in.bytes + p.all())
+        return fail(error, cap, "gated linear workspace too small or not 16-byte aligned");
+    const int size = d->type == BFHIP_F32 ? 4 : 2;
     const long long stride = slope_stride(d);
     SlopeArgs e{};
     const auto step = [&](const bfhip_matrix *t, long long rows, int bytes) { return rows > 1 ? t->stride * bytes : 0; };
@@ -796,7 +798,6 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     const long long grid = std::min<long long>(8192, (d->rows * (stride / 8) + kChunkThreads - 1) / kChunkThreads);
     const bfhip_matrix slopes_g{e.dg, stride}, slopes_u{e.du, stride};
     hipStream_t s = (hipStream_t)stream;
-    if ((dx && !gated_fits(p.inputs)) || (dw_gate && !gated_fits(p.weights))) return fail(error, cap, "gated linear has too many rows");
     with_element(d->type, [&](auto el) {
         using E = decltype(el);
         if (d->rows) {

@@ -322,9 +322,12 @@ int bfhip_paged_attention(const bfhip_paged_desc *desc, const bfhip_rows *q,
  * Any alignment will do; x and weights whose pointers, strides and rows are
  * multiples of 16 bytes (and strides below 2 Mi elements) need no copy.  Wg and Wu
  * have one stride.  Results overlap nothing.  rows at most 0x7fff0000, features and
- * hidden 1 .. 2^20, no matrix of more than 2^40 elements.  The workspace holds dg and
+ * hidden 1 .. 2^20, no matrix of more than 2^40 elements; calls of which a product has
+ * 2^23 tiles or more are refused (of 128 rows by 64 hidden elements forward, of 128 by 128
+ * elements of dx or of both dWg and dWu backward; in 16 bits of twice as many both ways).  The workspace holds dg and
  * du (and what their rounding left), copies of x and the weights where they need them
- * (more than 16 rows, or backward), and, where results are few beside the sums'
+ * (backward, and forward with more than 32 rows, or 16 where hidden * features is above
+ * 12 Mi, in fp32 4 Mi), and, where results are few beside the sums'
  * lengths, parts of sums (at most 256 MiB). */
 enum { BFHIP_SILU = 0, BFHIP_GELU = 1, BFHIP_RELU = 2 };
 

@@ -97,6 +97,20 @@ def test_refuses_what_no_launch_holds():
         assert b"too many" in backward(d, **dict(dict.fromkeys(("x", "w_gate", "w_up"), x), **named))[1]
 
 
+@pytest.mark.parametrize("hidden", [1, 64])
+def test_takes_as_many_tiles_as_stated(hidden):
+    """Up to 2^23 - 1 tiles of 128 rows in fp32: 2^30 - 128 rows."""
+    none = dict(work=None, size=0)
+    for rows, message in (((1 << 30) - 128, b"workspace"), (1 << 30, b"too many")):
+        d = desc(type=0, rows=rows, features=2, hidden=hidden)
+        x = {n: mat(4100, 64) for n in ("x", "w_gate", "w_up")}  # (off 16 bytes: copied, so that there is a workspace)
+        assert message in forward(d, **x, **none)[1]
+        for left in (dict(), dict(dw_gate=None, dw_up=None)):
+            assert message in backward(d, **x, **left, **none)[1]
+    d = desc(type=2, rows=0x7fff0000, features=2, hidden=1)
+    assert b"workspace" in forward(d, **x, **none)[1] and b"workspace" in backward(d, **x, **none)[1]
+
+
 def test_nothing_to_do():
     none = mat(None)
     assert forward(desc(rows=0), x=none, h=none, gate=none, up=none, work=None, size=0)[0]
