@@ -969,18 +969,22 @@ def gated_linear(x, w_gate, w_up, activation="silu", out=None, save=False, strea
     return (out, gate, up) if save else out
 
 
-def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation="silu", stream=None):
+def gated_linear_backward(dh, x, w_gate, w_up, gate, up, activation="silu", stream=None,
+                          inputs=True, weights=True):
     """Gradients of gated_linear (bfhip_gated_linear_backward) from that of h:
-    (dx, dw_gate, dw_up)."""
+    (dx, dw_gate, dw_up).  Without `inputs` (a first layer) dx is not
+    computed and None, without `weights` (frozen ones) the other two."""
+    if not (inputs or weights):
+        raise BfHipError("no gradient is wanted")
     desc, given, rows, hidden, dtype, device = _gated_desc(x, w_gate, w_up, activation)
     lib, float32 = hip_lib(), _torch().float32
     md = _gated_matrix("dh", dh, rows, hidden, dtype, device)
     mg = _gated_matrix("gate", gate, rows, hidden, float32, device)
     mu = _gated_matrix("up", up, rows, hidden, float32, device)
     with _place(stream, x, dh, w_gate, w_up, gate, up) as queue:
-        dx, mx = _matrix_like(x)
-        dw_gate, mwg = _matrix_like(w_gate)
-        dw_up, mwu = _matrix_like(w_gate)
+        dx, mx = _matrix_like(x) if inputs else (None, None)
+        dw_gate, mwg = _matrix_like(w_gate) if weights else (None, None)
+        dw_up, mwu = _matrix_like(w_gate) if weights else (None, None)
         size = lib.bfhip_gated_linear_backward_workspace(desc, *given)
         work, pw = _scratch(size, x)
         err = _err()

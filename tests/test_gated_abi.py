@@ -152,3 +152,9 @@ def test_python_refuses():
             bfhip.gated_linear(*args, **named)
     with pytest.raises(bfhip.BfHipError):
         bfhip.gated_linear_backward(torch.zeros((4, 5)), x, w, w, torch.zeros((4, 6)), torch.zeros((4, 6)))
+
+
+def test_python_refuses_no_gradient():
+    x, w, rows = torch.zeros((4, 8)), torch.zeros((6, 8)), torch.zeros((4, 6))
+    with pytest.raises(bfhip.BfHipError, match="no gradient"):
+        bfhip.gated_linear_backward(rows, x, w, w, rows, rows, inputs=False, weights=False)

@@ -430,3 +430,17 @@ def test_infinite_operands_of_few_slopes(device, dtype, size):
         far = want[name].isinf()
         assert far.any() and torch.equal(t[far].double(), want[name][far]), name
         check(name, t[~far], bounds[name][0][~far], bounds[name][1][~far])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [(0, 24, 40), (3, 64, 100), (300, 72, 136), (999, 771, 2055)], ids=str)
+def test_gradients_that_are_not_wanted(device, dtype, size):
+    """Are None, and the others have the bits that they have beside them."""
+    call, dh = inputs(device, dtype, *size)
+    h, gate, up = bfhip.gated_linear(**call, save=True)
+    call.update(gate=gate, up=up)
+    want = bfhip.gated_linear_backward(dh, **call)
+    dx, *none = bfhip.gated_linear_backward(dh, **call, weights=False)
+    assert none == [None, None] and torch.equal(dx, want[0])
+    none, *dw = bfhip.gated_linear_backward(dh, **call, inputs=False)
+    assert none is None and torch.equal(dw[0], want[1]) and torch.equal(dw[1], want[2])
