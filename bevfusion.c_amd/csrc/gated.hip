@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "bfhip_debug.h"
 #include "gated.h"
 
 using namespace bfhip;
@@ -845,4 +846,27 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
         }
     });
     return launch_ok(error, cap, "gated linear launch");
+}
+
+// ---- Plan probe (include/bfhip_debug.h) --------------------------------------
+extern "C" int bfhip_debug_gated_plan(const bfhip_gated_desc *d, int product, int plan[6], char *error, size_t cap) {
+    if (bad_gated(d) || product < 0 || product > 2 || !plan) return fail(error, cap, "invalid gated plan contract");
+    const auto put = [&](const GatedPlan &p) {
+        plan[0] = p.kind;
+        plan[1] = p.whole;
+        plan[2] = (int)((long long)p.tiles_m * p.tiles_n - p.whole);
+        plan[3] = p.parts;
+    };
+    std::fill(plan, plan + 6, 0);
+    if (product) {
+        const BackwardPlan b = backward_plan(d);
+        put(product == 1 ? b.inputs : b.weights);
+        plan[4] = b.together;
+        plan[5] = b.low != 0;
+    } else if (few_rows(d)) {
+        plan[0] = kLarge + 1;
+    } else {
+        with_element(d->type, [&](auto e) { put(gated_plan<decltype(e), kForward>(d->rows, d->hidden, d->features)); });
+    }
+    return 1;
 }

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import bfhip
+from gated_paths import HALF, SINGLE, paths
 
 P = C.c_void_p(4096)
 
@@ -158,3 +159,36 @@ def test_python_refuses_no_gradient():
     x, w, rows = torch.zeros((4, 8)), torch.zeros((6, 8)), torch.zeros((4, 6))
     with pytest.raises(bfhip.BfHipError, match="no gradient"):
         bfhip.gated_linear_backward(rows, x, w, w, rows, rows, inputs=False, weights=False)
+
+
+@pytest.mark.parametrize("dtype,sizes", [(torch.float32, SINGLE), (torch.float16, HALF), (torch.bfloat16, HALF)])
+def test_sizes_that_go_by_every_kernel(dtype, sizes):
+    """What random sizes go by is what the sizes that are run on the GPU go by: a
+    change of the rules that leaves a kernel without a test is found here."""
+    covered = set().union(*(paths(dtype, s) for s in sizes))
+    kinds = {k for name, (k, *_), *_ in covered if name != "both"}
+    assert kinds == {"small", "low", "few"} | (set() if dtype == torch.float32 else {"deep", "large"})
+    for kind in kinds - {"few", "small"}:  # every kind in every product that it is for, with and without a split
+        for name in ("forward", "inputs") + (("weights",) if kind == "large" else ()):
+            found = {p[1][1:] for p in covered if p[0] == name and p[1][0] == kind}
+            assert found >= {(True, False), (False, True)} | ({(True, True)} if kind == "large" else set()), (kind, name)
+    rng = random.Random(2)
+    log = lambda most: int(most ** rng.random())
+    tried = 0
+    while tried < 6000:
+        size = log(20000), log(9000), log(12000)
+        if rng.random() < 0.3:
+            size = size[0], -(-size[1] // 64) * 64, -(-size[2] // 64) * 64
+        if size[0] * size[1] * size[2] <= 1 << 33:
+            assert paths(dtype, size) <= covered, size
+            tried += 1
+
+
+def test_plan_refuses():
+    lib, plan = bfhip.hip_lib(), (C.c_int * 6)()
+    for bad in (dict(hidden=0), dict(type=3)):
+        assert not lib.bfhip_debug_gated_plan(desc(**bad), 0, plan, None, 0)
+    for product in (-1, 3):
+        assert not lib.bfhip_debug_gated_plan(desc(), product, plan, None, 0)
+    e = C.create_string_buffer(64)
+    assert not lib.bfhip_debug_gated_plan(desc(), 0, None, e, 64) and b"plan" in e.value

@@ -8,6 +8,7 @@ import torch
 
 import bfhip
 import decoder_ref as ref
+from gated_paths import HALF, SINGLE
 from transformer_ref import check
 
 pytestmark = pytest.mark.gpu
@@ -444,3 +445,16 @@ def test_gradients_that_are_not_wanted(device, dtype, size):
     assert none == [None, None] and torch.equal(dx, want[0])
     none, *dw = bfhip.gated_linear_backward(dh, **call, inputs=False)
     assert none is None and torch.equal(dw[0], want[1]) and torch.equal(dw[1], want[2])
+
+
+@pytest.mark.parametrize("dtype,size", [(t, s) for t, sizes in ((F32, SINGLE), (F16, HALF), (BF16, HALF)) for s in sizes], ids=str)
+def test_every_kernel(device, dtype, size):
+    """Sizes that go by every kind of tiles in every product, whole, split and in
+    part, and each gradient by itself."""
+    activation = ("silu", "gelu", "relu")[sum(size) % 3]
+    call, dh = inputs(device, dtype, *size)
+    forward, back = compare(call, dh, activation)
+    call.update(gate=forward["gate"], up=forward["up"], activation=activation)
+    dx, *_ = bfhip.gated_linear_backward(dh, **call, weights=False)
+    _, dw_gate, dw_up = bfhip.gated_linear_backward(dh, **call, inputs=False)
+    assert torch.equal(dx, back["dx"]) and torch.equal(dw_gate, back["dw_gate"]) and torch.equal(dw_up, back["dw_up"])
