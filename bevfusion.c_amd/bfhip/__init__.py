@@ -272,7 +272,7 @@ TRANSFORMER_SIGNATURES = {
     "bfhip_gated_linear": (_i, [_gatedp] + [_matrixp] * 6 + [_vp, _sz, _vp, C.c_char_p, _sz]),
     "bfhip_gated_linear_backward": (_i, [_gatedp] + [_matrixp] * 9 + [_vp, _sz, _vp, C.c_char_p,
                                                                        _sz]),
-    "bfhip_debug_gated_plan": (_i, [_gatedp, _i, C.POINTER(_i), C.c_char_p, _sz]),
+    "bfhip_gated_linear_plan": (_i, [_gatedp, _i, C.POINTER(_i), C.c_char_p, _sz]),
 }
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
@@ -1001,13 +1001,13 @@ GatedPlan = collections.namedtuple("GatedPlan", "kind whole split parts together
 
 
 def gated_plan(dtype, rows, features, hidden, product):
-    """Which kernel a product of the gated linear goes by (bfhip_debug_gated_plan,
-    include/bfhip_debug.h): product "forward", "inputs" or "weights"."""
+    """Which kernel a product of the gated linear goes by (bfhip_gated_linear_plan):
+    product "forward", "inputs" or "weights"."""
     torch = _torch()
     desc = GatedDesc(_type_code(torch.empty(0, dtype=dtype)), 0, rows, features, hidden)
     plan, err = (_i * 6)(), _err()
-    _check(hip_lib().bfhip_debug_gated_plan(desc, ("forward", "inputs", "weights").index(product),
-                                            plan, err, 512), err, "bfhip_debug_gated_plan")
+    _check(hip_lib().bfhip_gated_linear_plan(desc, ("forward", "inputs", "weights").index(product),
+                                            plan, err, 512), err, "bfhip_gated_linear_plan")
     kind, whole, split, parts, together, two = plan
     return GatedPlan(GATED_KINDS[kind], whole, split, parts, bool(together), bool(two))
 

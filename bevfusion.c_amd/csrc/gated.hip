@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 
-#include "bfhip_debug.h"
 #include "gated.h"
 
 using namespace bfhip;
@@ -15,10 +14,10 @@ namespace {
 // LDS; while one is multiplied the others are on their way.  Small ones have two: two
 // workgroups then share a CU and cover each other's waits, ways in and ways out.  (With
 // four a workgroup is alone there: forward, 999 rows of 776 -> 2056 fp16, 264 tiles: 17
-// us, 26 with four; gradient of 5632 x 2048 weights by 512 rows bf16: 36 and 60.)  With
+// us, 25 with four; both gradients of 512 rows of 2048 -> 5632 bf16: 74 and 102.)  With
 // four they are `deep` ones, for tiles that are no more than the CUs and stream weights from
-// memory (128 rows of 4096 -> 11008 bf16: 53 us, 65 with two).  Low ones have three, and share
-// a CU by twos (64 rows of 4096 -> 11008 bf16: 44 us, 59 with two stages).
+// memory (128 rows of 4096 -> 11008 bf16: 48 us, 60 with two).  Low ones have three, and share
+// a CU by twos (64 rows of 4096 -> 11008 bf16: 41 us, 57 with two stages).
 constexpr int kSmallStages = 2, kDeepStages = 4, kLowStages = 3;
 
 template <class E, Form F, class S, int kStages>
@@ -588,9 +587,17 @@ void gated_gradients(GatedArgs inputs, const GatedPlan &pi, GatedArgs weights, c
 }
 
 // Whether a forward pass goes by the kernel for few rows: up to 16, or up to 32 where the
-// weights are small.  17 rows, few or tiles, us: 1024 -> 4096 bf16 9.1 and 12.5, 2048 -> 5632
-// 15.4 and 16.3, 4096 -> 11008 43 and 43; 512 -> 2048 fp32 10.8 and 16.6, 1024 -> 4096 20 and
-// 20, 2048 -> 5632 45 and 39.
+// weights are small.  us, few or tiles (rows that lie on 16 bytes: others would be copied for the
+// tiles):
+//              1 row       8           16          17          32
+//   bf16 1024 -> 4096   5.8, 10.0   6.1,  9.8   6.3,  9.7   8.9,  9.7   9.3,  9.8
+//        2048 -> 5632  13.2, 14.9  13.5, 14.4  14.5, 14.4  15.1, 14.6  15.2, 14.5
+//        4096 -> 11008 35.3, 37.5  41.0, 36.0  46.1, 40.7
+//   fp32 512 -> 2048    5.5, 16.6   5.8, 15.8   6.0, 16.0  10.5, 16.8  11.1, 16.0
+//        2048 -> 5632  28.0, 41.1  30.0, 40.3  32.0, 40.5
+//        4096 -> 11008 82.9, 116   82.9, 115   91.9, 115
+// So 4 to 16 rows of large 16-bit weights would be 5 to 13 % faster by tiles: each of the few
+// kernel's workgroups reads all of x for 16 hidden elements.
 bool few_rows(const bfhip_gated_desc *d) {
     return d->rows <= 16 || (d->rows <= 32 && d->features * d->hidden <= (d->type == BFHIP_F32 ? 4 : 12) << 20);
 }
@@ -848,8 +855,7 @@ extern "C" int bfhip_gated_linear_backward(const bfhip_gated_desc *d, const bfhi
     return launch_ok(error, cap, "gated linear launch");
 }
 
-// ---- Plan probe (include/bfhip_debug.h) --------------------------------------
-extern "C" int bfhip_debug_gated_plan(const bfhip_gated_desc *d, int product, int plan[6], char *error, size_t cap) {
+extern "C" int bfhip_gated_linear_plan(const bfhip_gated_desc *d, int product, int plan[6], char *error, size_t cap) {
     if (bad_gated(d) || product < 0 || product > 2 || !plan) return fail(error, cap, "invalid gated plan contract");
     const auto put = [&](const GatedPlan &p) {
         plan[0] = p.kind;

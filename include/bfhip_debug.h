@@ -75,18 +75,7 @@
  *       Lets a test check that the calibration cache stays consistent with
  *       the queued cell lists across a failed frame.
  *
- *   bfhip_debug_gated_plan
- *       Which kernel a product of the gated linear goes by (host only, nothing
- *       is launched): product 0 the forward pass, 1 the inputs' gradient, 2 the
- *       weights'.  plan[0] the kind: 0 small tiles, 1 deep, 2 low, 3 large, 4
- *       the forward kernel for few rows (whose other entries are zero);
- *       plan[1] tiles that one workgroup computes, plan[2] tiles that are
- *       split along the contraction, plan[3] into how many parts, plan[4]
- *       whether both gradients go in one launch where both are wanted,
- *       plan[5] whether the slopes enter in two parts.  Lets a test see that its
- *       sizes reach every kernel.
- *
- * All pointers are device pointers (but plan); stream is a hipStream_t.  Returns 1 on
+ * All pointers are device pointers; stream is a hipStream_t.  Returns 1 on
  * success, 0 with a message in error[0..error_cap).
  */
 #ifndef BFHIP_DEBUG_H
@@ -95,7 +84,6 @@
 #include "bf_cuda_camera.h"
 #include "bf_cuda_runtime.h"
 #include "bf_cuda_swin.h"
-#include "bfhip_transformer.h"
 
 #include <stddef.h>
 
@@ -130,9 +118,6 @@ int bfhip_debug_fpn_upsample(bf_cuda_camera_neck *neck, int level, const float *
 
 int bfhip_debug_swin_merge_gather(bf_cuda_swin *swin, int stage, const void *xh_f16, float *out,
                                   void *stream, char *error, size_t error_cap);
-
-int bfhip_debug_gated_plan(const bfhip_gated_desc *desc, int product, int plan[6],
-                           char *error, size_t error_cap);
 
 #ifdef __cplusplus
 }

@@ -285,7 +285,8 @@ int bfhip_cache_append(const bfhip_paged_desc *desc, const bfhip_rows *k, const 
  * bfhip_attention_forward, and so is what is said there of rows without keys and
  * of rows outside every sequence; but probabilities meet the values with what their
  * rounding left, as if they had twice the type's precision.  Made for few tokens per sequence: a key head's
- * keys are read once for each 16 rows (token, head of its group); the work is
+ * keys are read once for each 16 rows (token, head of its group), so that long
+ * prompts take several times as long as by bfhip_attention_forward; the work is
  * split over the keys as the lengths on the device say.  Keys past a query's
  * position and what pages hold past a length reach no result, but a NaN or
  * infinity in the value of a token reaches the queries of the same sequence in
@@ -362,6 +363,16 @@ int bfhip_gated_linear_backward(const bfhip_gated_desc *desc, const bfhip_matrix
                                 const bfhip_matrix *dw_gate, const bfhip_matrix *dw_up,
                                 void *workspace, size_t workspace_bytes,
                                 void *stream, char *error, size_t error_cap);
+
+/* Which kernel a product goes by; on the host, nothing is launched.  For tests,
+ * which see by it that their sizes reach every kernel.  product: 0 the forward
+ * pass, 1 dx, 2 dWg and dWu.  plan[0] the kind: 0 small tiles, 1 deep, 2 low, 3
+ * large, 4 the forward kernel for few rows (whose other entries are zero); plan[1]
+ * tiles that one workgroup computes, plan[2] tiles that are split along the
+ * contraction, plan[3] into how many parts, plan[4] whether both gradients go in
+ * one launch where both are wanted, plan[5] whether dg and du enter in two parts. */
+int bfhip_gated_linear_plan(const bfhip_gated_desc *desc, int product, int plan[6], char *error,
+                            size_t error_cap);
 
 #ifdef __cplusplus
 }

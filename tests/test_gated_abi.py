@@ -187,8 +187,8 @@ def test_sizes_that_go_by_every_kernel(dtype, sizes):
 def test_plan_refuses():
     lib, plan = bfhip.hip_lib(), (C.c_int * 6)()
     for bad in (dict(hidden=0), dict(type=3)):
-        assert not lib.bfhip_debug_gated_plan(desc(**bad), 0, plan, None, 0)
+        assert not lib.bfhip_gated_linear_plan(desc(**bad), 0, plan, None, 0)
     for product in (-1, 3):
-        assert not lib.bfhip_debug_gated_plan(desc(), product, plan, None, 0)
+        assert not lib.bfhip_gated_linear_plan(desc(), product, plan, None, 0)
     e = C.create_string_buffer(64)
-    assert not lib.bfhip_debug_gated_plan(desc(), 0, None, e, 64) and b"plan" in e.value
+    assert not lib.bfhip_gated_linear_plan(desc(), 0, None, e, 64) and b"plan" in e.value
