@@ -52,10 +52,10 @@ __device__ __forceinline__ float over(float a, float b) {
 }
 
 // erfc, which keeps gelu's relative precision where it is small.  For 16-bit types with
-// t = 1 / (1 + |v| / 2) as t 2^(p(t) - v^2 log2 e), p a polynomial fitted to
-// log2(e^(v^2) erfc(v) / t) at Chebyshev's nodes: off by 3e-6 of it for |v| < 4, beyond
-// by 1e-5 (v^2's rounding); half a step of fp16 is 2.4e-4.  17 instructions, the exact
-// one takes 50 (the epilogue of a tile of 256 x 256: 8 us less).
+// t = 1 / (1 + |v| / 2), the substitution that approximations of erfc use since Hastings (1955), as
+// t 2^(p(t) - v^2 log2 e), p a polynomial fitted here to log2(e^(v^2) erfc(v) / t) at Chebyshev's
+// nodes: off by 3e-6 of it for |v| < 4, beyond by 1e-5 (v^2's rounding); half a step of fp16 is
+// 2.4e-4.  17 instructions, erfcf takes 50 (the epilogue of a tile of 256 x 256: 8 us more).
 template <class E>
 __device__ __forceinline__ float erfc_of(float v) {
     if constexpr (E::kSize == 4) {
